@@ -325,6 +325,109 @@ PA_API int pa_prefill(pa_layer* layer, uint32_t seq, uint32_t pos, uint32_t n_co
 PA_API int pa_sigmoid_mul(pa_ctx* ctx, void* a, uint64_t a_col_stride, const void* g, uint64_t g_col_stride,
                           uint64_t g_head_stride, uint32_t n_cols, void* stream);
 
+/* ---- rotary positions of other layouts and scalings ---------------------------------------------------------- */
+
+/* A rotation other than the context's own: pairs of neighbouring dims, frequencies scaled for contexts longer than the
+ * trained one, positions that come from the device, cache rows that are not positions.  Pair i < n_rot / 2 of every head
+ * turns by position * f_i radians, and cos and sin are multiplied by mscale:
+ *   (a, b) -> mscale * (a cos - b sin, b cos + a sin);  dims past n_rot are left as they are.
+ * f_i = theta^(-2i/n_rot), scaled by one of:
+ *   PA_ROPE_SCALE_LINEAR  f_i / factor
+ *   PA_ROPE_SCALE_NTK     theta * factor^(n_rot / (n_rot - 2)) in theta's place
+ *   PA_ROPE_SCALE_YARN    pairs that turn more than `fast` times over the `original` positions stay, those that turn less
+ *                         than `slow` times are divided by factor, and a ramp over the pairs' numbers between: with
+ *                         at(r) = n_rot ln(original / (2 pi r)) / (2 ln theta), lo = max(floor(at(fast)), 0),
+ *                         hi = min(ceil(at(slow)), n_rot - 1), t = clamp((i - lo) / max(hi - lo, 0.001), 0, 1):
+ *                         (1 - t) f_i + t f_i / factor; mscale 1 + 0.1 ln(factor) for a factor above 1
+ *   PA_ROPE_SCALE_BANDS   the same idea by turns: pairs of more than `fast` turns over `original` stay, of fewer than
+ *                         `slow` are divided by factor, between them linear in the number of turns
+ * The frequencies and the angles (reduced to one turn) are float64, everything else f32 (relative error of a rotated pair
+ * below 2^-21 of its length; positions up to 2^31 cost no more than the angle's own 2^-52). */
+typedef enum pa_rope_layout {
+  PA_ROPE_HALF = 0,        /* pair i is dims i and i + n_rot / 2 (the context's own rotation) */
+  PA_ROPE_INTERLEAVED = 1  /* pair i is dims 2i and 2i + 1 */
+} pa_rope_layout;
+typedef enum pa_rope_scaling {
+  PA_ROPE_SCALE_NONE = 0, PA_ROPE_SCALE_LINEAR = 1, PA_ROPE_SCALE_NTK = 2, PA_ROPE_SCALE_YARN = 3, PA_ROPE_SCALE_BANDS = 4
+} pa_rope_scaling;
+typedef struct pa_rotary_config {
+  uint32_t n_rot;     /* rotated dims per head, even, 2 .. head_dim (at least 4 for PA_ROPE_SCALE_NTK) */
+  uint32_t layout;    /* pa_rope_layout */
+  uint32_t scaling;   /* pa_rope_scaling */
+  uint32_t original;  /* trained positions (YARN, BANDS) */
+  double theta;       /* above 1 */
+  double factor;      /* above 0; ignored without scaling */
+  double fast, slow;  /* YARN (0: 32 and 1), BANDS (0: 4 and 1); fast > slow > 0 */
+  double mscale;      /* factor on cos and sin; 0: the scaling's own (1 but for YARN) */
+  uint32_t reserved[4];
+} pa_rotary_config;
+typedef struct pa_rotary pa_rotary;   /* one per (context, rotation) */
+PA_API int pa_rotary_create(pa_ctx* ctx, const pa_rotary_config* cfg, pa_rotary** out);
+PA_API int pa_rotary_destroy(pa_rotary* rotary);   /* before its context */
+/* The frequencies in use, radians per position: n_rot / 2 values, and mscale (either may be NULL).  Host arithmetic only. */
+PA_API int pa_rotary_freqs(const pa_rotary* rotary, double* freqs, double* mscale);
+/* Rotates x into y.  x: x_dtype [n_cols][x_col_stride], head h at h * x_head_stride; y: y_dtype, the same with its own strides;
+ * y may be x with equal type and strides, and otherwise does not overlap it.  Column c is at position positions[c] (int32 on
+ * the device, read when the kernel runs), or, without positions, at pos + c.  A negative position turns back: with mscale 1
+ * the rotation by -p undoes the rotation by p.  Any number of columns and heads; beside pa_rope, which keeps the context's
+ * own rotation bit for bit. */
+PA_API int pa_rotary_apply(pa_rotary* rotary, const void* x, int x_dtype, uint64_t x_col_stride, uint64_t x_head_stride, uint32_t n_heads_x,
+                           const int32_t* positions, int32_t pos, uint32_t n_cols, void* y, int y_dtype, uint64_t y_col_stride,
+                           uint64_t y_head_stride, void* stream);
+/* The front of a layer call with this rotation, for one or many sequences: items[i] = (seq, pos, n_cols) owns the next n_cols
+ * rows of q, k, v (act_dtype) and q_out.  q is rotated into q_out (q_out_dtype, heads packed; q = NULL: k and v only); k is
+ * rotated, k and v are rounded to f16 (as pa_kv_append rounds) and stored in rows rows[i] .. rows[i] + n_cols - 1 of the sequence, or, with
+ * rows = NULL, in the rows of their positions.  Rows and positions part when a cache holds only some of the positions
+ * (pa_evict) or begins behind a shared prefix (pa_decode_shared).  At most 128 items; two items may not store the same row.  f16 caches. */
+PA_API int pa_rotary_append(pa_rotary* rotary, pa_layer* layer, const pa_item* items, uint32_t n_items, const uint32_t* rows, const void* q,
+                            uint64_t q_col_stride, uint64_t q_head_stride, const void* k, const void* v, uint64_t kv_col_stride,
+                            void* q_out, int q_out_dtype, uint64_t q_out_col_stride, void* stream);
+
+/* ---- batches that share a prefix ------------------------------------------------------------------------------ */
+
+/* pa_decode for a batch whose sequences begin with the same prefix_len rows, which are kept once and read once for all:
+ * items[i] = (seq, pos, 1) is one token (its q rotated) that attends the prefix -- rows [0, prefix_len) of sequence
+ * prefix_seq of prefix_layer -- and its own rows, the positions [prefix_len, pos] at rows position - own_base of sequence
+ * seq of layer.  own_base = 0: sequences that keep every position in the row of that number (the first prefix_len of them
+ * unused); own_base = prefix_len: sequences that hold nothing but their own rows.  pos + 1 >= prefix_len; own rows may be
+ * none.  prefix_layer = NULL: layer itself; else any f16 layer of the same device and kv heads x head_dim, its context's too.
+ * Items may repeat a sequence (each is one query against the rows it names).  q, gate, out: as pa_decode's, q strides
+ * multiples of 16 bytes and q 16-byte aligned.  At most 128 items and 64 query heads per kv head; f16 caches, no KV shards
+ * (origin 0). */
+PA_API int pa_decode_shared(pa_layer* layer, pa_layer* prefix_layer, uint32_t prefix_seq, uint32_t prefix_len, uint32_t own_base,
+                            const pa_item* items, uint32_t n_items, const void* q, int q_dtype, uint64_t q_col_stride,
+                            uint64_t q_head_stride, const void* gate, uint64_t gate_col_stride, uint64_t gate_head_stride, void* out,
+                            uint64_t out_col_stride, void* stream);
+
+/* ---- caches that keep what attention uses ---------------------------------------------------------------------- */
+
+/* Gives a layer a sum of attention weights per cached row: f32 [n_seqs][n_kv_heads][max_seq], zeroed, the layer's own, and
+ * the context room for the scores of a call.  f16 caches.  Allocates: not inside a stream capture. */
+PA_API int pa_layer_track_weights(pa_layer* layer);
+PA_API float* pa_weights_ptr(pa_layer* layer);   /* NULL: not tracked */
+/* Zeroes the sums of one sequence, as a new conversation begins with. */
+PA_API int pa_weights_clear(pa_layer* layer, uint32_t seq, void* stream);
+/* pa_decode of one token per item, items[i] = (seq, pos, 1), that attends rows [0, pos + 1) of its sequence (a cache that has
+ * evicted rows counts rows here, not positions) and adds what it gave each row to the row's sum: for every kv head and row,
+ * the softmax weights of the group's query heads.  Sums have a fixed order (head after head, item after item), so repeated
+ * runs give the same bits.  Items may repeat a sequence: a prompt's last tokens, each with the rows it sees.  Limits as
+ * pa_decode_shared's; a call whose scores exceed the context's room runs in parts. */
+PA_API int pa_decode_weights(pa_layer* layer, const pa_item* items, uint32_t n_items, const void* q, int q_dtype, uint64_t q_col_stride,
+                             uint64_t q_head_stride, const void* gate, uint64_t gate_col_stride, uint64_t gate_head_stride, void* out,
+                             uint64_t out_col_stride, void* stream);
+/* Brings a sequence's n_rows rows down to n_keep, for each kv head by itself: the first n_first and the last n_recent stay, and
+ * of those between them the ones with the largest sums (equal sums: the lower row; NaN counts as the largest).  What stays is moved together in its order to
+ * rows [0, n_keep) of sequence dst_seq (dst_seq = src_seq: in place), K, V and sums; the sums behind it are zeroed, the
+ * K and V rows behind it are left as they were.  A sequence of no more than n_keep rows keeps them all.  kept (device, may be NULL): u32
+ * [n_items][n_kv_heads][n_keep], the rows that stayed, ascending, 0xffffffff behind the last.  K rows keep the rotation of the
+ * position they were appended at; the next token goes to row n_keep (pa_rotary_append).  No dst_seq may be named by another item, be it
+ * as its source or its destination.  At most 32 items, 393216 rows; needs pa_layer_track_weights; f16 caches, origin 0. */
+typedef struct pa_evict_item {
+  uint32_t src_seq, dst_seq, n_rows, reserved;
+} pa_evict_item;
+PA_API int pa_evict(pa_layer* layer, const pa_evict_item* items, uint32_t n_items, uint32_t n_keep, uint32_t n_first, uint32_t n_recent,
+                    uint32_t* kept, void* stream);
+
 /* ---- the path in one call --------------------------------------------------------------------------- */
 
 enum { PA_MODE_AUTO = 0, PA_MODE_DECODE = 1, PA_MODE_PREFILL = 2 };

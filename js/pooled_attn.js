@@ -67,6 +67,17 @@ export const SYMBOLS = {
   pa_attn_step_host: { parameters: [BUF, U32, U32, U32, U32, I32, BUF, U64, U64, U64, BUF, BUF, U64, U64, BUF, U64, U64, U64, BUF, U64, U64, P], result: I32, nonblocking: true },
   pa_decode_static: { parameters: [I32, P, P, U32, U32, U32, U32, U32, U32, P, P, P, P, BUF, U64], result: I32 },
   pa_decode_static_status: { parameters: [I32, P, BUF], result: I32, nonblocking: true },
+  pa_rotary_create: { parameters: [P, BUF, BUF], result: I32 },
+  pa_rotary_destroy: { parameters: [P], result: I32 },
+  pa_rotary_freqs: { parameters: [P, BUF, BUF], result: I32 },
+  pa_rotary_apply: { parameters: [P, P, I32, U64, U64, U32, P, I32, U32, P, I32, U64, U64, P], result: I32 },
+  pa_rotary_append: { parameters: [P, P, BUF, U32, BUF, P, U64, U64, P, P, U64, P, I32, U64, P], result: I32 },
+  pa_decode_shared: { parameters: [P, P, U32, U32, U32, BUF, U32, P, I32, U64, U64, P, U64, U64, P, U64, P], result: I32 },
+  pa_layer_track_weights: { parameters: [P], result: I32 },
+  pa_weights_ptr: { parameters: [P], result: P },
+  pa_weights_clear: { parameters: [P, U32, P], result: I32 },
+  pa_decode_weights: { parameters: [P, BUF, U32, P, I32, U64, U64, P, U64, U64, P, U64, P], result: I32 },
+  pa_evict: { parameters: [P, BUF, U32, U32, U32, U32, P, P], result: I32 },
   pa_set_wait_limit: { parameters: [P, U32], result: I32 },
   pa_get_stats: { parameters: [P, BUF], result: I32 },
   pa_timing_begin: { parameters: [P, U32], result: I32 },

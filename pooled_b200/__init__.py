@@ -7,5 +7,5 @@ pooled's engines (engine/qwen35.js _encodeLayerR / _encAttnCore, engine/wgsl/att
 without a GPU, every compute call needs the CUDA library and a B200.
 """
 from .lib import PA_F16, PA_F32, PaError, Lib, load  # noqa: F401
-from .attn import (AttnConfig, AttnEngine, DEC_CQ, attn_dec_config, attn_tile_config, dec_split_len, dec_splits,  # noqa: F401
+from .attn import (AttnConfig, AttnEngine, DEC_CQ, Rotary, attn_dec_config, attn_tile_config, dec_split_len, dec_splits,  # noqa: F401
                    tile_split_len)

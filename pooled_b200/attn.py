@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import weakref
 from dataclasses import dataclass
 
 import torch
@@ -108,6 +109,61 @@ class _DevArray:
         self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": typestr, "data": (ptr, False), "version": 3}
 
 
+_LAYOUT = {"half": _l.PA_ROPE_HALF, "interleaved": _l.PA_ROPE_INTERLEAVED}
+_SCALING = {"none": _l.PA_ROPE_SCALE_NONE, "linear": _l.PA_ROPE_SCALE_LINEAR, "ntk": _l.PA_ROPE_SCALE_NTK, "yarn": _l.PA_ROPE_SCALE_YARN,
+            "bands": _l.PA_ROPE_SCALE_BANDS}
+
+
+class Rotary:
+    """A rotation of its own layout and scaling (pa_rotary), made by AttnEngine.rotary."""
+
+    def __init__(self, eng: "AttnEngine", cfg: "_l.PaRotaryConfig"):
+        self.eng, self.n_rot, self.handle = eng, cfg.n_rot, None
+        h = C.c_void_p()
+        eng._ck(eng.L.pa_rotary_create(eng.ctx, C.byref(cfg), C.byref(h)))
+        self.handle = h
+        eng._rotaries.add(self)
+        self._apply, self._f_apply = eng._call.rotary_apply, eng.L.entry["pa_rotary_apply"]
+
+    def destroy(self):
+        if self.handle and self.eng.ctx:
+            self.eng.L.pa_rotary_destroy(self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+    def freqs(self):
+        """(radians per position of every rotated pair, the factor on cos and sin)."""
+        f, m = (C.c_double * (self.n_rot // 2))(), C.c_double()
+        self.eng._ck(self.eng.L.pa_rotary_freqs(self.handle, f, C.byref(m)))
+        return list(f), m.value
+
+    def apply(self, x: torch.Tensor, n_heads: int, pos: int = 0, positions: torch.Tensor | None = None, head_stride: int | None = None,
+              out: torch.Tensor | None = None, out_head_stride: int | None = None) -> torch.Tensor:
+        """x [n_cols, stride] (float16 or float32) rotated: column c at pos + c, or at positions[c] (int32 on the device).  Into a
+        new [n_cols, n_heads * head_dim] of x's type, or `out`, which may be x itself (with x's head_stride)."""
+        eng = self.eng
+        hd = eng.cfg.head_dim
+        eng._on_device(x, out, positions)
+        if positions is not None and (positions.dtype != torch.int32 or positions.dim() != 1 or positions.shape[0] != x.shape[0] or positions.stride(0) != 1):
+            raise _l.PaError(-1, "positions are a contiguous int32 tensor of one value per column")
+        if out is None:
+            out = torch.empty((x.shape[0], n_heads * hd), dtype=x.dtype, device=x.device)
+        elif out.shape[0] != x.shape[0]:
+            raise _l.PaError(-1, f"out has {out.shape[0]} columns for {x.shape[0]}")
+        hs, ohs = head_stride or hd, out_head_stride or (head_stride if out is x and head_stride else hd)
+        if (n_heads - 1) * hs + hd > x.shape[1] or (n_heads - 1) * ohs + hd > out.shape[1]:
+            raise _l.PaError(-1, f"{n_heads} heads do not fit the columns of x or out")
+        rc = self._apply(self._f_apply, self.handle.value, x, _dt(x.dtype), hs, n_heads, positions, pos, out, _dt(out.dtype), ohs, eng._raw_st())
+        if rc:
+            eng._ck(rc)
+        return out
+
+
 class AttnEngine:
     """The attention part of an engine: per-layer f16 K/V caches and the per-layer attention step."""
 
@@ -116,6 +172,7 @@ class AttnEngine:
         self.L = _l.load()
         self._call, e = self.L.call, self.L.entry
         self._f_layer, self._f_items, self._f_rope, self._f_gather = e["pa_attn_layer"], e["pa_attn_items"], e["pa_rope_append"], e["pa_decode_gather"]
+        self._f_rot_append, self._f_shared, self._f_weights, self._f_evict = e["pa_rotary_append"], e["pa_decode_shared"], e["pa_decode_weights"], e["pa_evict"]
         pc = _l.PaConfig(n_heads=cfg.n_heads, n_kv_heads=cfg.n_kv_heads, head_dim=cfg.head_dim, n_rot=cfg.n_rot, rope_theta=cfg.rope_theta,
                          rope_mode=_ROPE[cfg.rope_mode], act_dtype=_dt(cfg.act_dtype), max_cols=cfg.max_cols, splits=cfg.splits,
                          flags=_l.PA_FLAG_FAST if cfg.fast else 0)
@@ -124,6 +181,7 @@ class AttnEngine:
         self.layers: list[C.c_void_p] = []
         self.slots: dict[str, dict] = {}
         self._xc_keep = None
+        self._rotaries = weakref.WeakSet()      # destroyed ahead of the context
         self.L.check(self.L.pa_create(device, C.byref(pc), C.byref(h)))
         self.ctx = h
         try:
@@ -163,6 +221,8 @@ class AttnEngine:
         for lh in self.layers:
             self.L.pa_layer_destroy(lh)
         self.layers = []
+        for r in list(getattr(self, "_rotaries", ())):
+            r.destroy()
         if self.ctx:
             self.L.pa_destroy(self.ctx)
             self.ctx = None
@@ -352,6 +412,113 @@ class AttnEngine:
     def sigmoid_mul(self, a: torch.Tensor, g: torch.Tensor, g_head_stride: int | None = None):
         self._ck(self.L.pa_sigmoid_mul(self.ctx, self._p(a), a.stride(0), self._p(g), g.stride(0), g_head_stride or self.cfg.head_dim,
                                        a.shape[0], self._st()))
+
+    # ---- rotations of other layouts and scalings ----
+    def rotary(self, n_rot: int | None = None, theta: float | None = None, layout: str = "half", scaling: str = "none", factor: float = 1.0, original: int = 0,
+               beta_fast: float = 0.0, beta_slow: float = 0.0, high: float = 0.0, low: float = 0.0, mscale: float = 0.0) -> Rotary:
+        """A rotation beside the engine's own: pairs of dims "half" a rotation apart or "interleaved", frequencies unscaled ("none"),
+        "linear", "ntk", "yarn" (beta_fast, beta_slow: 32 and 1 unless given) or "bands" (high, low: 4 and 1) for a context `factor` times the
+        `original` one; mscale 0: the scaling's own factor on cos and sin.  The formulas stand in include/pooled_attn.h."""
+        fast, slow = (high, low) if scaling == "bands" else (beta_fast, beta_slow)
+        return Rotary(self, _l.PaRotaryConfig(n_rot=self.cfg.n_rot if n_rot is None else n_rot, layout=_LAYOUT[layout], scaling=_SCALING[scaling], original=original,
+                                              theta=self.cfg.rope_theta if theta is None else theta, factor=factor, fast=fast, slow=slow, mscale=mscale))
+
+    def rotary_append(self, li: int, rot: Rotary, items, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, rows=None, q_head_stride: int | None = None,
+                      q_dtype: torch.dtype = torch.float32, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+        """rope_append with `rot`, for one or many sequences: items = [(seq, pos, n_cols)] own consecutive rows of q, k and v.  Item i's k and v go to
+        cache rows rows[i] .. (None: the rows of their positions).  Returns the rotated q, [n_cols, q_dim] of q_dtype (None without q)."""
+        total = sum(it[2] for it in items)
+        self._columns(total, q, k, v, q_out)
+        if q is not None and q_out is None:
+            q_out = torch.empty((total, self.cfg.q_dim), dtype=q_dtype, device=k.device)
+        if k.stride(0) != v.stride(0):
+            raise _l.PaError(-1, "k and v have different column strides")
+        rc = self._call.rotary_append(self._f_rot_append, rot.handle.value, self.layers[li].value, items, rows, q, q_head_stride or self.cfg.head_dim, k, v, q_out,
+                                      _l.PA_F32 if q is None else _dt(q_out.dtype), self._raw_st())
+        if rc:
+            self._ck(rc)
+        return q_out
+
+    def _on_device(self, *tensors):
+        for t in tensors:
+            if t is not None and (t.device.index != self.device or t.stride(-1) != 1):
+                raise _l.PaError(-1, f"a tensor on {t.device} with strides {t.stride()}: the engine takes rows of consecutive values on cuda:{self.device}")
+
+    def _columns(self, n: int, q, k, v, out):
+        """Columns of the engine's own types: q, k, v of act_dtype, n of each."""
+        c = self.cfg
+        self._on_device(q, k, v, out)
+        for t, width in ((q, c.head_dim), (k, c.kv_dim), (v, c.kv_dim)):
+            if t is not None and (t.dtype != c.act_dtype or t.dim() != 2 or t.shape[0] != n or t.shape[1] < width):
+                raise _l.PaError(-1, f"{t.dtype} {tuple(t.shape)}: {n} columns of {c.act_dtype} are wanted")
+        if out is not None and (out.dim() != 2 or out.shape[0] != n or out.shape[1] < c.q_dim):
+            raise _l.PaError(-1, f"an output of shape {tuple(out.shape)} for {n} columns of {c.q_dim}")
+
+    def _batch(self, n: int, q, q_head_stride, gate, gate_head_stride, out):
+        """The tensors of a decode of n single tokens; returns out, made where it is None."""
+        c = self.cfg
+        hd, last = c.head_dim, c.n_heads - 1
+        if out is None:
+            out = torch.empty((n, c.q_dim), dtype=c.act_dtype, device=q.device)
+        self._on_device(q, gate, out)
+        if q.dim() != 2 or q.shape[0] != n or last * (q_head_stride or hd) + hd > q.shape[1]:
+            raise _l.PaError(-1, f"q of shape {tuple(q.shape)} for {n} items of {c.n_heads} heads")
+        if gate is not None and (gate.dtype != c.act_dtype or gate.dim() != 2 or gate.shape[0] != n or last * (gate_head_stride or hd) + hd > gate.shape[1]):
+            raise _l.PaError(-1, f"{gate.dtype} gate of shape {tuple(gate.shape)} for {n} items of {c.n_heads} heads")
+        if out.dtype != c.act_dtype or out.dim() != 2 or out.shape[0] != n or out.shape[1] < c.q_dim:
+            raise _l.PaError(-1, f"{out.dtype} output of shape {tuple(out.shape)} for {n} columns of {c.q_dim}")
+        return out
+
+    # ---- batches that share a prefix ----
+    def decode_shared(self, li: int, prefix: "AttnEngine | None", prefix_seq: int, prefix_len: int, seqs_pos, q: torch.Tensor, gate: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None, own_base: int = 0, q_head_stride: int | None = None, gate_head_stride: int | None = None) -> torch.Tensor:
+        """One token of each of several sequences that begin with the same rows: seqs_pos = [(seq, pos)], row i of q (rotated), gate and out belongs to
+        item i, which attends rows [0, prefix_len) of sequence prefix_seq of layer li of `prefix` (an engine with caches of their own; None: this
+        one's) and its own rows, the positions [prefix_len, pos] at rows position - own_base of its sequence.  The prefix is read once for all."""
+        out = self._batch(len(seqs_pos), q, q_head_stride, gate, gate_head_stride, out)
+        hd = self.cfg.head_dim
+        rc = self._call.decode_shared(self._f_shared, self.layers[li].value, (prefix or self).layers[li].value, prefix_seq, prefix_len, own_base, seqs_pos, q, _dt(q.dtype),
+                                      q_head_stride or hd, gate, gate_head_stride or hd, out, self._raw_st())
+        if rc:
+            self._ck(rc)
+        return out
+
+    # ---- caches that keep what attention uses ----
+    def track_weights(self, li: int):
+        """Gives layer li a sum of attention weights per cached row (zeros at first)."""
+        self._ck(self.L.pa_layer_track_weights(self.layers[li]))
+
+    def weights(self, li: int) -> torch.Tensor:
+        """The sums of a tracked layer: float32 [n_seqs, n_kv_heads, max_seq] (no copy)."""
+        ptr = self.L.pa_weights_ptr(self.layers[li])
+        if not ptr:
+            raise _l.PaError(-1, "the layer's weights are not tracked: call track_weights first")
+        return torch.as_tensor(_DevArray(ptr, (self.cfg.n_seqs, self.cfg.n_kv_heads, self.cfg.max_seq), "<f4"), device=f"cuda:{self.device}")
+
+    def clear_weights(self, li: int, seq: int):
+        self._ck(self.L.pa_weights_clear(self.layers[li], seq, self._st()))
+
+    def decode_weights(self, li: int, seqs_pos, q: torch.Tensor, gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                       q_head_stride: int | None = None, gate_head_stride: int | None = None) -> torch.Tensor:
+        """decode() of one token per item (seqs_pos = [(seq, pos)]: rows [0, pos] of its sequence), which adds the softmax weights to the rows' sums:
+        weights(li)[seq, kv head, row] grows by what the group's query heads gave the row."""
+        out = self._batch(len(seqs_pos), q, q_head_stride, gate, gate_head_stride, out)
+        hd = self.cfg.head_dim
+        rc = self._call.decode_weights(self._f_weights, self.layers[li].value, seqs_pos, q, _dt(q.dtype), q_head_stride or hd, gate, gate_head_stride or hd, out,
+                                       self._raw_st())
+        if rc:
+            self._ck(rc)
+        return out
+
+    def evict(self, li: int, items, n_keep: int, n_first: int = 0, n_recent: int = 0) -> torch.Tensor:
+        """Brings sequences down to n_keep rows per kv head, the first n_first, the last n_recent and the rows with the largest sums between them:
+        items = [(src_seq, dst_seq, n_rows)], dst_seq = src_seq in place.  Returns the rows that stayed, int32 [n_items, n_kv_heads, n_keep],
+        ascending, -1 behind the last."""
+        kept = torch.empty((len(items), self.cfg.n_kv_heads, max(0, n_keep)), dtype=torch.int32, device=f"cuda:{self.device}")
+        rc = self._call.evict(self._f_evict, self.layers[li].value, items, n_keep, n_first, n_recent, kept, self._raw_st())
+        if rc:
+            self._ck(rc)
+        return kept
 
     # ---- the path in one call ----
     def encode_layer(self, li: int, pos: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gate: torch.Tensor | None = None,

@@ -10,7 +10,7 @@
 #include <new>
 
 #include "pa_common.cuh"
-
+#include "pa_host.cuh"
 #include "pa_params.cuh"
 
 namespace pa {
@@ -43,7 +43,7 @@ using namespace pa;
 
 static thread_local std::string g_err;  // for failures before a context exists
 
-static int fail(pa_ctx* ctx, int code, const char* fmt, ...) {
+int pa::fail(pa_ctx* ctx, int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -52,14 +52,6 @@ static int fail(pa_ctx* ctx, int code, const char* fmt, ...) {
   if (ctx) ctx->err = buf; else g_err = buf;
   return code;
 }
-#define CU_TRY(ctx, expr)                                                                         \
-  do {                                                                                            \
-    cudaError_t e_ = (expr);                                                                      \
-    if (e_ != cudaSuccess) {                                                                      \
-      (ctx)->failed = true;                                                                       \
-      return fail((ctx), PA_ECUDA, "%s failed: %s", #expr, cudaGetErrorString(e_));               \
-    }                                                                                             \
-  } while (0)
 
 typedef CUresult (*encode_tiled_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                     const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -225,6 +217,8 @@ extern "C" int pa_destroy(pa_ctx* ctx) {
   cudaSetDevice(ctx->device);
   cudaFree(ctx->inv_freq); cudaFree(ctx->angles); cudaFree(ctx->norm_q); cudaFree(ctx->norm_k); cudaFree(ctx->q_rot); cudaFree(ctx->k_rot); cudaFree(ctx->part_o); cudaFree(ctx->part_ml); cudaFree(ctx->dev_err); cudaFree(ctx->merge_rec); cudaFree(ctx->merge_ctr);
   cudaFree(ctx->stage_dev);
+  cudaFree(ctx->scores);
+  for (void* p : ctx->outgrown) cudaFree(p);
   for (cudaEvent_t e : ctx->side_ev) if (e) cudaEventDestroy(e);
   if (ctx->side) cudaStreamDestroy(ctx->side);
   for (cudaEvent_t e : ctx->ev) cudaEventDestroy(e);
@@ -282,7 +276,7 @@ extern "C" int pa_layer_create(pa_ctx* ctx, uint32_t n_seqs, uint32_t max_seq, p
 extern "C" int pa_layer_destroy(pa_layer* L) {
   if (!L) return PA_OK;
   cudaSetDevice(L->ctx->device);
-  cudaFree(L->k); cudaFree(L->v); cudaFree(L->k_alt); cudaFree(L->v_alt); cudaFree(L->k_scale); cudaFree(L->v_scale);
+  cudaFree(L->k); cudaFree(L->v); cudaFree(L->k_alt); cudaFree(L->v_alt); cudaFree(L->k_scale); cudaFree(L->v_scale); cudaFree(L->sums);
   delete L;
   return PA_OK;
 }
@@ -424,12 +418,6 @@ extern "C" int pa_download(pa_ctx* ctx, void* h, const void* d, size_t n, void* 
 }
 
 // ------------------------------------------------------------------------------ the path --
-
-#define GUARD(ctx)                                                                                       \
-  do {                                                                                                   \
-    if (!(ctx)) return PA_EINVAL;                                                                        \
-    if ((ctx)->failed) return fail((ctx), PA_ESTATE, "an earlier step failed (%s); call pa_reset() first", (ctx)->err.c_str()); \
-  } while (0)
 
 // own_rows: the call writes or reads rows pos .. pos+n_cols-1 themselves, which must lie inside this layer's cache
 // (for a shard: inside [origin, origin + max_seq)); otherwise any position at or past the origin's sequence is fine

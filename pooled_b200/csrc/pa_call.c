@@ -19,6 +19,13 @@ typedef int (*fn_rope_append)(pa_layer*, uint32_t, uint32_t, uint32_t, const voi
                               void*);
 typedef int (*fn_decode_gather)(pa_layer*, uint32_t, uint32_t, const uint32_t*, uint32_t, const void*, int, uint64_t, uint64_t, const void*, uint64_t,
                                 uint64_t, void*, uint64_t, void*);
+typedef int (*fn_rotary_apply)(pa_rotary*, const void*, int, uint64_t, uint64_t, uint32_t, const int32_t*, int32_t, uint32_t, void*, int, uint64_t, uint64_t, void*);
+typedef int (*fn_rotary_append)(pa_rotary*, pa_layer*, const pa_item*, uint32_t, const uint32_t*, const void*, uint64_t, uint64_t, const void*, const void*, uint64_t,
+                                void*, int, uint64_t, void*);
+typedef int (*fn_decode_shared)(pa_layer*, pa_layer*, uint32_t, uint32_t, uint32_t, const pa_item*, uint32_t, const void*, int, uint64_t, uint64_t, const void*,
+                                uint64_t, uint64_t, void*, uint64_t, void*);
+typedef int (*fn_decode_weights)(pa_layer*, const pa_item*, uint32_t, const void*, int, uint64_t, uint64_t, const void*, uint64_t, uint64_t, void*, uint64_t, void*);
+typedef int (*fn_evict)(pa_layer*, const pa_evict_item*, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t*, void*);
 /* Every call names the entry point (its address in the library the engine loaded) as its first argument: the module keeps
  * nothing of its own. */
 static PyObject *s_data_ptr, *s_stride, *s_size, *i_zero;
@@ -142,11 +149,154 @@ static PyObject* decode_gather(PyObject* self, PyObject* const* a, Py_ssize_t n)
   return PyLong_FromLong(rc);
 }
 
+/* a sequence of `width`-tuples of integers as `width` words each of a four-word struct, the others `rest`; NULL with an error set.  Freed by the caller. */
+static uint32_t* words_of(PyObject* o, Py_ssize_t width, uint32_t rest, const char* what, Py_ssize_t* cnt) {
+  PyObject* list = PySequence_Fast(o, what);
+  if (!list) return NULL;
+  *cnt = PySequence_Fast_GET_SIZE(list);
+  uint32_t* w = (uint32_t*)calloc((size_t)(*cnt ? *cnt : 1) * 4, sizeof(uint32_t));
+  if (!w) { Py_DECREF(list); PyErr_NoMemory(); return NULL; }
+  for (Py_ssize_t i = 0; i < *cnt; ++i) {
+    PyObject* t = PySequence_Fast(PySequence_Fast_GET_ITEM(list, i), what);
+    int bad = !t;
+    if (t && PySequence_Fast_GET_SIZE(t) != width) { PyErr_SetString(PyExc_ValueError, what); bad = 1; }
+    for (Py_ssize_t k = 0; !bad && k < width; ++k) bad = u32_of(PySequence_Fast_GET_ITEM(t, k), &w[4 * i + k]);
+    Py_XDECREF(t);
+    if (bad) { free(w); Py_DECREF(list); return NULL; }
+    if (width == 2) w[4 * i + 2] = rest;
+  }
+  Py_DECREF(list);
+  return w;
+}
+static const char* const kPairs = "the items are a sequence of (seq, pos) pairs";
+static const char* const kTriples = "the items are a sequence of triples";
+
+/* rotary_apply(entry, rotary, x, x_dtype, head_stride, n_heads, positions, pos, y, y_dtype, y_head_stride, stream) -> status */
+static PyObject* rotary_apply(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  uint64_t fn, rot, xcs, xhs, ycs, yhs, stream;
+  uint32_t xdt, ydt, heads, pos, cols;
+  void *x, *ps, *y;
+  (void)self;
+  if (args_are(n, 12, "rotary_apply") || u64_of(a[0], &fn) || u64_of(a[1], &rot) || ptr_of(a[2], &x) || stride0(a[2], &xcs) || rows_of(a[2], &cols) || u32_of(a[3], &xdt) ||
+      u64_of(a[4], &xhs) || u32_of(a[5], &heads) || ptr_of(a[6], &ps) || u32_of(a[7], &pos) || ptr_of(a[8], &y) || stride0(a[8], &ycs) || u32_of(a[9], &ydt) ||
+      u64_of(a[10], &yhs) || u64_of(a[11], &stream))
+    return NULL;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = ((fn_rotary_apply)(uintptr_t)fn)((pa_rotary*)(uintptr_t)rot, x, (int)xdt, xcs, xhs, heads, (const int32_t*)ps, (int32_t)pos, cols, y, (int)ydt, ycs, yhs,
+                    (void*)(uintptr_t)stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+/* rotary_append(entry, rotary, layer, [(seq, pos, n_cols)], rows, q, q_head_stride, k, v, q_out, q_out_dtype, stream) -> status */
+static PyObject* rotary_append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  uint64_t fn, rot, layer, qcs = 0, qhs = 0, kcs, ocs = 0, stream;
+  uint32_t odt;
+  void *q, *k, *v, *o;
+  (void)self;
+  if (args_are(n, 12, "rotary_append") || u64_of(a[0], &fn) || u64_of(a[1], &rot) || u64_of(a[2], &layer) || ptr_of(a[5], &q) ||
+      (a[5] != Py_None && (stride0(a[5], &qcs) || u64_of(a[6], &qhs))) || ptr_of(a[7], &k) || stride0(a[7], &kcs) || ptr_of(a[8], &v) || ptr_of(a[9], &o) ||
+      (a[9] != Py_None && stride0(a[9], &ocs)) || u32_of(a[10], &odt) || u64_of(a[11], &stream))
+    return NULL;
+  Py_ssize_t cnt, nr = 0;
+  uint32_t *items = words_of(a[3], 3, 0, kTriples, &cnt), *rows = NULL;
+  if (!items) return NULL;
+  if (a[4] != Py_None) {
+    PyObject* list = PySequence_Fast(a[4], "the rows are a sequence of integers");
+    int bad = !list;
+    if (list) {
+      nr = PySequence_Fast_GET_SIZE(list);
+      if (nr != cnt) { PyErr_SetString(PyExc_ValueError, "one row per item"); bad = 1; }
+      rows = bad ? NULL : (uint32_t*)calloc((size_t)(nr ? nr : 1), sizeof(uint32_t));
+      if (!bad && !rows) { PyErr_NoMemory(); bad = 1; }
+      for (Py_ssize_t i = 0; !bad && i < nr; ++i) bad = u32_of(PySequence_Fast_GET_ITEM(list, i), &rows[i]);
+      Py_DECREF(list);
+    }
+    if (bad) { free(rows); free(items); return NULL; }
+  }
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = ((fn_rotary_append)(uintptr_t)fn)((pa_rotary*)(uintptr_t)rot, (pa_layer*)(uintptr_t)layer, (const pa_item*)items, (uint32_t)cnt, rows, q, qcs, qhs, k, v, kcs, o,
+                    (int)odt, ocs, (void*)(uintptr_t)stream);
+  Py_END_ALLOW_THREADS
+  free(rows); free(items);
+  return PyLong_FromLong(rc);
+}
+
+/* decode_shared(entry, layer, prefix_layer, prefix_seq, prefix_len, own_base, [(seq, pos)], q, q_dtype, q_head_stride, gate, gate_head_stride, out, stream) -> status */
+static PyObject* decode_shared(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  uint64_t fn, layer, pre, qcs, qhs, gcs = 0, ghs = 0, ocs, stream;
+  uint32_t seq, len, base, qdt;
+  void *q, *g, *out;
+  (void)self;
+  if (args_are(n, 14, "decode_shared") || u64_of(a[0], &fn) || u64_of(a[1], &layer) || u64_of(a[2], &pre) || u32_of(a[3], &seq) || u32_of(a[4], &len) || u32_of(a[5], &base) ||
+      ptr_of(a[7], &q) || stride0(a[7], &qcs) || u32_of(a[8], &qdt) || u64_of(a[9], &qhs) || ptr_of(a[10], &g) ||
+      (a[10] != Py_None && (stride0(a[10], &gcs) || u64_of(a[11], &ghs))) || ptr_of(a[12], &out) || stride0(a[12], &ocs) || u64_of(a[13], &stream))
+    return NULL;
+  Py_ssize_t cnt;
+  uint32_t* items = words_of(a[6], 2, 1, kPairs, &cnt);
+  if (!items) return NULL;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = ((fn_decode_shared)(uintptr_t)fn)((pa_layer*)(uintptr_t)layer, (pa_layer*)(uintptr_t)pre, seq, len, base, (const pa_item*)items, (uint32_t)cnt, q, (int)qdt, qcs,
+                    qhs, g, gcs, ghs, out, ocs, (void*)(uintptr_t)stream);
+  Py_END_ALLOW_THREADS
+  free(items);
+  return PyLong_FromLong(rc);
+}
+
+/* decode_weights(entry, layer, [(seq, pos)], q, q_dtype, q_head_stride, gate, gate_head_stride, out, stream) -> status */
+static PyObject* decode_weights(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  uint64_t fn, layer, qcs, qhs, gcs = 0, ghs = 0, ocs, stream;
+  uint32_t qdt;
+  void *q, *g, *out;
+  (void)self;
+  if (args_are(n, 10, "decode_weights") || u64_of(a[0], &fn) || u64_of(a[1], &layer) || ptr_of(a[3], &q) || stride0(a[3], &qcs) || u32_of(a[4], &qdt) || u64_of(a[5], &qhs) ||
+      ptr_of(a[6], &g) || (a[6] != Py_None && (stride0(a[6], &gcs) || u64_of(a[7], &ghs))) || ptr_of(a[8], &out) || stride0(a[8], &ocs) || u64_of(a[9], &stream))
+    return NULL;
+  Py_ssize_t cnt;
+  uint32_t* items = words_of(a[2], 2, 1, kPairs, &cnt);
+  if (!items) return NULL;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = ((fn_decode_weights)(uintptr_t)fn)((pa_layer*)(uintptr_t)layer, (const pa_item*)items, (uint32_t)cnt, q, (int)qdt, qcs, qhs, g, gcs, ghs, out, ocs,
+                    (void*)(uintptr_t)stream);
+  Py_END_ALLOW_THREADS
+  free(items);
+  return PyLong_FromLong(rc);
+}
+
+/* evict(entry, layer, [(src_seq, dst_seq, n_rows)], n_keep, n_first, n_recent, kept, stream) -> status */
+static PyObject* evict(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  uint64_t fn, layer, stream;
+  uint32_t keep, first, recent;
+  void* kept;
+  (void)self;
+  if (args_are(n, 8, "evict") || u64_of(a[0], &fn) || u64_of(a[1], &layer) || u32_of(a[3], &keep) || u32_of(a[4], &first) || u32_of(a[5], &recent) || ptr_of(a[6], &kept) ||
+      u64_of(a[7], &stream))
+    return NULL;
+  Py_ssize_t cnt;
+  uint32_t* items = words_of(a[2], 3, 0, kTriples, &cnt);
+  if (!items) return NULL;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = ((fn_evict)(uintptr_t)fn)((pa_layer*)(uintptr_t)layer, (const pa_evict_item*)items, (uint32_t)cnt, keep, first, recent, (uint32_t*)kept, (void*)(uintptr_t)stream);
+  Py_END_ALLOW_THREADS
+  free(items);
+  return PyLong_FromLong(rc);
+}
+
 static PyMethodDef methods[] = {
     {"attn_layer", (PyCFunction)(void (*)(void))attn_layer, METH_FASTCALL, "pa_attn_layer on tensors"},
     {"attn_items", (PyCFunction)(void (*)(void))attn_items, METH_FASTCALL, "pa_attn_items on tensors"},
     {"rope_append", (PyCFunction)(void (*)(void))rope_append, METH_FASTCALL, "pa_rope_append on tensors"},
     {"decode_gather", (PyCFunction)(void (*)(void))decode_gather, METH_FASTCALL, "pa_decode_gather on tensors"},
+    {"rotary_apply", (PyCFunction)(void (*)(void))rotary_apply, METH_FASTCALL, "pa_rotary_apply on tensors"},
+    {"rotary_append", (PyCFunction)(void (*)(void))rotary_append, METH_FASTCALL, "pa_rotary_append on tensors"},
+    {"decode_shared", (PyCFunction)(void (*)(void))decode_shared, METH_FASTCALL, "pa_decode_shared on tensors"},
+    {"decode_weights", (PyCFunction)(void (*)(void))decode_weights, METH_FASTCALL, "pa_decode_weights on tensors"},
+    {"evict", (PyCFunction)(void (*)(void))evict, METH_FASTCALL, "pa_evict on tensors"},
     {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pa_call", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__pa_call(void) {

@@ -420,6 +420,11 @@ struct pa_ctx {
     bool no_merge = false;       // POOLED_ATTN_NO_MERGE: always merge the split records in the combine kernel
     uint32_t wait_polls = 0;     // pa_set_wait_limit: limit of the waits for other CTAs' and other GPUs' records (0: the built-in limits)
   } tune;
+  // device: the scores of one pa_decode_weights call, or the lists of a pa_evict call (pa_layer_track_weights makes it as large as
+  // the largest tracked layer wants it); `outgrown`: earlier ones, which captured graphs may still use
+  float* scores = nullptr;
+  size_t scores_floats = 0;
+  std::vector<void*> outgrown;
   bool failed = false;
   std::string err;
   pa_stats stats{};
@@ -442,4 +447,5 @@ struct pa_layer {
   const float* qnorm_w = nullptr;   // QK head-norm weights of this layer (device, f32 [head_dim]); nullptr: the layer
   const float* knorm_w = nullptr;   // call takes q and k as they come
   double norm_eps = 0.0;
+  float* sums = nullptr;            // summed attention weights, f32 [n_seqs][n_kv_heads][max_seq] (pa_layer_track_weights)
 };

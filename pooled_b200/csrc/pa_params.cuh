@@ -200,4 +200,71 @@ struct PrefillParams {
   uint32_t out_tma;             // prefill, f16 out: the CTA's output tile leaves through shared memory by one TMA store (tm_o)
 };
 
+constexpr int kMaxShared = 128;   // items of one pa_rotary_append / pa_decode_shared / pa_decode_weights call
+
+// rotation by a pa_rotary, and the append behind it (pa_rotary_kernel)
+struct RotaryParams {
+  const double* turns;     // [n_rot / 2] turns of a pair per position
+  float mscale;
+  uint32_t hd, n_rot, layout, n_cols, cpb;                                   // cpb: columns of a CTA (the launcher sets it)
+  const void* q; uint64_t q_col_stride, q_head_stride; uint32_t q_heads;    // q == nullptr: k and v only
+  void* q_out; uint64_t q_out_col_stride, q_out_head_stride;
+  int in_f16, out_f16;
+  const int32_t* positions;                                                 // no append: per column, or nullptr: pos[0] + column
+  // append: rows of f16 caches; item i owns columns col0[i] .., at positions pos[i] .. and cache rows row[i] .. (over all sequences)
+  const void* k; const void* v; uint64_t kv_col_stride; uint32_t kv_heads;
+  __half* k_cache; __half* v_cache;
+  uint32_t n_items, one_each;                                               // one_each: every item has one column
+  int32_t pos[kMaxShared];
+  uint32_t col0[kMaxShared];
+  uint64_t row[kMaxShared];
+};
+
+// attention of one token per item against rows all items share and rows of its own (pa_shared_kernel), and the merge of its
+// records, with or without the sums of the weights (pa_shared_finish_kernel)
+struct SharedParams {
+  const void* q; int q_f16; uint64_t q_col_stride, q_head_stride;           // rotated queries: item i is column i
+  uint32_t n_items, n_heads, G;
+  float scale_log2;
+  float* part_o; float* part_ml; uint32_t n_rec;                            // records of a row (column, head): n_rec apart; m in log2 units
+  // the shared rows [0, p_rows) from row p_row0 of their cache on: units 0 .. p_splits * row_tiles - 1, a row tile being the
+  // heads of items_per_tile items
+  uint32_t p_row0, p_rows, p_tps, p_splits, row_tiles, items_per_tile;
+  // the items' own rows, rows[i] of them from row own_row0 of sequence seq[i] on: units cta0[i] .. cta0[i + 1] - 1 behind those
+  uint32_t max_seq, own_row0, tps, units;
+  uint32_t seq[kMaxShared], rows[kMaxShared];
+  uint32_t cta0[kMaxShared + 1];
+  float* scores;                                                            // != nullptr: q . k of every own row, f32 [item][kv head][G][rows up to 64]
+  uint64_t score0[kMaxShared];                                              // an item's first float
+  uint32_t* err;
+};
+
+struct SharedFinishParams {
+  const float* part_o; const float* part_ml; uint32_t n_rec, p_splits;
+  uint32_t n_items, n_heads, G, n_kv;
+  const void* gate; uint64_t gate_col_stride, gate_head_stride;
+  void* out; uint64_t out_col_stride; int act_f16;
+  uint16_t n_own[kMaxShared];                                               // records of an item's own rows
+  // sums of the weights: CTAs merge_ctas .. of the grid, chunks of kSumRows rows of a sequence and kv head
+  uint32_t merge_ctas;
+  const float* scores; float* sums; float scale_log2;
+  uint32_t max_seq, n_leads;                                                // sequences, each with its items in their order
+  uint32_t seq[kMaxShared], rows[kMaxShared];                               // of the items
+  uint64_t score0[kMaxShared];
+  uint32_t sum0[kMaxShared + 1];                                            // first chunk of a lead, over all kv heads
+  uint8_t lead[kMaxShared], next[kMaxShared];                               // a lead's first item; the next item of the same sequence (255: none)
+};
+constexpr uint32_t kSumRows = 1024;   // rows of one CTA's sums
+
+// eviction by summed weights (pa_evict_select_kernel, pa_evict_move_kernel)
+constexpr int kMaxEvict = 32;                       // items of one pa_evict call
+constexpr uint32_t kEvictKeys = 49152;              // rows of one CTA of the selection
+struct EvictParams {
+  uint32_t n_items, n_kv, hd, max_seq, n_keep, n_first, n_recent;
+  __half* k; __half* v; float* sums;
+  uint32_t* list;                                   // [n_items][n_kv][n_keep]: the rows that stay
+  uint32_t chunks;                                  // CTAs that share the rows of an item that goes to another sequence
+  uint32_t src[kMaxEvict], dst[kMaxEvict], rows[kMaxEvict];
+};
+
 }  // namespace pa

@@ -1,0 +1,284 @@
+// C entry points of the shared-prefix and the weighing decode, and of the eviction (include/pooled_attn.h): checks, the plan of
+// the units, launches.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+
+#include "pa_host.cuh"
+#include "pa_params.cuh"
+
+namespace pa {
+cudaError_t launch_shared(const SharedParams& p, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v, uint32_t hd, uint32_t n_kv,
+                          int dev, cudaStream_t st);
+cudaError_t launch_shared_finish(const SharedFinishParams& p, uint32_t hd, uint32_t sum_ctas, cudaStream_t st);
+cudaError_t launch_evict(const EvictParams& p, uint32_t sms, int dev, cudaStream_t st);
+}  // namespace pa
+using namespace pa;
+
+static uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+static uint32_t pad64(uint32_t rows) { return (rows + 63) & ~63u; }
+static uint64_t scores_of(const pa_ctx* ctx, uint32_t rows) { return (uint64_t)ctx->cfg.n_heads * pad64(rows); }
+
+// Tiles per unit: all units of a call have the same number T, so that no CTA is the last for long.  For each number of waves
+// the least T whose units fit it; the waves with the least waves * (T + start and end of a unit, in tiles).
+static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_items, uint32_t p_tiles, uint32_t row_tiles, uint32_t most_records) {
+  uint32_t longest = std::max(1u, p_tiles), least = p_tiles ? row_tiles : 0;
+  for (uint32_t i = 0; i < n_items; ++i) { longest = std::max(longest, ceil_div(rows[i], 64)); least += rows[i] > 0; }
+  auto units = [&](uint32_t T) { uint32_t n = row_tiles * ceil_div(p_tiles, T); for (uint32_t i = 0; i < n_items; ++i) n += ceil_div(ceil_div(rows[i], 64), T); return n; };
+  const uint32_t per_wave = std::max(1u, (uint32_t)ctx->sm_count / ctx->cfg.n_kv_heads), start = ctx->cfg.head_dim == 256 ? 5 : ctx->cfg.head_dim == 128 ? 8 : 12;
+  uint32_t best = longest;
+  uint64_t cost = ~0ull;
+  const uint32_t w0 = std::max(1u, ceil_div(least, per_wave));
+  for (uint32_t w = w0; w < w0 + 6; ++w) {
+    uint32_t lo = 1, hi = longest;
+    while (lo < hi) { const uint32_t mid = (lo + hi) / 2; if (units(mid) <= w * per_wave) hi = mid; else lo = mid + 1; }
+    if ((uint64_t)w * (lo + start) < cost) { cost = (uint64_t)w * (lo + start); best = lo; }
+  }
+  // a row's records: those of the shared rows and the longest item's own
+  uint32_t own = 0;
+  for (uint32_t i = 0; i < n_items; ++i) own = std::max(own, ceil_div(rows[i], 64));
+  while (best < longest && ceil_div(p_tiles, best) + ceil_div(own, best) > most_records) ++best;
+  return best;
+}
+
+struct SharedCall {
+  const char* who;
+  pa_layer* L;
+  pa_layer* prefix;             // nullptr: own rows only
+  uint32_t prefix_seq, prefix_len, own_row0;
+  const void* q; int q_f16; uint64_t qcs, qhs;
+  const void* gate; uint64_t gcs, ghs;
+  void* out; uint64_t ocs;
+  bool sums;
+};
+
+// one launch of each kernel for items [first, first + n) with these own rows
+static int shared_launch(const SharedCall& c, const pa_item* items, const uint32_t* rows, uint32_t first, uint32_t n, cudaStream_t st) {
+  pa_layer* L = c.L;
+  pa_ctx* ctx = L->ctx;
+  const uint32_t hd = ctx->cfg.head_dim, nH = ctx->cfg.n_heads, n_kv = ctx->cfg.n_kv_heads, G = ctx->G;
+  SharedParams p{};
+  SharedFinishParams f{};
+  p.n_items = n; p.n_heads = nH; p.G = G; p.max_seq = L->max_seq; p.err = ctx->dev_err;
+  p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)hd));
+  const size_t aes = ctx->cfg.act_dtype == PA_F16 ? 2 : 4;
+  p.q = reinterpret_cast<const uint8_t*>(c.q) + (uint64_t)first * c.qcs * (c.q_f16 ? 2 : 4); p.q_f16 = c.q_f16; p.q_col_stride = c.qcs; p.q_head_stride = c.qhs;
+  p.part_o = ctx->part_o; p.part_ml = ctx->part_ml;
+  p.items_per_tile = 64 / G; p.row_tiles = ceil_div(n, p.items_per_tile);
+  const uint32_t p_tiles = c.prefix ? ceil_div(c.prefix_len, 64) : 0;
+  const uint32_t most = (uint32_t)std::min<size_t>(512, ctx->pf_slots / ((size_t)n * nH));
+  const uint32_t T = plan_units(ctx, rows + first, n, p_tiles, p.row_tiles, most);
+  if (c.prefix) { p.p_row0 = c.prefix_seq * c.prefix->max_seq; p.p_rows = c.prefix_len; p.p_tps = T; p.p_splits = ceil_div(p_tiles, T); }
+  p.tps = T; p.own_row0 = c.own_row0;
+  uint32_t units = p.p_splits * p.row_tiles, own_most = 0;
+  uint64_t floats = 0;
+  for (uint32_t i = 0; i < n; ++i) {
+    const uint32_t r = rows[first + i], u = ceil_div(ceil_div(r, 64), T);
+    p.seq[i] = f.seq[i] = items[first + i].seq; p.rows[i] = f.rows[i] = r; p.cta0[i] = units; f.n_own[i] = (uint16_t)u;
+    p.score0[i] = f.score0[i] = floats;
+    floats += scores_of(ctx, r);
+    units += u; own_most = std::max(own_most, u);
+  }
+  p.cta0[n] = units; p.units = units;
+  p.n_rec = p.p_splits + own_most;
+  if (c.sums) p.scores = ctx->scores;
+  f.part_o = p.part_o; f.part_ml = p.part_ml; f.n_rec = p.n_rec; f.p_splits = p.p_splits; f.n_items = n; f.n_heads = nH; f.G = G; f.n_kv = n_kv;
+  f.gate = c.gate ? reinterpret_cast<const uint8_t*>(c.gate) + (uint64_t)first * c.gcs * aes : nullptr; f.gate_col_stride = c.gcs; f.gate_head_stride = c.ghs;
+  f.out = reinterpret_cast<uint8_t*>(c.out) + (uint64_t)first * c.ocs * aes; f.out_col_stride = c.ocs; f.act_f16 = ctx->cfg.act_dtype == PA_F16;
+  f.merge_ctas = n * nH * (hd / 64);
+  uint32_t sum_ctas = 0;
+  if (c.sums) {
+    f.scores = ctx->scores; f.sums = L->sums; f.scale_log2 = p.scale_log2; f.max_seq = L->max_seq;
+    uint8_t last[kMaxShared];            // of each lead: its last item so far
+    for (uint32_t i = 0; i < n; ++i) {
+      f.next[i] = 255;
+      uint32_t l = 0;
+      while (l < f.n_leads && f.seq[f.lead[l]] != f.seq[i]) ++l;
+      if (l == f.n_leads) { f.lead[l] = (uint8_t)i; f.n_leads++; } else f.next[last[l]] = (uint8_t)i;
+      last[l] = (uint8_t)i;
+    }
+    for (uint32_t l = 0; l < f.n_leads; ++l) {
+      uint32_t longest = 0;
+      for (uint32_t i = f.lead[l]; i != 255; i = f.next[i]) longest = std::max(longest, f.rows[i]);
+      f.sum0[l] = sum_ctas;
+      sum_ctas += n_kv * ceil_div(longest, kSumRows);
+    }
+    f.sum0[f.n_leads] = sum_ctas;
+  }
+  const pa_layer* P = c.prefix ? c.prefix : L;
+  CU_TRY(ctx, launch_shared(p, P->tm_k64, P->tm_v64, L->tm_k64, L->tm_v64, hd, n_kv, ctx->device, st));
+  CU_TRY(ctx, launch_shared_finish(f, hd, sum_ctas, st));
+  ctx->stats.kernel_launches += 2;
+  uint64_t read = c.prefix ? c.prefix_len : 0;
+  for (uint32_t i = 0; i < n; ++i) read += p.rows[i];
+  ctx->stats.kv_bytes_streamed += read * ctx->kv_dim * 4;
+  return PA_OK;
+}
+
+static int shared_impl(const SharedCall& c, const pa_item* items, uint32_t n_items, const uint32_t* rows, cudaStream_t st) {
+  pa_ctx* ctx = c.L->ctx;
+  const uint64_t am = c.q_f16 ? 7 : 3;
+  if ((c.qcs & am) || (c.qhs & am) || ((uintptr_t)c.q & 15)) return fail(ctx, PA_EINVAL, "%s: q strides must be multiples of 16 bytes and q 16-byte aligned", c.who);
+  const uint32_t ae = ctx->cfg.act_dtype == PA_F16 ? 2 : 4;
+  if ((uintptr_t)c.gate % ae || (uintptr_t)c.out % ae) return fail(ctx, PA_EINVAL, "%s: a pointer is not aligned to its type", c.who);
+  if (n_items > 1 && c.ocs < ctx->q_dim) return fail(ctx, PA_EINVAL, "%s: the column stride of out is below %u", c.who, ctx->q_dim);
+  DeviceScope on(ctx->device);
+  // items that fit the records (two a row at least) and the room for scores go in one launch
+  const uint32_t by_records = std::max<uint32_t>(1, (uint32_t)(ctx->pf_slots / (2 * (size_t)ctx->cfg.n_heads)));
+  for (uint32_t i = 0; i < n_items;) {
+    uint32_t n = 0;
+    uint64_t floats = 0;
+    while (i + n < n_items && n < by_records) {
+      floats += c.sums ? scores_of(ctx, rows[i + n]) : 0;
+      if (floats > ctx->scores_floats && c.sums && n) break;
+      ++n;
+    }
+    if (int rc = shared_launch(c, items, rows, i, n, st)) return rc;
+    i += n;
+  }
+  ctx->stats.calls++;
+  ctx->inflight_layer = nullptr;         // these kernels wait for everything before them and write no cache row
+  return PA_OK;
+}
+
+// what both decodes want of the layer and the items
+static int shared_checks(pa_layer* L, const pa_item* items, uint32_t n_items, const void* q, int q_dtype, const void* out, const char* who) {
+  pa_ctx* ctx = L->ctx;
+  if (L->kv_format != PA_KV_F16) return fail(ctx, PA_EUNSUPPORTED, "%s: f16 caches only", who);
+  if (L->origin) return fail(ctx, PA_EUNSUPPORTED, "%s: not on a shard of longer sequences", who);
+  if (ctx->G > 64) return fail(ctx, PA_EUNSUPPORTED, "%s: more than 64 query heads per kv head", who);
+  if ((size_t)ctx->cfg.n_heads * 2 > ctx->pf_slots) return fail(ctx, PA_EUNSUPPORTED, "%s: more than %zu query heads", who, ctx->pf_slots / 2);
+  if (!items || !q || !out) return fail(ctx, PA_EINVAL, "%s: null items, q or out", who);
+  if (q_dtype != PA_F32 && q_dtype != PA_F16) return fail(ctx, PA_EINVAL, "%s: unknown q dtype", who);
+  if (n_items < 1 || n_items > (uint32_t)kMaxShared) return fail(ctx, PA_EINVAL, "%s: 1 to %d items per call", who, kMaxShared);
+  for (uint32_t i = 0; i < n_items; ++i) {
+    if (items[i].n_cols != 1) return fail(ctx, PA_EINVAL, "%s: item %u has %u columns; one token per item", who, i, items[i].n_cols);
+    if (items[i].seq >= L->n_seqs) return fail(ctx, PA_EINVAL, "%s: sequence %u of %u", who, items[i].seq, L->n_seqs);
+    if (items[i].pos >= 0x7fffffffu) return fail(ctx, PA_EINVAL, "%s: position %u is out of range", who, items[i].pos);
+  }
+  return PA_OK;
+}
+
+extern "C" int pa_decode_shared(pa_layer* L, pa_layer* prefix_layer, uint32_t prefix_seq, uint32_t prefix_len, uint32_t own_base, const pa_item* items,
+                                uint32_t n_items, const void* q, int q_dtype, uint64_t qcs, uint64_t qhs, const void* gate, uint64_t gcs, uint64_t ghs, void* out,
+                                uint64_t ocs, void* stream) {
+  if (!L) return PA_EINVAL;
+  pa_ctx* ctx = L->ctx;
+  GUARD(ctx);
+  const char* who = "pa_decode_shared";
+  if (int rc = shared_checks(L, items, n_items, q, q_dtype, out, who)) return rc;
+  pa_layer* P = prefix_layer ? prefix_layer : L;
+  const pa_ctx* pc = P->ctx;
+  if (P->kv_format != PA_KV_F16 || P->origin) return fail(ctx, PA_EUNSUPPORTED, "%s: the prefix must lie in an f16 cache that is no shard", who);
+  if (pc->device != ctx->device || pc->cfg.n_kv_heads != ctx->cfg.n_kv_heads || pc->cfg.head_dim != ctx->cfg.head_dim)
+    return fail(ctx, PA_EINVAL, "%s: the prefix layer is of another device or shape", who);
+  if (prefix_seq >= P->n_seqs || prefix_len > P->max_seq)
+    return fail(ctx, PA_EINVAL, "%s: rows [0, %u) of sequence %u: the prefix layer has %u sequences of %u rows", who, prefix_len, prefix_seq, P->n_seqs, P->max_seq);
+  if (own_base && own_base != prefix_len) return fail(ctx, PA_EINVAL, "%s: own_base %u must be 0 or prefix_len %u", who, own_base, prefix_len);
+  uint32_t rows[kMaxShared];
+  for (uint32_t i = 0; i < n_items; ++i) {
+    if (items[i].pos + 1 < prefix_len) return fail(ctx, PA_EINVAL, "%s: position %u lies inside the prefix of %u", who, items[i].pos, prefix_len);
+    if (items[i].pos + 1 - own_base > L->max_seq) return fail(ctx, PA_EINVAL, "%s: position %u passes the layer's %u rows", who, items[i].pos, L->max_seq);
+    rows[i] = items[i].pos + 1 - prefix_len;
+  }
+  SharedCall c{who, L, prefix_len ? P : nullptr, prefix_seq, prefix_len, prefix_len - own_base, q, q_dtype == PA_F16, qcs, qhs, gate, gcs, ghs, out, ocs, false};
+  return shared_impl(c, items, n_items, rows, (cudaStream_t)stream);
+}
+
+extern "C" int pa_layer_track_weights(pa_layer* L) {
+  if (!L) return PA_EINVAL;
+  pa_ctx* ctx = L->ctx;
+  GUARD(ctx);
+  if (L->kv_format != PA_KV_F16) return fail(ctx, PA_EUNSUPPORTED, "pa_layer_track_weights: f16 caches only");
+  if (L->sums) return PA_OK;
+  DeviceScope on(ctx->device);
+  const size_t sums = (size_t)L->n_seqs * ctx->cfg.n_kv_heads * L->max_seq;
+  // scores: a token of every sequence, up to 2^28 of them; never less than one item wants, nor than an eviction's lists
+  const size_t one = scores_of(ctx, L->max_seq), want = std::max(std::max(one, sums), std::min<size_t>(one * L->n_seqs, (size_t)1 << 28));
+  float *s = nullptr, *w = nullptr;
+  cudaError_t e = cudaMalloc(&s, sums * 4);
+  if (e == cudaSuccess) e = cudaMemset(s, 0, sums * 4);
+  if (e == cudaSuccess && want > ctx->scores_floats) e = cudaMalloc(&w, want * 4);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    cudaFree(s); cudaFree(w);
+    return fail(ctx, e == cudaErrorMemoryAllocation ? PA_ENOMEM : PA_ECUDA, "pa_layer_track_weights: %.0f MiB of sums and %.0f MiB of scores: %s", sums * 4 / 1048576.0,
+                want * 4 / 1048576.0, cudaGetErrorString(e));
+  }
+  L->sums = s;
+  if (w) {
+    if (ctx->scores) ctx->outgrown.push_back(ctx->scores);
+    ctx->scores = w; ctx->scores_floats = want;
+  }
+  return PA_OK;
+}
+extern "C" float* pa_weights_ptr(pa_layer* L) { return L ? L->sums : nullptr; }
+
+extern "C" int pa_weights_clear(pa_layer* L, uint32_t seq, void* stream) {
+  if (!L) return PA_EINVAL;
+  pa_ctx* ctx = L->ctx;
+  GUARD(ctx);
+  if (!L->sums) return fail(ctx, PA_EINVAL, "pa_weights_clear: call pa_layer_track_weights first");
+  if (seq >= L->n_seqs) return fail(ctx, PA_EINVAL, "pa_weights_clear: sequence %u of %u", seq, L->n_seqs);
+  const size_t n = (size_t)ctx->cfg.n_kv_heads * L->max_seq;
+  DeviceScope on(ctx->device);
+  CU_TRY(ctx, cudaMemsetAsync(L->sums + seq * n, 0, n * 4, (cudaStream_t)stream));
+  return PA_OK;
+}
+
+extern "C" int pa_decode_weights(pa_layer* L, const pa_item* items, uint32_t n_items, const void* q, int q_dtype, uint64_t qcs, uint64_t qhs, const void* gate,
+                                 uint64_t gcs, uint64_t ghs, void* out, uint64_t ocs, void* stream) {
+  if (!L) return PA_EINVAL;
+  pa_ctx* ctx = L->ctx;
+  GUARD(ctx);
+  const char* who = "pa_decode_weights";
+  if (int rc = shared_checks(L, items, n_items, q, q_dtype, out, who)) return rc;
+  if (!L->sums) return fail(ctx, PA_EINVAL, "%s: call pa_layer_track_weights first", who);
+  uint32_t rows[kMaxShared];
+  for (uint32_t i = 0; i < n_items; ++i) {
+    if (items[i].pos >= L->max_seq) return fail(ctx, PA_EINVAL, "%s: position %u passes the layer's %u rows", who, items[i].pos, L->max_seq);
+    rows[i] = items[i].pos + 1;
+  }
+  SharedCall c{who, L, nullptr, 0, 0, 0, q, q_dtype == PA_F16, qcs, qhs, gate, gcs, ghs, out, ocs, true};
+  return shared_impl(c, items, n_items, rows, (cudaStream_t)stream);
+}
+
+extern "C" int pa_evict(pa_layer* L, const pa_evict_item* items, uint32_t n_items, uint32_t n_keep, uint32_t n_first, uint32_t n_recent, uint32_t* kept, void* stream) {
+  if (!L) return PA_EINVAL;
+  pa_ctx* ctx = L->ctx;
+  GUARD(ctx);
+  if (L->kv_format != PA_KV_F16) return fail(ctx, PA_EUNSUPPORTED, "pa_evict: f16 caches only");
+  if (L->origin) return fail(ctx, PA_EUNSUPPORTED, "pa_evict: not on a shard of longer sequences");
+  if (!L->sums) return fail(ctx, PA_EINVAL, "pa_evict: call pa_layer_track_weights first");
+  if (!items || n_items < 1 || n_items > (uint32_t)kMaxEvict) return fail(ctx, PA_EINVAL, "pa_evict: 1 to %d items per call", kMaxEvict);
+  if (n_keep < 1 || n_keep > L->max_seq || (uint64_t)n_first + n_recent > n_keep)
+    return fail(ctx, PA_EINVAL, "pa_evict: n_keep %u must be 1 .. %u and hold the first %u and the last %u rows", n_keep, L->max_seq, n_first, n_recent);
+  if ((uintptr_t)kept & 3) return fail(ctx, PA_EINVAL, "pa_evict: kept is not aligned to its type");
+  EvictParams p{};
+  p.n_items = n_items; p.n_kv = ctx->cfg.n_kv_heads; p.hd = ctx->cfg.head_dim; p.max_seq = L->max_seq; p.n_keep = n_keep; p.n_first = n_first; p.n_recent = n_recent;
+  p.k = L->k; p.v = L->v; p.sums = L->sums;
+  uint64_t moved = 0;
+  for (uint32_t i = 0; i < n_items; ++i) {
+    const pa_evict_item& it = items[i];
+    if (it.src_seq >= L->n_seqs || it.dst_seq >= L->n_seqs) return fail(ctx, PA_EINVAL, "pa_evict: sequence %u of %u", std::max(it.src_seq, it.dst_seq), L->n_seqs);
+    if (it.n_rows > L->max_seq) return fail(ctx, PA_EINVAL, "pa_evict: %u rows pass the layer's %u", it.n_rows, L->max_seq);
+    if (it.n_rows > kEvictKeys * 8) return fail(ctx, PA_EUNSUPPORTED, "pa_evict: %u rows, at most %u", it.n_rows, kEvictKeys * 8);
+    for (uint32_t j = 0; j < i; ++j)
+      if (items[j].dst_seq == it.dst_seq || items[j].src_seq == it.dst_seq || items[j].dst_seq == it.src_seq)
+        return fail(ctx, PA_EINVAL, "pa_evict: the destination of item %u or %u is named by the other", j, i);
+    p.src[i] = it.src_seq; p.dst[i] = it.dst_seq; p.rows[i] = it.n_rows;
+    moved += std::min(it.n_rows, n_keep);
+  }
+  const uint64_t words = (uint64_t)n_items * p.n_kv * n_keep;
+  if (!kept && words > ctx->scores_floats) return fail(ctx, PA_EUNSUPPORTED, "pa_evict: the lists of %u items do not fit the context's room; pass `kept` or fewer items", n_items);
+  p.list = kept ? kept : reinterpret_cast<uint32_t*>(ctx->scores);
+  DeviceScope on(ctx->device);
+  CU_TRY(ctx, launch_evict(p, (uint32_t)ctx->sm_count, ctx->device, (cudaStream_t)stream));
+  ctx->stats.kernel_launches += 2; ctx->stats.calls++;
+  // rows of any number may still be on the move: what follows on this layer fetches nothing ahead of its wait
+  ctx->inflight_layer = L; ctx->inflight_row0 = 0;
+  return PA_OK;
+}

@@ -15,6 +15,8 @@ PA_F32, PA_F16 = 0, 1
 PA_ROPE_NONE, PA_ROPE_F64, PA_ROPE_TABLE = 0, 1, 2
 PA_KV_F16, PA_KV_Q8, PA_KV_F32 = 0, 1, 2
 PA_FLAG_FAST = 1
+PA_ROPE_HALF, PA_ROPE_INTERLEAVED = 0, 1
+PA_ROPE_SCALE_NONE, PA_ROPE_SCALE_LINEAR, PA_ROPE_SCALE_NTK, PA_ROPE_SCALE_YARN, PA_ROPE_SCALE_BANDS = 0, 1, 2, 3, 4
 PA_MODE_AUTO, PA_MODE_DECODE, PA_MODE_PREFILL = 0, 1, 2
 STATUS = {0: "PA_OK", -1: "PA_EINVAL", -2: "PA_EUNSUPPORTED", -3: "PA_ENOMEM", -4: "PA_ECUDA", -5: "PA_ETIMEOUT", -6: "PA_ESTATE"}
 
@@ -33,6 +35,15 @@ class PaConfig(C.Structure):
 
 class PaItem(C.Structure):
     _fields_ = [("seq", C.c_uint32), ("pos", C.c_uint32), ("n_cols", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class PaRotaryConfig(C.Structure):
+    _fields_ = [("n_rot", C.c_uint32), ("layout", C.c_uint32), ("scaling", C.c_uint32), ("original", C.c_uint32), ("theta", C.c_double),
+                ("factor", C.c_double), ("fast", C.c_double), ("slow", C.c_double), ("mscale", C.c_double), ("reserved", C.c_uint32 * 4)]
+
+
+class PaEvictItem(C.Structure):
+    _fields_ = [("src_seq", C.c_uint32), ("dst_seq", C.c_uint32), ("n_rows", C.c_uint32), ("reserved", C.c_uint32)]
 
 
 class PaStats(C.Structure):
@@ -97,6 +108,17 @@ SYMBOLS = {
     "pa_attn_step_host": (_i, [C.POINTER(_vp), _u32, _u32, _u32, _u32, _i, _vp, _u64, _u64, _u64, _vp, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _vp]),
     "pa_decode_static": (_i, [_i, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, C.c_char_p, _sz]),
     "pa_decode_static_status": (_i, [_i, _vp, C.POINTER(_u32)]),
+    "pa_rotary_create": (_i, [_vp, C.POINTER(PaRotaryConfig), C.POINTER(_vp)]),
+    "pa_rotary_destroy": (_i, [_vp]),
+    "pa_rotary_freqs": (_i, [_vp, C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+    "pa_rotary_apply": (_i, [_vp, _vp, _i, _u64, _u64, _u32, _vp, C.c_int32, _u32, _vp, _i, _u64, _u64, _vp]),
+    "pa_rotary_append": (_i, [_vp, _vp, _vp, _u32, _vp, _vp, _u64, _u64, _vp, _vp, _u64, _vp, _i, _u64, _vp]),
+    "pa_decode_shared": (_i, [_vp, _vp, _u32, _u32, _u32, _vp, _u32, _vp, _i, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _vp]),
+    "pa_layer_track_weights": (_i, [_vp]),
+    "pa_weights_ptr": (_vp, [_vp]),
+    "pa_weights_clear": (_i, [_vp, _u32, _vp]),
+    "pa_decode_weights": (_i, [_vp, _vp, _u32, _vp, _i, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _vp]),
+    "pa_evict": (_i, [_vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp]),
     "pa_set_wait_limit": (_i, [_vp, _u32]),
     "pa_get_stats": (_i, [_vp, C.POINTER(PaStats)]),
     "pa_timing_begin": (_i, [_vp, _u32]),
@@ -137,6 +159,33 @@ class CtypesCalls:
                                          *_gate(gate, gate_head_stride), _ptr(out), out.stride(0), stream)
 
 
+    def _items(self, items, n_cols=True):
+        return (PaItem * max(1, len(items)))(*[PaItem(*it, 0) if n_cols else PaItem(*it, 1, 0) for it in items])
+
+    def rotary_apply(self, entry, rotary, x, x_dtype, head_stride, n_heads, positions, pos, y, y_dtype, y_head_stride, stream):
+        return self.lib.pa_rotary_apply(rotary, _ptr(x), x_dtype, x.stride(0), head_stride, n_heads, _ptr(positions), pos, x.shape[0], _ptr(y), y_dtype, y.stride(0),
+                                        y_head_stride, stream)
+
+    def rotary_append(self, entry, rotary, layer, items, rows, q, q_head_stride, k, v, q_out, q_out_dtype, stream):
+        if rows is not None and len(rows) != len(items):
+            raise ValueError("one row per item")
+        r = None if rows is None else (C.c_uint32 * max(1, len(rows)))(*rows)
+        return self.lib.pa_rotary_append(rotary, layer, self._items(items), len(items), r, *_gate(q, q_head_stride), _ptr(k), _ptr(v), k.stride(0), _ptr(q_out),
+                                         q_out_dtype, 0 if q_out is None else q_out.stride(0), stream)
+
+    def decode_shared(self, entry, layer, prefix_layer, prefix_seq, prefix_len, own_base, seqs_pos, q, q_dtype, q_head_stride, gate, gate_head_stride, out, stream):
+        return self.lib.pa_decode_shared(layer, prefix_layer, prefix_seq, prefix_len, own_base, self._items(seqs_pos, False), len(seqs_pos), _ptr(q), q_dtype, q.stride(0),
+                                         q_head_stride, *_gate(gate, gate_head_stride), _ptr(out), out.stride(0), stream)
+
+    def decode_weights(self, entry, layer, seqs_pos, q, q_dtype, q_head_stride, gate, gate_head_stride, out, stream):
+        return self.lib.pa_decode_weights(layer, self._items(seqs_pos, False), len(seqs_pos), _ptr(q), q_dtype, q.stride(0), q_head_stride,
+                                          *_gate(gate, gate_head_stride), _ptr(out), out.stride(0), stream)
+
+    def evict(self, entry, layer, items, n_keep, n_first, n_recent, kept, stream):
+        arr = (PaEvictItem * max(1, len(items)))(*[PaEvictItem(*it, 0) for it in items])
+        return self.lib.pa_evict(layer, arr, len(items), n_keep, n_first, n_recent, _ptr(kept), stream)
+
+
 class Lib:
     """The loaded shared library with typed entry points."""
 
@@ -155,7 +204,9 @@ class Lib:
     def _load_call(self):
         """The CPython module with the per-layer calls (csrc/pa_call.c), which takes their addresses in this library from
         `entry`; the same calls through ctypes where it was not built for this interpreter."""
-        self.entry = {n: C.cast(getattr(self.dll, n), C.c_void_p).value for n in ("pa_attn_layer", "pa_attn_items", "pa_rope_append", "pa_decode_gather")}
+        self.entry = {n: C.cast(getattr(self.dll, n), C.c_void_p).value for n in
+                      ("pa_attn_layer", "pa_attn_items", "pa_rope_append", "pa_decode_gather", "pa_rotary_apply", "pa_rotary_append", "pa_decode_shared",
+                       "pa_decode_weights", "pa_evict")}
         if not os.path.exists(CALL_PATH):
             return CtypesCalls(self)
         loader = importlib.machinery.ExtensionFileLoader("_pa_call", CALL_PATH)

@@ -1,0 +1,119 @@
+"""The calls of the rotary, shared-prefix, weighing and evicting operators without a GPU: the CPython module and ctypes make the same
+ones, null handles are refused, and the host refuses tensors that do not fit before anything is called."""
+import ctypes as C
+
+import pytest
+import torch
+
+from pooled_b200 import AttnConfig, AttnEngine, PaError, Rotary
+from pooled_b200 import lib as L
+
+
+@pytest.fixture(scope="module")
+def pa():
+    from pooled_b200 import build
+    build.build()
+    return L.load()
+
+
+def test_struct_layouts_match_the_header():
+    assert C.sizeof(L.PaRotaryConfig) == 72 and L.PaRotaryConfig.theta.offset == 16 and L.PaRotaryConfig.mscale.offset == 48
+    assert C.sizeof(L.PaEvictItem) == 16
+
+
+def test_call_module_calls_as_ctypes_does(pa):
+    seen = []
+
+    def items(a, i, n, struct):
+        it = C.cast(a[i], C.POINTER(struct))
+        return tuple(tuple(getattr(it[j], f) for f, _ in struct._fields_) for j in range(a[n]))
+
+    def fake(name):
+        res, args = L.SYMBOLS[name]
+
+        def record(*a):
+            a = list(a)
+            if name == "pa_rotary_append":
+                rows = C.cast(a[4], C.POINTER(C.c_uint32))
+                a[4] = a[4] and [rows[j] for j in range(a[3])]
+                a[2] = items(a, 2, 3, L.PaItem)
+            elif name == "pa_decode_shared":
+                a[5] = items(a, 5, 6, L.PaItem)
+            elif name == "pa_decode_weights":
+                a[1] = items(a, 1, 2, L.PaItem)
+            elif name == "pa_evict":
+                a[1] = items(a, 1, 2, L.PaEvictItem)
+            seen.append((name, *a))
+            return len(seen)
+        return C.CFUNCTYPE(res, *args)(record)
+
+    class FakeLib:
+        pass
+    lib = FakeLib()
+    names = ["pa_rotary_apply", "pa_rotary_append", "pa_decode_shared", "pa_decode_weights", "pa_evict"]
+    for name in names:
+        setattr(lib, name, fake(name))
+    by_ctypes = L.CtypesCalls(lib)
+    entry = {name: C.cast(getattr(lib, name), C.c_void_p).value for name in names}
+    q, k, v, g, o = (torch.zeros((3, n + 2 * i))[:, :n] for i, n in enumerate((64, 16, 16, 64, 64)))
+    p, kept = torch.zeros(3, dtype=torch.int32), torch.zeros((2, 2, 5), dtype=torch.int32)
+    pairs, triples = [(0, 5), (2, 2 ** 32 - 1), (1, 0)], [(3, 7, 1), (0, 2 ** 31, 2)]
+    calls = [("rotary_apply", (4096, q, 0, 16, 4, ps, pos, o, 1, 32, 7)) for ps in (None, p) for pos in (0, -5, 2 ** 31 - 1)]
+    calls += [("rotary_append", (4096, 8192, triples, rows, qq, 16, k, v, qo, 1, 7)) for rows in (None, [9, 2 ** 32 - 1]) for qq, qo in ((q, o), (None, None))]
+    calls += [("decode_shared", (4096, 8192, 2, 100, 50, pairs, q, 1, 16, gate, 32, o, 7)) for gate in (None, g)]
+    calls += [("decode_weights", (4096, pairs, q, 1, 16, gate, 32, o, 7)) for gate in (None, g)]
+    calls += [("evict", (4096, triples, 5, 1, 2, kp, 7)) for kp in (None, kept)]
+    for method, args in calls:
+        seen.clear()
+        name = "pa_" + method
+        assert getattr(pa.call, method)(entry[name], *args) == 1 and getattr(by_ctypes, method)(entry[name], *args) == 2
+        assert seen[0] == seen[1] and seen[0][0] == name, method
+    for bad in ([(1,)], [3], [(1, 2, 3, 4)], [(1, "a", 2)]):
+        for method, args in (("rotary_append", (4096, 8192, bad, None, q, 16, k, v, o, 1, 7)), ("decode_shared", (4096, 8192, 2, 100, 50, bad, q, 1, 16, None, 32, o, 7)),
+                             ("decode_weights", (4096, bad, q, 1, 16, None, 32, o, 7)), ("evict", (4096, bad, 5, 1, 2, None, 7))):
+            with pytest.raises((TypeError, ValueError)):
+                getattr(pa.call, method)(entry["pa_" + method], *args)
+    with pytest.raises(ValueError):
+        pa.call.rotary_append(entry["pa_rotary_append"], 4096, 8192, triples, [1], q, 16, k, v, o, 1, 7)
+
+
+def test_null_handles_are_refused(pa):
+    h = C.c_void_p()
+    assert pa.pa_rotary_create(None, None, C.byref(h)) == -1 and pa.pa_rotary_freqs(None, None, None) == -1
+    assert pa.pa_rotary_destroy(None) == 0
+    assert pa.pa_rotary_apply(None, None, 0, 0, 0, 0, None, 0, 0, None, 0, 0, 0, None) == -1
+    assert pa.pa_rotary_append(None, None, None, 0, None, None, 0, 0, None, None, 0, None, 0, 0, None) == -1
+    assert pa.pa_decode_shared(None, None, 0, 0, 0, None, 0, None, 0, 0, 0, None, 0, 0, None, 0, None) == -1
+    assert pa.pa_decode_weights(None, None, 0, None, 0, 0, 0, None, 0, 0, None, 0, None) == -1
+    assert pa.pa_layer_track_weights(None) == -1 and pa.pa_weights_ptr(None) is None and pa.pa_weights_clear(None, 0, None) == -1
+    assert pa.pa_evict(None, None, 0, 0, 0, 0, None, None) == -1
+
+
+def test_the_host_refuses_what_does_not_fit():
+    class Calls:
+        def __getattr__(self, name):
+            return lambda *a: pytest.fail(f"{name} was called")
+
+    eng = object.__new__(AttnEngine)                                  # an engine without a device: nothing may reach the library
+    eng.cfg = AttnConfig(n_heads=4, n_kv_heads=2, head_dim=64, n_rot=64, rope_theta=1e4, max_seq=32, act_dtype=torch.float32)
+    eng.device, eng.layers, eng._call, eng.ctx, eng.slots, eng._xc_keep = 0, [C.c_void_p(8)], Calls(), None, {}, None
+    eng._f_rot_append = eng._f_shared = eng._f_weights = 0
+    rot = object.__new__(Rotary)
+    rot.eng, rot.handle, rot._apply, rot._f_apply = eng, C.c_void_p(8), Calls(), 0
+    q, kv = torch.zeros((2, 256)), torch.zeros((2, 128))             # of another device than the engine's
+    for call in (lambda: rot.apply(q, 4), lambda: eng.rotary_append(0, rot, [(0, 0, 2)], q, kv, kv, q_out=q), lambda: eng.decode_shared(0, None, 0, 0, [(0, 1), (0, 2)], q, out=q),
+                 lambda: eng.decode_weights(0, [(0, 1), (0, 2)], q, out=q)):
+        with pytest.raises(PaError):
+            call()
+    eng.device = None                                                 # ... of the same: the shapes
+    meta = lambda *s, dt=torch.float32: torch.zeros(s, dtype=dt)
+    for call in (lambda: rot.apply(q, 5, out=meta(2, 320)), lambda: rot.apply(q, 4, out=meta(1, 256)), lambda: rot.apply(q, 4, positions=meta(2), out=q),
+                 lambda: rot.apply(q, 4, positions=meta(3, dt=torch.int32), out=q), lambda: rot.apply(q.t(), 4, out=q),
+                 lambda: eng.rotary_append(0, rot, [(0, 0, 1)], q, kv, kv, q_out=q), lambda: eng.rotary_append(0, rot, [(0, 0, 2)], q.half(), kv, kv, q_out=q),
+                 lambda: eng.rotary_append(0, rot, [(0, 0, 2)], q, kv, meta(2, 136)[:, :128], q_out=q), lambda: eng.rotary_append(0, rot, [(0, 0, 2)], q, kv[:, :64], kv, q_out=q),
+                 lambda: eng.decode_shared(0, None, 0, 0, [(0, 1)], q, out=q), lambda: eng.decode_shared(0, None, 0, 0, [(0, 1), (0, 2)], q, out=q[:, :128]),
+                 lambda: eng.decode_weights(0, [(0, 1), (0, 2)], q, gate=q.half(), out=q), lambda: eng.decode_weights(0, [(0, 1), (0, 2)], q, out=q.half()),
+                 lambda: eng.decode_weights(0, [(0, 1), (0, 2)], q, q_head_stride=128, out=q)):
+        with pytest.raises(PaError):
+            call()
+    eng.layers = []
