@@ -121,14 +121,14 @@ class Rotary:
         self.eng, self.n_rot, self.handle = eng, cfg.n_rot, None
         h = C.c_void_p()
         eng._ck(eng.L.pa_rotary_create(eng.ctx, C.byref(cfg), C.byref(h)))
-        self.handle = h
+        self.handle, self._h = h, h.value
         eng._rotaries.add(self)
         self._apply, self._f_apply = eng._call.rotary_apply, eng.L.entry["pa_rotary_apply"]
 
     def destroy(self):
         if self.handle and self.eng.ctx:
             self.eng.L.pa_rotary_destroy(self.handle)
-        self.handle = None
+        self.handle, self._h = None, 0
 
     def __del__(self):
         try:
@@ -151,14 +151,20 @@ class Rotary:
         eng._on_device(x, out, positions)
         if positions is not None and (positions.dtype != torch.int32 or positions.dim() != 1 or positions.shape[0] != x.shape[0] or positions.stride(0) != 1):
             raise _l.PaError(-1, "positions are a contiguous int32 tensor of one value per column")
+        cols, have = x.shape
+        hs, ohs, last, dt = head_stride or hd, out_head_stride or hd, n_heads - 1, _dt(x.dtype)
         if out is None:
-            out = torch.empty((x.shape[0], n_heads * hd), dtype=x.dtype, device=x.device)
-        elif out.shape[0] != x.shape[0]:
-            raise _l.PaError(-1, f"out has {out.shape[0]} columns for {x.shape[0]}")
-        hs, ohs = head_stride or hd, out_head_stride or (head_stride if out is x and head_stride else hd)
-        if (n_heads - 1) * hs + hd > x.shape[1] or (n_heads - 1) * ohs + hd > out.shape[1]:
+            out, out_have, out_dt, ohs = x.new_empty((cols, n_heads * hd)), n_heads * hd, dt, hd
+        else:
+            out_cols, out_have = out.shape
+            out_dt = _dt(out.dtype)
+            if out is x and not out_head_stride:
+                ohs = hs
+            if out_cols != cols:
+                raise _l.PaError(-1, f"out has {out_cols} columns for {cols}")
+        if last * hs + hd > have or last * ohs + hd > out_have:
             raise _l.PaError(-1, f"{n_heads} heads do not fit the columns of x or out")
-        rc = self._apply(self._f_apply, self.handle.value, x, _dt(x.dtype), hs, n_heads, positions, pos, out, _dt(out.dtype), ohs, eng._raw_st())
+        rc = self._apply(self._f_apply, self._h, x, dt, hs, n_heads, positions, pos, out, out_dt, ohs, eng._raw_st())
         if rc:
             eng._ck(rc)
         return out
@@ -181,6 +187,8 @@ class AttnEngine:
         self.layers: list[C.c_void_p] = []
         self.slots: dict[str, dict] = {}
         self._xc_keep = None
+        self._q_dim, self._kv_dim = cfg.q_dim, cfg.kv_dim
+        self._views: dict = {}                  # cache() and the like: the device arrays as tensors, made once
         self._rotaries = weakref.WeakSet()      # destroyed ahead of the context
         self.L.check(self.L.pa_create(device, C.byref(pc), C.byref(h)))
         self.ctx = h
@@ -218,6 +226,7 @@ class AttnEngine:
         if self.ctx:
             self.drop_all_slots()
             self._exchange_release()
+        self._views = {}
         for lh in self.layers:
             self.L.pa_layer_destroy(lh)
         self.layers = []
@@ -267,16 +276,19 @@ class AttnEngine:
     def cache(self, li: int, which: str) -> torch.Tensor:
         """The K ("k") or V ("v") cache of layer li as a tensor [n_seqs, max_seq, kv_dim] (no copy): int16 words of the
         f16 values, int8 values of a "q8" layer, float32 of an "f32" one."""
-        ptr = self.L.pa_cache_ptr(self.layers[li], 0 if which == "k" else 1)
         ts = {"f16": "<i2", "q8": "|i1", "f32": "<f4"}[self.cfg.kv_format]
-        arr = _DevArray(ptr, (self.cfg.n_seqs, self.cfg.max_seq, self.cfg.kv_dim), ts)
-        return torch.as_tensor(arr, device=f"cuda:{self.device}")
+        return self._view((li, which), lambda: self.L.pa_cache_ptr(self.layers[li], 0 if which == "k" else 1), (self.cfg.n_seqs, self.cfg.max_seq, self.cfg.kv_dim), ts)
 
     def cache_scales(self, li: int, which: str) -> torch.Tensor:
         """The scales of a "q8" layer's K or V cache: float32 [n_seqs, max_seq, kv_dim / 32]."""
-        ptr = self.L.pa_cache_ptr(self.layers[li], 2 if which == "k" else 3)
-        arr = _DevArray(ptr, (self.cfg.n_seqs, self.cfg.max_seq, self.cfg.kv_dim // 32), "<f4")
-        return torch.as_tensor(arr, device=f"cuda:{self.device}")
+        return self._view((li, which + "s"), lambda: self.L.pa_cache_ptr(self.layers[li], 2 if which == "k" else 3),
+                          (self.cfg.n_seqs, self.cfg.max_seq, self.cfg.kv_dim // 32), "<f4")
+
+    def _view(self, key, ptr, shape, typestr) -> torch.Tensor:
+        t = self._views.get(key)
+        if t is None:
+            t = self._views[key] = torch.as_tensor(_DevArray(ptr(), shape, typestr), device=f"cuda:{self.device}")
+        return t.detach()                       # a tensor of the caller's own over the same memory
 
     # ---- the path, step by step ----
     def rope(self, x: torch.Tensor, n_heads: int, pos: int, head_stride: int | None = None, cs_table: torch.Tensor | None = None) -> torch.Tensor:
@@ -427,13 +439,13 @@ class AttnEngine:
                       q_dtype: torch.dtype = torch.float32, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
         """rope_append with `rot`, for one or many sequences: items = [(seq, pos, n_cols)] own consecutive rows of q, k and v.  Item i's k and v go to
         cache rows rows[i] .. (None: the rows of their positions).  Returns the rotated q, [n_cols, q_dim] of q_dtype (None without q)."""
-        total = sum(it[2] for it in items)
+        total = sum([it[2] for it in items])
         self._columns(total, q, k, v, q_out)
         if q is not None and q_out is None:
-            q_out = torch.empty((total, self.cfg.q_dim), dtype=q_dtype, device=k.device)
-        if k.stride(0) != v.stride(0):
+            q_out = q.new_empty((total, self._q_dim), dtype=q_dtype)
+        if k.stride(0) != v.stride(0) and total > 1:
             raise _l.PaError(-1, "k and v have different column strides")
-        rc = self._call.rotary_append(self._f_rot_append, rot.handle.value, self.layers[li].value, items, rows, q, q_head_stride or self.cfg.head_dim, k, v, q_out,
+        rc = self._call.rotary_append(self._f_rot_append, rot._h, self.layers[li].value, items, rows, q, q_head_stride or self.cfg.head_dim, k, v, q_out,
                                       _l.PA_F32 if q is None else _dt(q_out.dtype), self._raw_st())
         if rc:
             self._ck(rc)
@@ -441,32 +453,41 @@ class AttnEngine:
 
     def _on_device(self, *tensors):
         for t in tensors:
-            if t is not None and (t.device.index != self.device or t.stride(-1) != 1):
+            if t is not None and (t.get_device() != self.device or not (t.is_contiguous() or t.stride(-1) == 1)):
                 raise _l.PaError(-1, f"a tensor on {t.device} with strides {t.stride()}: the engine takes rows of consecutive values on cuda:{self.device}")
 
     def _columns(self, n: int, q, k, v, out):
         """Columns of the engine's own types: q, k, v of act_dtype, n of each."""
         c = self.cfg
         self._on_device(q, k, v, out)
-        for t, width in ((q, c.head_dim), (k, c.kv_dim), (v, c.kv_dim)):
-            if t is not None and (t.dtype != c.act_dtype or t.dim() != 2 or t.shape[0] != n or t.shape[1] < width):
-                raise _l.PaError(-1, f"{t.dtype} {tuple(t.shape)}: {n} columns of {c.act_dtype} are wanted")
-        if out is not None and (out.dim() != 2 or out.shape[0] != n or out.shape[1] < c.q_dim):
-            raise _l.PaError(-1, f"an output of shape {tuple(out.shape)} for {n} columns of {c.q_dim}")
+        for t, width in ((q, c.head_dim), (k, self._kv_dim), (v, self._kv_dim)):
+            if t is not None:
+                cols, have = t.shape
+                if t.dtype != c.act_dtype or cols != n or have < width:
+                    raise _l.PaError(-1, f"{t.dtype} {tuple(t.shape)}: {n} columns of {c.act_dtype} are wanted")
+        if out is not None:
+            cols, have = out.shape
+            if cols != n or have < self._q_dim:
+                raise _l.PaError(-1, f"an output of shape {tuple(out.shape)} for {n} columns of {self._q_dim}")
 
     def _batch(self, n: int, q, q_head_stride, gate, gate_head_stride, out):
         """The tensors of a decode of n single tokens; returns out, made where it is None."""
         c = self.cfg
-        hd, last = c.head_dim, c.n_heads - 1
-        if out is None:
-            out = torch.empty((n, c.q_dim), dtype=c.act_dtype, device=q.device)
-        self._on_device(q, gate, out)
-        if q.dim() != 2 or q.shape[0] != n or last * (q_head_stride or hd) + hd > q.shape[1]:
+        hd, last, act = c.head_dim, c.n_heads - 1, c.act_dtype
+        self._on_device(q, gate)
+        cols, have = q.shape
+        if cols != n or last * (q_head_stride or hd) + hd > have:
             raise _l.PaError(-1, f"q of shape {tuple(q.shape)} for {n} items of {c.n_heads} heads")
-        if gate is not None and (gate.dtype != c.act_dtype or gate.dim() != 2 or gate.shape[0] != n or last * (gate_head_stride or hd) + hd > gate.shape[1]):
-            raise _l.PaError(-1, f"{gate.dtype} gate of shape {tuple(gate.shape)} for {n} items of {c.n_heads} heads")
-        if out.dtype != c.act_dtype or out.dim() != 2 or out.shape[0] != n or out.shape[1] < c.q_dim:
-            raise _l.PaError(-1, f"{out.dtype} output of shape {tuple(out.shape)} for {n} columns of {c.q_dim}")
+        if gate is not None:
+            cols, have = gate.shape
+            if gate.dtype != act or cols != n or last * (gate_head_stride or hd) + hd > have:
+                raise _l.PaError(-1, f"{gate.dtype} gate of shape {tuple(gate.shape)} for {n} items of {c.n_heads} heads")
+        if out is None:
+            return q.new_empty((n, self._q_dim), dtype=act)
+        self._on_device(out)
+        cols, have = out.shape
+        if out.dtype != act or cols != n or have < self._q_dim:
+            raise _l.PaError(-1, f"{out.dtype} output of shape {tuple(out.shape)} for {n} columns of {self._q_dim}")
         return out
 
     # ---- batches that share a prefix ----
@@ -490,10 +511,12 @@ class AttnEngine:
 
     def weights(self, li: int) -> torch.Tensor:
         """The sums of a tracked layer: float32 [n_seqs, n_kv_heads, max_seq] (no copy)."""
-        ptr = self.L.pa_weights_ptr(self.layers[li])
-        if not ptr:
-            raise _l.PaError(-1, "the layer's weights are not tracked: call track_weights first")
-        return torch.as_tensor(_DevArray(ptr, (self.cfg.n_seqs, self.cfg.n_kv_heads, self.cfg.max_seq), "<f4"), device=f"cuda:{self.device}")
+        def ptr():
+            p = self.L.pa_weights_ptr(self.layers[li])
+            if not p:
+                raise _l.PaError(-1, "the layer's weights are not tracked: call track_weights first")
+            return p
+        return self._view((li, "w"), ptr, (self.cfg.n_seqs, self.cfg.n_kv_heads, self.cfg.max_seq), "<f4")
 
     def clear_weights(self, li: int, seq: int):
         self._ck(self.L.pa_weights_clear(self.layers[li], seq, self._st()))

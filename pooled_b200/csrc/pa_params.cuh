@@ -241,7 +241,7 @@ struct SharedParams {
 
 struct SharedFinishParams {
   const float* part_o; const float* part_ml; uint32_t n_rec, p_splits;
-  uint32_t n_items, n_heads, G, n_kv;
+  uint32_t n_items, n_heads, G, n_kv, lanes;                                // lanes: float4 lanes of a merging CTA, 16 (a slice of 64 dims) or head_dim / 4
   const void* gate; uint64_t gate_col_stride, gate_head_stride;
   void* out; uint64_t out_col_stride; int act_f16;
   uint16_t n_own[kMaxShared];                                               // records of an item's own rows
@@ -254,7 +254,7 @@ struct SharedFinishParams {
   uint32_t sum0[kMaxShared + 1];                                            // first chunk of a lead, over all kv heads
   uint8_t lead[kMaxShared], next[kMaxShared];                               // a lead's first item; the next item of the same sequence (255: none)
 };
-constexpr uint32_t kSumRows = 1024;   // rows of one CTA's sums
+constexpr uint32_t kSumRows = 256;    // rows of one CTA's sums
 
 // eviction by summed weights (pa_evict_select_kernel, pa_evict_move_kernel)
 constexpr int kMaxEvict = 32;                       // items of one pa_evict call

@@ -16,8 +16,8 @@
 //   warp 1      issues the scores: S = Q K^T into one of three tiles of tensor memory (128 x 64 f32)
 //   warp 2      tensor memory; issues O += P V into the accumulator (128 x head_dim f32)
 //   warps 4-11  two softmax groups on alternate tiles.  Even rows of the 128 carry the f16 high parts of q and of the
-//               weights, odd rows the low parts of the same query row: some 22 bits of both, S_hi + S_lo and O_hi + O_lo one
-//               shuffle each.  A row's reference lies 2^7 below its maximum, moves only when a tile passes it by 2^15, and travels
+//               weights, odd rows the low parts of the same query row: some 22 bits of both, added by shuffles.  The two lanes
+//               share the row's keys out (each with all 64, a tile took 2 us of a group instead of 1.2).  A row's reference lies 2^7 below its maximum, moves only when a tile passes it by 2^15, and travels
 //               with the tiles: weights of up to 2^15 keep the low parts of small ones above f16's last place (with a
 //               reference at the maximum, a long row's error was 2.2e-6 of the result, 3e-7 now).
 //               Warps whose rows hold no query take no part.
@@ -85,6 +85,7 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
   }
   const CUtensorMap* mk = shared ? &tm_pk : &tm_k;
   const CUtensorMap* mv = shared ? &tm_pv : &tm_v;
+  const bool once = !shared || p.row_tiles == 1;                       // nobody else reads the unit's rows: they need not stay in L2
   const uint32_t tiles = (n_rows + 63) / 64, tile0 = split * tps, n_tiles = min(tiles, tile0 + tps) - tile0;
   const uint32_t pairs = n_q * p.G;                                     // query rows, two lanes each
   const uint32_t live_warps = (2 * pairs + 31) / 32;                    // of each softmax group
@@ -123,7 +124,9 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
         if (j == 2) mbar_wait(BAR(Q_READ, 0), 0, s_err, WAIT_QFULL);         // the third slot stages query rows until then
         mbar_wait(BAR(K_EMPTY, st), (u & 1) ^ 1, s_err, WAIT_EMPTY);
         mbar_expect_tx(BAR(K_FULL, st), L::KV_BYTES);
-        tma_load_3d(smem_u32(base + L::OFF_K + st * L::KV_BYTES), mk, 0, (int)(row0 + (tile0 + j) * 64), (int)(g * CH), BAR(K_FULL, st));
+        const uint32_t dst = smem_u32(base + L::OFF_K + st * L::KV_BYTES);
+        if (once) tma_load_3d_hint(dst, mk, 0, (int)(row0 + (tile0 + j) * 64), (int)(g * CH), BAR(K_FULL, st), l2_policy_evict_first());
+        else tma_load_3d(dst, mk, 0, (int)(row0 + (tile0 + j) * 64), (int)(g * CH), BAR(K_FULL, st));
       }
     }
   } else if (warp == 3) {
@@ -134,7 +137,9 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
         if (j == 1) mbar_wait(BAR(Q_READ, 0), 0, s_err, WAIT_QFULL);         // ... and the second V slot
         mbar_wait(BAR(V_EMPTY, st), (u & 1) ^ 1, s_err, WAIT_EMPTY);
         mbar_expect_tx(BAR(V_FULL, st), L::KV_BYTES);
-        tma_load_3d(smem_u32(base + L::OFF_V + st * L::KV_BYTES), mv, 0, (int)(row0 + (tile0 + j) * 64), (int)(g * CH), BAR(V_FULL, st));
+        const uint32_t dst = smem_u32(base + L::OFF_V + st * L::KV_BYTES);
+        if (once) tma_load_3d_hint(dst, mv, 0, (int)(row0 + (tile0 + j) * 64), (int)(g * CH), BAR(V_FULL, st), l2_policy_evict_first());
+        else tma_load_3d(dst, mv, 0, (int)(row0 + (tile0 + j) * 64), (int)(g * CH), BAR(V_FULL, st));
       }
     }
     __syncwarp();
@@ -269,30 +274,34 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
         const uint32_t b = j % SB, u = j / SB, kv0 = (tile0 + j) * 64;
         mbar_wait(BAR(S_FULL, b), u & 1, s_err, WAIT_MMA);
         tc_fence_after();
-        float s[64];
-        tmem_ld32_async(t_s0 + b * 64 + lane_addr, s);
-        tmem_ld32_async(t_s0 + b * 64 + 32 + lane_addr, s + 32);
-        tmem_wait_ld(s);
+        // the two lanes of a query row share its keys out, 32 each: a lane sends the other's half of its own row (high or low
+        // parts) and adds what comes back to its half
+        float s[32];
+        {
+          float t[64];
+          tmem_ld32_async(t_s0 + b * 64 + lane_addr, t);
+          tmem_ld32_async(t_s0 + b * 64 + 32 + lane_addr, t + 32);
+          tmem_wait_ld(t);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], 1);
+          for (int i = 0; i < 32; ++i) {
+            const float give = is_lo ? t[i] : t[32 + i], keep = is_lo ? t[32 + i] : t[i];
+            s[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+          }
+        }
+        const uint32_t key0 = kv0 + (is_lo ? 32 : 0);
         if (sc) {
           float4* d = reinterpret_cast<float4*>(sc + j * 64);
-          if (is_lo) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = make_float4(s[32 + 4 * i], s[33 + 4 * i], s[34 + 4 * i], s[35 + 4 * i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-          }
+          for (int i = 0; i < 8; ++i) d[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
         }
         if (kv0 + 64 > n_rows) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) if (kv0 + i >= n_rows) s[i] = -INFINITY;
+          for (int i = 0; i < 32; ++i) if (key0 + i >= n_rows) s[i] = -INFINITY;
         }
         float mt = s[0];
 #pragma unroll
-        for (int i = 1; i < 64; ++i) mt = fmaxf(mt, s[i]);
-        mt *= p.scale_log2;
+        for (int i = 1; i < 32; ++i) mt = fmaxf(mt, s[i]);
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1)) * p.scale_log2;
         if (j > 0) {
           mbar_wait(BAR(M_READY, (j - 1) & 1), ((j - 1) >> 1) & 1, s_err, WAIT_MMA);
           m_st = s_rm[row];
@@ -316,14 +325,19 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
             tmem_st32(t_o + c * 32 + lane_addr, o);
           }
         }
+        // weights of this lane's keys as f16 pairs, high and low parts; the even lane's row takes the high parts of all 64 keys, the odd one's the low parts
         uint32_t pw[32];
         float ls = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float e0 = ex2_approx(fmaf(s[2 * i], p.scale_log2, -m_st)), e1 = ex2_approx(fmaf(s[2 * i + 1], p.scale_log2, -m_st));
+        for (int i = 0; i < 16; ++i) {
+          const float e0 = ex2_approx(fmaf(s[2 * i], p.scale_log2, -m_st)), e1 = ex2_approx(fmaf(s[2 * i + 1], p.scale_log2, -m_st));
           ls += e0 + e1;
-          if (is_lo) { e0 -= __half2float(__float2half_rn(e0)); e1 -= __half2float(__float2half_rn(e1)); }
-          pw[i] = pack_h2(e0, e1);
+          const __half2 h = __floats2half2_rn(e0, e1);
+          const float2 f = __half22float2(h);
+          const uint32_t hi = *reinterpret_cast<const uint32_t*>(&h), lo = pack_h2(e0 - f.x, e1 - f.y);
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, is_lo ? hi : lo, 1);
+          pw[i] = is_lo ? got : hi;
+          pw[16 + i] = is_lo ? lo : got;
         }
         l_sum += ls;
         tmem_st32u(t_s0 + b * 64 + lane_addr, pw);
@@ -333,6 +347,7 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
       }
       // the row sum: the two groups' shares brought to the final reference
       mbar_wait(BAR(M_READY, (n_tiles - 1) & 1), ((n_tiles - 1) >> 1) & 1, s_err, WAIT_MMA);    // published after the last scores: the K ring is idle
+      l_sum += __shfl_xor_sync(0xffffffffu, l_sum, 1);
       s_rl[wg * 128 + row] = l_sum; s_rr[wg * 128 + row] = m_l;
     }
     named_bar_sync(2, 128 * GRP);
@@ -378,113 +393,136 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
 
 // ------------------------------------------------------------------------------ merge and sums --
 
-// CTAs below merge_ctas: one (item, head, 64-dim slice) each, 16 groups of 16 lanes over the row's records, sums in a fixed
-// order, gate, store.  The others: kSumRows rows of a sequence and kv head; the final (m, l) of the group's heads from
-// their records, then per row sum_h 2^(s_h - m_h) / l_h, head after head and item after item, added to the row's sum.
+// CTAs below merge_ctas merge: one (item, head) each, or one 64-dim slice of it where there are many records and few rows to
+// share them out (p.lanes: float4 lanes of a CTA's part of the row).  Every warp finds the row's maximum and sum by itself, over
+// records requested together with the (m, l) pairs, so that nothing waits for a barrier but the sum of the groups of lanes.
+// The others: kSumRows rows of a sequence and kv head; the final (m, l) of the group's heads from their records while the
+// scores are on their way, then per row sum_h 2^(s_h - m_h) / l_h, added to the row's sum: four threads a row, each with
+// every fourth head, then the four in order, item after item.
 template <int HD>
-__global__ void __launch_bounds__(256) pa_shared_finish_kernel(const __grid_constant__ SharedFinishParams p) {
-  __shared__ float s_w[512], s_red[8], s_red2[8];
-  __shared__ float4 s_acc[16][16];
+__global__ void __launch_bounds__(256, 2) pa_shared_finish_kernel(const __grid_constant__ SharedFinishParams p) {
+  __shared__ float4 s_acc[256];
+  __shared__ float s_m[64], s_il[64];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // (m, l) of a row from its records, the same in every lane of the warp
+  auto row_ml = [&](const float2* ml, uint32_t ns, float& M, float& l) {
+    float2 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = lane + 32 * k < ns ? ml[lane + 32 * k] : make_float2(-3.0e38f, 0.f);
+    M = fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x));
+    for (uint32_t s = lane + 128; s < ns; s += 32) M = fmaxf(M, ml[s].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    l = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) l = fmaf(v[k].y, ex2_approx(v[k].x - M), l);
+    for (uint32_t s = lane + 128; s < ns; s += 32) { const float2 w = ml[s]; l = fmaf(w.y, ex2_approx(w.x - M), l); }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  };
   pdl_wait();
   pdl_trigger();
   if (blockIdx.x < p.merge_ctas) {
-    const uint32_t prow = blockIdx.x / (HD / 64), slice = blockIdx.x % (HD / 64), item = prow / p.n_heads, h = prow % p.n_heads;
-    const uint32_t ns = p.p_splits + p.n_own[item], grp = tid >> 4, ln = tid & 15;
+    const uint32_t slices = HD / 4 / p.lanes, prow = blockIdx.x / slices, slice = blockIdx.x % slices, item = prow / p.n_heads, h = prow % p.n_heads;
+    const uint32_t ns = p.p_splits + p.n_own[item], groups = 256 / p.lanes, grp = tid / p.lanes, ln = tid % p.lanes, dims = p.lanes * 4, d = slice * dims + tid;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + (uint64_t)prow * p.n_rec;
-    const float* ob = p.part_o + (uint64_t)prow * p.n_rec * HD + slice * 64 + ln * 4;
-    float gv = 0.f;
-    const bool gated = p.gate && tid < 64;
-    if (gated) gv = ld_act(p.gate, (uint64_t)item * p.gate_col_stride + (uint64_t)h * p.gate_head_stride + slice * 64 + tid, p.act_f16);
-    float2 v0 = make_float2(-3.0e38f, 0.f), v1 = v0;
-    if (tid < ns) v0 = ml[tid];
-    if (tid + 256 < ns) v1 = ml[tid + 256];
-    float4 x[4];
+    const float* ob = p.part_o + (uint64_t)prow * p.n_rec * HD + slice * dims + ln * 4;
+    constexpr int U = 8;
+    float4 x[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t s = grp + 16 * u;
+    for (int u = 0; u < U; ++u) {
+      const uint32_t s = grp + u * groups;
       x[u] = s < ns ? *reinterpret_cast<const float4*>(ob + (uint64_t)s * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    float M = fmaxf(v0.x, v1.x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (lane == 0) s_red[warp] = M;
-    __syncthreads();
-    M = s_red[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) M = fmaxf(M, s_red[i]);
-    const float w0 = tid < ns ? exp2f(v0.x - M) : 0.f, w1 = tid + 256 < ns ? exp2f(v1.x - M) : 0.f;
-    s_w[tid] = w0; s_w[tid + 256] = w1;
-    float l = fmaf(v1.y, w1, v0.y * w0);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane == 0) s_red2[warp] = l;
-    __syncthreads();
-    l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) l += s_red2[i];
+    float gv = 0.f;
+    const bool gated = p.gate && tid < dims;
+    if (gated) gv = ld_act(p.gate, (uint64_t)item * p.gate_col_stride + (uint64_t)h * p.gate_head_stride + d, p.act_f16);
+    float M, l;
+    row_ml(ml, ns, M, l);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float4& r, float w) { acc.x = fmaf(r.x, w, acc.x); acc.y = fmaf(r.y, w, acc.y); acc.z = fmaf(r.z, w, acc.z); acc.w = fmaf(r.w, w, acc.w); };
+    auto add = [&](const float4& r, uint32_t s) {
+      const float w = s < ns ? ex2_approx(ml[s].x - M) : 0.f;
+      acc.x = fmaf(r.x, w, acc.x); acc.y = fmaf(r.y, w, acc.y); acc.z = fmaf(r.z, w, acc.z); acc.w = fmaf(r.w, w, acc.w);
+    };
 #pragma unroll
-    for (int u = 0; u < 4; ++u) { const uint32_t s = grp + 16 * u; add(x[u], s < ns ? s_w[s] : 0.f); }
-    for (uint32_t s = grp + 64; s < ns; s += 16) add(*reinterpret_cast<const float4*>(ob + (uint64_t)s * HD), s_w[s]);
-    s_acc[grp][ln] = acc;
+    for (int u = 0; u < U; ++u) add(x[u], grp + u * groups);
+    for (uint32_t s0 = grp + U * groups; s0 < ns; s0 += U * groups) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t s = s0 + u * groups;
+        x[u] = s < ns ? *reinterpret_cast<const float4*>(ob + (uint64_t)s * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(x[u], s0 + u * groups);
+    }
+    s_acc[tid] = acc;
     __syncthreads();
-    if (tid < 64) {
+    if (tid < dims) {
       const float* sa = reinterpret_cast<const float*>(s_acc);
       float t = sa[tid];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) t += sa[i * 64 + tid];
+      for (uint32_t i = 1; i < groups; ++i) t += sa[i * dims + tid];
       t = __fdiv_rn(t, l);
       if (gated) t *= __fdiv_rn(1.0f, 1.0f + __expf(-gv));
-      const uint64_t oo = (uint64_t)item * p.out_col_stride + (uint64_t)h * HD + slice * 64 + tid;
+      const uint64_t oo = (uint64_t)item * p.out_col_stride + (uint64_t)h * HD + d;
       if (p.act_f16) reinterpret_cast<__half*>(p.out)[oo] = __float2half_rn(t);
       else reinterpret_cast<float*>(p.out)[oo] = t;
     }
     return;
   }
   // ---- sums of the weights ----
-  const uint32_t u = blockIdx.x - p.merge_ctas;
+  const uint32_t u0 = blockIdx.x - p.merge_ctas;
   uint32_t lo = 0, hi = p.n_leads - 1;
-  while (lo < hi) { const uint32_t mid = (lo + hi + 1) / 2; if (u >= p.sum0[mid]) lo = mid; else hi = mid - 1; }
-  const uint32_t per_head = (p.sum0[lo + 1] - p.sum0[lo]) / p.n_kv, w = u - p.sum0[lo], kvh = w / per_head, r0 = (w % per_head) * kSumRows + tid * 4;
-  uint32_t item = p.lead[lo];
-  float* sums = p.sums + ((uint64_t)p.seq[item] * p.n_kv + kvh) * p.max_seq;
-  float add[4] = {0.f, 0.f, 0.f, 0.f};
+  while (lo < hi) { const uint32_t mid = (lo + hi + 1) / 2; if (u0 >= p.sum0[mid]) lo = mid; else hi = mid - 1; }
+  const uint32_t per_head = (p.sum0[lo + 1] - p.sum0[lo]) / p.n_kv, w = u0 - p.sum0[lo], kvh = w / per_head;
+  const uint32_t hg = tid >> 6, r0 = (w % per_head) * kSumRows + (tid & 63) * 4;     // this thread's heads: hg, hg + 4, ...; its rows
+  uint32_t item = p.lead[lo], most = 0;
+  for (uint32_t i = item; i != 255; i = p.next[i]) most = max(most, p.rows[i]);
+  float* sums = p.sums + ((uint64_t)p.seq[item] * p.n_kv + kvh) * p.max_seq + r0;
+  float old[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) old[e] = hg == 0 && r0 + e < most ? sums[e] : 0.f;
+  float4 add = make_float4(0.f, 0.f, 0.f, 0.f);
   for (; item != 255; item = p.next[item]) {
-    const uint32_t ns = p.p_splits + p.n_own[item], rows = p.rows[item];
-    __syncthreads();                                       // the heads' values of the item before have been read
+    const uint32_t ns = p.p_splits + p.n_own[item], rows = p.rows[item], pad = (rows + 63) & ~63u;
+    const float* sc = p.scores + p.score0[item] + (uint64_t)kvh * p.G * pad + r0;
+    constexpr int U = 4;
+    float4 s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (r0 < rows && hg + 4 * u < p.G) s[u] = *reinterpret_cast<const float4*>(sc + (uint64_t)(hg + 4 * u) * pad);
     for (uint32_t h = warp; h < p.G; h += 8) {
-      const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + ((uint64_t)item * p.n_heads + kvh * p.G + h) * p.n_rec;
-      float M = -3.0e38f, l = 0.f;
-      for (uint32_t s = lane; s < ns; s += 32) M = fmaxf(M, ml[s].x);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      for (uint32_t s = lane; s < ns; s += 32) l = fmaf(ml[s].y, exp2f(ml[s].x - M), l);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      if (lane == 0) { s_w[h] = M; s_w[256 + h] = __fdiv_rn(1.0f, l); }
+      float M, l;
+      row_ml(reinterpret_cast<const float2*>(p.part_ml) + ((uint64_t)item * p.n_heads + kvh * p.G + h) * p.n_rec, ns, M, l);
+      if (lane == 0) { s_m[h] = M; s_il[h] = __fdiv_rn(1.0f, l); }
     }
     __syncthreads();
+    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r0 < rows) {
-      const uint32_t pad = (rows + 63) & ~63u;
-      const float* sc = p.scores + p.score0[item] + (uint64_t)kvh * p.G * pad + r0;
-      float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (uint32_t h = 0; h < p.G; ++h) {
-        const float4 s = *reinterpret_cast<const float4*>(sc + (uint64_t)h * pad);
-        const float m = s_w[h], il = s_w[256 + h];
-        t[0] = fmaf(ex2_approx(fmaf(s.x, p.scale_log2, -m)), il, t[0]); t[1] = fmaf(ex2_approx(fmaf(s.y, p.scale_log2, -m)), il, t[1]);
-        t[2] = fmaf(ex2_approx(fmaf(s.z, p.scale_log2, -m)), il, t[2]); t[3] = fmaf(ex2_approx(fmaf(s.w, p.scale_log2, -m)), il, t[3]);
-      }
+      auto weigh = [&](const float4& v, uint32_t h) {
+        const float m = s_m[h], il = s_il[h];
+        t.x = fmaf(ex2_approx(fmaf(v.x, p.scale_log2, -m)), il, t.x); t.y = fmaf(ex2_approx(fmaf(v.y, p.scale_log2, -m)), il, t.y);
+        t.z = fmaf(ex2_approx(fmaf(v.z, p.scale_log2, -m)), il, t.z); t.w = fmaf(ex2_approx(fmaf(v.w, p.scale_log2, -m)), il, t.w);
+      };
 #pragma unroll
-      for (int e = 0; e < 4; ++e) if (r0 + e < rows) add[e] += t[e];
+      for (int u = 0; u < U; ++u) if (hg + 4 * u < p.G) weigh(s[u], hg + 4 * u);
+      for (uint32_t h = hg + 4 * U; h < p.G; h += 4) weigh(*reinterpret_cast<const float4*>(sc + (uint64_t)h * pad), h);
+    }
+    s_acc[tid] = t;
+    __syncthreads();
+    if (hg == 0 && r0 < rows) {
+#pragma unroll
+      for (int i = 1; i < 4; ++i) { const float4 v = s_acc[tid + 64 * i]; t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w; }
+      add.x += t.x;
+      if (r0 + 1 < rows) add.y += t.y;
+      if (r0 + 2 < rows) add.z += t.z;
+      if (r0 + 3 < rows) add.w += t.w;
     }
   }
-  uint32_t most = 0;
-  for (uint32_t i = p.lead[lo]; i != 255; i = p.next[i]) most = max(most, p.rows[i]);
+  if (hg == 0) {
+    const float a[4] = {add.x, add.y, add.z, add.w};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) if (r0 + e < most) sums[r0 + e] += add[e];
+    for (int e = 0; e < 4; ++e) if (r0 + e < most) sums[e] = old[e] + a[e];
+  }
 }
 
 template <int HD>

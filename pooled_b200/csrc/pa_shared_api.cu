@@ -21,25 +21,41 @@ static uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 static uint32_t pad64(uint32_t rows) { return (rows + 63) & ~63u; }
 static uint64_t scores_of(const pa_ctx* ctx, uint32_t rows) { return (uint64_t)ctx->cfg.n_heads * pad64(rows); }
 
-// Tiles per unit: all units of a call have the same number T, so that no CTA is the last for long.  For each number of waves
-// the least T whose units fit it; the waves with the least waves * (T + start and end of a unit, in tiles).
+// Tiles per unit (T).  The units of a call are launched longest first, one CTA an SM at a time, so a call takes about
+// max(its longest unit, all its tiles and starts / SMs).  A unit costs `start` tiles of its own: launch, q, the first
+// scores, the record; some 6.5 us, a tile 0.72 us where several row tiles read the shared rows (the tensor cores' time) and 1.45
+// where HBM feeds every SM (head_dim 256).  Tried: every number of splits of the shared rows, or of the longest item without them.
 static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_items, uint32_t p_tiles, uint32_t row_tiles, uint32_t most_records) {
-  uint32_t longest = std::max(1u, p_tiles), least = p_tiles ? row_tiles : 0;
-  for (uint32_t i = 0; i < n_items; ++i) { longest = std::max(longest, ceil_div(rows[i], 64)); least += rows[i] > 0; }
-  auto units = [&](uint32_t T) { uint32_t n = row_tiles * ceil_div(p_tiles, T); for (uint32_t i = 0; i < n_items; ++i) n += ceil_div(ceil_div(rows[i], 64), T); return n; };
-  const uint32_t per_wave = std::max(1u, (uint32_t)ctx->sm_count / ctx->cfg.n_kv_heads), start = ctx->cfg.head_dim == 256 ? 5 : ctx->cfg.head_dim == 128 ? 8 : 12;
-  uint32_t best = longest;
-  uint64_t cost = ~0ull;
-  const uint32_t w0 = std::max(1u, ceil_div(least, per_wave));
-  for (uint32_t w = w0; w < w0 + 6; ++w) {
-    uint32_t lo = 1, hi = longest;
-    while (lo < hi) { const uint32_t mid = (lo + hi) / 2; if (units(mid) <= w * per_wave) hi = mid; else lo = mid + 1; }
-    if ((uint64_t)w * (lo + start) < cost) { cost = (uint64_t)w * (lo + start); best = lo; }
+  const uint32_t n_kv = ctx->cfg.n_kv_heads, sms = (uint32_t)ctx->sm_count;
+  uint32_t own_longest = 0, own_tiles = 0, own_items = 0;
+  for (uint32_t i = 0; i < n_items; ++i) {
+    const uint32_t t = ceil_div(rows[i], 64);
+    own_longest = std::max(own_longest, t); own_tiles += t; own_items += t > 0;
   }
-  // a row's records: those of the shared rows and the longest item's own
-  uint32_t own = 0;
-  for (uint32_t i = 0; i < n_items; ++i) own = std::max(own, ceil_div(rows[i], 64));
-  while (best < longest && ceil_div(p_tiles, best) + ceil_div(own, best) > most_records) ++best;
+  const uint32_t longest = std::max(1u, std::max(p_tiles, own_longest)), hd = ctx->cfg.head_dim;
+  const float start = p_tiles && row_tiles > 1 ? (hd == 256 ? 9.f : 12.f) : hd == 256 ? 4.5f : hd == 128 ? 8.f : 12.f;
+  uint32_t best = longest;
+  float least = 3.0e38f;
+  const uint32_t split = p_tiles ? p_tiles : longest, most_splits = std::min(split, std::min(most_records, 4 * sms));
+  for (uint32_t n = 1; n <= most_splits; ++n) {
+    const uint32_t T = ceil_div(split, n);
+    if (n > 1 && T == ceil_div(split, n - 1)) continue;
+    // records of a row: the shared rows' and the longest item's
+    if (ceil_div(p_tiles, T) + ceil_div(own_longest, T) > most_records) break;
+    const float t = (float)std::min(T, longest) + start;
+    const float own_units = own_longest <= T ? (float)own_items : (float)own_tiles / T + 0.5f * own_items;
+    const float shared_units = (float)(p_tiles ? row_tiles * ceil_div(p_tiles, T) : 0) * n_kv, own_work = ((float)own_tiles + own_units * start) * n_kv;
+    const float units = shared_units + own_units * n_kv;
+    float time;
+    if (units <= sms) time = t;
+    else if (shared_units > 0) {   // full waves of the equal, longest units; the others fill what the last wave leaves
+      const float full = ceilf(shared_units / sms) * t;
+      time = full + std::max(0.f, own_work - (sms * full - shared_units * t)) / sms;
+    } else {
+      time = std::max(own_work / sms + 0.5f * t, t);
+    }
+    if (time < least) { least = time; best = T; }
+  }
   return best;
 }
 
@@ -87,7 +103,9 @@ static int shared_launch(const SharedCall& c, const pa_item* items, const uint32
   f.part_o = p.part_o; f.part_ml = p.part_ml; f.n_rec = p.n_rec; f.p_splits = p.p_splits; f.n_items = n; f.n_heads = nH; f.G = G; f.n_kv = n_kv;
   f.gate = c.gate ? reinterpret_cast<const uint8_t*>(c.gate) + (uint64_t)first * c.gcs * aes : nullptr; f.gate_col_stride = c.gcs; f.gate_head_stride = c.ghs;
   f.out = reinterpret_cast<uint8_t*>(c.out) + (uint64_t)first * c.ocs * aes; f.out_col_stride = c.ocs; f.act_f16 = ctx->cfg.act_dtype == PA_F16;
-  f.merge_ctas = n * nH * (hd / 64);
+  // few rows of many records: their dims are shared out among CTAs, else a CTA takes a row
+  f.lanes = (uint64_t)n * nH * 2 <= (uint64_t)ctx->sm_count * 4 && p.n_rec > 16 ? 16 : hd / 4;
+  f.merge_ctas = n * nH * (hd / 4 / f.lanes);
   uint32_t sum_ctas = 0;
   if (c.sums) {
     f.scores = ctx->scores; f.sums = L->sums; f.scale_log2 = p.scale_log2; f.max_seq = L->max_seq;

@@ -99,13 +99,13 @@ def test_the_host_refuses_what_does_not_fit():
     eng.device, eng.layers, eng._call, eng.ctx, eng.slots, eng._xc_keep = 0, [C.c_void_p(8)], Calls(), None, {}, None
     eng._f_rot_append = eng._f_shared = eng._f_weights = 0
     rot = object.__new__(Rotary)
-    rot.eng, rot.handle, rot._apply, rot._f_apply = eng, C.c_void_p(8), Calls(), 0
+    rot.eng, rot.handle, rot._h, rot._apply, rot._f_apply = eng, C.c_void_p(8), 8, Calls(), 0
     q, kv = torch.zeros((2, 256)), torch.zeros((2, 128))             # of another device than the engine's
     for call in (lambda: rot.apply(q, 4), lambda: eng.rotary_append(0, rot, [(0, 0, 2)], q, kv, kv, q_out=q), lambda: eng.decode_shared(0, None, 0, 0, [(0, 1), (0, 2)], q, out=q),
                  lambda: eng.decode_weights(0, [(0, 1), (0, 2)], q, out=q)):
         with pytest.raises(PaError):
             call()
-    eng.device = None                                                 # ... of the same: the shapes
+    eng._q_dim, eng._kv_dim, eng.device = 256, 128, -1                                                 # ... of the same: the shapes
     meta = lambda *s, dt=torch.float32: torch.zeros(s, dtype=dt)
     for call in (lambda: rot.apply(q, 5, out=meta(2, 320)), lambda: rot.apply(q, 4, out=meta(1, 256)), lambda: rot.apply(q, 4, positions=meta(2), out=q),
                  lambda: rot.apply(q, 4, positions=meta(3, dt=torch.int32), out=q), lambda: rot.apply(q.t(), 4, out=q),
