@@ -154,7 +154,7 @@ class Rotary:
         cols, have = x.shape
         hs, ohs, last, dt = head_stride or hd, out_head_stride or hd, n_heads - 1, _dt(x.dtype)
         if out is None:
-            out, out_have, out_dt, ohs = x.new_empty((cols, n_heads * hd)), n_heads * hd, dt, hd
+            out, out_have, out_dt, ohs = torch.empty_strided((cols, n_heads * hd), (n_heads * hd, 1), dtype=x.dtype, device=eng._dev), n_heads * hd, dt, hd
         else:
             out_cols, out_have = out.shape
             out_dt = _dt(out.dtype)
@@ -188,6 +188,7 @@ class AttnEngine:
         self.slots: dict[str, dict] = {}
         self._xc_keep = None
         self._q_dim, self._kv_dim = cfg.q_dim, cfg.kv_dim
+        self._dev = torch.device("cuda", device)
         self._views: dict = {}                  # cache() and the like: the device arrays as tensors, made once
         self._rotaries = weakref.WeakSet()      # destroyed ahead of the context
         self.L.check(self.L.pa_create(device, C.byref(pc), C.byref(h)))
@@ -287,7 +288,7 @@ class AttnEngine:
     def _view(self, key, ptr, shape, typestr) -> torch.Tensor:
         t = self._views.get(key)
         if t is None:
-            t = self._views[key] = torch.as_tensor(_DevArray(ptr(), shape, typestr), device=f"cuda:{self.device}")
+            t = self._views[key] = torch.as_tensor(_DevArray(ptr(), shape, typestr), device=self._dev)
         return t.detach()                       # a tensor of the caller's own over the same memory
 
     # ---- the path, step by step ----
@@ -442,7 +443,7 @@ class AttnEngine:
         total = sum([it[2] for it in items])
         self._columns(total, q, k, v, q_out)
         if q is not None and q_out is None:
-            q_out = q.new_empty((total, self._q_dim), dtype=q_dtype)
+            q_out = torch.empty_strided((total, self._q_dim), (self._q_dim, 1), dtype=q_dtype, device=self._dev)
         if k.stride(0) != v.stride(0) and total > 1:
             raise _l.PaError(-1, "k and v have different column strides")
         rc = self._call.rotary_append(self._f_rot_append, rot._h, self.layers[li].value, items, rows, q, q_head_stride or self.cfg.head_dim, k, v, q_out,
@@ -483,7 +484,7 @@ class AttnEngine:
             if gate.dtype != act or cols != n or last * (gate_head_stride or hd) + hd > have:
                 raise _l.PaError(-1, f"{gate.dtype} gate of shape {tuple(gate.shape)} for {n} items of {c.n_heads} heads")
         if out is None:
-            return q.new_empty((n, self._q_dim), dtype=act)
+            return torch.empty_strided((n, self._q_dim), (self._q_dim, 1), dtype=act, device=self._dev)
         self._on_device(out)
         cols, have = out.shape
         if out.dtype != act or cols != n or have < self._q_dim:
@@ -537,7 +538,7 @@ class AttnEngine:
         """Brings sequences down to n_keep rows per kv head, the first n_first, the last n_recent and the rows with the largest sums between them:
         items = [(src_seq, dst_seq, n_rows)], dst_seq = src_seq in place.  Returns the rows that stayed, int32 [n_items, n_kv_heads, n_keep],
         ascending, -1 behind the last."""
-        kept = torch.empty((len(items), self.cfg.n_kv_heads, max(0, n_keep)), dtype=torch.int32, device=f"cuda:{self.device}")
+        kept = torch.empty((len(items), self.cfg.n_kv_heads, max(0, n_keep)), dtype=torch.int32, device=self._dev)
         rc = self._call.evict(self._f_evict, self.layers[li].value, items, n_keep, n_first, n_recent, kept, self._raw_st())
         if rc:
             self._ck(rc)
