@@ -258,12 +258,13 @@ constexpr uint32_t kSumRows = 256;    // rows of one CTA's sums
 
 // eviction by summed weights (pa_evict_select_kernel, pa_evict_move_kernel)
 constexpr int kMaxEvict = 32;                       // items of one pa_evict call
-constexpr uint32_t kEvictKeys = 49152;              // rows of one CTA of the selection
+constexpr uint32_t kEvictKeys = 49152;              // rows of one CTA where eight share them out
+constexpr uint32_t kEvictAlone = 8192;              // rows that one CTA ranks by itself
 struct EvictParams {
   uint32_t n_items, n_kv, hd, max_seq, n_keep, n_first, n_recent;
   __half* k; __half* v; float* sums;
   uint32_t* list;                                   // [n_items][n_kv][n_keep]: the rows that stay
-  uint32_t chunks;                                  // CTAs that share the rows of an item that goes to another sequence
+  uint32_t chunks;                                  // CTAs that share the rows of an item that goes to another sequence (the launcher sets it)
   uint32_t src[kMaxEvict], dst[kMaxEvict], rows[kMaxEvict];
 };
 

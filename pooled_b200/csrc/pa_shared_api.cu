@@ -277,7 +277,6 @@ extern "C" int pa_evict(pa_layer* L, const pa_evict_item* items, uint32_t n_item
   EvictParams p{};
   p.n_items = n_items; p.n_kv = ctx->cfg.n_kv_heads; p.hd = ctx->cfg.head_dim; p.max_seq = L->max_seq; p.n_keep = n_keep; p.n_first = n_first; p.n_recent = n_recent;
   p.k = L->k; p.v = L->v; p.sums = L->sums;
-  uint64_t moved = 0;
   for (uint32_t i = 0; i < n_items; ++i) {
     const pa_evict_item& it = items[i];
     if (it.src_seq >= L->n_seqs || it.dst_seq >= L->n_seqs) return fail(ctx, PA_EINVAL, "pa_evict: sequence %u of %u", std::max(it.src_seq, it.dst_seq), L->n_seqs);
@@ -287,11 +286,13 @@ extern "C" int pa_evict(pa_layer* L, const pa_evict_item* items, uint32_t n_item
       if (items[j].dst_seq == it.dst_seq || items[j].src_seq == it.dst_seq || items[j].dst_seq == it.src_seq)
         return fail(ctx, PA_EINVAL, "pa_evict: the destination of item %u or %u is named by the other", j, i);
     p.src[i] = it.src_seq; p.dst[i] = it.dst_seq; p.rows[i] = it.n_rows;
-    moved += std::min(it.n_rows, n_keep);
   }
-  const uint64_t words = (uint64_t)n_items * p.n_kv * n_keep;
-  if (!kept && words > ctx->scores_floats) return fail(ctx, PA_EUNSUPPORTED, "pa_evict: the lists of %u items do not fit the context's room; pass `kept` or fewer items", n_items);
-  p.list = kept ? kept : reinterpret_cast<uint32_t*>(ctx->scores);
+  p.list = kept;
+  if (!kept) {
+    if ((uint64_t)n_items * p.n_kv * n_keep > ctx->scores_floats)
+      return fail(ctx, PA_EUNSUPPORTED, "pa_evict: the lists of %u items do not fit the context's room; pass `kept` or fewer items", n_items);
+    p.list = reinterpret_cast<uint32_t*>(ctx->scores);
+  }
   DeviceScope on(ctx->device);
   CU_TRY(ctx, launch_evict(p, (uint32_t)ctx->sm_count, ctx->device, (cudaStream_t)stream));
   ctx->stats.kernel_launches += 2; ctx->stats.calls++;

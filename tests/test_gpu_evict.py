@@ -113,7 +113,7 @@ def check_eviction(eng, items, keep, first, recent):
 
 @pytest.mark.parametrize("nKV,hd", [(2, 256), (8, 128), (1, 64)])
 @pytest.mark.parametrize("rows,keep,first,recent", [(300, 299, 0, 0), (300, 1, 0, 0), (300, 100, 4, 50), (301, 128, 0, 128), (1111, 700, 700, 0), (1111, 64, 32, 32), (2, 1, 0, 1),
-                                                    (2500, 2000, 4, 256), (9000, 1024, 16, 100), (17001, 3000, 1, 1), (40000, 39000, 5, 7)])
+                                                    (2500, 2000, 4, 256), (9000, 1024, 16, 100), (8192, 5000, 0, 9), (8193, 8000, 3, 0), (17001, 3000, 1, 1), (40000, 39000, 5, 7)])
 @pytest.mark.parametrize("in_place", [True, False])
 def test_evict(nKV, hd, rows, keep, first, recent, in_place):
     eng = tracked(nKV, nKV, hd, rows + 3, 3, F16)
@@ -151,14 +151,15 @@ def test_evict_short_sequences_keep_all_and_forks():
     assert eng.evict(0, [(0, 0, 10)], 5).shape == (1, 4, 5)
 
 
-def test_evict_lists_of_the_context():
+@pytest.mark.parametrize("n", [500, 9000])
+def test_evict_without_lists(n):
     # without `kept` the lists live in the context's room
-    eng = tracked(2, 2, 128, 500, 2, F16)
+    eng = tracked(2, 2, 128, n, 2, F16)
     fill(eng, 7)
     eng.weights(0).uniform_()
-    rows = [reference_rows(eng.weights(0)[0, h].tolist(), 500, 200, 0, 0) for h in (0, 1)]
-    want = torch.stack([eng.cache(0, "k")[0].view(500, 2, 128)[rows[h], h] for h in (0, 1)], 1)
-    rc = eng._call.evict(eng._f_evict, eng.layers[0].value, [(0, 1, 500)], 200, 0, 0, None, eng._raw_st())
+    rows = [reference_rows(eng.weights(0)[0, h].tolist(), n, 200, 0, 0) for h in (0, 1)]
+    want = torch.stack([eng.cache(0, "k")[0].view(n, 2, 128)[rows[h], h] for h in (0, 1)], 1)
+    rc = eng._call.evict(eng._f_evict, eng.layers[0].value, [(0, 1, n)], 200, 0, 0, None, eng._raw_st())
     assert rc == 0 and torch.equal(eng.cache(0, "k")[1, :200].view(200, 2, 128), want)
 
 
