@@ -229,7 +229,7 @@ struct SharedParams {
   float* part_o; float* part_ml; uint32_t n_rec;                            // records of a row (column, head): n_rec apart; m in log2 units
   // the shared rows [0, p_rows) from row p_row0 of their cache on: units 0 .. p_splits * row_tiles - 1, a row tile being the
   // heads of items_per_tile items
-  uint32_t p_row0, p_rows, p_tps, p_splits, row_tiles, items_per_tile;
+  uint32_t p_row0, p_rows, p_tps, p_splits, row_tiles, items_per_tile, wide;   // wide: 128 query rows a tile, else up to 64
   // the items' own rows, rows[i] of them from row own_row0 of sequence seq[i] on: units cta0[i] .. cta0[i + 1] - 1 behind those
   uint32_t max_seq, own_row0, tps, units;
   uint32_t seq[kMaxShared], rows[kMaxShared];

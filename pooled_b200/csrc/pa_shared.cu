@@ -3,26 +3,30 @@
 //
 //   o = sum_r e^(q.k_r / sqrt(hd) - M) v_r / sum_r e^(q.k_r / sqrt(hd) - M)   over the shared rows and the item's own
 //
-// A unit is a run of 64-row K / V tiles of one kv head and up to 64 query rows that attend them: for the shared rows the
-// heads of several items (so that each shared byte is read once per 64 query rows, from HBM once in all), for own rows the
-// heads of one.  A CTA per unit walks its tiles on the 5th-generation tensor cores and leaves an unnormalised (o, m, l)
-// record per query row; the second kernel merges a row's records, gates and stores.  All units have the same number of
-// tiles, whatever they are units of (plan_shared), so that a batch of long shared rows and short own ones fills the
-// machine like one long conversation.
+// A unit is a run of 64-row K / V tiles of one kv head and the query rows that attend them: for the shared rows the heads of
+// several items (so that a shared byte is read once for all of these, from HBM once in all), for own rows the heads of one.
+// A CTA per unit walks its tiles on the 5th-generation tensor cores and leaves an unnormalised (o, m, l) record per query
+// row; the second kernel merges a row's records, gates and stores.  All units have the same number of tiles, whatever they
+// are units of (plan_units), so that a batch of long shared rows and short own ones fills the machine like one long conversation.
 //
 //   warps 0, 3  TMA producers: K tiles and V tiles (64 x head_dim f16, 128-byte swizzle), a ring of three and of two slots;
 //               warp 3 then clears the rows of the last V tile that lie behind the unit's last: a weight of zero does not
 //               make up for an infinity or NaN that the cache holds there
-//   warp 1      issues the scores: S = Q K^T into one of three tiles of tensor memory (128 x 64 f32)
+//   warp 1      issues the scores: S = Q K^T into one of two or three tiles of tensor memory (128 x 64 f32)
 //   warp 2      tensor memory; issues O += P V into the accumulator (128 x head_dim f32)
-//   warps 4-11  two softmax groups on alternate tiles.  Even rows of the 128 carry the f16 high parts of q and of the
-//               weights, odd rows the low parts of the same query row: some 22 bits of both, added by shuffles.  The two lanes
-//               share the row's keys out (each with all 64, a tile took 2 us of a group instead of 1.2).  A row's reference lies 2^7 below its maximum, moves only when a tile passes it by 2^15, and travels
-//               with the tiles: weights of up to 2^15 keep the low parts of small ones above f16's last place (with a
-//               reference at the maximum, a long row's error was 2.2e-6 of the result, 3e-7 now).
-//               Warps whose rows hold no query take no part.
-// What bounds it: one query tile per kv head, HBM; several, the tensor cores (1394 cycles for both products of 64 keys at
-// head_dim 256).
+//   warps 4-11  softmax, two groups of four warps with half of a tile's keys each (on alternate tiles, a call of one tile a CTA took
+//               0.4 us longer, and wide tiles 1.5 us each).  A row's reference lies 2^7 below its maximum and moves only when a tile
+//               passes it by 2^15: weights of up to 2^15 keep the low parts of small ones above f16's last place (with a reference at the
+//               maximum, a long row's error was 2.2e-6 of the result, 3e-7 now).  Warps whose rows hold no query take no part.
+// q and the weights enter as pairs of f16 values, high and low parts, some 22 bits of both, in one of two ways:
+//   narrow (up to 64 query rows)   even rows of the 128 carry the high parts, odd rows the low parts of the same query row, added by
+//               shuffles: both products at the cost of one, 1394 cycles for 64 keys at head_dim 256.  The two lanes share the
+//               row's keys out
+//   wide (shared rows of more)     128 query rows; the products of the low parts are issued after those of the high ones into the same
+//               accumulators (none of q's where q is f16): 1906 cycles with f16 queries, 2788 with f32 ones, and half the bytes
+//               through L2, which at 64 KB a tile and 0.87 us fed narrow tiles no faster
+// What bounds it: one query tile per kv head, HBM; several, the tensor cores; short calls the chain of launch, q, scores,
+// weights, products and records, 6.5 us.
 #include <algorithm>
 
 #include "pa_tc.cuh"
@@ -31,102 +35,62 @@ namespace pa {
 
 template <int HD>
 struct ShSmem {
-  static constexpr int SBUF = 3, NK = 3, NV = 2;
+  static constexpr int NK = 3, NV = 2;
   static constexpr int KV_BYTES = HD * 128;          // [HD/64][64 rows][128 B]
-  static constexpr int TQC = HD / 128;               // 64-dim chunks of Q in tensor memory, the others in shared memory
-  static constexpr int QS_BYTES = (HD / 64 - TQC) * 128 * 128;
   static constexpr int THREADS = 384;
-  static constexpr int OFF_K = 0, OFF_V = NK * KV_BYTES, OFF_Q = (NK + NV) * KV_BYTES, OFF_BAR = OFF_Q + QS_BYTES;
-  static constexpr int OFF_ROW = OFF_BAR + 256;      // [128] reference maximum of each row
-  static constexpr int TOTAL = 1024 + OFF_ROW + 128 * 4;
-  static_assert(TOTAL <= 227 * 1024, "shared memory of one CTA");
-  // the records leave through the K ring: row sums of the groups, then 64 rows of HD + 4 floats and their slots
-  static_assert(2048 + 64 * (HD + 4) * 4 + 64 * 8 <= (NK + NV) * KV_BYTES, "staging of the records");
-  static constexpr int T_Q = 0, T_S = TQC * 32, T_O = TQC * 32 + SBUF * 64;
-  static constexpr int TMEM_COLS = T_O + HD <= 256 ? 256 : 512;
+  static constexpr int OFF_K = 0, OFF_V = NK * KV_BYTES, OFF_BAR = (NK + NV) * KV_BYTES;
+  static constexpr int OFF_MAX = OFF_BAR + 256;      // wide: [2][128] maxima of the rows
+  static constexpr int OFF_Q = OFF_BAR + 2048;       // narrow: the chunks of Q that are not in tensor memory; wide: the low parts
+  static constexpr int OFF_MAX2 = OFF_Q + (HD / 64 - HD / 128) * 128 * 128;     // narrow: [2][2][128] maxima of the rows, two tiles in turn
+  static constexpr int total(bool wide_lo) { return 1024 + std::max(OFF_MAX2 + 2048, wide_lo ? OFF_Q + HD / 64 * 128 * 128 : 0); }
+  static_assert(total(true) <= 227 * 1024, "shared memory of one CTA");
+  // the records leave through the rings: row sums of the groups, then 64 (in the K ring) or 128 rows of HD + 4 floats
+  static_assert(2048 + 64 * (HD + 4) * 4 <= NK * KV_BYTES && 2048 + 128 * (HD + 4) * 4 <= (NK + NV) * KV_BYTES, "staging of the records");
+};
+template <int HD, bool WIDE>
+struct ShLay {
+  static constexpr int SB = WIDE ? 2 : 3;            // tiles of scores in tensor memory; the weights take their scores' place
+  static constexpr int TQC = WIDE ? HD / 64 : HD / 128;     // 64-dim chunks of Q in tensor memory, 32 columns each
+  static constexpr int T_S = TQC * 32, T_O = T_S + SB * 64;
   static_assert(T_O + HD <= 512, "tensor memory columns");
 };
-
 template <int HD>
-__global__ void __launch_bounds__(384, 1)
-pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv, const __grid_constant__ CUtensorMap tm_k,
-                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedParams p) {
+constexpr int sh_tmem_cols() { return std::max(ShLay<HD, false>::T_O, ShLay<HD, true>::T_O) + HD <= 256 ? 256 : 512; }
+
+enum { SH_K_FULL = 0, SH_K_EMPTY = 3, SH_V_FULL = 6, SH_V_EMPTY = 8, SH_S_FULL = 10, SH_P_FULL = 13, SH_PV_DONE = 16, SH_O_DONE = 19, SH_Q_FULL, SH_Q_READ, SH_V_CLEAN, SH_BARS };
+static_assert(SH_BARS <= 31, "barrier slots");
+
+// a CTA's unit
+struct ShUnit {
+  const CUtensorMap* mk;
+  const CUtensorMap* mv;
+  uint32_t item0, slot, row0, n_rows, tile0, n_tiles;       // first item; record of a row; first row in the map; the unit's rows end here; its tiles
+  uint32_t pairs, live_warps;                               // query rows; warps of a softmax group that hold them
+  bool shared, once, ragged;                                // shared rows; nobody else reads the unit's rows; the last tile reaches past them
+};
+
+template <int HD, bool WIDE>
+__device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit& un, uint8_t* base, uint32_t bar0, volatile uint32_t* s_err, uint32_t tmem) {
   using L = ShSmem<HD>;
-  constexpr int CH = HD / 64, NK = L::NK, NV = L::NV, SB = L::SBUF, GRP = 2;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base + L::OFF_BAR);
-  volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(bars + 31);
-  volatile uint32_t* s_err = s_tmem + 1;
-  float* s_rm = reinterpret_cast<float*>(base + L::OFF_ROW);
-  float* s_rl = reinterpret_cast<float*>(base + L::OFF_K);       // [2][128] the groups' row sums and [2][128] what they are expressed in,
-  float* s_rr = s_rl + 256;                                      // in the first K slot once the last tile's scores exist
-  const uint32_t bar0 = smem_u32(bars);
-  enum { K_FULL = 0, K_EMPTY = NK, V_FULL = 2 * NK, V_EMPTY = V_FULL + NV, S_FULL = V_EMPTY + NV, P_FULL = S_FULL + SB, PV_DONE = P_FULL + SB, O_DONE = PV_DONE + SB,
-         Q_FULL, Q_READ, M_READY /* [2] */, V_CLEAN = M_READY + 2, N_BARS };
-  static_assert(N_BARS <= 31, "barrier slots");
-  uint8_t* q_s = base + L::OFF_Q;
-  auto BAR = [&](int which, int idx) { return bar0 + 8u * (uint32_t)(which + idx); };
-
+  using T = ShLay<HD, WIDE>;
+  constexpr int CH = HD / 64, NK = L::NK, NV = L::NV, SB = T::SB, GRP = 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t g = blockIdx.y, unit = blockIdx.x, p_units = p.p_splits * p.row_tiles;
-  const bool shared = unit < p_units;
-  uint32_t item0, n_q, split, row0, n_rows, tps;       // first item, items, split, first row in the map, the unit's rows end here, tiles per split
-  if (shared) {
-    split = unit / p.row_tiles;
-    item0 = (unit % p.row_tiles) * p.items_per_tile;
-    n_q = min(p.items_per_tile, p.n_items - item0);
-    row0 = p.p_row0; n_rows = p.p_rows; tps = p.p_tps;
-  } else {
-    uint32_t lo = 0, hi = p.n_items - 1;
-    while (lo < hi) { const uint32_t mid = (lo + hi + 1) / 2; if (unit >= p.cta0[mid]) lo = mid; else hi = mid - 1; }
-    item0 = lo; n_q = 1; split = unit - p.cta0[lo];
-    row0 = p.seq[lo] * p.max_seq + p.own_row0; n_rows = p.rows[lo]; tps = p.tps;
-  }
-  const CUtensorMap* mk = shared ? &tm_pk : &tm_k;
-  const CUtensorMap* mv = shared ? &tm_pv : &tm_v;
-  const bool once = !shared || p.row_tiles == 1;                       // nobody else reads the unit's rows: they need not stay in L2
-  const uint32_t tiles = (n_rows + 63) / 64, tile0 = split * tps, n_tiles = min(tiles, tile0 + tps) - tile0;
-  const uint32_t pairs = n_q * p.G;                                     // query rows, two lanes each
-  const uint32_t live_warps = (2 * pairs + 31) / 32;                    // of each softmax group
-  const bool ragged = (tile0 + n_tiles) * 64 > n_rows;                  // the last tile reaches past the unit's rows
-
-  if (warp == 1 && lane == 0) {
-    *s_err = 0;
-    for (int i = 0; i < NK; ++i) { mbar_init(BAR(K_FULL, i), 1); mbar_init(BAR(K_EMPTY, i), 1); }
-    for (int i = 0; i < NV; ++i) { mbar_init(BAR(V_FULL, i), 1); mbar_init(BAR(V_EMPTY, i), 1); }
-    for (int i = 0; i < SB; ++i) { mbar_init(BAR(S_FULL, i), 1); mbar_init(BAR(P_FULL, i), 32 * live_warps); mbar_init(BAR(PV_DONE, i), 1); }
-    mbar_init(BAR(O_DONE, 0), 1);
-    mbar_init(BAR(Q_FULL, 0), 128 * GRP);
-    mbar_init(BAR(Q_READ, 0), 128 * GRP);
-    mbar_init(BAR(M_READY, 0), 32 * live_warps); mbar_init(BAR(M_READY, 1), 32 * live_warps);
-    mbar_init(BAR(V_CLEAN, 0), 1);
-    fence_barrier_init();
-  }
-  if (warp == 2) {
-    tmem_alloc(smem_u32((const void*)s_tmem), L::TMEM_COLS);
-    tmem_relinquish();
-    tc_fence_before();
-  }
-  if (warp == 0 && lane == 0) { prefetch_tmap(mk); prefetch_tmap(mv); }
-  pdl_wait();
-  pdl_trigger();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *s_tmem;
-  const uint32_t t_q = tmem + L::T_Q, t_s0 = tmem + L::T_S, t_o = tmem + L::T_O;
+  const uint32_t g = blockIdx.y, n_tiles = un.n_tiles, tile0 = un.tile0;
+  auto BAR = [&](int which, int idx) { return bar0 + 8u * (uint32_t)(which + idx); };
+  uint8_t* q_s = base + L::OFF_Q;
+  const uint32_t t_q = tmem, t_s0 = tmem + T::T_S, t_o = tmem + T::T_O;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer, K ----
     if (lane == 0) {
       for (uint32_t j = 0; j < n_tiles; ++j) {
         const uint32_t st = j % NK, u = j / NK;
-        if (j == 2) mbar_wait(BAR(Q_READ, 0), 0, s_err, WAIT_QFULL);         // the third slot stages query rows until then
-        mbar_wait(BAR(K_EMPTY, st), (u & 1) ^ 1, s_err, WAIT_EMPTY);
-        mbar_expect_tx(BAR(K_FULL, st), L::KV_BYTES);
+        if (j == 2) mbar_wait(BAR(SH_Q_READ, 0), 0, s_err, WAIT_QFULL);      // the third slot stages query rows until then
+        mbar_wait(BAR(SH_K_EMPTY, st), (u & 1) ^ 1, s_err, WAIT_EMPTY);
+        mbar_expect_tx(BAR(SH_K_FULL, st), L::KV_BYTES);
         const uint32_t dst = smem_u32(base + L::OFF_K + st * L::KV_BYTES);
-        if (once) tma_load_3d_hint(dst, mk, 0, (int)(row0 + (tile0 + j) * 64), (int)(g * CH), BAR(K_FULL, st), l2_policy_evict_first());
-        else tma_load_3d(dst, mk, 0, (int)(row0 + (tile0 + j) * 64), (int)(g * CH), BAR(K_FULL, st));
+        if (un.once) tma_load_3d_hint(dst, un.mk, 0, (int)(un.row0 + (tile0 + j) * 64), (int)(g * CH), BAR(SH_K_FULL, st), l2_policy_evict_first());
+        else tma_load_3d(dst, un.mk, 0, (int)(un.row0 + (tile0 + j) * 64), (int)(g * CH), BAR(SH_K_FULL, st));
       }
     }
   } else if (warp == 3) {
@@ -134,25 +98,25 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
     if (lane == 0) {
       for (uint32_t j = 0; j < n_tiles; ++j) {
         const uint32_t st = j % NV, u = j / NV;
-        if (j == 1) mbar_wait(BAR(Q_READ, 0), 0, s_err, WAIT_QFULL);         // ... and the second V slot
-        mbar_wait(BAR(V_EMPTY, st), (u & 1) ^ 1, s_err, WAIT_EMPTY);
-        mbar_expect_tx(BAR(V_FULL, st), L::KV_BYTES);
+        if (j == 1) mbar_wait(BAR(SH_Q_READ, 0), 0, s_err, WAIT_QFULL);      // ... and the second V slot
+        mbar_wait(BAR(SH_V_EMPTY, st), (u & 1) ^ 1, s_err, WAIT_EMPTY);
+        mbar_expect_tx(BAR(SH_V_FULL, st), L::KV_BYTES);
         const uint32_t dst = smem_u32(base + L::OFF_V + st * L::KV_BYTES);
-        if (once) tma_load_3d_hint(dst, mv, 0, (int)(row0 + (tile0 + j) * 64), (int)(g * CH), BAR(V_FULL, st), l2_policy_evict_first());
-        else tma_load_3d(dst, mv, 0, (int)(row0 + (tile0 + j) * 64), (int)(g * CH), BAR(V_FULL, st));
+        if (un.once) tma_load_3d_hint(dst, un.mv, 0, (int)(un.row0 + (tile0 + j) * 64), (int)(g * CH), BAR(SH_V_FULL, st), l2_policy_evict_first());
+        else tma_load_3d(dst, un.mv, 0, (int)(un.row0 + (tile0 + j) * 64), (int)(g * CH), BAR(SH_V_FULL, st));
       }
     }
     __syncwarp();
-    if (ragged) {
-      const uint32_t j = n_tiles - 1, st = j % NV, from = n_rows - (tile0 + j) * 64;
-      mbar_wait(BAR(V_FULL, st), (j / NV) & 1, s_err, WAIT_VFULL);
+    if (un.ragged) {
+      const uint32_t j = n_tiles - 1, st = j % NV, from = un.n_rows - (tile0 + j) * 64;
+      mbar_wait(BAR(SH_V_FULL, st), (j / NV) & 1, s_err, WAIT_VFULL);
       for (uint32_t i = lane; i < (64 - from) * 8 * CH; i += 32) {
         const uint32_t c = i / ((64 - from) * 8), w = i % ((64 - from) * 8);
         *reinterpret_cast<uint4*>(base + L::OFF_V + st * L::KV_BYTES + c * (64 * 128) + from * 128 + w * 16) = make_uint4(0, 0, 0, 0);
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(BAR(V_CLEAN, 0));
+      if (lane == 0) mbar_arrive(BAR(SH_V_CLEAN, 0));
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer, scores ----
@@ -162,25 +126,31 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
 #pragma unroll
     for (int i = 0; i < NK; ++i) k_desc[i] = smem_desc(smem_u32(base + L::OFF_K + i * L::KV_BYTES), 16, 1024);
     const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024);
-    mbar_wait(BAR(Q_FULL, 0), 0, s_err, WAIT_QFULL);
+    mbar_wait(BAR(SH_Q_FULL, 0), 0, s_err, WAIT_QFULL);
     tc_fence_after();
     for (uint32_t j = 0; j < n_tiles; ++j) {
       const uint32_t sb = j % SB, st = j % NK;
-      if (j >= (uint32_t)SB) mbar_wait(BAR(PV_DONE, sb), ((j - SB) / SB) & 1, s_err, WAIT_MMA);
-      mbar_wait(BAR(K_FULL, st), (j / NK) & 1, s_err, WAIT_KFULL);
+      if (j >= (uint32_t)SB) mbar_wait(BAR(SH_PV_DONE, sb), ((j - SB) / SB) & 1, s_err, WAIT_MMA);
+      mbar_wait(BAR(SH_K_FULL, st), (j / NK) & 1, s_err, WAIT_KFULL);
       tc_fence_after();
       const uint64_t kd = st == 0 ? k_desc[0] : (st == 1 ? k_desc[1] : k_desc[2]);
       const uint32_t ts = t_s0 + sb * 64;
-      constexpr int TS_STEPS = L::TQC * 4;     // the dims whose Q chunks sit in tensor memory, then those from shared memory
+      auto k_at = [&](int ks) { return kd + (uint64_t)(((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4); };
+      auto q_at = [&](int ks) { return q_desc + (uint64_t)(((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4); };
+      constexpr int TS = T::TQC * 4;           // the dims whose Q chunks sit in tensor memory
 #pragma unroll
-      for (int ks = 0; ks < TS_STEPS; ++ks)
-        umma_f16_ts(leader, ts, t_q + ks * 8, kd + (uint64_t)(((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4), idesc_qk, ks > 0);
+      for (int ks = 0; ks < TS; ++ks) umma_f16_ts(leader, ts, t_q + ks * 8, k_at(ks), idesc_qk, ks > 0);
+      if constexpr (WIDE) {
+        if (!p.q_f16) {                        // the low parts, in shared memory
 #pragma unroll
-      for (int ks = TS_STEPS; ks < HD / 16; ++ks)
-        umma_f16_ss(leader, ts, q_desc + (uint64_t)((((ks - TS_STEPS) >> 2) * (128 * 128) + (ks & 3) * 32) >> 4),
-                    kd + (uint64_t)(((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4), idesc_qk, ks > 0 ? 1u : 0u);
-      umma_commit_elected(leader, BAR(K_EMPTY, st));
-      umma_commit_elected(leader, BAR(S_FULL, sb));
+          for (int ks = 0; ks < HD / 16; ++ks) umma_f16_ss(leader, ts, q_at(ks), k_at(ks), idesc_qk, 1u);
+        }
+      } else {
+#pragma unroll
+        for (int ks = TS; ks < HD / 16; ++ks) umma_f16_ss(leader, ts, q_at(ks - TS), k_at(ks), idesc_qk, ks > 0 ? 1u : 0u);
+      }
+      umma_commit_elected(leader, BAR(SH_K_EMPTY, st));
+      umma_commit_elected(leader, BAR(SH_S_FULL, sb));
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ MMA issuer, P V ----
@@ -191,133 +161,157 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
     for (int i = 0; i < NV; ++i) v_desc[i] = smem_desc(smem_u32(base + L::OFF_V + i * L::KV_BYTES), 64 * 128, 1024);
     for (uint32_t j = 0; j < n_tiles; ++j) {
       const uint32_t sb = j % SB, st = j % NV;
-      mbar_wait(BAR(P_FULL, sb), (j / SB) & 1, s_err, WAIT_QFULL);
-      mbar_wait(BAR(V_FULL, st), (j / NV) & 1, s_err, WAIT_VFULL);
-      if (ragged && j == n_tiles - 1) mbar_wait(BAR(V_CLEAN, 0), 0, s_err, WAIT_VFULL);
+      mbar_wait(BAR(SH_P_FULL, sb), (j / SB) & 1, s_err, WAIT_QFULL);
+      mbar_wait(BAR(SH_V_FULL, st), (j / NV) & 1, s_err, WAIT_VFULL);
+      if (un.ragged && j == n_tiles - 1) mbar_wait(BAR(SH_V_CLEAN, 0), 0, s_err, WAIT_VFULL);
       tc_fence_after();
       const uint64_t vd = st == 0 ? v_desc[0] : v_desc[1];
-      const uint32_t tp = t_s0 + sb * 64;      // P(j): packed f16 pairs in the first 32 columns of S(j)'s tile
+      const uint32_t tp = t_s0 + sb * 64;      // P(j): packed f16 pairs over S(j): 32 columns, wide: 32 of high and 32 of low parts
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-        umma_f16_ts(leader, t_o, tp + ks * 8, vd + (uint64_t)((ks * 2048) >> 4), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
-      umma_commit_elected(leader, BAR(V_EMPTY, st));
-      umma_commit_elected(leader, BAR(PV_DONE, sb));
+      for (int ks = 0; ks < (WIDE ? 8 : 4); ++ks)
+        umma_f16_ts(leader, t_o, tp + ks * 8, vd + (uint64_t)(((ks & 3) * 2048) >> 4), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
+      umma_commit_elected(leader, BAR(SH_V_EMPTY, st));
+      umma_commit_elected(leader, BAR(SH_PV_DONE, sb));
     }
-    umma_commit_elected(leader, BAR(O_DONE, 0));
+    umma_commit_elected(leader, BAR(SH_O_DONE, 0));
   } else {
     // ------------------------------------------------------------------ softmax + epilogue ----
+    float* s_rl = reinterpret_cast<float*>(base + L::OFF_K);     // [2][128] the groups' row sums, in the first K slot once the last tile's scores exist
     const uint32_t wg = (warp - 4) >> 2, qd = (warp - 4) & 3, row = qd * 32 + lane;
     const uint32_t lane_addr = (qd * 32) << 16;
-    const bool is_lo = (row & 1u) != 0, in_use = qd < live_warps;
-    const uint32_t lr = row >> 1;                      // query row: (item, head of the group)
-    const bool live = lr < pairs;
-    // the query rows come by cp.async into the K and the V slot that the producers leave alone until Q_READ, 32 rows each, a row's
-    // 16-byte chunks XOR-swizzled against the per-row reads
-    auto stage_row = [&](uint32_t pr) {
-      return (pr < 32 ? base + L::OFF_K + 2 * L::KV_BYTES : base + L::OFF_V + L::KV_BYTES) + (size_t)(pr & 31u) * (HD * 4);
-    };
-    const uint32_t q_es = p.q_f16 ? 2u : 4u, q_ch = HD * q_es / 16, st_tid = tid - 128;
-    for (uint32_t idx = st_tid; idx < pairs * q_ch; idx += 128 * GRP) {
-      const uint32_t pr = idx / q_ch, c = idx % q_ch;
-      const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
-                           ((uint64_t)(item0 + pr / p.G) * p.q_col_stride + (uint64_t)(g * p.G + pr % p.G) * p.q_head_stride) * q_es + (uint64_t)c * 16;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stage_row(pr) + ((c ^ (pr & 7u)) << 4))), "l"(src) : "memory");
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    named_bar_sync(1, 128 * GRP);
-    const uint8_t* my_stage = stage_row(lr);
-    auto stage_ld = [&](uint32_t c) { return *reinterpret_cast<const uint4*>(my_stage + ((c ^ (lr & 7u)) << 4)); };
-    // this thread's Q row as f16 pairs, 64 dims at a time (the groups share the chunks out): high or low parts
+    const bool is_lo = !WIDE && (row & 1u) != 0, in_use = qd < un.live_warps;
+    const uint32_t lr = WIDE ? row : row >> 1;         // query row: (item, head of the group)
+    const bool live = lr < un.pairs;
+    const uint32_t st_tid = tid - 128, G = p.G;
+    // The query rows come by cp.async into the K and the V slot that the producers leave alone until Q_READ, a row's 16-byte chunks
+    // XOR-swizzled against the per-row reads; in two rounds where they do not fit at once (wide, f32).
+    {
+      const uint32_t es = p.q_f16 ? 2u : 4u, cap = 128 / es, q_ch = HD * es / 16;
+      const uint32_t warp_lr = WIDE ? qd * 32 : qd * 16, my_round = warp_lr < un.pairs ? warp_lr / (2 * cap) : 0;
+      for (uint32_t r0 = 0, round = 0; r0 < un.pairs; r0 += 2 * cap, ++round) {
+        auto stage_row = [&](uint32_t r) { return base + (r < cap ? L::OFF_K + 2 * L::KV_BYTES : L::OFF_V + L::KV_BYTES) + (size_t)(r & (cap - 1)) * (HD * es); };
+        if (round) named_bar_sync(1, 128 * GRP);
+        const uint32_t n = min(un.pairs - r0, 2 * cap);
+        for (uint32_t idx = st_tid; idx < n * q_ch; idx += 128 * GRP) {
+          const uint32_t r = idx / q_ch, c = idx % q_ch, pr = r0 + r;
+          const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
+                               ((uint64_t)(un.item0 + pr / G) * p.q_col_stride + (uint64_t)(g * G + pr % G) * p.q_head_stride) * es + (uint64_t)c * 16;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stage_row(r) + ((c ^ (r & 7u)) << 4))), "l"(src) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        named_bar_sync(1, 128 * GRP);
+        if (round != my_round) continue;
+        const uint32_t mr = live ? lr - r0 : 0;
+        const uint8_t* my_stage = stage_row(mr);
+        auto stage_ld = [&](uint32_t c) { return live ? *reinterpret_cast<const uint4*>(my_stage + ((c ^ (mr & 7u)) << 4)) : make_uint4(0, 0, 0, 0); };
+        auto to_smem = [&](int c, const uint32_t (&w)[32]) {
+          uint8_t* dst = q_s + c * (128 * 128) + row * 128;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(dst + ((i ^ (row & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        };
+        // this thread's Q row as f16 pairs, 64 dims at a time (the groups share the chunks out)
 #pragma unroll 1
-    for (int c = 0; c < CH; ++c) {
-      if (CH >= 2 ? (uint32_t)(c >= CH / 2) != wg : wg != 0) continue;
-      uint32_t w[32];
-      if (p.q_f16) {
+        for (int c = 0; c < CH; ++c) {
+          if (CH >= 2 ? (uint32_t)(c >= CH / 2) != wg : wg != 0) continue;
+          uint32_t w[32], lo[32];
+          if (p.q_f16) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint4 x = live && !is_lo ? stage_ld(c * 8 + i) : make_uint4(0, 0, 0, 0);      // f16 queries have no low part
-          w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
-        }
-      } else {
+            for (int i = 0; i < 8; ++i) {
+              const uint4 x = is_lo ? make_uint4(0, 0, 0, 0) : stage_ld(c * 8 + i);       // f16 queries have no low part
+              w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+            }
+          } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint4 r4 = live ? stage_ld(c * 16 + i) : make_uint4(0, 0, 0, 0);
-          float4 x = *reinterpret_cast<const float4*>(&r4);
-          if (is_lo) {
-            x.x -= __half2float(__float2half_rn(x.x)); x.y -= __half2float(__float2half_rn(x.y));
-            x.z -= __half2float(__float2half_rn(x.z)); x.w -= __half2float(__float2half_rn(x.w));
+            for (int i = 0; i < 16; ++i) {
+              const uint4 r4 = stage_ld(c * 16 + i);
+              const float4 x = *reinterpret_cast<const float4*>(&r4);
+              float4 y;                                                                   // what the high part leaves over
+              y.x = x.x - __half2float(__float2half_rn(x.x)); y.y = x.y - __half2float(__float2half_rn(x.y));
+              y.z = x.z - __half2float(__float2half_rn(x.z)); y.w = x.w - __half2float(__float2half_rn(x.w));
+              if (WIDE) { lo[2 * i] = pack_h2(y.x, y.y); lo[2 * i + 1] = pack_h2(y.z, y.w); }
+              w[2 * i] = is_lo ? pack_h2(y.x, y.y) : pack_h2(x.x, x.y); w[2 * i + 1] = is_lo ? pack_h2(y.z, y.w) : pack_h2(x.z, x.w);
+            }
           }
-          w[2 * i] = pack_h2(x.x, x.y); w[2 * i + 1] = pack_h2(x.z, x.w);
+          if (c < T::TQC) tmem_st32u(t_q + c * 32 + lane_addr, w);
+          else to_smem(c - T::TQC, w);
+          if (WIDE && !p.q_f16) to_smem(c, lo);
         }
-      }
-      if (c < L::TQC) {
-        tmem_st32u(t_q + c * 32 + lane_addr, w);
-      } else {
-        uint8_t* dst = q_s + (c - L::TQC) * (128 * 128) + row * 128;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(dst + ((i ^ (row & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       }
     }
     fence_proxy_async();
-    mbar_arrive(BAR(Q_READ, 0));
+    mbar_arrive(BAR(SH_Q_READ, 0));
     tmem_wait_st();
     tc_fence_before();
-    mbar_arrive(BAR(Q_FULL, 0));
+    mbar_arrive(BAR(SH_Q_FULL, 0));
 
-    float m_st = -1.0e30f, l_sum = 0.f, m_l = m_st;
-    float* sc = nullptr;                                  // where this lane's half of its row's scores goes
-    if (p.scores && !shared && live)
-      sc = p.scores + p.score0[item0] + ((uint64_t)g * p.G + lr) * ((n_rows + 63) & ~63u) + tile0 * 64 + (is_lo ? 32 : 0);
+    // Both groups work on the same tile: of this lane's row the 32 keys of its group (narrow: shared with the row's other lane, 16 each).
+    constexpr int NS = WIDE ? 32 : 16;
+    const uint32_t mine = wg * 32 + (is_lo ? 16 : 0);     // this lane's first key of a tile
+    float m_st = -1.0e30f, l_sum = 0.f;
+    float* sc = nullptr;                                  // where the scores of this lane's keys go
+    if (!WIDE && p.scores && !un.shared && live) sc = p.scores + p.score0[un.item0] + ((uint64_t)g * G + lr) * ((un.n_rows + 63) & ~63u) + tile0 * 64 + mine;
+    // the maximum of a row over both groups, whose warps of the same rows meet at a barrier of their own.  Narrow: two buffers in turn;
+    // wide, where 64 KB of low parts leave room for one: the first group decides
+    float* s_max = reinterpret_cast<float*>(base + (WIDE ? L::OFF_MAX : L::OFF_MAX2));
+    auto row_max = [&](float m, uint32_t j) {
+      tc_fence_before();                                  // this warp's scores have been read: the other's weights may take their place
+      if constexpr (WIDE) {
+        if (wg) s_max[row] = m;
+        named_bar_sync(3 + qd, 64);
+        if (!wg) { m = fmaxf(m, s_max[row]); s_max[128 + row] = m; }
+        named_bar_sync(3 + qd, 64);
+        if (wg) m = s_max[128 + row];
+      } else {
+        float* at = s_max + (j & 1) * 256 + row;
+        at[wg * 128] = m;
+        named_bar_sync(3 + qd, 64);
+        m = fmaxf(m, at[(wg ^ 1) * 128]);
+      }
+      tc_fence_after();
+      return m;
+    };
     if (in_use) {
-      for (uint32_t j = wg; j < n_tiles; j += GRP) {
+      for (uint32_t j = 0; j < n_tiles; ++j) {
         const uint32_t b = j % SB, u = j / SB, kv0 = (tile0 + j) * 64;
-        mbar_wait(BAR(S_FULL, b), u & 1, s_err, WAIT_MMA);
+        mbar_wait(BAR(SH_S_FULL, b), u & 1, s_err, WAIT_MMA);
         tc_fence_after();
-        // the two lanes of a query row share its keys out, 32 each: a lane sends the other's half of its own row (high or low
-        // parts) and adds what comes back to its half
-        float s[32];
-        {
-          float t[64];
-          tmem_ld32_async(t_s0 + b * 64 + lane_addr, t);
-          tmem_ld32_async(t_s0 + b * 64 + 32 + lane_addr, t + 32);
-          tmem_wait_ld(t);
+        float s[NS];
+        if constexpr (WIDE) {
+          tmem_ld32(t_s0 + b * 64 + wg * 32 + lane_addr, s);
+        } else {
+          // a lane sends the half of its row (high or low parts) that the other lane has the keys of, and adds what comes back to its own
+          float t[32];
+          tmem_ld32(t_s0 + b * 64 + wg * 32 + lane_addr, t);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float give = is_lo ? t[i] : t[32 + i], keep = is_lo ? t[32 + i] : t[i];
+          for (int i = 0; i < 16; ++i) {
+            const float give = is_lo ? t[i] : t[16 + i], keep = is_lo ? t[16 + i] : t[i];
             s[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
           }
         }
-        const uint32_t key0 = kv0 + (is_lo ? 32 : 0);
-        if (sc) {
+        if (!WIDE && sc) {
           float4* d = reinterpret_cast<float4*>(sc + j * 64);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+          for (int i = 0; i < 4; ++i) d[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
         }
-        if (kv0 + 64 > n_rows) {
+        if (kv0 + 64 > un.n_rows) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) if (key0 + i >= n_rows) s[i] = -INFINITY;
+          for (int i = 0; i < NS; ++i) if (kv0 + mine + i >= un.n_rows) s[i] = -INFINITY;
         }
         float mt = s[0];
 #pragma unroll
-        for (int i = 1; i < 32; ++i) mt = fmaxf(mt, s[i]);
-        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1)) * p.scale_log2;
-        if (j > 0) {
-          mbar_wait(BAR(M_READY, (j - 1) & 1), ((j - 1) >> 1) & 1, s_err, WAIT_MMA);
-          m_st = s_rm[row];
-        }
+        for (int i = 1; i < NS; ++i) mt = fmaxf(mt, s[i]);
+        if (!WIDE) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+        mt = row_max(mt, j) * p.scale_log2;
         float alpha = 1.f;
         bool grow = false;
-        if (mt > m_st + 15.f) { alpha = ex2_approx(m_st - (mt - 7.f)); m_st = mt - 7.f; grow = true; }
-        s_rm[row] = m_st;
-        mbar_arrive(BAR(M_READY, j & 1));
-        if (m_st != m_l) { l_sum *= ex2_approx(m_l - m_st); m_l = m_st; }
+        if (mt > m_st + 15.f) { alpha = ex2_approx(m_st - (mt - 7.f)); m_st = mt - 7.f; l_sum *= alpha; grow = true; }
         if (j > 0 && __any_sync(0xffffffffu, grow)) {
           const uint32_t jb = (j - 1) % SB, ju = (j - 1) / SB;
-          mbar_wait(BAR(PV_DONE, jb), ju & 1, s_err, WAIT_MMA);
+          mbar_wait(BAR(SH_PV_DONE, jb), ju & 1, s_err, WAIT_MMA);
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
+          for (int c = wg; c < HD / 32; c += GRP) {       // the groups share the columns out
             float o[32];
             tmem_ld32(t_o + c * 32 + lane_addr, o);
 #pragma unroll
@@ -325,68 +319,136 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
             tmem_st32(t_o + c * 32 + lane_addr, o);
           }
         }
-        // weights of this lane's keys as f16 pairs, high and low parts; the even lane's row takes the high parts of all 64 keys, the odd one's the low parts
-        uint32_t pw[32];
-        float ls = 0.f;
+        // weights as f16 pairs, high and low parts
+        uint32_t hi[NS / 2], lo[NS / 2];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < NS / 2; ++i) {
           const float e0 = ex2_approx(fmaf(s[2 * i], p.scale_log2, -m_st)), e1 = ex2_approx(fmaf(s[2 * i + 1], p.scale_log2, -m_st));
-          ls += e0 + e1;
+          l_sum += e0 + e1;
           const __half2 h = __floats2half2_rn(e0, e1);
           const float2 f = __half22float2(h);
-          const uint32_t hi = *reinterpret_cast<const uint32_t*>(&h), lo = pack_h2(e0 - f.x, e1 - f.y);
-          const uint32_t got = __shfl_xor_sync(0xffffffffu, is_lo ? hi : lo, 1);
-          pw[i] = is_lo ? got : hi;
-          pw[16 + i] = is_lo ? lo : got;
+          hi[i] = *reinterpret_cast<const uint32_t*>(&h); lo[i] = pack_h2(e0 - f.x, e1 - f.y);
         }
-        l_sum += ls;
-        tmem_st32u(t_s0 + b * 64 + lane_addr, pw);
+        if constexpr (WIDE) {
+          tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, hi);
+          tmem_st16u(t_s0 + b * 64 + 32 + 16 * wg + lane_addr, lo);
+        } else {
+          // the even lane's row takes the high parts of the group's 32 keys, the odd one's the low parts
+          uint32_t pw[16];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, is_lo ? hi[i] : lo[i], 1);
+            pw[i] = is_lo ? got : hi[i];
+            pw[8 + i] = is_lo ? lo[i] : got;
+          }
+          tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, pw);
+        }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(BAR(P_FULL, b));
+        mbar_arrive(BAR(SH_P_FULL, b));
       }
-      // the row sum: the two groups' shares brought to the final reference
-      mbar_wait(BAR(M_READY, (n_tiles - 1) & 1), ((n_tiles - 1) >> 1) & 1, s_err, WAIT_MMA);    // published after the last scores: the K ring is idle
-      l_sum += __shfl_xor_sync(0xffffffffu, l_sum, 1);
-      s_rl[wg * 128 + row] = l_sum; s_rr[wg * 128 + row] = m_l;
+      if (!WIDE) l_sum += __shfl_xor_sync(0xffffffffu, l_sum, 1);
+      s_rl[wg * 128 + row] = l_sum;
     }
     named_bar_sync(2, 128 * GRP);
-    mbar_wait(BAR(O_DONE, 0), 0, s_err, WAIT_MMA);
+    mbar_wait(BAR(SH_O_DONE, 0), 0, s_err, WAIT_MMA);
     tc_fence_after();
     // ---- the records: rows to shared memory (every product has retired), whole records from there ----
     constexpr int RP = HD / 4 + 1;                       // row pitch in float4
     float4* xs = reinterpret_cast<float4*>(base + 2048);
-    const uint32_t s_idx = shared ? split : p.p_splits + split;
-    auto slot_of = [&](uint32_t pr) { return ((uint64_t)(item0 + pr / p.G) * p.n_heads + g * p.G + pr % p.G) * p.n_rec + s_idx; };
+    auto slot_of = [&](uint32_t pr) { return ((uint64_t)(un.item0 + pr / G) * p.n_heads + g * G + pr % G) * p.n_rec + un.slot; };
     if (in_use) {
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         if ((uint32_t)(c & 1) != wg) continue;           // the groups share the columns out
         float o[32];
         tmem_ld32(t_o + c * 32 + lane_addr, o);
+        if (!WIDE) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], 1);
+          for (int i = 0; i < 32; ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], 1);
+        }
         if (live && !is_lo) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) xs[lr * RP + c * 8 + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
-      if (live && !is_lo && wg == 0) {
-        const float m = s_rm[row], l = s_rl[row] * ex2_approx(s_rr[row] - m) + s_rl[128 + row] * ex2_approx(s_rr[128 + row] - m);
-        reinterpret_cast<float2*>(p.part_ml)[slot_of(lr)] = make_float2(m, l);
-      }
+      if (live && !is_lo && wg == 0) reinterpret_cast<float2*>(p.part_ml)[slot_of(lr)] = make_float2(m_st, s_rl[row] + s_rl[128 + row]);
     }
     named_bar_sync(1, 128 * GRP);
-    for (uint32_t idx = st_tid; idx < pairs * (HD / 4); idx += 128 * GRP) {
+    for (uint32_t idx = st_tid; idx < un.pairs * (HD / 4); idx += 128 * GRP) {
       const uint32_t rr = idx / (HD / 4), c4 = idx % (HD / 4);
       reinterpret_cast<float4*>(p.part_o + slot_of(rr) * HD)[c4] = xs[rr * RP + c4];
     }
     tc_fence_before();
   }
+}
+
+// grid (units, kv heads): the shared rows' units first.  MIXED: they are wide (an instantiation of its own: calls without wide
+// units run a kernel of half the code, most of whose time at short rows is fetching it)
+template <int HD, bool MIXED>
+__global__ void __launch_bounds__(384, 1)
+pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv, const __grid_constant__ CUtensorMap tm_k,
+                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedParams p) {
+  using L = ShSmem<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + L::OFF_BAR);
+  volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(bars + 31);
+  volatile uint32_t* s_err = s_tmem + 1;
+  const uint32_t bar0 = smem_u32(bars);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t unit = blockIdx.x;
+  ShUnit un;
+  un.shared = unit < p.p_splits * p.row_tiles;
+  uint32_t split, n_q, tps;
+  if (un.shared) {
+    split = unit / p.row_tiles;
+    un.item0 = (unit % p.row_tiles) * p.items_per_tile;
+    n_q = min(p.items_per_tile, p.n_items - un.item0);
+    un.row0 = p.p_row0; un.n_rows = p.p_rows; tps = p.p_tps; un.slot = split;
+    un.mk = &tm_pk; un.mv = &tm_pv;
+  } else {
+    uint32_t lo = 0, hi = p.n_items - 1;
+    while (lo < hi) { const uint32_t mid = (lo + hi + 1) / 2; if (unit >= p.cta0[mid]) lo = mid; else hi = mid - 1; }
+    un.item0 = lo; n_q = 1; split = unit - p.cta0[lo];
+    un.row0 = p.seq[lo] * p.max_seq + p.own_row0; un.n_rows = p.rows[lo]; tps = p.tps; un.slot = p.p_splits + split;
+    un.mk = &tm_k; un.mv = &tm_v;
+  }
+  un.once = !un.shared || p.row_tiles == 1;
+  un.tile0 = split * tps;
+  un.n_tiles = min((un.n_rows + 63) / 64, un.tile0 + tps) - un.tile0;
+  un.pairs = n_q * p.G;
+  const bool wide = MIXED && un.shared;
+  un.live_warps = ((wide ? 1 : 2) * un.pairs + 31) / 32;
+  un.ragged = (un.tile0 + un.n_tiles) * 64 > un.n_rows;
+
+  if (warp == 1 && lane == 0) {
+    *s_err = 0;
+    auto init = [&](int which, int n, uint32_t count) { for (int i = 0; i < n; ++i) mbar_init(bar0 + 8u * (uint32_t)(which + i), count); };
+    init(SH_K_FULL, 3, 1); init(SH_K_EMPTY, 3, 1); init(SH_V_FULL, 2, 1); init(SH_V_EMPTY, 2, 1);
+    init(SH_S_FULL, 3, 1); init(SH_P_FULL, 3, 64 * un.live_warps); init(SH_PV_DONE, 3, 1);
+    init(SH_O_DONE, 1, 1); init(SH_Q_FULL, 1, 256); init(SH_Q_READ, 1, 256); init(SH_V_CLEAN, 1, 1);
+    fence_barrier_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(smem_u32((const void*)s_tmem), sh_tmem_cols<HD>());
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  if (warp == 0 && lane == 0) { prefetch_tmap(un.mk); prefetch_tmap(un.mv); }
+  pdl_wait();
+  pdl_trigger();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  if constexpr (MIXED) {
+    if (wide) shared_roles<HD, true>(p, un, base, bar0, s_err, tmem);
+  }
+  if (!wide) shared_roles<HD, false>(p, un, base, bar0, s_err, tmem);
   __syncthreads();
   if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc(tmem, L::TMEM_COLS);
+    tmem_dealloc(tmem, sh_tmem_cols<HD>());
   }
   if (tid == 0 && *s_err) atomicMax(p.err, *s_err);
 }
@@ -525,23 +587,24 @@ __global__ void __launch_bounds__(256, 2) pa_shared_finish_kernel(const __grid_c
   }
 }
 
-template <int HD>
+template <int HD, bool MIXED>
 static cudaError_t launch_shared_t(const SharedParams& p, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v, uint32_t n_kv,
                                    int dev, cudaStream_t st) {
   using S = ShSmem<HD>;
   static std::atomic<bool> attr_set[64];
   if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(pa_shared_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
+    cudaError_t e = cudaFuncSetAttribute(pa_shared_kernel<HD, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::total(MIXED));
     if (e != cudaSuccess) return e;
     attr_set[dev & 63].store(true, std::memory_order_release);
   }
-  return launch_pdl(pa_shared_kernel<HD>, dim3(p.units, n_kv), dim3(S::THREADS), (size_t)S::TOTAL, st, pk, pv, k, v, p);
+  return launch_pdl(pa_shared_kernel<HD, MIXED>, dim3(p.units, n_kv), dim3(S::THREADS), (size_t)S::total(MIXED && !p.q_f16), st, pk, pv, k, v, p);
 }
 cudaError_t launch_shared(const SharedParams& p, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v, uint32_t hd, uint32_t n_kv,
                           int dev, cudaStream_t st) {
-  if (hd == 256) return launch_shared_t<256>(p, pk, pv, k, v, n_kv, dev, st);
-  if (hd == 128) return launch_shared_t<128>(p, pk, pv, k, v, n_kv, dev, st);
-  if (hd == 64) return launch_shared_t<64>(p, pk, pv, k, v, n_kv, dev, st);
+  const bool mixed = p.wide && p.p_splits;
+  if (hd == 256) return mixed ? launch_shared_t<256, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<256, false>(p, pk, pv, k, v, n_kv, dev, st);
+  if (hd == 128) return mixed ? launch_shared_t<128, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<128, false>(p, pk, pv, k, v, n_kv, dev, st);
+  if (hd == 64) return mixed ? launch_shared_t<64, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<64, false>(p, pk, pv, k, v, n_kv, dev, st);
   return cudaErrorInvalidValue;
 }
 cudaError_t launch_shared_finish(const SharedFinishParams& p, uint32_t hd, uint32_t sum_ctas, cudaStream_t st) {
