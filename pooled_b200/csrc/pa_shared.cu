@@ -20,13 +20,14 @@
 //               maximum, a long row's error was 2.2e-6 of the result, 3e-7 now).  Warps whose rows hold no query take no part.
 // q and the weights enter as pairs of f16 values, high and low parts, some 22 bits of both, in one of two ways:
 //   narrow (up to 64 query rows)   even rows of the 128 carry the high parts, odd rows the low parts of the same query row, added by
-//               shuffles: both products at the cost of one, 1394 cycles for 64 keys at head_dim 256.  The two lanes share the
-//               row's keys out
-//   wide (shared rows of more)     128 query rows; the products of the low parts are issued after those of the high ones into the same
-//               accumulators (none of q's where q is f16): 1906 cycles with f16 queries, 2788 with f32 ones, and half the bytes
-//               through L2, which at 64 KB a tile and 0.87 us fed narrow tiles no faster
-// What bounds it: one query tile per kv head, HBM; several, the tensor cores; short calls the chain of launch, q, scores,
-// weights, products and records, 6.5 us.
+//               shuffles: both products at the cost of one, and the two lanes share the row's keys out.  0.75 us a tile of 64 keys
+//               at head_dim 256 (the tensor cores: 1394 cycles), 0.67 at 128 and 64 (the softmax)
+//   wide (shared rows of more, f16 queries, where plan_shared finds it faster)   128 query rows without low parts of q; the low parts
+//               of the weights are multiplied behind the high ones into the same accumulator.  1.17 us a tile at head_dim 256, 0.64 at 128,
+//               and a start 5 us longer.  (With f32 queries and the products of their low parts: 1.43 us and 13 us of start, slower than two
+//               narrow tiles at every size tried.)
+// What bounds it: HBM, one query tile per kv head and long rows; the tensor cores, several; short calls the chain of launch, q,
+// scores, weights, products and records, and fetching the code for it: without wide units a kernel of half the code runs.
 #include <algorithm>
 
 #include "pa_tc.cuh"
@@ -39,11 +40,10 @@ struct ShSmem {
   static constexpr int KV_BYTES = HD * 128;          // [HD/64][64 rows][128 B]
   static constexpr int THREADS = 384;
   static constexpr int OFF_K = 0, OFF_V = NK * KV_BYTES, OFF_BAR = (NK + NV) * KV_BYTES;
-  static constexpr int OFF_MAX = OFF_BAR + 256;      // wide: [2][128] maxima of the rows
-  static constexpr int OFF_Q = OFF_BAR + 2048;       // narrow: the chunks of Q that are not in tensor memory; wide: the low parts
-  static constexpr int OFF_MAX2 = OFF_Q + (HD / 64 - HD / 128) * 128 * 128;     // narrow: [2][2][128] maxima of the rows, two tiles in turn
-  static constexpr int total(bool wide_lo) { return 1024 + std::max(OFF_MAX2 + 2048, wide_lo ? OFF_Q + HD / 64 * 128 * 128 : 0); }
-  static_assert(total(true) <= 227 * 1024, "shared memory of one CTA");
+  static constexpr int OFF_MAX = OFF_BAR + 256;      // [2][2][128] maxima of the rows, two tiles in turn
+  static constexpr int OFF_Q = OFF_BAR + 4096;       // narrow: the chunks of Q that are not in tensor memory
+  static constexpr int TOTAL = 1024 + OFF_Q + (HD / 64 - HD / 128) * 128 * 128;
+  static_assert(TOTAL <= 227 * 1024, "shared memory of one CTA");
   // the records leave through the rings: row sums of the groups, then 64 (in the K ring) or 128 rows of HD + 4 floats
   static_assert(2048 + 64 * (HD + 4) * 4 <= NK * KV_BYTES && 2048 + 128 * (HD + 4) * 4 <= (NK + NV) * KV_BYTES, "staging of the records");
 };
@@ -75,7 +75,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
   using T = ShLay<HD, WIDE>;
   constexpr int CH = HD / 64, NK = L::NK, NV = L::NV, SB = T::SB, GRP = 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t g = blockIdx.y, n_tiles = un.n_tiles, tile0 = un.tile0;
+  const uint32_t g = blockIdx.x, n_tiles = un.n_tiles, tile0 = un.tile0;
   auto BAR = [&](int which, int idx) { return bar0 + 8u * (uint32_t)(which + idx); };
   uint8_t* q_s = base + L::OFF_Q;
   const uint32_t t_q = tmem, t_s0 = tmem + T::T_S, t_o = tmem + T::T_O;
@@ -140,15 +140,8 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       constexpr int TS = T::TQC * 4;           // the dims whose Q chunks sit in tensor memory
 #pragma unroll
       for (int ks = 0; ks < TS; ++ks) umma_f16_ts(leader, ts, t_q + ks * 8, k_at(ks), idesc_qk, ks > 0);
-      if constexpr (WIDE) {
-        if (!p.q_f16) {                        // the low parts, in shared memory
 #pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) umma_f16_ss(leader, ts, q_at(ks), k_at(ks), idesc_qk, 1u);
-        }
-      } else {
-#pragma unroll
-        for (int ks = TS; ks < HD / 16; ++ks) umma_f16_ss(leader, ts, q_at(ks - TS), k_at(ks), idesc_qk, ks > 0 ? 1u : 0u);
-      }
+      for (int ks = TS; ks < HD / 16; ++ks) umma_f16_ss(leader, ts, q_at(ks - TS), k_at(ks), idesc_qk, ks > 0 ? 1u : 0u);
       umma_commit_elected(leader, BAR(SH_K_EMPTY, st));
       umma_commit_elected(leader, BAR(SH_S_FULL, sb));
     }
@@ -183,59 +176,51 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
     const uint32_t lr = WIDE ? row : row >> 1;         // query row: (item, head of the group)
     const bool live = lr < un.pairs;
     const uint32_t st_tid = tid - 128, G = p.G;
-    // The query rows come by cp.async into the K and the V slot that the producers leave alone until Q_READ, a row's 16-byte chunks
-    // XOR-swizzled against the per-row reads; in two rounds where they do not fit at once (wide, f32).
+    // The query rows come by cp.async into the K and the V slot that the producers leave alone until Q_READ, half of them each, a
+    // row's 16-byte chunks XOR-swizzled against the per-row reads.
     {
-      const uint32_t es = p.q_f16 ? 2u : 4u, cap = 128 / es, q_ch = HD * es / 16;
-      const uint32_t warp_lr = WIDE ? qd * 32 : qd * 16, my_round = warp_lr < un.pairs ? warp_lr / (2 * cap) : 0;
-      for (uint32_t r0 = 0, round = 0; r0 < un.pairs; r0 += 2 * cap, ++round) {
-        auto stage_row = [&](uint32_t r) { return base + (r < cap ? L::OFF_K + 2 * L::KV_BYTES : L::OFF_V + L::KV_BYTES) + (size_t)(r & (cap - 1)) * (HD * es); };
-        if (round) named_bar_sync(1, 128 * GRP);
-        const uint32_t n = min(un.pairs - r0, 2 * cap);
-        for (uint32_t idx = st_tid; idx < n * q_ch; idx += 128 * GRP) {
-          const uint32_t r = idx / q_ch, c = idx % q_ch, pr = r0 + r;
-          const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
-                               ((uint64_t)(un.item0 + pr / G) * p.q_col_stride + (uint64_t)(g * G + pr % G) * p.q_head_stride) * es + (uint64_t)c * 16;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stage_row(r) + ((c ^ (r & 7u)) << 4))), "l"(src) : "memory");
+      const uint32_t es = WIDE || p.q_f16 ? 2u : 4u, cap = 128 / es, q_ch = HD * es / 16;
+      auto stage_row = [&](uint32_t r) { return base + (r < cap ? L::OFF_K + 2 * L::KV_BYTES : L::OFF_V + L::KV_BYTES) + (size_t)(r & (cap - 1)) * (HD * es); };
+      for (uint32_t idx = st_tid; idx < un.pairs * q_ch; idx += 128 * GRP) {
+        const uint32_t pr = idx / q_ch, c = idx % q_ch;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
+                             ((uint64_t)(un.item0 + pr / G) * p.q_col_stride + (uint64_t)(g * G + pr % G) * p.q_head_stride) * es + (uint64_t)c * 16;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stage_row(pr) + ((c ^ (pr & 7u)) << 4))), "l"(src) : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      named_bar_sync(1, 128 * GRP);
+      const uint8_t* my_stage = stage_row(lr);
+      auto stage_ld = [&](uint32_t c) { return live ? *reinterpret_cast<const uint4*>(my_stage + ((c ^ (lr & 7u)) << 4)) : make_uint4(0, 0, 0, 0); };
+      // this thread's Q row as f16 pairs, 64 dims at a time (the groups share the chunks out)
+#pragma unroll 1
+      for (int c = 0; c < CH; ++c) {
+        if (CH >= 2 ? (uint32_t)(c >= CH / 2) != wg : wg != 0) continue;
+        uint32_t w[32];
+        if (WIDE || p.q_f16) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint4 x = is_lo ? make_uint4(0, 0, 0, 0) : stage_ld(c * 8 + i);         // f16 queries have no low part
+            w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint4 r4 = stage_ld(c * 16 + i);
+            float4 x = *reinterpret_cast<const float4*>(&r4);
+            if (is_lo) {                                                                  // what the high part leaves over
+              x.x -= __half2float(__float2half_rn(x.x)); x.y -= __half2float(__float2half_rn(x.y));
+              x.z -= __half2float(__float2half_rn(x.z)); x.w -= __half2float(__float2half_rn(x.w));
+            }
+            w[2 * i] = pack_h2(x.x, x.y); w[2 * i + 1] = pack_h2(x.z, x.w);
+          }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        named_bar_sync(1, 128 * GRP);
-        if (round != my_round) continue;
-        const uint32_t mr = live ? lr - r0 : 0;
-        const uint8_t* my_stage = stage_row(mr);
-        auto stage_ld = [&](uint32_t c) { return live ? *reinterpret_cast<const uint4*>(my_stage + ((c ^ (mr & 7u)) << 4)) : make_uint4(0, 0, 0, 0); };
-        auto to_smem = [&](int c, const uint32_t (&w)[32]) {
-          uint8_t* dst = q_s + c * (128 * 128) + row * 128;
+        if (c < T::TQC) {
+          tmem_st32u(t_q + c * 32 + lane_addr, w);
+        } else {
+          uint8_t* dst = q_s + (c - T::TQC) * (128 * 128) + row * 128;
 #pragma unroll
           for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(dst + ((i ^ (row & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        };
-        // this thread's Q row as f16 pairs, 64 dims at a time (the groups share the chunks out)
-#pragma unroll 1
-        for (int c = 0; c < CH; ++c) {
-          if (CH >= 2 ? (uint32_t)(c >= CH / 2) != wg : wg != 0) continue;
-          uint32_t w[32], lo[32];
-          if (p.q_f16) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint4 x = is_lo ? make_uint4(0, 0, 0, 0) : stage_ld(c * 8 + i);       // f16 queries have no low part
-              w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const uint4 r4 = stage_ld(c * 16 + i);
-              const float4 x = *reinterpret_cast<const float4*>(&r4);
-              float4 y;                                                                   // what the high part leaves over
-              y.x = x.x - __half2float(__float2half_rn(x.x)); y.y = x.y - __half2float(__float2half_rn(x.y));
-              y.z = x.z - __half2float(__float2half_rn(x.z)); y.w = x.w - __half2float(__float2half_rn(x.w));
-              if (WIDE) { lo[2 * i] = pack_h2(y.x, y.y); lo[2 * i + 1] = pack_h2(y.z, y.w); }
-              w[2 * i] = is_lo ? pack_h2(y.x, y.y) : pack_h2(x.x, x.y); w[2 * i + 1] = is_lo ? pack_h2(y.z, y.w) : pack_h2(x.z, x.w);
-            }
-          }
-          if (c < T::TQC) tmem_st32u(t_q + c * 32 + lane_addr, w);
-          else to_smem(c - T::TQC, w);
-          if (WIDE && !p.q_f16) to_smem(c, lo);
         }
       }
     }
@@ -251,25 +236,15 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
     float m_st = -1.0e30f, l_sum = 0.f;
     float* sc = nullptr;                                  // where the scores of this lane's keys go
     if (!WIDE && p.scores && !un.shared && live) sc = p.scores + p.score0[un.item0] + ((uint64_t)g * G + lr) * ((un.n_rows + 63) & ~63u) + tile0 * 64 + mine;
-    // the maximum of a row over both groups, whose warps of the same rows meet at a barrier of their own.  Narrow: two buffers in turn;
-    // wide, where 64 KB of low parts leave room for one: the first group decides
-    float* s_max = reinterpret_cast<float*>(base + (WIDE ? L::OFF_MAX : L::OFF_MAX2));
+    // the maximum of a row over both groups, whose warps of the same rows meet at a barrier of their own; two buffers in turn
+    float* s_max = reinterpret_cast<float*>(base + L::OFF_MAX);
     auto row_max = [&](float m, uint32_t j) {
       tc_fence_before();                                  // this warp's scores have been read: the other's weights may take their place
-      if constexpr (WIDE) {
-        if (wg) s_max[row] = m;
-        named_bar_sync(3 + qd, 64);
-        if (!wg) { m = fmaxf(m, s_max[row]); s_max[128 + row] = m; }
-        named_bar_sync(3 + qd, 64);
-        if (wg) m = s_max[128 + row];
-      } else {
-        float* at = s_max + (j & 1) * 256 + row;
-        at[wg * 128] = m;
-        named_bar_sync(3 + qd, 64);
-        m = fmaxf(m, at[(wg ^ 1) * 128]);
-      }
+      float* at = s_max + (j & 1) * 256 + row;
+      at[wg * 128] = m;
+      named_bar_sync(3 + qd, 64);
       tc_fence_after();
-      return m;
+      return fmaxf(m, at[(wg ^ 1) * 128]);
     };
     if (in_use) {
       for (uint32_t j = 0; j < n_tiles; ++j) {
@@ -383,7 +358,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
   }
 }
 
-// grid (units, kv heads): the shared rows' units first.  MIXED: they are wide (an instantiation of its own: calls without wide
+// grid (kv heads, units): the shared rows' units of all heads first.  MIXED: they are wide (an instantiation of its own: calls without wide
 // units run a kernel of half the code, most of whose time at short rows is fetching it)
 template <int HD, bool MIXED>
 __global__ void __launch_bounds__(384, 1)
@@ -397,7 +372,7 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
   volatile uint32_t* s_err = s_tmem + 1;
   const uint32_t bar0 = smem_u32(bars);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t unit = blockIdx.x;
+  const uint32_t unit = blockIdx.y;
   ShUnit un;
   un.shared = unit < p.p_splits * p.row_tiles;
   uint32_t split, n_q, tps;
@@ -461,8 +436,8 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
 // The others: kSumRows rows of a sequence and kv head; the final (m, l) of the group's heads from their records while the
 // scores are on their way, then per row sum_h 2^(s_h - m_h) / l_h, added to the row's sum: four threads a row, each with
 // every fourth head, then the four in order, item after item.
-template <int HD>
-__global__ void __launch_bounds__(256, 2) pa_shared_finish_kernel(const __grid_constant__ SharedFinishParams p) {
+template <int HD, bool SUMS>
+__global__ void __launch_bounds__(256, SUMS ? 3 : 4) pa_shared_finish_kernel(const __grid_constant__ SharedFinishParams p) {
   __shared__ float4 s_acc[256];
   __shared__ float s_m[64], s_il[64];
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -484,12 +459,12 @@ __global__ void __launch_bounds__(256, 2) pa_shared_finish_kernel(const __grid_c
   };
   pdl_wait();
   pdl_trigger();
-  if (blockIdx.x < p.merge_ctas) {
+  if (!SUMS || blockIdx.x < p.merge_ctas) {
     const uint32_t slices = HD / 4 / p.lanes, prow = blockIdx.x / slices, slice = blockIdx.x % slices, item = prow / p.n_heads, h = prow % p.n_heads;
     const uint32_t ns = p.p_splits + p.n_own[item], groups = 256 / p.lanes, grp = tid / p.lanes, ln = tid % p.lanes, dims = p.lanes * 4, d = slice * dims + tid;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + (uint64_t)prow * p.n_rec;
     const float* ob = p.part_o + (uint64_t)prow * p.n_rec * HD + slice * dims + ln * 4;
-    constexpr int U = 8;
+    constexpr int U = 4;      // (eight: two CTAs an SM, a second wave for 512 rows)
     float4 x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -531,6 +506,7 @@ __global__ void __launch_bounds__(256, 2) pa_shared_finish_kernel(const __grid_c
     }
     return;
   }
+  if constexpr (SUMS) {
   // ---- sums of the weights ----
   const uint32_t u0 = blockIdx.x - p.merge_ctas;
   uint32_t lo = 0, hi = p.n_leads - 1;
@@ -585,6 +561,7 @@ __global__ void __launch_bounds__(256, 2) pa_shared_finish_kernel(const __grid_c
 #pragma unroll
     for (int e = 0; e < 4; ++e) if (r0 + e < most) sums[e] = old[e] + a[e];
   }
+  }
 }
 
 template <int HD, bool MIXED>
@@ -593,11 +570,11 @@ static cudaError_t launch_shared_t(const SharedParams& p, const CUtensorMap& pk,
   using S = ShSmem<HD>;
   static std::atomic<bool> attr_set[64];
   if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(pa_shared_kernel<HD, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::total(MIXED));
+    cudaError_t e = cudaFuncSetAttribute(pa_shared_kernel<HD, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
     if (e != cudaSuccess) return e;
     attr_set[dev & 63].store(true, std::memory_order_release);
   }
-  return launch_pdl(pa_shared_kernel<HD, MIXED>, dim3(p.units, n_kv), dim3(S::THREADS), (size_t)S::total(MIXED && !p.q_f16), st, pk, pv, k, v, p);
+  return launch_pdl(pa_shared_kernel<HD, MIXED>, dim3(n_kv, p.units), dim3(S::THREADS), (size_t)S::TOTAL, st, pk, pv, k, v, p);
 }
 cudaError_t launch_shared(const SharedParams& p, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v, uint32_t hd, uint32_t n_kv,
                           int dev, cudaStream_t st) {
@@ -609,9 +586,9 @@ cudaError_t launch_shared(const SharedParams& p, const CUtensorMap& pk, const CU
 }
 cudaError_t launch_shared_finish(const SharedFinishParams& p, uint32_t hd, uint32_t sum_ctas, cudaStream_t st) {
   const dim3 grid(p.merge_ctas + sum_ctas);
-  if (hd == 256) return launch_pdl(pa_shared_finish_kernel<256>, grid, dim3(256), 0, st, p);
-  if (hd == 128) return launch_pdl(pa_shared_finish_kernel<128>, grid, dim3(256), 0, st, p);
-  if (hd == 64) return launch_pdl(pa_shared_finish_kernel<64>, grid, dim3(256), 0, st, p);
+  if (hd == 256) return sum_ctas ? launch_pdl(pa_shared_finish_kernel<256, true>, grid, dim3(256), 0, st, p) : launch_pdl(pa_shared_finish_kernel<256, false>, grid, dim3(256), 0, st, p);
+  if (hd == 128) return sum_ctas ? launch_pdl(pa_shared_finish_kernel<128, true>, grid, dim3(256), 0, st, p) : launch_pdl(pa_shared_finish_kernel<128, false>, grid, dim3(256), 0, st, p);
+  if (hd == 64) return sum_ctas ? launch_pdl(pa_shared_finish_kernel<64, true>, grid, dim3(256), 0, st, p) : launch_pdl(pa_shared_finish_kernel<64, false>, grid, dim3(256), 0, st, p);
   return cudaErrorInvalidValue;
 }
 

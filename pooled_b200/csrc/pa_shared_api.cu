@@ -21,39 +21,51 @@ static uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 static uint32_t pad64(uint32_t rows) { return (rows + 63) & ~63u; }
 static uint64_t scores_of(const pa_ctx* ctx, uint32_t rows) { return (uint64_t)ctx->cfg.n_heads * pad64(rows); }
 
-// Tiles per unit (T).  The units of a call are launched longest first, one CTA an SM at a time, so a call takes about
-// max(its longest unit, all its tiles and starts / SMs).  A unit costs `start` us of its own: launch, q, the first scores, the
-// record.  p_tile, o_tile: us a tile of the shared and of own rows.  Tried: every number of splits of the shared rows, or of
-// the longest item without them (beyond 24 in steps of 4 %).
-static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_items, uint32_t p_tiles, uint32_t row_tiles, float p_tile, float o_tile, uint32_t most_records) {
-  const uint32_t n_kv = ctx->cfg.n_kv_heads, sms = (uint32_t)ctx->sm_count;
-  uint32_t own_longest = 0, own_tiles = 0, own_items = 0;
+// What a call's units cost, in us on the device (measured: a unit of T tiles takes T * tile + start; start: launch, q, the first
+// scores, the record).  tile: 0.75 at head_dim 256 (the tensor cores), 0.67 below (the softmax); of 128 query rows 1.17 and 0.64.
+struct UnitCost { float p_tile, p_start, o_tile, o_start; };
+static UnitCost unit_cost(uint32_t hd, bool wide) {
+  const float tile = hd == 256 ? 0.75f : 0.67f;
+  return wide ? UnitCost{hd == 256 ? 1.17f : 0.64f, 10.5f, tile, 5.5f} : UnitCost{tile, 5.5f, tile, 5.5f};
+}
+
+// Tiles per unit (T) and the time the call takes with them.  The units run one CTA an SM at a time, in the grid's order: the shared
+// rows' units, all equal, then those of own rows, which fill what the last wave of the others leaves.  Tried: every number of splits
+// of the shared rows, or of the longest item without them (beyond 24 in steps of 4 %).
+static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_items, uint32_t p_tiles, uint32_t row_tiles, const UnitCost& c, uint32_t most_records, float* us) {
+  const uint32_t n_kv = ctx->cfg.n_kv_heads;
+  const float sms = (float)ctx->sm_count;
+  float tiles[kMaxShared], own_tiles = 0.f, own_longest = 0.f;
   for (uint32_t i = 0; i < n_items; ++i) {
-    const uint32_t t = ceil_div(rows[i], 64);
-    own_longest = std::max(own_longest, t); own_tiles += t; own_items += t > 0;
+    tiles[i] = (float)ceil_div(rows[i], 64);
+    own_tiles += tiles[i]; own_longest = std::max(own_longest, tiles[i]);
   }
-  const uint32_t longest = std::max(1u, std::max(p_tiles, own_longest));
-  const float start = 6.5f;
+  const uint32_t longest = std::max(1u, std::max(p_tiles, (uint32_t)own_longest));
+  const uint32_t split = p_tiles ? p_tiles : longest, most_splits = std::min(split, std::min(most_records, 4 * (uint32_t)ctx->sm_count));
+  const float hbm = ((float)p_tiles + own_tiles) * n_kv * (float)(ctx->cfg.head_dim * 256) / 6.0e6f;      // us for its bytes
   uint32_t best = longest;
-  float least = 3.0e38f;
-  const uint32_t split = p_tiles ? p_tiles : longest, most_splits = std::min(split, std::min(most_records, 4 * sms));
+  *us = 3.0e38f;
   for (uint32_t n = 1; n <= most_splits; n += 1 + n / 24) {
     const uint32_t T = ceil_div(split, n);
     // records of a row: the shared rows' and the longest item's
-    if (ceil_div(p_tiles, T) + ceil_div(own_longest, T) > most_records) break;
-    const float tp = (float)T * p_tile + start, to = (float)std::min(T, own_longest) * o_tile + start, t = p_tiles ? std::max(tp, to) : to;
-    const float own_units = own_longest <= T ? (float)own_items : (float)own_tiles / T + 0.5f * own_items;
-    const float shared_units = (float)(p_tiles ? row_tiles * ceil_div(p_tiles, T) : 0) * n_kv, own_work = ((float)own_tiles * o_tile + own_units * start) * n_kv;
-    const float units = shared_units + own_units * n_kv;
-    float time;
-    if (units <= sms) time = t;
-    else if (shared_units > 0) {   // full waves of the equal, longest units; the others fill what the last wave leaves
-      const float full = ceilf(shared_units / sms) * tp;
-      time = full + std::max(0.f, own_work - (sms * full - shared_units * tp)) / sms;
-    } else {
-      time = std::max(own_work / sms + 0.5f * t, t);
+    if (ceil_div(p_tiles, T) + ceil_div((uint32_t)own_longest, T) > most_records) break;
+    const float inv = 1.0f / (float)T, tp = (float)T * c.p_tile + c.p_start, to = std::min((float)T, own_longest) * c.o_tile + c.o_start;
+    float own_units = 0.f;
+    for (uint32_t i = 0; i < n_items; ++i) own_units += (float)(int)(tiles[i] * inv + 0.999f);
+    own_units *= n_kv;
+    const float p_units = (float)(row_tiles * ceil_div(p_tiles, T) * n_kv), waves = floorf(p_units / sms), rest = p_units - waves * sms;
+    const float own_work = own_tiles * n_kv * c.o_tile + own_units * c.o_start;
+    float time = (waves + (rest > 0.f ? 1.f : 0.f)) * tp;            // the shared rows
+    if (own_units > 0.f) {
+      if (own_units <= sms - rest) time = std::max(time, waves * tp + to);
+      else {                                                         // sms - rest SMs from the last full wave on, the others a wave later
+        float level = waves * tp + own_work / (sms - rest + 1.0e-3f);
+        if (rest > 0.f && level > (waves + 1.f) * tp) level = (waves + 1.f) * tp + (own_work - (sms - rest) * tp) / sms;
+        time = std::max(time, level + 0.5f * to);
+      }
     }
-    if (time < least) { least = time; best = T; }
+    time = std::max(time, hbm + c.o_start) + 0.05f * time;           // (bound by HBM, the smaller T: more CTAs stream)
+    if (time < *us) { *us = time; best = T; }
   }
   return best;
 }
@@ -81,16 +93,16 @@ static int shared_launch(const SharedCall& c, const pa_item* items, const uint32
   const size_t aes = ctx->cfg.act_dtype == PA_F16 ? 2 : 4;
   p.q = reinterpret_cast<const uint8_t*>(c.q) + (uint64_t)first * c.qcs * (c.q_f16 ? 2 : 4); p.q_f16 = c.q_f16; p.q_col_stride = c.qcs; p.q_head_stride = c.qhs;
   p.part_o = ctx->part_o; p.part_ml = ctx->part_ml;
-  // Row tiles of the shared rows: of 64 query rows, or of 128 where that takes less time.  us a tile, by HBM (one row tile, every
-  // SM streaming) or by what the tensor cores and L2 give narrow and wide tiles, as measured at head_dim 256
-  const float hds = (float)hd / 256.f, hbm = 1.45f * hds, narrow = 0.87f * hds, wide = (c.q_f16 ? 1.0f : 1.45f) * hds;
-  const uint32_t tiles64 = ceil_div(n, 64 / G), tiles128 = ceil_div(n, 128 / G);
-  p.wide = tiles64 > 1 && tiles128 * wide < tiles64 * narrow;
-  p.items_per_tile = (p.wide ? 128 : 64) / G; p.row_tiles = p.wide ? tiles128 : tiles64;
-  const float p_tile = p.wide ? wide : p.row_tiles > 1 ? narrow : hbm;
   const uint32_t p_tiles = c.prefix ? ceil_div(c.prefix_len, 64) : 0;
   const uint32_t most = (uint32_t)std::min<size_t>(512, ctx->pf_slots / ((size_t)n * nH));
-  const uint32_t T = plan_units(ctx, rows + first, n, p_tiles, p.row_tiles, p_tile, hbm, most);
+  // row tiles of the shared rows: of 64 query rows, or of 128 where that promises less time
+  p.items_per_tile = 64 / G; p.row_tiles = ceil_div(n, p.items_per_tile);
+  float us = 0.f, wide_us = 0.f;
+  uint32_t T = plan_units(ctx, rows + first, n, p_tiles, p.row_tiles, unit_cost(hd, false), most, &us);
+  if (p_tiles && p.row_tiles > 1 && c.q_f16) {
+    const uint32_t tiles128 = ceil_div(n, 128 / G), T128 = plan_units(ctx, rows + first, n, p_tiles, tiles128, unit_cost(hd, true), most, &wide_us);
+    if (wide_us < us) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }
+  }
   if (c.prefix) { p.p_row0 = c.prefix_seq * c.prefix->max_seq; p.p_rows = c.prefix_len; p.p_tps = T; p.p_splits = ceil_div(p_tiles, T); }
   p.tps = T; p.own_row0 = c.own_row0;
   uint32_t units = p.p_splits * p.row_tiles, own_most = 0;
