@@ -175,16 +175,18 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
     const bool is_lo = !WIDE && (row & 1u) != 0, in_use = qd < un.live_warps;
     const uint32_t lr = WIDE ? row : row >> 1;         // query row: (item, head of the group)
     const bool live = lr < un.pairs;
-    const uint32_t st_tid = tid - 128, G = p.G;
+    const uint32_t st_tid = tid - 128, G = p.G, by_g = (65536 + G - 1) / G;
+    auto row_item = [&](uint32_t pr) { return (pr * by_g) >> 16; };       // pr / G, pr < 128
     // The query rows come by cp.async into the K and the V slot that the producers leave alone until Q_READ, half of them each, a
     // row's 16-byte chunks XOR-swizzled against the per-row reads.
     {
-      const uint32_t es = WIDE || p.q_f16 ? 2u : 4u, cap = 128 / es, q_ch = HD * es / 16;
+      const bool f16 = WIDE || p.q_f16;
+      const uint32_t es = f16 ? 2u : 4u, cap = f16 ? 64u : 32u, q_ch = f16 ? HD / 8 : HD / 4;
       auto stage_row = [&](uint32_t r) { return base + (r < cap ? L::OFF_K + 2 * L::KV_BYTES : L::OFF_V + L::KV_BYTES) + (size_t)(r & (cap - 1)) * (HD * es); };
       for (uint32_t idx = st_tid; idx < un.pairs * q_ch; idx += 128 * GRP) {
-        const uint32_t pr = idx / q_ch, c = idx % q_ch;
+        const uint32_t pr = idx / q_ch, c = idx % q_ch, it = row_item(pr);
         const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
-                             ((uint64_t)(un.item0 + pr / G) * p.q_col_stride + (uint64_t)(g * G + pr % G) * p.q_head_stride) * es + (uint64_t)c * 16;
+                             ((uint64_t)(un.item0 + it) * p.q_col_stride + (uint64_t)(g * G + pr - it * G) * p.q_head_stride) * es + (uint64_t)c * 16;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stage_row(pr) + ((c ^ (pr & 7u)) << 4))), "l"(src) : "memory");
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -195,9 +197,9 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       // this thread's Q row as f16 pairs, 64 dims at a time (the groups share the chunks out)
 #pragma unroll 1
       for (int c = 0; c < CH; ++c) {
-        if (CH >= 2 ? (uint32_t)(c >= CH / 2) != wg : wg != 0) continue;
+        if (!in_use || (CH >= 2 ? (uint32_t)(c >= CH / 2) != wg : wg != 0)) continue;     // (rows without a query: whatever is there)
         uint32_t w[32];
-        if (WIDE || p.q_f16) {
+        if (f16) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint4 x = is_lo ? make_uint4(0, 0, 0, 0) : stage_ld(c * 8 + i);         // f16 queries have no low part
@@ -331,20 +333,26 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
     // ---- the records: rows to shared memory (every product has retired), whole records from there ----
     constexpr int RP = HD / 4 + 1;                       // row pitch in float4
     float4* xs = reinterpret_cast<float4*>(base + 2048);
-    auto slot_of = [&](uint32_t pr) { return ((uint64_t)(un.item0 + pr / G) * p.n_heads + g * G + pr % G) * p.n_rec + un.slot; };
+    auto slot_of = [&](uint32_t pr) { const uint32_t it = row_item(pr); return ((uint64_t)(un.item0 + it) * p.n_heads + g * G + pr - it * G) * p.n_rec + un.slot; };
     if (in_use) {
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        if ((uint32_t)(c & 1) != wg) continue;           // the groups share the columns out
-        float o[32];
-        tmem_ld32(t_o + c * 32 + lane_addr, o);
+      for (int c = wg; c < HD / 32; c += 2 * GRP) {      // the groups share the columns out, two chunks of 32 at a time
+        constexpr bool TWO = HD / 32 > GRP;
+        float o[TWO ? 64 : 32];
+        tmem_ld32_async(t_o + c * 32 + lane_addr, o);
+        if (TWO) tmem_ld32_async(t_o + (c + GRP) * 32 + lane_addr, o + 32);
+        tmem_wait_ld(o);
         if (!WIDE) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], 1);
+          for (int i = 0; i < (TWO ? 64 : 32); ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], 1);
         }
         if (live && !is_lo) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) xs[lr * RP + c * 8 + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          if (TWO) {
+#pragma unroll
+            for (int i = 8; i < 16; ++i) xs[lr * RP + (c + GRP) * 8 + i - 8] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
         }
       }
       if (live && !is_lo && wg == 0) reinterpret_cast<float2*>(p.part_ml)[slot_of(lr)] = make_float2(m_st, s_rl[row] + s_rl[128 + row]);
