@@ -342,7 +342,11 @@ PA_API int pa_sigmoid_mul(pa_ctx* ctx, void* a, uint64_t a_col_stride, const voi
  *   PA_ROPE_SCALE_BANDS   the same idea by turns: pairs of more than `fast` turns over `original` stay, of fewer than
  *                         `slow` are divided by factor, between them linear in the number of turns
  * The frequencies and the angles (reduced to one turn) are float64, everything else f32 (relative error of a rotated pair
- * below 2^-21 of its length; positions up to 2^31 cost no more than the angle's own 2^-52). */
+ * below 2^-21 of its length; positions up to 2^31 cost no more than the angle's own 2^-52).
+ *
+ * For these entry points and the ones below, as for all of the library: the records, scores and lists of a call live in its
+ * context, so the calls of one context, and the graphs that captured them, run one after another, on whatever streams.  Creating
+ * a pa_rotary and pa_layer_track_weights allocate: not inside a stream capture. */
 typedef enum pa_rope_layout {
   PA_ROPE_HALF = 0,        /* pair i is dims i and i + n_rot / 2 (the context's own rotation) */
   PA_ROPE_INTERLEAVED = 1  /* pair i is dims 2i and 2i + 1 */
@@ -367,7 +371,7 @@ PA_API int pa_rotary_destroy(pa_rotary* rotary);   /* before its context */
 /* The frequencies in use, radians per position: n_rot / 2 values, and mscale (either may be NULL).  Host arithmetic only. */
 PA_API int pa_rotary_freqs(const pa_rotary* rotary, double* freqs, double* mscale);
 /* Rotates x into y.  x: x_dtype [n_cols][x_col_stride], head h at h * x_head_stride; y: y_dtype, the same with its own strides;
- * y may be x with equal type and strides, and otherwise does not overlap it.  Column c is at position positions[c] (int32 on
+ * y may be x with equal type and strides (rows of a cache too), and otherwise does not overlap it.  Column c is at position positions[c] (int32 on
  * the device, read when the kernel runs), or, without positions, at pos + c.  A negative position turns back: with mscale 1
  * the rotation by -p undoes the rotation by p.  Any number of columns and heads; beside pa_rope, which keeps the context's
  * own rotation bit for bit. */
@@ -375,7 +379,7 @@ PA_API int pa_rotary_apply(pa_rotary* rotary, const void* x, int x_dtype, uint64
                            const int32_t* positions, int32_t pos, uint32_t n_cols, void* y, int y_dtype, uint64_t y_col_stride,
                            uint64_t y_head_stride, void* stream);
 /* The front of a layer call with this rotation, for one or many sequences: items[i] = (seq, pos, n_cols) owns the next n_cols
- * rows of q, k, v (act_dtype) and q_out.  q is rotated into q_out (q_out_dtype, heads packed; q = NULL: k and v only); k is
+ * rows of q, k, v (act_dtype) and q_out.  q is rotated into q_out (q_out_dtype, heads packed, no overlap with q; q = NULL: k and v only); k is
  * rotated, k and v are rounded to f16 (as pa_kv_append rounds) and stored in rows rows[i] .. rows[i] + n_cols - 1 of the sequence, or, with
  * rows = NULL, in the rows of their positions.  Rows and positions part when a cache holds only some of the positions
  * (pa_evict) or begins behind a shared prefix (pa_decode_shared).  At most 128 items; two items may not store the same row.  f16 caches. */
@@ -402,7 +406,7 @@ PA_API int pa_decode_shared(pa_layer* layer, pa_layer* prefix_layer, uint32_t pr
 /* ---- caches that keep what attention uses ---------------------------------------------------------------------- */
 
 /* Gives a layer a sum of attention weights per cached row: f32 [n_seqs][n_kv_heads][max_seq], zeroed, the layer's own, and
- * the context room for the scores of a call.  f16 caches.  Allocates: not inside a stream capture. */
+ * the context room for the scores of a call.  f16 caches.  Appends, imports and slots leave the sums alone. */
 PA_API int pa_layer_track_weights(pa_layer* layer);
 PA_API float* pa_weights_ptr(pa_layer* layer);   /* NULL: not tracked */
 /* Zeroes the sums of one sequence, as a new conversation begins with. */

@@ -6,7 +6,8 @@
 // A unit is a run of 64-row K / V tiles of one kv head and the query rows that attend them: for the shared rows the heads of
 // several items (so that a shared byte is read once for all of these, from HBM once in all), for own rows the heads of one.
 // A CTA per unit walks its tiles on the 5th-generation tensor cores and leaves an unnormalised (o, m, l) record per query
-// row; the second kernel merges a row's records, gates and stores.  All units have the same number of tiles, whatever they
+// row (with f32 outputs one every p.seg tiles: the tensor cores' sums round towards zero, which after 32 tiles has cost 2.3e-6 of the
+// result, after four 6e-7); the second kernel merges a row's records, gates and stores.  All units have the same number of tiles, whatever they
 // are units of (plan_units), so that a batch of long shared rows and short own ones fills the machine like one long conversation.
 //
 //   warps 0, 3  TMA producers: K tiles and V tiles (64 x head_dim f16, 128-byte swizzle), a ring of three and of two slots;
@@ -16,8 +17,7 @@
 //   warp 2      tensor memory; issues O += P V into the accumulator (128 x head_dim f32)
 //   warps 4-11  softmax, two groups of four warps with half of a tile's keys each (on alternate tiles, a call of one tile a CTA took
 //               0.4 us longer, and wide tiles 1.5 us each).  A row's reference lies 2^7 below its maximum and moves only when a tile
-//               passes it by 2^15: weights of up to 2^15 keep the low parts of small ones above f16's last place (with a reference at the
-//               maximum, a long row's error was 2.2e-6 of the result, 3e-7 now).  Warps whose rows hold no query take no part.
+//               passes it by 2^15: weights of up to 2^15 keep the low parts of small ones above f16's last place.  Warps whose rows hold no query take no part.
 // q and the weights enter as pairs of f16 values, high and low parts, some 22 bits of both, in one of two ways:
 //   narrow (up to 64 query rows)   even rows of the 128 carry the high parts, odd rows the low parts of the same query row, added by
 //               shuffles: both products at the cost of one, and the two lanes share the row's keys out.  0.75 us a tile of 64 keys
@@ -40,12 +40,13 @@ struct ShSmem {
   static constexpr int KV_BYTES = HD * 128;          // [HD/64][64 rows][128 B]
   static constexpr int THREADS = 384;
   static constexpr int OFF_K = 0, OFF_V = NK * KV_BYTES, OFF_BAR = (NK + NV) * KV_BYTES;
-  static constexpr int OFF_MAX = OFF_BAR + 256;      // [2][2][128] maxima of the rows, two tiles in turn
+  static constexpr int OFF_MAX = OFF_BAR + 256;      // [2][2][128] maxima of the rows, two tiles in turn, and [2][128] row sums
   static constexpr int OFF_Q = OFF_BAR + 4096;       // narrow: the chunks of Q that are not in tensor memory
-  static constexpr int TOTAL = 1024 + OFF_Q + (HD / 64 - HD / 128) * 128 * 128;
+  static constexpr int QS_BYTES = (HD / 64 - HD / 128) * 128 * 128;
+  static constexpr int XP = 36;                      // a chunk of the records on its way out: 64 or 128 rows of 32 floats, 36 apart, for each group
+  static constexpr int X_BYTES = 64 * XP * 4;
+  static constexpr int TOTAL = 1024 + OFF_Q + std::max(QS_BYTES + 2 * X_BYTES, 4 * X_BYTES);
   static_assert(TOTAL <= 227 * 1024, "shared memory of one CTA");
-  // the records leave through the rings: row sums of the groups, then 64 (in the K ring) or 128 rows of HD + 4 floats
-  static_assert(2048 + 64 * (HD + 4) * 4 <= NK * KV_BYTES && 2048 + 128 * (HD + 4) * 4 <= (NK + NV) * KV_BYTES, "staging of the records");
 };
 template <int HD, bool WIDE>
 struct ShLay {
@@ -57,7 +58,7 @@ struct ShLay {
 template <int HD>
 constexpr int sh_tmem_cols() { return std::max(ShLay<HD, false>::T_O, ShLay<HD, true>::T_O) + HD <= 256 ? 256 : 512; }
 
-enum { SH_K_FULL = 0, SH_K_EMPTY = 3, SH_V_FULL = 6, SH_V_EMPTY = 8, SH_S_FULL = 10, SH_P_FULL = 13, SH_PV_DONE = 16, SH_O_DONE = 19, SH_Q_FULL, SH_Q_READ, SH_V_CLEAN, SH_BARS };
+enum { SH_K_FULL = 0, SH_K_EMPTY = 3, SH_V_FULL = 6, SH_V_EMPTY = 8, SH_S_FULL = 10, SH_P_FULL = 13, SH_PV_DONE = 16, SH_O_DONE = 19, SH_O_FREE, SH_Q_FULL, SH_Q_READ, SH_V_CLEAN, SH_BARS };
 static_assert(SH_BARS <= 31, "barrier slots");
 
 // a CTA's unit
@@ -152,24 +153,27 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
     uint64_t v_desc[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) v_desc[i] = smem_desc(smem_u32(base + L::OFF_V + i * L::KV_BYTES), 64 * 128, 1024);
-    for (uint32_t j = 0; j < n_tiles; ++j) {
+    for (uint32_t j = 0, seg = 0, in_seg = 0; j < n_tiles; ++j) {
       const uint32_t sb = j % SB, st = j % NV;
       mbar_wait(BAR(SH_P_FULL, sb), (j / SB) & 1, s_err, WAIT_QFULL);
       mbar_wait(BAR(SH_V_FULL, st), (j / NV) & 1, s_err, WAIT_VFULL);
       if (un.ragged && j == n_tiles - 1) mbar_wait(BAR(SH_V_CLEAN, 0), 0, s_err, WAIT_VFULL);
+      if (in_seg == 0 && j > 0) mbar_wait(BAR(SH_O_FREE, 0), (seg - 1) & 1, s_err, WAIT_MMA);      // the record before is out
       tc_fence_after();
       const uint64_t vd = st == 0 ? v_desc[0] : v_desc[1];
       const uint32_t tp = t_s0 + sb * 64;      // P(j): packed f16 pairs over S(j): 32 columns, wide: 32 of high and 32 of low parts
 #pragma unroll
       for (int ks = 0; ks < (WIDE ? 8 : 4); ++ks)
-        umma_f16_ts(leader, t_o, tp + ks * 8, vd + (uint64_t)(((ks & 3) * 2048) >> 4), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
+        umma_f16_ts(leader, t_o, tp + ks * 8, vd + (uint64_t)(((ks & 3) * 2048) >> 4), idesc_pv, (in_seg > 0 || ks > 0) ? 1u : 0u);
       umma_commit_elected(leader, BAR(SH_V_EMPTY, st));
       umma_commit_elected(leader, BAR(SH_PV_DONE, sb));
+      if (++in_seg == p.seg || j == n_tiles - 1) {
+        umma_commit_elected(leader, BAR(SH_O_DONE, 0));
+        in_seg = 0; ++seg;
+      }
     }
-    umma_commit_elected(leader, BAR(SH_O_DONE, 0));
   } else {
     // ------------------------------------------------------------------ softmax + epilogue ----
-    float* s_rl = reinterpret_cast<float*>(base + L::OFF_K);     // [2][128] the groups' row sums, in the first K slot once the last tile's scores exist
     const uint32_t wg = (warp - 4) >> 2, qd = (warp - 4) & 3, row = qd * 32 + lane;
     const uint32_t lane_addr = (qd * 32) << 16;
     const bool is_lo = !WIDE && (row & 1u) != 0, in_use = qd < un.live_warps;
@@ -248,8 +252,76 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       tc_fence_after();
       return fmaxf(m, at[(wg ^ 1) * 128]);
     };
+    // The record of the tiles since the last one.  Up to 16 query rows the lanes store what they have, 64 bytes of a chunk of 32 dims;
+    // more rows go through shared memory, a chunk at a time, so that whole lines leave (a lane has a row: its own stores are 16 bytes
+    // each in 32 records 1 KB apart).
+    float* s_rl = s_max + 512;
+    auto record = [&](uint32_t seg) {
+      const uint32_t threads = 32 * un.live_warps, gt = (tid - 128) & 127;
+      auto slot_of = [&](uint32_t pr) { const uint32_t it = row_item(pr); return ((uint64_t)(un.item0 + it) * p.n_heads + g * G + pr - it * G) * p.n_rec + un.slot + seg; };
+      float l = l_sum;
+      if (!WIDE) l += __shfl_xor_sync(0xffffffffu, l, 1);
+      if (wg) s_rl[row] = l;
+      named_bar_sync(3 + qd, 64);
+      if (!wg && live && !is_lo) reinterpret_cast<float2*>(p.part_ml)[slot_of(lr)] = make_float2(m_st, l + s_rl[row]);
+      l_sum = 0.f;
+      float* xs = reinterpret_cast<float*>(base + L::OFF_Q + (WIDE ? 2 * wg * L::X_BYTES : L::QS_BYTES + wg * L::X_BYTES));
+      mbar_wait(BAR(SH_O_DONE, 0), seg & 1, s_err, WAIT_MMA);
+      tc_fence_after();
+      // high and low rows of a chunk added, each lane with half of it
+      auto add_rows = [&](const float* o, float (&t)[16]) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float give = is_lo ? o[i] : o[16 + i], keep = is_lo ? o[16 + i] : o[i];
+          t[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+        }
+      };
+      if (!WIDE && un.live_warps == 1) {
+        constexpr int N = HD / 32 > GRP ? 2 : 1;          // chunks at a time
+        float* to = p.part_o + slot_of(live ? lr : 0) * HD + (is_lo ? 16 : 0);
+#pragma unroll 1
+        for (int c = wg; c < HD / 32; c += N * GRP) {
+          float o[32 * N], t[16];
+#pragma unroll
+          for (int k = 0; k < N; ++k) tmem_ld32_async(t_o + (c + k * GRP) * 32 + lane_addr, o + 32 * k);
+          tmem_wait_ld(o);
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            add_rows(o + 32 * k, t);
+            if (live) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(to + (c + k * GRP) * 32 + 4 * i) = make_float4(t[4 * i], t[4 * i + 1], t[4 * i + 2], t[4 * i + 3]);
+            }
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(BAR(SH_O_FREE, 0));
+        return;
+      }
+#pragma unroll 1
+      for (int c = wg; c < HD / 32; c += GRP) {           // the groups share the chunks out
+        float o[32];
+        tmem_ld32(t_o + c * 32 + lane_addr, o);
+        if (c != (int)wg) named_bar_sync(7 + wg, threads);
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(xs + row * L::XP + 4 * i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else {
+          float t[16];
+          add_rows(o, t);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(xs + lr * L::XP + (is_lo ? 16 : 0) + 4 * i) = make_float4(t[4 * i], t[4 * i + 1], t[4 * i + 2], t[4 * i + 3]);
+        }
+        named_bar_sync(7 + wg, threads);
+        for (uint32_t i = gt; i < un.pairs * 8; i += threads)
+          reinterpret_cast<float4*>(p.part_o + slot_of(i >> 3) * HD + c * 32)[i & 7] = *reinterpret_cast<const float4*>(xs + (i >> 3) * L::XP + (i & 7) * 4);
+      }
+      named_bar_sync(7 + wg, threads);                    // the next record may take the place
+      tc_fence_before();
+      mbar_arrive(BAR(SH_O_FREE, 0));
+    };
     if (in_use) {
-      for (uint32_t j = 0; j < n_tiles; ++j) {
+      for (uint32_t j = 0, seg = 0, in_seg = 0; j < n_tiles; ++j) {
         const uint32_t b = j % SB, u = j / SB, kv0 = (tile0 + j) * 64;
         mbar_wait(BAR(SH_S_FULL, b), u & 1, s_err, WAIT_MMA);
         tc_fence_after();
@@ -283,7 +355,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
         float alpha = 1.f;
         bool grow = false;
         if (mt > m_st + 15.f) { alpha = ex2_approx(m_st - (mt - 7.f)); m_st = mt - 7.f; l_sum *= alpha; grow = true; }
-        if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        if (in_seg > 0 && __any_sync(0xffffffffu, grow)) {
           const uint32_t jb = (j - 1) % SB, ju = (j - 1) / SB;
           mbar_wait(BAR(SH_PV_DONE, jb), ju & 1, s_err, WAIT_MMA);
           tc_fence_after();
@@ -323,46 +395,9 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(BAR(SH_P_FULL, b));
+        if (++in_seg == p.seg || j == n_tiles - 1) { record(seg++); in_seg = 0; }
       }
-      if (!WIDE) l_sum += __shfl_xor_sync(0xffffffffu, l_sum, 1);
-      s_rl[wg * 128 + row] = l_sum;
     }
-    named_bar_sync(2, 128 * GRP);
-    mbar_wait(BAR(SH_O_DONE, 0), 0, s_err, WAIT_MMA);
-    tc_fence_after();
-    // ---- the records: rows to shared memory (every product has retired), whole records from there ----
-    constexpr int RP = HD / 4 + 1;                       // row pitch in float4
-    float4* xs = reinterpret_cast<float4*>(base + 2048);
-    auto slot_of = [&](uint32_t pr) { const uint32_t it = row_item(pr); return ((uint64_t)(un.item0 + it) * p.n_heads + g * G + pr - it * G) * p.n_rec + un.slot; };
-    if (in_use) {
-#pragma unroll 1
-      for (int c = wg; c < HD / 32; c += 2 * GRP) {      // the groups share the columns out, two chunks of 32 at a time
-        constexpr bool TWO = HD / 32 > GRP;
-        float o[TWO ? 64 : 32];
-        tmem_ld32_async(t_o + c * 32 + lane_addr, o);
-        if (TWO) tmem_ld32_async(t_o + (c + GRP) * 32 + lane_addr, o + 32);
-        tmem_wait_ld(o);
-        if (!WIDE) {
-#pragma unroll
-          for (int i = 0; i < (TWO ? 64 : 32); ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], 1);
-        }
-        if (live && !is_lo) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) xs[lr * RP + c * 8 + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          if (TWO) {
-#pragma unroll
-            for (int i = 8; i < 16; ++i) xs[lr * RP + (c + GRP) * 8 + i - 8] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          }
-        }
-      }
-      if (live && !is_lo && wg == 0) reinterpret_cast<float2*>(p.part_ml)[slot_of(lr)] = make_float2(m_st, s_rl[row] + s_rl[128 + row]);
-    }
-    named_bar_sync(1, 128 * GRP);
-    for (uint32_t idx = st_tid; idx < un.pairs * (HD / 4); idx += 128 * GRP) {
-      const uint32_t rr = idx / (HD / 4), c4 = idx % (HD / 4);
-      reinterpret_cast<float4*>(p.part_o + slot_of(rr) * HD)[c4] = xs[rr * RP + c4];
-    }
-    tc_fence_before();
   }
 }
 
@@ -388,17 +423,18 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
     split = unit / p.row_tiles;
     un.item0 = (unit % p.row_tiles) * p.items_per_tile;
     n_q = min(p.items_per_tile, p.n_items - un.item0);
-    un.row0 = p.p_row0; un.n_rows = p.p_rows; tps = p.p_tps; un.slot = split;
+    un.row0 = p.p_row0; un.n_rows = p.p_rows; tps = p.p_tps; un.slot = 0;
     un.mk = &tm_pk; un.mv = &tm_pv;
   } else {
     uint32_t lo = 0, hi = p.n_items - 1;
     while (lo < hi) { const uint32_t mid = (lo + hi + 1) / 2; if (unit >= p.cta0[mid]) lo = mid; else hi = mid - 1; }
     un.item0 = lo; n_q = 1; split = unit - p.cta0[lo];
-    un.row0 = p.seq[lo] * p.max_seq + p.own_row0; un.n_rows = p.rows[lo]; tps = p.tps; un.slot = p.p_splits + split;
+    un.row0 = p.seq[lo] * p.max_seq + p.own_row0; un.n_rows = p.rows[lo]; tps = p.tps; un.slot = p.p_recs;
     un.mk = &tm_k; un.mv = &tm_v;
   }
   un.once = !un.shared || p.row_tiles == 1;
   un.tile0 = split * tps;
+  un.slot += un.tile0 / p.seg;                                        // (tiles per unit: a multiple of seg)
   un.n_tiles = min((un.n_rows + 63) / 64, un.tile0 + tps) - un.tile0;
   un.pairs = n_q * p.G;
   const bool wide = MIXED && un.shared;
@@ -410,7 +446,7 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
     auto init = [&](int which, int n, uint32_t count) { for (int i = 0; i < n; ++i) mbar_init(bar0 + 8u * (uint32_t)(which + i), count); };
     init(SH_K_FULL, 3, 1); init(SH_K_EMPTY, 3, 1); init(SH_V_FULL, 2, 1); init(SH_V_EMPTY, 2, 1);
     init(SH_S_FULL, 3, 1); init(SH_P_FULL, 3, 64 * un.live_warps); init(SH_PV_DONE, 3, 1);
-    init(SH_O_DONE, 1, 1); init(SH_Q_FULL, 1, 256); init(SH_Q_READ, 1, 256); init(SH_V_CLEAN, 1, 1);
+    init(SH_O_DONE, 1, 1); init(SH_O_FREE, 1, 64 * un.live_warps); init(SH_Q_FULL, 1, 256); init(SH_Q_READ, 1, 256); init(SH_V_CLEAN, 1, 1);
     fence_barrier_init();
   }
   if (warp == 2) {
@@ -469,7 +505,7 @@ __global__ void __launch_bounds__(256, SUMS ? 3 : 4) pa_shared_finish_kernel(con
   pdl_trigger();
   if (!SUMS || blockIdx.x < p.merge_ctas) {
     const uint32_t slices = HD / 4 / p.lanes, prow = blockIdx.x / slices, slice = blockIdx.x % slices, item = prow / p.n_heads, h = prow % p.n_heads;
-    const uint32_t ns = p.p_splits + p.n_own[item], groups = 256 / p.lanes, grp = tid / p.lanes, ln = tid % p.lanes, dims = p.lanes * 4, d = slice * dims + tid;
+    const uint32_t ns = p.p_recs + p.n_own[item], groups = 256 / p.lanes, grp = tid / p.lanes, ln = tid % p.lanes, dims = p.lanes * 4, d = slice * dims + tid;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + (uint64_t)prow * p.n_rec;
     const float* ob = p.part_o + (uint64_t)prow * p.n_rec * HD + slice * dims + ln * 4;
     constexpr int U = 4;      // (eight: two CTAs an SM, a second wave for 512 rows)
@@ -529,7 +565,7 @@ __global__ void __launch_bounds__(256, SUMS ? 3 : 4) pa_shared_finish_kernel(con
   for (int e = 0; e < 4; ++e) old[e] = hg == 0 && r0 + e < most ? sums[e] : 0.f;
   float4 add = make_float4(0.f, 0.f, 0.f, 0.f);
   for (; item != 255; item = p.next[item]) {
-    const uint32_t ns = p.p_splits + p.n_own[item], rows = p.rows[item], pad = (rows + 63) & ~63u;
+    const uint32_t ns = p.p_recs + p.n_own[item], rows = p.rows[item], pad = (rows + 63) & ~63u;
     const float* sc = p.scores + p.score0[item] + (uint64_t)kvh * p.G * pad + r0;
     constexpr int U = 4;
     float4 s[U];

@@ -103,21 +103,31 @@ static int shared_launch(const SharedCall& c, const pa_item* items, const uint32
     const uint32_t tiles128 = ceil_div(n, 128 / G), T128 = plan_units(ctx, rows + first, n, p_tiles, tiles128, unit_cost(hd, true), most, &wide_us);
     if (wide_us < us) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }
   }
+  // tiles of a record: those of a unit, or with f32 outputs four (which HBM hides), sixteen where the tensor cores bound it
+  uint32_t own_longest = 0;
+  for (uint32_t i = 0; i < n; ++i) own_longest = std::max(own_longest, ceil_div(rows[first + i], 64));
+  p.seg = T;
+  if (ctx->cfg.act_dtype == PA_F32) {
+    p.seg = std::min(T, p.row_tiles > 1 && p_tiles ? 16u : 4u);
+    while (p.seg < T && ceil_div(p_tiles, p.seg) + ceil_div(own_longest, p.seg) > most) p.seg = std::min(T, 2 * p.seg);
+    T = ceil_div(T, p.seg) * p.seg;
+  }
   if (c.prefix) { p.p_row0 = c.prefix_seq * c.prefix->max_seq; p.p_rows = c.prefix_len; p.p_tps = T; p.p_splits = ceil_div(p_tiles, T); }
+  p.p_recs = ceil_div(p_tiles, p.seg);
   p.tps = T; p.own_row0 = c.own_row0;
-  uint32_t units = p.p_splits * p.row_tiles, own_most = 0;
+  uint32_t units = p.p_splits * p.row_tiles;
   uint64_t floats = 0;
   for (uint32_t i = 0; i < n; ++i) {
-    const uint32_t r = rows[first + i], u = ceil_div(ceil_div(r, 64), T);
-    p.seq[i] = f.seq[i] = items[first + i].seq; p.rows[i] = f.rows[i] = r; p.cta0[i] = units; f.n_own[i] = (uint16_t)u;
+    const uint32_t r = rows[first + i], tiles = ceil_div(r, 64);
+    p.seq[i] = f.seq[i] = items[first + i].seq; p.rows[i] = f.rows[i] = r; p.cta0[i] = units; f.n_own[i] = (uint16_t)ceil_div(tiles, p.seg);
     p.score0[i] = f.score0[i] = floats;
     floats += scores_of(ctx, r);
-    units += u; own_most = std::max(own_most, u);
+    units += ceil_div(tiles, T);
   }
   p.cta0[n] = units; p.units = units;
-  p.n_rec = p.p_splits + own_most;
+  p.n_rec = p.p_recs + ceil_div(own_longest, p.seg);
   if (c.sums) p.scores = ctx->scores;
-  f.part_o = p.part_o; f.part_ml = p.part_ml; f.n_rec = p.n_rec; f.p_splits = p.p_splits; f.n_items = n; f.n_heads = nH; f.G = G; f.n_kv = n_kv;
+  f.part_o = p.part_o; f.part_ml = p.part_ml; f.n_rec = p.n_rec; f.p_recs = p.p_recs; f.n_items = n; f.n_heads = nH; f.G = G; f.n_kv = n_kv;
   f.gate = c.gate ? reinterpret_cast<const uint8_t*>(c.gate) + (uint64_t)first * c.gcs * aes : nullptr; f.gate_col_stride = c.gcs; f.gate_head_stride = c.ghs;
   f.out = reinterpret_cast<uint8_t*>(c.out) + (uint64_t)first * c.ocs * aes; f.out_col_stride = c.ocs; f.act_f16 = ctx->cfg.act_dtype == PA_F16;
   // few rows of many records: their dims are shared out among CTAs, else a CTA takes a row
@@ -206,6 +216,7 @@ extern "C" int pa_decode_shared(pa_layer* L, pa_layer* prefix_layer, uint32_t pr
   if (int rc = shared_checks(L, items, n_items, q, q_dtype, out, who)) return rc;
   pa_layer* P = prefix_layer ? prefix_layer : L;
   const pa_ctx* pc = P->ctx;
+  if (pc->failed) return fail(ctx, PA_ESTATE, "%s: an earlier step of the prefix layer's context failed (%s)", who, pc->err.c_str());
   if (P->kv_format != PA_KV_F16 || P->origin) return fail(ctx, PA_EUNSUPPORTED, "%s: the prefix must lie in an f16 cache that is no shard", who);
   if (pc->device != ctx->device || pc->cfg.n_kv_heads != ctx->cfg.n_kv_heads || pc->cfg.head_dim != ctx->cfg.head_dim)
     return fail(ctx, PA_EINVAL, "%s: the prefix layer is of another device or shape", who);
@@ -233,6 +244,7 @@ extern "C" int pa_layer_track_weights(pa_layer* L) {
   // scores: a token of every sequence, up to 2^28 of them; never less than one item wants, nor than an eviction's lists
   const size_t one = scores_of(ctx, L->max_seq), want = std::max(std::max(one, sums), std::min<size_t>(one * L->n_seqs, (size_t)1 << 28));
   float *s = nullptr, *w = nullptr;
+  try { ctx->outgrown.reserve(ctx->outgrown.size() + 1); } catch (...) { return fail(ctx, PA_ENOMEM, "pa_layer_track_weights: out of host memory"); }
   cudaError_t e = cudaMalloc(&s, sums * 4);
   if (e == cudaSuccess) e = cudaMemset(s, 0, sums * 4);
   if (e == cudaSuccess && want > ctx->scores_floats) e = cudaMalloc(&w, want * 4);
