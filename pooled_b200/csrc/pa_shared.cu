@@ -22,7 +22,7 @@
 //   narrow (up to 64 query rows)   even rows of the 128 carry the high parts, odd rows the low parts of the same query row, added by
 //               shuffles: both products at the cost of one, and the two lanes share the row's keys out.  0.75 us a tile of 64 keys
 //               at head_dim 256 (the tensor cores: 1394 cycles), 0.67 at 128 and 64 (the softmax)
-//   wide (shared rows of more, f16 queries, where plan_shared finds it faster)   128 query rows without low parts of q; the low parts
+//   wide (shared rows of more, f16 queries and outputs, where the plan finds it faster)   128 query rows without low parts of q; the low parts
 //               of the weights are multiplied behind the high ones into the same accumulator.  1.17 us a tile at head_dim 256, 0.64 at 128,
 //               and a start 5 us longer.  (With f32 queries and the products of their low parts: 1.43 us and 13 us of start, slower than two
 //               narrow tiles at every size tried.)
@@ -45,8 +45,10 @@ struct ShSmem {
   static constexpr int QS_BYTES = (HD / 64 - HD / 128) * 128 * 128;
   static constexpr int XP = 36;                      // a chunk of the records on its way out: 64 or 128 rows of 32 floats, 36 apart, for each group
   static constexpr int X_BYTES = 64 * XP * 4;
-  static constexpr int TOTAL = 1024 + OFF_Q + std::max(QS_BYTES + 2 * X_BYTES, 4 * X_BYTES);
-  static_assert(TOTAL <= 227 * 1024, "shared memory of one CTA");
+  // a unit's only record leaves by way of the rings, which are idle by then: without room for others the merging kernel's CTAs find
+  // place beside this one's (at 220 KB they came 2 us later)
+  static constexpr int total(bool more_records) { return 1024 + OFF_Q + QS_BYTES + (more_records ? 2 * X_BYTES : 0); }
+  static_assert(total(true) <= 227 * 1024 && 4 * X_BYTES * (HD / 64) <= (NK + NV) * KV_BYTES, "shared memory of one CTA");
 };
 template <int HD, bool WIDE>
 struct ShLay {
@@ -67,10 +69,44 @@ struct ShUnit {
   const CUtensorMap* mv;
   uint32_t item0, slot, row0, n_rows, tile0, n_tiles;       // first item; record of a row; first row in the map; the unit's rows end here; its tiles
   uint32_t pairs, live_warps;                               // query rows; warps of a softmax group that hold them
-  bool shared, once, ragged;                                // shared rows; nobody else reads the unit's rows; the last tile reaches past them
+  bool shared, ragged;                                      // shared rows; the last tile reaches past them
 };
 
-template <int HD, bool WIDE>
+// warps 0 (K) and 3 (V), the same for both kinds of units; the tiles are read once, or by neighbouring CTAs at the same time, and
+// enter L2 as its first to go
+template <int HD>
+__device__ __forceinline__ void shared_producer(const ShUnit& un, bool is_v, uint8_t* base, uint32_t bar0, volatile uint32_t* s_err) {
+  using L = ShSmem<HD>;
+  constexpr int CH = HD / 64;
+  const uint32_t lane = threadIdx.x & 31, slots = is_v ? L::NV : L::NK, full = bar0 + 8 * (is_v ? SH_V_FULL : SH_K_FULL), empty = bar0 + 8 * (is_v ? SH_V_EMPTY : SH_K_EMPTY);
+  uint8_t* ring = base + (is_v ? L::OFF_V : L::OFF_K);
+  const CUtensorMap* map = is_v ? un.mv : un.mk;
+  if (lane == 0) {
+    const uint64_t policy = l2_policy_evict_first();
+    for (uint32_t j = 0, st = 0, u = 0; j < un.n_tiles; ++j) {
+      if (j == slots - 1) mbar_wait(bar0 + 8 * SH_Q_READ, 0, s_err, WAIT_QFULL);      // the last slot stages query rows until then
+      mbar_wait(empty + 8 * st, (u & 1) ^ 1, s_err, WAIT_EMPTY);
+      mbar_expect_tx(full + 8 * st, L::KV_BYTES);
+      tma_load_3d_hint(smem_u32(ring + st * L::KV_BYTES), map, 0, (int)(un.row0 + (un.tile0 + j) * 64), (int)(blockIdx.x * CH), full + 8 * st, policy);
+      if (++st == slots) { st = 0; ++u; }
+    }
+  }
+  __syncwarp();
+  if (is_v && un.ragged) {
+    const uint32_t j = un.n_tiles - 1, st = j % L::NV, from = un.n_rows - (un.tile0 + j) * 64;
+    mbar_wait(full + 8 * st, (j / L::NV) & 1, s_err, WAIT_VFULL);
+    for (uint32_t i = lane; i < (64 - from) * 8 * CH; i += 32) {
+      const uint32_t c = i / ((64 - from) * 8), w = i % ((64 - from) * 8);
+      *reinterpret_cast<uint4*>(ring + st * L::KV_BYTES + c * (64 * 128) + from * 128 + w * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar0 + 8 * SH_V_CLEAN);
+  }
+}
+
+// the other warps.  DIRECT: records of few rows may leave the lanes as they are
+template <int HD, bool WIDE, bool DIRECT>
 __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit& un, uint8_t* base, uint32_t bar0, volatile uint32_t* s_err, uint32_t tmem) {
   using L = ShSmem<HD>;
   using T = ShLay<HD, WIDE>;
@@ -81,45 +117,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
   uint8_t* q_s = base + L::OFF_Q;
   const uint32_t t_q = tmem, t_s0 = tmem + T::T_S, t_o = tmem + T::T_O;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer, K ----
-    if (lane == 0) {
-      for (uint32_t j = 0; j < n_tiles; ++j) {
-        const uint32_t st = j % NK, u = j / NK;
-        if (j == 2) mbar_wait(BAR(SH_Q_READ, 0), 0, s_err, WAIT_QFULL);      // the third slot stages query rows until then
-        mbar_wait(BAR(SH_K_EMPTY, st), (u & 1) ^ 1, s_err, WAIT_EMPTY);
-        mbar_expect_tx(BAR(SH_K_FULL, st), L::KV_BYTES);
-        const uint32_t dst = smem_u32(base + L::OFF_K + st * L::KV_BYTES);
-        if (un.once) tma_load_3d_hint(dst, un.mk, 0, (int)(un.row0 + (tile0 + j) * 64), (int)(g * CH), BAR(SH_K_FULL, st), l2_policy_evict_first());
-        else tma_load_3d(dst, un.mk, 0, (int)(un.row0 + (tile0 + j) * 64), (int)(g * CH), BAR(SH_K_FULL, st));
-      }
-    }
-  } else if (warp == 3) {
-    // ------------------------------------------------------------------ TMA producer, V ----
-    if (lane == 0) {
-      for (uint32_t j = 0; j < n_tiles; ++j) {
-        const uint32_t st = j % NV, u = j / NV;
-        if (j == 1) mbar_wait(BAR(SH_Q_READ, 0), 0, s_err, WAIT_QFULL);      // ... and the second V slot
-        mbar_wait(BAR(SH_V_EMPTY, st), (u & 1) ^ 1, s_err, WAIT_EMPTY);
-        mbar_expect_tx(BAR(SH_V_FULL, st), L::KV_BYTES);
-        const uint32_t dst = smem_u32(base + L::OFF_V + st * L::KV_BYTES);
-        if (un.once) tma_load_3d_hint(dst, un.mv, 0, (int)(un.row0 + (tile0 + j) * 64), (int)(g * CH), BAR(SH_V_FULL, st), l2_policy_evict_first());
-        else tma_load_3d(dst, un.mv, 0, (int)(un.row0 + (tile0 + j) * 64), (int)(g * CH), BAR(SH_V_FULL, st));
-      }
-    }
-    __syncwarp();
-    if (un.ragged) {
-      const uint32_t j = n_tiles - 1, st = j % NV, from = un.n_rows - (tile0 + j) * 64;
-      mbar_wait(BAR(SH_V_FULL, st), (j / NV) & 1, s_err, WAIT_VFULL);
-      for (uint32_t i = lane; i < (64 - from) * 8 * CH; i += 32) {
-        const uint32_t c = i / ((64 - from) * 8), w = i % ((64 - from) * 8);
-        *reinterpret_cast<uint4*>(base + L::OFF_V + st * L::KV_BYTES + c * (64 * 128) + from * 128 + w * 16) = make_uint4(0, 0, 0, 0);
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(BAR(SH_V_CLEAN, 0));
-    }
-  } else if (warp == 1) {
+  if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer, scores ----
     const uint32_t leader = elect_one();
     constexpr uint32_t idesc_qk = umma_idesc(128, 64, 0);
@@ -256,16 +254,17 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
     // more rows go through shared memory, a chunk at a time, so that whole lines leave (a lane has a row: its own stores are 16 bytes
     // each in 32 records 1 KB apart).
     float* s_rl = s_max + 512;
-    auto record = [&](uint32_t seg) {
+    auto record = [&](uint32_t seg, float m, float l) {
       const uint32_t threads = 32 * un.live_warps, gt = (tid - 128) & 127;
       auto slot_of = [&](uint32_t pr) { const uint32_t it = row_item(pr); return ((uint64_t)(un.item0 + it) * p.n_heads + g * G + pr - it * G) * p.n_rec + un.slot + seg; };
-      float l = l_sum;
       if (!WIDE) l += __shfl_xor_sync(0xffffffffu, l, 1);
-      if (wg) s_rl[row] = l;
+      float* sums = s_rl + (seg & 1) * 128 + row;          // two in turn: nothing else may come between two records
+      if (wg) *sums = l;
       named_bar_sync(3 + qd, 64);
-      if (!wg && live && !is_lo) reinterpret_cast<float2*>(p.part_ml)[slot_of(lr)] = make_float2(m_st, l + s_rl[row]);
-      l_sum = 0.f;
-      float* xs = reinterpret_cast<float*>(base + L::OFF_Q + (WIDE ? 2 * wg * L::X_BYTES : L::QS_BYTES + wg * L::X_BYTES));
+      if (!wg && live && !is_lo) reinterpret_cast<float2*>(p.part_ml)[slot_of(lr)] = make_float2(m, l + *sums);
+      const bool only = WIDE || n_tiles <= p.seg;
+      constexpr uint32_t XW = WIDE ? 2 * L::X_BYTES : L::X_BYTES;
+      uint8_t* xb = only ? base + L::OFF_K + wg * XW : base + L::OFF_Q + L::QS_BYTES + wg * L::X_BYTES;
       mbar_wait(BAR(SH_O_DONE, 0), seg & 1, s_err, WAIT_MMA);
       tc_fence_after();
       // high and low rows of a chunk added, each lane with half of it
@@ -276,7 +275,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
           t[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
         }
       };
-      if (!WIDE && un.live_warps == 1) {
+      if (DIRECT && un.live_warps == 1) {
         constexpr int N = HD / 32 > GRP ? 2 : 1;          // chunks at a time
         float* to = p.part_o + slot_of(live ? lr : 0) * HD + (is_lo ? 16 : 0);
 #pragma unroll 1
@@ -302,7 +301,8 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       for (int c = wg; c < HD / 32; c += GRP) {           // the groups share the chunks out
         float o[32];
         tmem_ld32(t_o + c * 32 + lane_addr, o);
-        if (c != (int)wg) named_bar_sync(7 + wg, threads);
+        if (!only && c != (int)wg) named_bar_sync(7 + wg, threads);
+        float* xs = reinterpret_cast<float*>(xb + (only ? (c / GRP) * GRP * XW : 0));       // (a place for each chunk of the only record)
         if constexpr (WIDE) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(xs + row * L::XP + 4 * i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -321,7 +321,9 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       mbar_arrive(BAR(SH_O_FREE, 0));
     };
     if (in_use) {
-      for (uint32_t j = 0, seg = 0, in_seg = 0; j < n_tiles; ++j) {
+      float m_old = -3.0e30f, l_old = 0.f;                // of the record to be written next (m below -2e30: none)
+      for (uint32_t j = 0, seg = 0, in_seg = 0;; ++j) {
+        if (j < n_tiles) {
         const uint32_t b = j % SB, u = j / SB, kv0 = (tile0 + j) * 64;
         mbar_wait(BAR(SH_S_FULL, b), u & 1, s_err, WAIT_MMA);
         tc_fence_after();
@@ -395,7 +397,13 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(BAR(SH_P_FULL, b));
-        if (++in_seg == p.seg || j == n_tiles - 1) { record(seg++); in_seg = 0; }
+        }
+        // a record is written behind the weights of the tile after its last, while the products of its last retire
+        const bool last = j == n_tiles;
+        if (last) { m_old = m_st; l_old = l_sum; }
+        if (m_old > -2.0e30f) { record(seg++, m_old, l_old); m_old = -3.0e30f; }
+        if (last) break;
+        if (++in_seg == p.seg && j != n_tiles - 1) { m_old = m_st; l_old = l_sum; l_sum = 0.f; in_seg = 0; }
       }
     }
   }
@@ -432,7 +440,6 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
     un.row0 = p.seq[lo] * p.max_seq + p.own_row0; un.n_rows = p.rows[lo]; tps = p.tps; un.slot = p.p_recs;
     un.mk = &tm_k; un.mv = &tm_v;
   }
-  un.once = !un.shared || p.row_tiles == 1;
   un.tile0 = split * tps;
   un.slot += un.tile0 / p.seg;                                        // (tiles per unit: a multiple of seg)
   un.n_tiles = min((un.n_rows + 63) / 64, un.tile0 + tps) - un.tile0;
@@ -460,10 +467,14 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  if constexpr (MIXED) {
-    if (wide) shared_roles<HD, true>(p, un, base, bar0, s_err, tmem);
+  if (warp == 0 || warp == 3) {
+    shared_producer<HD>(un, warp == 3, base, bar0, s_err);
+  } else {
+    if constexpr (MIXED) {
+      if (wide) shared_roles<HD, true, false>(p, un, base, bar0, s_err, tmem);
+    }
+    if (!wide) shared_roles<HD, false, !MIXED>(p, un, base, bar0, s_err, tmem);
   }
-  if (!wide) shared_roles<HD, false>(p, un, base, bar0, s_err, tmem);
   __syncthreads();
   if (warp == 2) {
     tc_fence_after();
@@ -614,11 +625,11 @@ static cudaError_t launch_shared_t(const SharedParams& p, const CUtensorMap& pk,
   using S = ShSmem<HD>;
   static std::atomic<bool> attr_set[64];
   if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(pa_shared_kernel<HD, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
+    cudaError_t e = cudaFuncSetAttribute(pa_shared_kernel<HD, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::total(true));
     if (e != cudaSuccess) return e;
     attr_set[dev & 63].store(true, std::memory_order_release);
   }
-  return launch_pdl(pa_shared_kernel<HD, MIXED>, dim3(n_kv, p.units), dim3(S::THREADS), (size_t)S::TOTAL, st, pk, pv, k, v, p);
+  return launch_pdl(pa_shared_kernel<HD, MIXED>, dim3(n_kv, p.units), dim3(S::THREADS), (size_t)S::total(p.seg < p.tps), st, pk, pv, k, v, p);
 }
 cudaError_t launch_shared(const SharedParams& p, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v, uint32_t hd, uint32_t n_kv,
                           int dev, cudaStream_t st) {

@@ -99,7 +99,7 @@ static int shared_launch(const SharedCall& c, const pa_item* items, const uint32
   p.items_per_tile = 64 / G; p.row_tiles = ceil_div(n, p.items_per_tile);
   float us = 0.f, wide_us = 0.f;
   uint32_t T = plan_units(ctx, rows + first, n, p_tiles, p.row_tiles, unit_cost(hd, false), most, &us);
-  if (p_tiles && p.row_tiles > 1 && c.q_f16) {
+  if (p_tiles && p.row_tiles > 1 && c.q_f16 && ctx->cfg.act_dtype == PA_F16) {
     const uint32_t tiles128 = ceil_div(n, 128 / G), T128 = plan_units(ctx, rows + first, n, p_tiles, tiles128, unit_cost(hd, true), most, &wide_us);
     if (wide_us < us) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }
   }

@@ -140,6 +140,23 @@ def test_long_prefix_in_many_splits():
         close(got[i], want, vv, delta, 20011 + n)
 
 
+@pytest.mark.parametrize("nH,nKV,hd,n,prefix_len", [(24, 4, 256, 11, 9001), (16, 2, 256, 5, 16000), (16, 8, 128, 40, 5000), (8, 8, 64, 70, 7000)])
+def test_f32_records_of_a_few_tiles(nH, nKV, hd, n, prefix_len):
+    # f32 outputs: a unit of many tiles leaves several records, whatever its last one holds.  What the tensor cores' sums lose by rounding
+    # towards zero stays below that of 16 tiles: 2^-24 of the running sum at each of 64 additions, half of them at half of it
+    eng, first = engine(nH, nKV, hd, 1300, n, F32), engine(nH, nKV, hd, prefix_len, 1, F32)
+    k, v = fill(eng, 13)
+    pk, pv = fill(first, 14)
+    own = [(97 * i * i) % 1301 for i in range(n)]
+    q = torch.randn((n, nH * hd), device="cuda")
+    got = eng.decode_shared(0, first, 0, prefix_len, [(i, prefix_len - 1 + own[i]) for i in range(n)], q, own_base=prefix_len)
+    for i in range(0, n, 3):
+        kk, vv = torch.cat([pk[0], k[i, :own[i]]]), torch.cat([pv[0], v[i, :own[i]]])
+        want, _, delta = attend(q[i].view(nH, hd), kk, vv)
+        close(got[i], want, vv, delta, prefix_len + own[i])
+        assert (got[i].double().view(want.shape) - want).norm() <= 3e-6 * want.norm()
+
+
 def test_rising_scores_move_the_reference_maximum():
     # every tile's maximum passes the last one's by far: each tile rescales what is summed so far
     eng = engine(2, 1, 128, 1000, 1, F32)
