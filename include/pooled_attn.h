@@ -395,8 +395,8 @@ PA_API int pa_rotary_append(pa_rotary* rotary, pa_layer* layer, const pa_item* i
  * seq of layer.  own_base = 0: sequences that keep every position in the row of that number (the first prefix_len of them
  * unused); own_base = prefix_len: sequences that hold nothing but their own rows.  pos + 1 >= prefix_len; own rows may be
  * none.  prefix_layer = NULL: layer itself; else any f16 layer of the same device and kv heads x head_dim, its context's too.
- * Items may repeat a sequence (each is one query against the rows it names).  q, gate, out: as pa_decode's, q strides
- * multiples of 16 bytes and q 16-byte aligned.  At most 128 items and 64 query heads per kv head; f16 caches, no KV shards
+ * Items may repeat a sequence (each is one query against the rows it names).  q, gate, out: as pa_decode's (f32 q within the
+ * range of f16, whose pairs it enters as; PA_FLAG_FAST changes nothing here), q strides multiples of 16 bytes and q 16-byte aligned.  At most 128 items and 64 query heads per kv head; f16 caches, no KV shards
  * (origin 0). */
 PA_API int pa_decode_shared(pa_layer* layer, pa_layer* prefix_layer, uint32_t prefix_seq, uint32_t prefix_len, uint32_t own_base,
                             const pa_item* items, uint32_t n_items, const void* q, int q_dtype, uint64_t q_col_stride,

@@ -6,9 +6,10 @@
 // A unit is a run of 64-row K / V tiles of one kv head and the query rows that attend them: for the shared rows the heads of
 // several items (so that a shared byte is read once for all of these, from HBM once in all), for own rows the heads of one.
 // A CTA per unit walks its tiles on the 5th-generation tensor cores and leaves an unnormalised (o, m, l) record per query
-// row (with f32 outputs one every p.seg tiles: the tensor cores' sums round towards zero, which after 32 tiles has cost 2.3e-6 of the
-// result, after four 6e-7); the second kernel merges a row's records, gates and stores.  All units have the same number of tiles, whatever they
-// are units of (plan_units), so that a batch of long shared rows and short own ones fills the machine like one long conversation.
+// row (with f32 outputs one every p.seg tiles: the tensor cores' sums round towards zero, which after 32 tiles has cost 2.3e-6
+// of the result, after four 6e-7); the second kernel merges a row's records, gates and stores.  All units have the same number
+// of tiles, whatever they are units of (plan_units), so that a batch of long shared rows and short own ones fills the machine
+// like one long conversation.
 //
 //   warps 0, 3  TMA producers: K tiles and V tiles (64 x head_dim f16, 128-byte swizzle), a ring of three and of two slots;
 //               warp 3 then clears the rows of the last V tile that lie behind the unit's last: a weight of zero does not
@@ -17,7 +18,8 @@
 //   warp 2      tensor memory; issues O += P V into the accumulator (128 x head_dim f32)
 //   warps 4-11  softmax, two groups of four warps with half of a tile's keys each (on alternate tiles, a call of one tile a CTA took
 //               0.4 us longer, and wide tiles 1.5 us each).  A row's reference lies 2^7 below its maximum and moves only when a tile
-//               passes it by 2^15: weights of up to 2^15 keep the low parts of small ones above f16's last place.  Warps whose rows hold no query take no part.
+//               passes it by 2^15: weights of up to 2^15 keep the low parts of small ones above f16's last place.  Warps whose rows
+//               hold no query take no part
 // q and the weights enter as pairs of f16 values, high and low parts, some 22 bits of both, in one of two ways:
 //   narrow (up to 64 query rows)   even rows of the 128 carry the high parts, odd rows the low parts of the same query row, added by
 //               shuffles: both products at the cost of one, and the two lanes share the row's keys out.  0.75 us a tile of 64 keys
@@ -324,79 +326,79 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       float m_old = -3.0e30f, l_old = 0.f;                // of the record to be written next (m below -2e30: none)
       for (uint32_t j = 0, seg = 0, in_seg = 0;; ++j) {
         if (j < n_tiles) {
-        const uint32_t b = j % SB, u = j / SB, kv0 = (tile0 + j) * 64;
-        mbar_wait(BAR(SH_S_FULL, b), u & 1, s_err, WAIT_MMA);
-        tc_fence_after();
-        float s[NS];
-        if constexpr (WIDE) {
-          tmem_ld32(t_s0 + b * 64 + wg * 32 + lane_addr, s);
-        } else {
-          // a lane sends the half of its row (high or low parts) that the other lane has the keys of, and adds what comes back to its own
-          float t[32];
-          tmem_ld32(t_s0 + b * 64 + wg * 32 + lane_addr, t);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float give = is_lo ? t[i] : t[16 + i], keep = is_lo ? t[16 + i] : t[i];
-            s[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
-          }
-        }
-        if (!WIDE && sc) {
-          float4* d = reinterpret_cast<float4*>(sc + j * 64);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) d[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-        }
-        if (kv0 + 64 > un.n_rows) {
-#pragma unroll
-          for (int i = 0; i < NS; ++i) if (kv0 + mine + i >= un.n_rows) s[i] = -INFINITY;
-        }
-        float mt = s[0];
-#pragma unroll
-        for (int i = 1; i < NS; ++i) mt = fmaxf(mt, s[i]);
-        if (!WIDE) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-        mt = row_max(mt, j) * p.scale_log2;
-        float alpha = 1.f;
-        bool grow = false;
-        if (mt > m_st + 15.f) { alpha = ex2_approx(m_st - (mt - 7.f)); m_st = mt - 7.f; l_sum *= alpha; grow = true; }
-        if (in_seg > 0 && __any_sync(0xffffffffu, grow)) {
-          const uint32_t jb = (j - 1) % SB, ju = (j - 1) / SB;
-          mbar_wait(BAR(SH_PV_DONE, jb), ju & 1, s_err, WAIT_MMA);
+          const uint32_t b = j % SB, u = j / SB, kv0 = (tile0 + j) * 64;
+          mbar_wait(BAR(SH_S_FULL, b), u & 1, s_err, WAIT_MMA);
           tc_fence_after();
+          float s[NS];
+          if constexpr (WIDE) {
+            tmem_ld32(t_s0 + b * 64 + wg * 32 + lane_addr, s);
+          } else {
+            // a lane sends the half of its row (high or low parts) that the other lane has the keys of, and adds what comes back to its own
+            float t[32];
+            tmem_ld32(t_s0 + b * 64 + wg * 32 + lane_addr, t);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float give = is_lo ? t[i] : t[16 + i], keep = is_lo ? t[16 + i] : t[i];
+              s[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+            }
+          }
+          if (!WIDE && sc) {
+            float4* d = reinterpret_cast<float4*>(sc + j * 64);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+          }
+          if (kv0 + 64 > un.n_rows) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) if (kv0 + mine + i >= un.n_rows) s[i] = -INFINITY;
+          }
+          float mt = s[0];
+#pragma unroll
+          for (int i = 1; i < NS; ++i) mt = fmaxf(mt, s[i]);
+          if (!WIDE) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+          mt = row_max(mt, j) * p.scale_log2;
+          float alpha = 1.f;
+          bool grow = false;
+          if (mt > m_st + 15.f) { alpha = ex2_approx(m_st - (mt - 7.f)); m_st = mt - 7.f; l_sum *= alpha; grow = true; }
+          if (in_seg > 0 && __any_sync(0xffffffffu, grow)) {
+            const uint32_t jb = (j - 1) % SB, ju = (j - 1) / SB;
+            mbar_wait(BAR(SH_PV_DONE, jb), ju & 1, s_err, WAIT_MMA);
+            tc_fence_after();
 #pragma unroll 1
-          for (int c = wg; c < HD / 32; c += GRP) {       // the groups share the columns out
-            float o[32];
-            tmem_ld32(t_o + c * 32 + lane_addr, o);
+            for (int c = wg; c < HD / 32; c += GRP) {       // the groups share the columns out
+              float o[32];
+              tmem_ld32(t_o + c * 32 + lane_addr, o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= alpha;
-            tmem_st32(t_o + c * 32 + lane_addr, o);
+              for (int i = 0; i < 32; ++i) o[i] *= alpha;
+              tmem_st32(t_o + c * 32 + lane_addr, o);
+            }
           }
-        }
-        // weights as f16 pairs, high and low parts
-        uint32_t hi[NS / 2], lo[NS / 2];
+          // weights as f16 pairs, high and low parts
+          uint32_t hi[NS / 2], lo[NS / 2];
 #pragma unroll
-        for (int i = 0; i < NS / 2; ++i) {
-          const float e0 = ex2_approx(fmaf(s[2 * i], p.scale_log2, -m_st)), e1 = ex2_approx(fmaf(s[2 * i + 1], p.scale_log2, -m_st));
-          l_sum += e0 + e1;
-          const __half2 h = __floats2half2_rn(e0, e1);
-          const float2 f = __half22float2(h);
-          hi[i] = *reinterpret_cast<const uint32_t*>(&h); lo[i] = pack_h2(e0 - f.x, e1 - f.y);
-        }
-        if constexpr (WIDE) {
-          tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, hi);
-          tmem_st16u(t_s0 + b * 64 + 32 + 16 * wg + lane_addr, lo);
-        } else {
-          // the even lane's row takes the high parts of the group's 32 keys, the odd one's the low parts
-          uint32_t pw[16];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, is_lo ? hi[i] : lo[i], 1);
-            pw[i] = is_lo ? got : hi[i];
-            pw[8 + i] = is_lo ? lo[i] : got;
+          for (int i = 0; i < NS / 2; ++i) {
+            const float e0 = ex2_approx(fmaf(s[2 * i], p.scale_log2, -m_st)), e1 = ex2_approx(fmaf(s[2 * i + 1], p.scale_log2, -m_st));
+            l_sum += e0 + e1;
+            const __half2 h = __floats2half2_rn(e0, e1);
+            const float2 f = __half22float2(h);
+            hi[i] = *reinterpret_cast<const uint32_t*>(&h); lo[i] = pack_h2(e0 - f.x, e1 - f.y);
           }
-          tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, pw);
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(BAR(SH_P_FULL, b));
+          if constexpr (WIDE) {
+            tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, hi);
+            tmem_st16u(t_s0 + b * 64 + 32 + 16 * wg + lane_addr, lo);
+          } else {
+            // the even lane's row takes the high parts of the group's 32 keys, the odd one's the low parts
+            uint32_t pw[16];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, is_lo ? hi[i] : lo[i], 1);
+              pw[i] = is_lo ? got : hi[i];
+              pw[8 + i] = is_lo ? lo[i] : got;
+            }
+            tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, pw);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(BAR(SH_P_FULL, b));
         }
         // a record is written behind the weights of the tile after its last, while the products of its last retire
         const bool last = j == n_tiles;
@@ -562,60 +564,60 @@ __global__ void __launch_bounds__(256, SUMS ? 3 : 4) pa_shared_finish_kernel(con
     return;
   }
   if constexpr (SUMS) {
-  // ---- sums of the weights ----
-  const uint32_t u0 = blockIdx.x - p.merge_ctas;
-  uint32_t lo = 0, hi = p.n_leads - 1;
-  while (lo < hi) { const uint32_t mid = (lo + hi + 1) / 2; if (u0 >= p.sum0[mid]) lo = mid; else hi = mid - 1; }
-  const uint32_t per_head = (p.sum0[lo + 1] - p.sum0[lo]) / p.n_kv, w = u0 - p.sum0[lo], kvh = w / per_head;
-  const uint32_t hg = tid >> 6, r0 = (w % per_head) * kSumRows + (tid & 63) * 4;     // this thread's heads: hg, hg + 4, ...; its rows
-  uint32_t item = p.lead[lo], most = 0;
-  for (uint32_t i = item; i != 255; i = p.next[i]) most = max(most, p.rows[i]);
-  float* sums = p.sums + ((uint64_t)p.seq[item] * p.n_kv + kvh) * p.max_seq + r0;
-  float old[4];
+    // ---- sums of the weights ----
+    const uint32_t u0 = blockIdx.x - p.merge_ctas;
+    uint32_t lo = 0, hi = p.n_leads - 1;
+    while (lo < hi) { const uint32_t mid = (lo + hi + 1) / 2; if (u0 >= p.sum0[mid]) lo = mid; else hi = mid - 1; }
+    const uint32_t per_head = (p.sum0[lo + 1] - p.sum0[lo]) / p.n_kv, w = u0 - p.sum0[lo], kvh = w / per_head;
+    const uint32_t hg = tid >> 6, r0 = (w % per_head) * kSumRows + (tid & 63) * 4;     // this thread's heads: hg, hg + 4, ...; its rows
+    uint32_t item = p.lead[lo], most = 0;
+    for (uint32_t i = item; i != 255; i = p.next[i]) most = max(most, p.rows[i]);
+    float* sums = p.sums + ((uint64_t)p.seq[item] * p.n_kv + kvh) * p.max_seq + r0;
+    float old[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) old[e] = hg == 0 && r0 + e < most ? sums[e] : 0.f;
-  float4 add = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (; item != 255; item = p.next[item]) {
-    const uint32_t ns = p.p_recs + p.n_own[item], rows = p.rows[item], pad = (rows + 63) & ~63u;
-    const float* sc = p.scores + p.score0[item] + (uint64_t)kvh * p.G * pad + r0;
-    constexpr int U = 4;
-    float4 s[U];
+    for (int e = 0; e < 4; ++e) old[e] = hg == 0 && r0 + e < most ? sums[e] : 0.f;
+    float4 add = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (; item != 255; item = p.next[item]) {
+      const uint32_t ns = p.p_recs + p.n_own[item], rows = p.rows[item], pad = (rows + 63) & ~63u;
+      const float* sc = p.scores + p.score0[item] + (uint64_t)kvh * p.G * pad + r0;
+      constexpr int U = 4;
+      float4 s[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (r0 < rows && hg + 4 * u < p.G) s[u] = *reinterpret_cast<const float4*>(sc + (uint64_t)(hg + 4 * u) * pad);
-    for (uint32_t h = warp; h < p.G; h += 8) {
-      float M, l;
-      row_ml(reinterpret_cast<const float2*>(p.part_ml) + ((uint64_t)item * p.n_heads + kvh * p.G + h) * p.n_rec, ns, M, l);
-      if (lane == 0) { s_m[h] = M; s_il[h] = __fdiv_rn(1.0f, l); }
+      for (int u = 0; u < U; ++u)
+        if (r0 < rows && hg + 4 * u < p.G) s[u] = *reinterpret_cast<const float4*>(sc + (uint64_t)(hg + 4 * u) * pad);
+      for (uint32_t h = warp; h < p.G; h += 8) {
+        float M, l;
+        row_ml(reinterpret_cast<const float2*>(p.part_ml) + ((uint64_t)item * p.n_heads + kvh * p.G + h) * p.n_rec, ns, M, l);
+        if (lane == 0) { s_m[h] = M; s_il[h] = __fdiv_rn(1.0f, l); }
+      }
+      __syncthreads();
+      float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r0 < rows) {
+        auto weigh = [&](const float4& v, uint32_t h) {
+          const float m = s_m[h], il = s_il[h];
+          t.x = fmaf(ex2_approx(fmaf(v.x, p.scale_log2, -m)), il, t.x); t.y = fmaf(ex2_approx(fmaf(v.y, p.scale_log2, -m)), il, t.y);
+          t.z = fmaf(ex2_approx(fmaf(v.z, p.scale_log2, -m)), il, t.z); t.w = fmaf(ex2_approx(fmaf(v.w, p.scale_log2, -m)), il, t.w);
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u) if (hg + 4 * u < p.G) weigh(s[u], hg + 4 * u);
+        for (uint32_t h = hg + 4 * U; h < p.G; h += 4) weigh(*reinterpret_cast<const float4*>(sc + (uint64_t)h * pad), h);
+      }
+      s_acc[tid] = t;
+      __syncthreads();
+      if (hg == 0 && r0 < rows) {
+#pragma unroll
+        for (int i = 1; i < 4; ++i) { const float4 v = s_acc[tid + 64 * i]; t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w; }
+        add.x += t.x;
+        if (r0 + 1 < rows) add.y += t.y;
+        if (r0 + 2 < rows) add.z += t.z;
+        if (r0 + 3 < rows) add.w += t.w;
+      }
     }
-    __syncthreads();
-    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r0 < rows) {
-      auto weigh = [&](const float4& v, uint32_t h) {
-        const float m = s_m[h], il = s_il[h];
-        t.x = fmaf(ex2_approx(fmaf(v.x, p.scale_log2, -m)), il, t.x); t.y = fmaf(ex2_approx(fmaf(v.y, p.scale_log2, -m)), il, t.y);
-        t.z = fmaf(ex2_approx(fmaf(v.z, p.scale_log2, -m)), il, t.z); t.w = fmaf(ex2_approx(fmaf(v.w, p.scale_log2, -m)), il, t.w);
-      };
+    if (hg == 0) {
+      const float a[4] = {add.x, add.y, add.z, add.w};
 #pragma unroll
-      for (int u = 0; u < U; ++u) if (hg + 4 * u < p.G) weigh(s[u], hg + 4 * u);
-      for (uint32_t h = hg + 4 * U; h < p.G; h += 4) weigh(*reinterpret_cast<const float4*>(sc + (uint64_t)h * pad), h);
+      for (int e = 0; e < 4; ++e) if (r0 + e < most) sums[e] = old[e] + a[e];
     }
-    s_acc[tid] = t;
-    __syncthreads();
-    if (hg == 0 && r0 < rows) {
-#pragma unroll
-      for (int i = 1; i < 4; ++i) { const float4 v = s_acc[tid + 64 * i]; t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w; }
-      add.x += t.x;
-      if (r0 + 1 < rows) add.y += t.y;
-      if (r0 + 2 < rows) add.z += t.z;
-      if (r0 + 3 < rows) add.w += t.w;
-    }
-  }
-  if (hg == 0) {
-    const float a[4] = {add.x, add.y, add.z, add.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) if (r0 + e < most) sums[e] = old[e] + a[e];
-  }
   }
 }
 
