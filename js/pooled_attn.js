@@ -139,6 +139,7 @@ export class NativeAttention {
     // the engine walks its layers in order, the last one followed by the first of the next token
     if (nLayers > 1) this.layers.forEach((L, i) => check(S.pa_layer_set_next(L, this.layers[(i + 1) % nLayers]), this.ctx));
     this.slots = new Map();
+    this.rotaries = [];
   }
   // device memory for the engine's q_full / k / v / attnOut when it has no CUDA binding of its own
   alloc(bytes) { const p = outPtr(); check(this.S.pa_alloc(this.ctx, BigInt(bytes), new Uint8Array(p.buffer)), this.ctx); return asPtr(p); }
@@ -176,6 +177,37 @@ export class NativeAttention {
     const { hd, qDim, kvDim } = this.dims, it = paItems(items.map(([s, p]) => [s, p, 1]));
     check(this.S.pa_attn_items(this.layers[li], new Uint8Array(it.buffer), items.length, q, BigInt(qDim), BigInt(hd), k, v, BigInt(kvDim), gate, BigInt(qDim), BigInt(hd),
       out, BigInt(qDim), sharded ? 1 : 0, stream), this.ctx);
+  }
+  // A rotation beside the context's own (include/pooled_attn.h, pa_rotary_config): layout 0 half, 1 interleaved; scaling 0 none, 1 linear,
+  // 2 ntk, 3 yarn, 4 bands.  u32 n_rot, layout, scaling, original; f64 theta, factor, fast, slow, mscale; u32 reserved[4]
+  rotary({ nRot, theta, layout = 0, scaling = 0, original = 0, factor = 1, fast = 0, slow = 0, mscale = 0 }) {
+    const b = new ArrayBuffer(72), u = new Uint32Array(b), f = new Float64Array(b), h = outPtr();
+    u.set([nRot, layout, scaling, original]); f.set([theta, factor, fast, slow, mscale], 2);
+    check(this.S.pa_rotary_create(this.ctx, new Uint8Array(b), new Uint8Array(h.buffer)), this.ctx);
+    this.rotaries.push(asPtr(h));
+    return this.rotaries.at(-1);
+  }
+  // the front of a layer call with it: items = [[seq, pos, nCols], ...], rows = the cache rows to store in (null: those of the positions)
+  rotaryAppend(li, rot, items, rows, q, k, v, qOut, { f16Out = false, stream = null } = {}) {
+    const { hd, qDim, kvDim } = this.dims, it = paItems(items), r = rows && new Uint8Array(Uint32Array.from(rows).buffer);
+    check(this.S.pa_rotary_append(rot, this.layers[li], new Uint8Array(it.buffer), items.length, r, q, BigInt(qDim), BigInt(hd), k, v, BigInt(kvDim), qOut,
+      f16Out ? PA_F16 : PA_F32, BigInt(qDim), stream), this.ctx);
+  }
+  // one token each of sequences that begin with the same prefixLen rows, kept once: items = [[seq, pos], ...], q rotated, of the activations' type
+  decodeShared(li, prefixLayer, prefixSeq, prefixLen, items, q, gate, out, { ownBase = 0, stream = null } = {}) {
+    const { hd, qDim } = this.dims, it = paItems(items.map(([s, p]) => [s, p, 1]));
+    check(this.S.pa_decode_shared(this.layers[li], prefixLayer, prefixSeq, prefixLen, ownBase, new Uint8Array(it.buffer), items.length, q, this.es === 2 ? PA_F16 : PA_F32,
+      BigInt(qDim), BigInt(hd), gate, BigInt(qDim), BigInt(hd), out, BigInt(qDim), stream), this.ctx);
+  }
+  // a cache kept to a budget: sums of attention weights per row, and the rows with the largest kept (items = [[srcSeq, dstSeq, nRows], ...])
+  trackWeights(li) { check(this.S.pa_layer_track_weights(this.layers[li]), this.ctx); }
+  decodeWeights(li, items, q, gate, out, { stream = null } = {}) {
+    const { hd, qDim } = this.dims, it = paItems(items.map(([s, p]) => [s, p, 1]));
+    check(this.S.pa_decode_weights(this.layers[li], new Uint8Array(it.buffer), items.length, q, this.es === 2 ? PA_F16 : PA_F32, BigInt(qDim), BigInt(hd), gate, BigInt(qDim),
+      BigInt(hd), out, BigInt(qDim), stream), this.ctx);
+  }
+  evict(li, items, nKeep, { nFirst = 0, nRecent = 0, kept = null, stream = null } = {}) {
+    check(this.S.pa_evict(this.layers[li], new Uint8Array(paItems(items).buffer), items.length, nKeep, nFirst, nRecent, kept, stream), this.ctx);
   }
   async sync(stream = null) { check(await this.S.pa_sync(this.ctx, stream), this.ctx); }
   reset() { check(this.S.pa_reset(this.ctx), this.ctx); }   // after a failed step every call rejects until here (engine/qwen35.js:111-119)
@@ -218,6 +250,7 @@ export class NativeAttention {
   destroy() {
     for (const k of [...this.slots.keys()]) this.dropSlot(k);
     this.layers.forEach((L) => this.S.pa_layer_destroy(L));
+    this.rotaries.forEach((r) => this.S.pa_rotary_destroy(r));
     this.S.pa_destroy(this.ctx);
     this.layers = []; this.ctx = null;
   }

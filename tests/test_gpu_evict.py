@@ -188,6 +188,40 @@ def test_decode_right_behind_an_eviction():
         close(got[0], want, vv, delta, len(kk))
 
 
+@pytest.mark.parametrize("act", [F16, F32])
+def test_layers_in_turn_behind_evictions_and_turned_caches(act):
+    # two layers of one context, each given up rows, its remaining keys turned back by what the rows have moved (in place, in the cache), then
+    # whole layer calls: the fused token fetches rows ahead of its own wait, and none of them may be of before
+    eng = AttnEngine(AttnConfig(n_heads=16, n_kv_heads=2, head_dim=256, n_rot=64, rope_theta=1e7, max_seq=2100, n_layers=2, act_dtype=act, max_cols=64))
+    rot = eng.rotary()
+    g = torch.Generator(device="cuda").manual_seed(7)
+    new = lambda *s: torch.empty(s, device="cuda").normal_(generator=g)
+    for _ in range(6):
+        for li in (0, 1):
+            for w in "kv":
+                eng.cache(li, w).view(F16).copy_(new(1, 2100, 512))
+            eng.track_weights(li)
+            eng.weights(li).copy_(new(1, 2, 2100).abs())
+        before = [[eng.cache(li, w)[0].view(F16).clone().view(2100, 2, 256) for w in "kv"] for li in (0, 1)]
+        kept = [eng.evict(li, [(0, 0, 2000)], 1500, n_first=2, n_recent=30) for li in (0, 1)]
+        back = torch.full((1500,), -500, dtype=torch.int32, device="cuda")
+        q, k, v = new(1, 4096).to(act), new(1, 512).to(act), new(1, 512).to(act)
+        for li in (0, 1):
+            rows = eng.cache(li, "k")[0, :1500].view(F16)
+            rot.apply(rows, 2, positions=back, out=rows)
+            got = eng.encode_layer(li, 1500, q, k, v)
+            eng.sync()
+            at = kept[li][0].long().t()[..., None].expand(-1, -1, 256)
+            kk, vv = [x.gather(0, at) for x in before[li]]
+            turned, _ = rotated(kk, [-500] * 1500, *frequencies(64, 1e7), "half")
+            kk = torch.from_numpy(turned).cuda()
+            held = eng.cache(li, "k")[0, :1501].view(F16).view(1501, 2, 256)
+            assert torch.all((held[:1500].double() - kk).abs() <= 2.0 ** -10 * kk.abs() + 2.0 ** -18)
+            qr, _ = rotated(q.view(1, 16, 256), [1500], *frequencies(64, 1e7), "half")
+            want, _, delta = attend(torch.from_numpy(qr[0]).cuda(), held, torch.cat([vv, v.half().view(1, 2, 256)]))
+            close(got[0], want, vv, delta, 1501)
+
+
 def test_streams_and_graphs():
     eng = tracked(16, 8, 128, 1000, 2, F16)
     fill(eng, 9)

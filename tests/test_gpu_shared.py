@@ -186,6 +186,26 @@ def test_rows_appended_just_before():
         close(got[0], want, vv, delta, 500 + n)
 
 
+def test_prefix_appended_just_before():
+    # the prefix's own context, and a layer of the same one, write rows that the next call attends
+    eng = engine(16, 8, 128, 400, 3, F32, max_cols=512)
+    other = engine(16, 8, 128, 400, 1, F32, max_cols=512)
+    rot = [e.rotary(n_rot=64) for e in (eng, other)]
+    fill(eng, 20)
+    q = torch.randn((2, 2048), device="cuda")
+    for turn in range(8):
+        k, v = [torch.randn((300, 1024), device="cuda") for _ in "kv"]
+        for e, r, pre in ((eng, rot[0], None), (other, rot[1], other)):
+            e.rotary_append(0, r, [(0, 0, 300)], None, k, v)
+            got = eng.decode_shared(0, pre, 0, 300, [(1, 320), (2, 299)], q)
+            pk, pv = [e.cache(0, w)[0, :300].view(F16).view(300, 8, 128) for w in "kv"]
+            for i, (s, n) in enumerate(((1, 21), (2, 0))):
+                ok, ov = [eng.cache(0, w)[s, 300:300 + n].view(F16).view(n, 8, 128) for w in "kv"]
+                vv = torch.cat([pv, ov])
+                want, _, delta = attend(q[i].view(16, 128), torch.cat([pk, ok]), vv)
+                close(got[i], want, vv, delta, 300 + n)
+
+
 def test_streams_graphs_and_repeats():
     eng, first = engine(24, 4, 256, 300, 3, F32), engine(24, 4, 256, 3000, 1, F32)
     fill(eng, 10); fill(first, 11)
