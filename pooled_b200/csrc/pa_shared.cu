@@ -23,11 +23,13 @@
 // q and the weights enter as pairs of f16 values, high and low parts, some 22 bits of both, in one of two ways:
 //   narrow (up to 64 query rows)   even rows of the 128 carry the high parts, odd rows the low parts of the same query row, added by
 //               shuffles: both products at the cost of one, and the two lanes share the row's keys out.  0.75 us a tile of 64 keys
-//               at head_dim 256 (the tensor cores: 1394 cycles), 0.67 at 128 and 64 (the softmax)
-//   wide (shared rows of more, f16 queries and outputs, where the plan finds it faster)   128 query rows without low parts of q; the low parts
-//               of the weights are multiplied behind the high ones into the same accumulator.  1.17 us a tile at head_dim 256, 0.64 at 128,
-//               and a start 5 us longer.  (With f32 queries and the products of their low parts: 1.43 us and 13 us of start, slower than two
-//               narrow tiles at every size tried.)
+//               at head_dim 256 (the tensor cores: 1394 cycles); 0.67 at 128 and 64 (the chain through the softmax), 0.8 of two
+//               CTAs an SM
+//   wide (head_dim 256, f16 queries and outputs, shared rows of more than 64 query rows, where the plan finds it faster)   128 query
+//               rows without low parts of q; the low parts of the weights are multiplied behind the high ones into the same
+//               accumulator.  1.17 us a tile and a start 5 us longer: 32 items of 8 heads behind 32768 rows 35 us, narrow 42.  (With f32
+//               queries and the products of their low parts 1.43 us and 13 us of start, slower than two narrow tiles at every size
+//               tried; at head_dim 128 0.64 us, slower than two narrow CTAs an SM.)
 // What bounds it: HBM, one query tile per kv head and long rows; the tensor cores, several; short calls the chain of launch, q,
 // scores, weights, products and records, and fetching the code for it: without wide units a kernel of half the code runs.
 #include <algorithm>
@@ -38,29 +40,30 @@ namespace pa {
 
 template <int HD>
 struct ShSmem {
-  static constexpr int NK = 3, NV = 2;
+  // head_dim 128 and 64: two CTAs an SM (80 registers, 256 columns of tensor memory, 102 KB), so that one fetches, starts or stores while
+  // the other multiplies
+  static constexpr int CTAS = HD == 256 ? 1 : 2;
+  static constexpr int NK = HD == 128 ? 2 : 3, NV = 2;
   static constexpr int KV_BYTES = HD * 128;          // [HD/64][64 rows][128 B]
   static constexpr int THREADS = 384;
   static constexpr int OFF_K = 0, OFF_V = NK * KV_BYTES, OFF_BAR = (NK + NV) * KV_BYTES;
   static constexpr int OFF_MAX = OFF_BAR + 256;      // [2][2][128] maxima of the rows, two tiles in turn, and [2][128] row sums
-  static constexpr int OFF_Q = OFF_BAR + 4096;       // narrow: the chunks of Q that are not in tensor memory
-  static constexpr int QS_BYTES = (HD / 64 - HD / 128) * 128 * 128;
-  static constexpr int XP = 36;                      // a chunk of the records on its way out: 64 or 128 rows of 32 floats, 36 apart, for each group
+  static constexpr int OFF_Q = OFF_BAR + 4096;       // the chunks of Q that are not in tensor memory: two, of head_dim 64 one (narrow only)
+  static constexpr int TOTAL = 1024 + OFF_Q + (HD == 64 ? 1 : 2) * 128 * 128;
+  static_assert(CTAS * (TOTAL + 1024) <= 228 * 1024, "shared memory of an SM");
+  static constexpr int XP = 36;                      // a chunk of a record on its way out through the rings: 64 or 128 rows of 32 floats, 36 apart
   static constexpr int X_BYTES = 64 * XP * 4;
-  // a unit's only record leaves by way of the rings, which are idle by then: without room for others the merging kernel's CTAs find
-  // place beside this one's (at 220 KB they came 2 us later)
-  static constexpr int total(bool more_records) { return 1024 + OFF_Q + QS_BYTES + (more_records ? 2 * X_BYTES : 0); }
-  static_assert(total(true) <= 227 * 1024 && 4 * X_BYTES * (HD / 64) <= (NK + NV) * KV_BYTES, "shared memory of one CTA");
 };
 template <int HD, bool WIDE>
 struct ShLay {
-  static constexpr int SB = WIDE ? 2 : 3;            // tiles of scores in tensor memory; the weights take their scores' place
-  static constexpr int TQC = WIDE ? HD / 64 : HD / 128;     // 64-dim chunks of Q in tensor memory, 32 columns each
+  static_assert(!WIDE || HD == 256, "wide units");
+  static constexpr int SB = WIDE || HD == 128 ? 2 : 3;      // tiles of scores in tensor memory; the weights take their scores' place
+  static constexpr int TQC = WIDE ? 4 : HD == 256 ? 2 : 0;     // 64-dim chunks of Q in tensor memory, 32 columns each
   static constexpr int T_S = TQC * 32, T_O = T_S + SB * 64;
-  static_assert(T_O + HD <= 512, "tensor memory columns");
+  static_assert(T_O + HD <= (HD == 256 ? 512 : 256), "tensor memory columns");
 };
 template <int HD>
-constexpr int sh_tmem_cols() { return std::max(ShLay<HD, false>::T_O, ShLay<HD, true>::T_O) + HD <= 256 ? 256 : 512; }
+constexpr int sh_tmem_cols() { return HD == 256 ? 512 : 256; }
 
 enum { SH_K_FULL = 0, SH_K_EMPTY = 3, SH_V_FULL = 6, SH_V_EMPTY = 8, SH_S_FULL = 10, SH_P_FULL = 13, SH_PV_DONE = 16, SH_O_DONE = 19, SH_O_FREE, SH_Q_FULL, SH_Q_READ, SH_V_CLEAN, SH_BARS };
 static_assert(SH_BARS <= 31, "barrier slots");
@@ -123,9 +126,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
     // ------------------------------------------------------------------ MMA issuer, scores ----
     const uint32_t leader = elect_one();
     constexpr uint32_t idesc_qk = umma_idesc(128, 64, 0);
-    uint64_t k_desc[NK];
-#pragma unroll
-    for (int i = 0; i < NK; ++i) k_desc[i] = smem_desc(smem_u32(base + L::OFF_K + i * L::KV_BYTES), 16, 1024);
+    const uint64_t k_desc = smem_desc(smem_u32(base + L::OFF_K), 16, 1024);
     const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024);
     mbar_wait(BAR(SH_Q_FULL, 0), 0, s_err, WAIT_QFULL);
     tc_fence_after();
@@ -134,7 +135,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       if (j >= (uint32_t)SB) mbar_wait(BAR(SH_PV_DONE, sb), ((j - SB) / SB) & 1, s_err, WAIT_MMA);
       mbar_wait(BAR(SH_K_FULL, st), (j / NK) & 1, s_err, WAIT_KFULL);
       tc_fence_after();
-      const uint64_t kd = st == 0 ? k_desc[0] : (st == 1 ? k_desc[1] : k_desc[2]);
+      const uint64_t kd = k_desc + (uint64_t)(st * (L::KV_BYTES >> 4));
       const uint32_t ts = t_s0 + sb * 64;
       auto k_at = [&](int ks) { return kd + (uint64_t)(((ks >> 2) * (64 * 128) + (ks & 3) * 32) >> 4); };
       auto q_at = [&](int ks) { return q_desc + (uint64_t)(((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4); };
@@ -150,9 +151,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
     // ------------------------------------------------------------------ MMA issuer, P V ----
     const uint32_t leader = elect_one();
     constexpr uint32_t idesc_pv = umma_idesc(128, HD, 1);
-    uint64_t v_desc[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) v_desc[i] = smem_desc(smem_u32(base + L::OFF_V + i * L::KV_BYTES), 64 * 128, 1024);
+    const uint64_t v_desc = smem_desc(smem_u32(base + L::OFF_V), 64 * 128, 1024);
     for (uint32_t j = 0, seg = 0, in_seg = 0; j < n_tiles; ++j) {
       const uint32_t sb = j % SB, st = j % NV;
       mbar_wait(BAR(SH_P_FULL, sb), (j / SB) & 1, s_err, WAIT_QFULL);
@@ -160,7 +159,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       if (un.ragged && j == n_tiles - 1) mbar_wait(BAR(SH_V_CLEAN, 0), 0, s_err, WAIT_VFULL);
       if (in_seg == 0 && j > 0) mbar_wait(BAR(SH_O_FREE, 0), (seg - 1) & 1, s_err, WAIT_MMA);      // the record before is out
       tc_fence_after();
-      const uint64_t vd = st == 0 ? v_desc[0] : v_desc[1];
+      const uint64_t vd = v_desc + (uint64_t)(st * (L::KV_BYTES >> 4));
       const uint32_t tp = t_s0 + sb * 64;      // P(j): packed f16 pairs over S(j): 32 columns, wide: 32 of high and 32 of low parts
 #pragma unroll
       for (int ks = 0; ks < (WIDE ? 8 : 4); ++ks)
@@ -181,12 +180,12 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
     const bool live = lr < un.pairs;
     const uint32_t st_tid = tid - 128, G = p.G, by_g = (65536 + G - 1) / G;
     auto row_item = [&](uint32_t pr) { return (pr * by_g) >> 16; };       // pr / G, pr < 128
-    // The query rows come by cp.async into the K and the V slot that the producers leave alone until Q_READ, half of them each, a
+    // The query rows come by cp.async into the last K and V slots, which the producers leave alone until Q_READ, half of them each, a
     // row's 16-byte chunks XOR-swizzled against the per-row reads.
     {
       const bool f16 = WIDE || p.q_f16;
       const uint32_t es = f16 ? 2u : 4u, cap = f16 ? 64u : 32u, q_ch = f16 ? HD / 8 : HD / 4;
-      auto stage_row = [&](uint32_t r) { return base + (r < cap ? L::OFF_K + 2 * L::KV_BYTES : L::OFF_V + L::KV_BYTES) + (size_t)(r & (cap - 1)) * (HD * es); };
+      auto stage_row = [&](uint32_t r) { return base + (r < cap ? L::OFF_K + (NK - 1) * L::KV_BYTES : L::OFF_V + (NV - 1) * L::KV_BYTES) + (size_t)(r & (cap - 1)) * (HD * es); };
       for (uint32_t idx = st_tid; idx < un.pairs * q_ch; idx += 128 * GRP) {
         const uint32_t pr = idx / q_ch, c = idx % q_ch, it = row_item(pr);
         const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
@@ -252,11 +251,11 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       tc_fence_after();
       return fmaxf(m, at[(wg ^ 1) * 128]);
     };
-    // The record of the tiles since the last one.  Up to 16 query rows the lanes store what they have, 64 bytes of a chunk of 32 dims;
-    // more rows go through shared memory, a chunk at a time, so that whole lines leave (a lane has a row: its own stores are 16 bytes
-    // each in 32 records 1 KB apart).
+    // The record of the tiles since the last one.  Of up to 16 query rows, or while the rings are in use, the lanes store what they have, 64
+    // bytes of a chunk of 32 dims; else a unit's only or last record goes through the rings, idle by then, so that whole lines leave
+    // (a lane has a row: its own stores are 16 bytes each in 32 records 1 KB apart).
     float* s_rl = s_max + 512;
-    auto record = [&](uint32_t seg, float m, float l) {
+    auto record = [&](uint32_t seg, float m, float l, bool last) {
       const uint32_t threads = 32 * un.live_warps, gt = (tid - 128) & 127;
       auto slot_of = [&](uint32_t pr) { const uint32_t it = row_item(pr); return ((uint64_t)(un.item0 + it) * p.n_heads + g * G + pr - it * G) * p.n_rec + un.slot + seg; };
       if (!WIDE) l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -264,9 +263,8 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       if (wg) *sums = l;
       named_bar_sync(3 + qd, 64);
       if (!wg && live && !is_lo) reinterpret_cast<float2*>(p.part_ml)[slot_of(lr)] = make_float2(m, l + *sums);
-      const bool only = WIDE || n_tiles <= p.seg;
       constexpr uint32_t XW = WIDE ? 2 * L::X_BYTES : L::X_BYTES;
-      uint8_t* xb = only ? base + L::OFF_K + wg * XW : base + L::OFF_Q + L::QS_BYTES + wg * L::X_BYTES;
+      static_assert(HD / 32 * XW <= (NK + NV) * L::KV_BYTES, "a place in the rings for every chunk");
       mbar_wait(BAR(SH_O_DONE, 0), seg & 1, s_err, WAIT_MMA);
       tc_fence_after();
       // high and low rows of a chunk added, each lane with half of it
@@ -277,8 +275,8 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
           t[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
         }
       };
-      if (DIRECT && un.live_warps == 1) {
-        constexpr int N = HD / 32 > GRP ? 2 : 1;          // chunks at a time
+      if (DIRECT && (un.live_warps == 1 || !last)) {
+        constexpr int N = HD == 256 ? 2 : 1;              // chunks at a time
         float* to = p.part_o + slot_of(live ? lr : 0) * HD + (is_lo ? 16 : 0);
 #pragma unroll 1
         for (int c = wg; c < HD / 32; c += N * GRP) {
@@ -303,8 +301,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       for (int c = wg; c < HD / 32; c += GRP) {           // the groups share the chunks out
         float o[32];
         tmem_ld32(t_o + c * 32 + lane_addr, o);
-        if (!only && c != (int)wg) named_bar_sync(7 + wg, threads);
-        float* xs = reinterpret_cast<float*>(xb + (only ? (c / GRP) * GRP * XW : 0));       // (a place for each chunk of the only record)
+        float* xs = reinterpret_cast<float*>(base + L::OFF_K + c * XW);
         if constexpr (WIDE) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(xs + row * L::XP + 4 * i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -318,9 +315,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
         for (uint32_t i = gt; i < un.pairs * 8; i += threads)
           reinterpret_cast<float4*>(p.part_o + slot_of(i >> 3) * HD + c * 32)[i & 7] = *reinterpret_cast<const float4*>(xs + (i >> 3) * L::XP + (i & 7) * 4);
       }
-      named_bar_sync(7 + wg, threads);                    // the next record may take the place
       tc_fence_before();
-      mbar_arrive(BAR(SH_O_FREE, 0));
     };
     if (in_use) {
       float m_old = -3.0e30f, l_old = 0.f;                // of the record to be written next (m below -2e30: none)
@@ -403,7 +398,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
         // a record is written behind the weights of the tile after its last, while the products of its last retire
         const bool last = j == n_tiles;
         if (last) { m_old = m_st; l_old = l_sum; }
-        if (m_old > -2.0e30f) { record(seg++, m_old, l_old); m_old = -3.0e30f; }
+        if (m_old > -2.0e30f) { record(seg++, m_old, l_old, last); m_old = -3.0e30f; }
         if (last) break;
         if (++in_seg == p.seg && j != n_tiles - 1) { m_old = m_st; l_old = l_sum; l_sum = 0.f; in_seg = 0; }
       }
@@ -414,7 +409,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
 // grid (kv heads, units): the shared rows' units of all heads first.  MIXED: they are wide (an instantiation of its own: calls without wide
 // units run a kernel of half the code, most of whose time at short rows is fetching it)
 template <int HD, bool MIXED>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(384, ShSmem<HD>::CTAS)
 pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedParams p) {
   using L = ShSmem<HD>;
@@ -627,18 +622,18 @@ static cudaError_t launch_shared_t(const SharedParams& p, const CUtensorMap& pk,
   using S = ShSmem<HD>;
   static std::atomic<bool> attr_set[64];
   if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(pa_shared_kernel<HD, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::total(true));
+    cudaError_t e = cudaFuncSetAttribute(pa_shared_kernel<HD, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
     if (e != cudaSuccess) return e;
     attr_set[dev & 63].store(true, std::memory_order_release);
   }
-  return launch_pdl(pa_shared_kernel<HD, MIXED>, dim3(n_kv, p.units), dim3(S::THREADS), (size_t)S::total(p.seg < p.tps), st, pk, pv, k, v, p);
+  return launch_pdl(pa_shared_kernel<HD, MIXED>, dim3(n_kv, p.units), dim3(S::THREADS), (size_t)S::TOTAL, st, pk, pv, k, v, p);
 }
 cudaError_t launch_shared(const SharedParams& p, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v, uint32_t hd, uint32_t n_kv,
                           int dev, cudaStream_t st) {
   const bool mixed = p.wide && p.p_splits;
   if (hd == 256) return mixed ? launch_shared_t<256, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<256, false>(p, pk, pv, k, v, n_kv, dev, st);
-  if (hd == 128) return mixed ? launch_shared_t<128, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<128, false>(p, pk, pv, k, v, n_kv, dev, st);
-  if (hd == 64) return mixed ? launch_shared_t<64, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<64, false>(p, pk, pv, k, v, n_kv, dev, st);
+  if (hd == 128 && !mixed) return launch_shared_t<128, false>(p, pk, pv, k, v, n_kv, dev, st);
+  if (hd == 64 && !mixed) return launch_shared_t<64, false>(p, pk, pv, k, v, n_kv, dev, st);
   return cudaErrorInvalidValue;
 }
 cudaError_t launch_shared_finish(const SharedFinishParams& p, uint32_t hd, uint32_t sum_ctas, cudaStream_t st) {

@@ -22,19 +22,19 @@ static uint32_t pad64(uint32_t rows) { return (rows + 63) & ~63u; }
 static uint64_t scores_of(const pa_ctx* ctx, uint32_t rows) { return (uint64_t)ctx->cfg.n_heads * pad64(rows); }
 
 // What a call's units cost, in us on the device (measured: a unit of T tiles takes T * tile + start; start: launch, q, the first
-// scores, the record).  tile: 0.75 at head_dim 256 (the tensor cores), 0.67 below (the softmax); of 128 query rows 1.17 and 0.64.
+// scores, the record).  tile: 0.75 at head_dim 256 (the tensor cores), 0.8 below, two CTAs an SM; of wide units 1.17.
 struct UnitCost { float p_tile, p_start, o_tile, o_start; };
 static UnitCost unit_cost(uint32_t hd, bool wide) {
-  const float tile = hd == 256 ? 0.75f : 0.67f;
-  return wide ? UnitCost{hd == 256 ? 1.17f : 0.64f, 10.5f, tile, 5.5f} : UnitCost{tile, 5.5f, tile, 5.5f};
+  const float tile = hd == 256 ? 0.75f : 0.8f;
+  return wide ? UnitCost{1.17f, 10.5f, tile, 5.5f} : UnitCost{tile, 5.5f, tile, 5.5f};
 }
 
-// Tiles per unit (T) and the time the call takes with them.  The units run one CTA an SM at a time, in the grid's order: the shared
+// Tiles per unit (T) and the time the call takes with them.  The units run one CTA an SM at a time (two of head_dim 128 and 64), in the grid's order: the shared
 // rows' units, all equal, then those of own rows, which fill what the last wave of the others leaves.  Tried: every number of splits
 // of the shared rows, or of the longest item without them (beyond 24 in steps of 4 %).
 static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_items, uint32_t p_tiles, uint32_t row_tiles, const UnitCost& c, uint32_t most_records, float* us) {
   const uint32_t n_kv = ctx->cfg.n_kv_heads;
-  const float sms = (float)ctx->sm_count;
+  const float sms = (float)(ctx->sm_count * (ctx->cfg.head_dim == 256 ? 1 : 2));      // CTAs at a time
   float tiles[kMaxShared], own_tiles = 0.f, own_longest = 0.f;
   for (uint32_t i = 0; i < n_items; ++i) {
     tiles[i] = (float)ceil_div(rows[i], 64);
@@ -99,7 +99,7 @@ static int shared_launch(const SharedCall& c, const pa_item* items, const uint32
   p.items_per_tile = 64 / G; p.row_tiles = ceil_div(n, p.items_per_tile);
   float us = 0.f, wide_us = 0.f;
   uint32_t T = plan_units(ctx, rows + first, n, p_tiles, p.row_tiles, unit_cost(hd, false), most, &us);
-  if (p_tiles && p.row_tiles > 1 && c.q_f16 && ctx->cfg.act_dtype == PA_F16) {
+  if (hd == 256 && p_tiles && p.row_tiles > 1 && c.q_f16 && ctx->cfg.act_dtype == PA_F16) {
     const uint32_t tiles128 = ceil_div(n, 128 / G), T128 = plan_units(ctx, rows + first, n, p_tiles, tiles128, unit_cost(hd, true), most, &wide_us);
     if (wide_us < us) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }
   }
