@@ -31,7 +31,7 @@ static UnitCost unit_cost(uint32_t hd, bool wide) {
 
 // Tiles per unit (T) and the time the call takes with them.  The units run one CTA an SM at a time (two of head_dim 128 and 64), in the grid's order: the shared
 // rows' units, all equal, then those of own rows, which fill what the last wave of the others leaves.  Tried: every number of splits
-// of the shared rows, or of the longest item without them (beyond 24 in steps of 4 %).
+// of the longest of the shared rows and the items' own (beyond 24 in steps of 4 %).
 static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_items, uint32_t p_tiles, uint32_t row_tiles, const UnitCost& c, uint32_t most_records, float* us) {
   const uint32_t n_kv = ctx->cfg.n_kv_heads;
   const float sms = (float)(ctx->sm_count * (ctx->cfg.head_dim == 256 ? 1 : 2));      // CTAs at a time
@@ -41,15 +41,15 @@ static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_i
     own_tiles += tiles[i]; own_longest = std::max(own_longest, tiles[i]);
   }
   const uint32_t longest = std::max(1u, std::max(p_tiles, (uint32_t)own_longest));
-  const uint32_t split = p_tiles ? p_tiles : longest, most_splits = std::min(split, std::min(most_records, 4 * (uint32_t)ctx->sm_count));
+  const uint32_t most_splits = std::min(longest, std::min(most_records, 4 * (uint32_t)ctx->sm_count));
   const float hbm = ((float)p_tiles + own_tiles) * n_kv * (float)(ctx->cfg.head_dim * 256) / 6.0e6f;      // us for its bytes
   uint32_t best = longest;
   *us = 3.0e38f;
   for (uint32_t n = 1; n <= most_splits; n += 1 + n / 24) {
-    const uint32_t T = ceil_div(split, n);
+    const uint32_t T = ceil_div(longest, n);
     // records of a row: the shared rows' and the longest item's
     if (ceil_div(p_tiles, T) + ceil_div((uint32_t)own_longest, T) > most_records) break;
-    const float inv = 1.0f / (float)T, tp = (float)T * c.p_tile + c.p_start, to = std::min((float)T, own_longest) * c.o_tile + c.o_start;
+    const float inv = 1.0f / (float)T, tp = (float)std::min(T, p_tiles) * c.p_tile + c.p_start, to = std::min((float)T, own_longest) * c.o_tile + c.o_start;
     float own_units = 0.f;
     for (uint32_t i = 0; i < n_items; ++i) own_units += (float)(int)(tiles[i] * inv + 0.999f);
     own_units *= n_kv;

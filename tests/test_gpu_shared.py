@@ -128,6 +128,24 @@ def test_many_items(nH, nKV, hd, n):
         close(got[i], want, vv, delta, 200 + own[i])
 
 
+@pytest.mark.parametrize("nH,nKV,hd", [(16, 8, 128), (16, 2, 256), (128, 8, 64)])
+@pytest.mark.parametrize("act", [F16, F32])
+@pytest.mark.parametrize("prefix_len,own", [(60, [4000, 1, 0, 2501]), (130, [3001])])
+def test_long_conversations_behind_a_short_prefix(nH, nKV, hd, act, prefix_len, own):
+    eng, first = engine(nH, nKV, hd, 4001, len(own), act), engine(nH, nKV, hd, prefix_len, 1, act)
+    k, v = fill(eng, 15)
+    pk, pv = fill(first, 16)
+    for s, rows in enumerate(own):
+        poison(eng, s, rows)
+    q = torch.randn((len(own), nH * hd), device="cuda").to(act)
+    got = eng.decode_shared(0, first, 0, prefix_len, [(s, prefix_len + rows - 1) for s, rows in enumerate(own)], q, own_base=prefix_len)
+    eng.sync()
+    for s, rows in enumerate(own):
+        kk, vv = torch.cat([pk[0], k[s, :rows]]), torch.cat([pv[0], v[s, :rows]])
+        want, _, delta = attend(q[s].view(nH, hd), kk, vv)
+        close(got[s], want, vv, delta, prefix_len + rows)
+
+
 def test_long_prefix_in_many_splits():
     eng, first = engine(16, 2, 256, 300, 3, F16), engine(16, 2, 256, 20011, 1, F16)
     k, v = fill(eng, 6)
