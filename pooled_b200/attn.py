@@ -538,7 +538,7 @@ class AttnEngine:
         """Brings sequences down to n_keep rows per kv head, the first n_first, the last n_recent and the rows with the largest sums between them:
         items = [(src_seq, dst_seq, n_rows)], dst_seq = src_seq in place.  Returns the rows that stayed, int32 [n_items, n_kv_heads, n_keep],
         ascending, -1 behind the last."""
-        kept = torch.empty((len(items), self.cfg.n_kv_heads, max(0, n_keep)), dtype=torch.int32, device=self._dev)
+        kept = torch.empty((len(items), self.cfg.n_kv_heads, max(0, min(n_keep, self.cfg.max_seq))), dtype=torch.int32, device=self._dev)
         rc = self._call.evict(self._f_evict, self.layers[li].value, items, n_keep, n_first, n_recent, kept, self._raw_st())
         if rc:
             self._ck(rc)

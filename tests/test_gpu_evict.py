@@ -354,3 +354,11 @@ def test_refused_calls():
     refused(lambda: shard.decode_weights(0, [(0, 70)], q), -2)
     eng.decode_weights(0, [(0, 63)], q)
     eng.sync()
+
+
+def test_a_budget_past_the_layer_is_refused_ahead_of_its_list():
+    eng = tracked(2, 1, 64, 64, 1, F16)
+    for keep in (65, 2 ** 31, 2 ** 32 - 1):
+        with pytest.raises(PaError) as e:
+            eng.evict(0, [(0, 0, 10)] * 32, keep)
+        assert e.value.code == -1
