@@ -242,6 +242,7 @@ extern "C" int pa_layer_create_fmt(pa_ctx* ctx, uint32_t n_seqs, uint32_t max_se
   if (rows >= (1ull << 31)) return fail(ctx, PA_EUNSUPPORTED, "pa_layer_create: %llu cache rows exceed the 2^31 row limit of one layer", (unsigned long long)rows);
   pa_layer* L = new (std::nothrow) pa_layer();
   if (!L) return fail(ctx, PA_ENOMEM, "pa_layer_create: out of host memory");
+  try { ctx->layers.reserve(ctx->layers.size() + 1); } catch (...) { delete L; return fail(ctx, PA_ENOMEM, "pa_layer_create: out of host memory"); }
   L->ctx = ctx; L->n_seqs = n_seqs; L->max_seq = max_seq; L->kv_format = kv_format;
   cudaSetDevice(ctx->device);
   const size_t bytes = rows * row_bytes_of(ctx, kv_format), sbytes = rows * scale_row_bytes_of(ctx, kv_format);
@@ -266,6 +267,7 @@ extern "C" int pa_layer_create_fmt(pa_ctx* ctx, uint32_t n_seqs, uint32_t max_se
   } else {
     L->k_alt = kp; L->v_alt = vp;
   }
+  ctx->layers.push_back(L);
   *out = L;
   return PA_OK;
 }
@@ -277,6 +279,9 @@ extern "C" int pa_layer_destroy(pa_layer* L) {
   if (!L) return PA_OK;
   cudaSetDevice(L->ctx->device);
   cudaFree(L->k); cudaFree(L->v); cudaFree(L->k_alt); cudaFree(L->v_alt); cudaFree(L->k_scale); cudaFree(L->v_scale); cudaFree(L->sums);
+  auto& all = L->ctx->layers;
+  all.erase(std::remove(all.begin(), all.end(), L), all.end());
+  if (L->ctx->inflight_layer == L) L->ctx->inflight_layer = nullptr;
   delete L;
   return PA_OK;
 }

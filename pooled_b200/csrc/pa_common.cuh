@@ -381,6 +381,7 @@ struct pa_ctx {
   unsigned long long angles_capture = 0;
   bool angles_valid = false, ever_captured = false, scope_active = false, scope_fresh = false;
   const pa_layer* inflight_layer = nullptr;
+  std::vector<const pa_layer*> layers;   // the context's layers: whose cache a pa_rotary_apply writes
   uint32_t inflight_row0 = 0;
   float* q_rot = nullptr;      // device: rotated q of the current call, f32 [max_cols][q_dim]
   float* k_rot = nullptr;      // device: rotated k of the current call, f32 [max_cols][kv_dim] (int8 / f32 caches; made with the first such layer)

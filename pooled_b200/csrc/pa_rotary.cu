@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kRotThreads) pa_rotary_kernel(const __grid_con
   const TI* src = reinterpret_cast<const TI*>(is_q ? p.q : is_k ? p.k : p.v) + (is_q ? (uint64_t)r.head * p.q_head_stride : r.head * p.hd);
   const uint64_t src_cs = is_q ? p.q_col_stride : p.kv_col_stride;
   pdl_wait();
-  if (APPEND) pdl_trigger();      // (without an append nobody knows whose rows y is: what follows may fetch ahead of its own wait, so it starts behind this kernel)
+  if (APPEND) pdl_trigger();      // (y of an application may be rows that the next kernel reads at once: it starts behind this one)
   uint4 ra[kRotCols], rb[kRotCols];                    // vectors as they come (V = 1: a value in the first word)
 #pragma unroll
   for (uint32_t k = 0; k < kRotCols; ++k) {

@@ -122,6 +122,13 @@ extern "C" int pa_rotary_apply(pa_rotary* r, const void* x, int x_dtype, uint64_
   DeviceScope on(ctx->device);
   CU_TRY(ctx, launch_rotary(p, false, (uint32_t)ctx->sm_count, (cudaStream_t)stream));
   ctx->stats.kernel_launches++; ctx->stats.calls++;
+  // into a cache: what follows on that layer fetches none of its rows ahead of its wait
+  const uintptr_t y0 = (uintptr_t)y, y1 = y0 + ((n_cols - 1) * ycs + (n_heads - 1) * yhs + hd) * esize(y_dtype);
+  for (const pa_layer* L : ctx->layers) {
+    const uint64_t bytes = (uint64_t)L->n_seqs * L->max_seq * ctx->kv_dim * (L->kv_format == PA_KV_F16 ? 2 : 4);
+    for (const void* cache : {L->k ? (const void*)L->k : L->k_alt, L->v ? (const void*)L->v : L->v_alt})
+      if (y0 < (uintptr_t)cache + bytes && (uintptr_t)cache < y1) { ctx->inflight_layer = L; ctx->inflight_row0 = 0; }
+  }
   return PA_OK;
 }
 

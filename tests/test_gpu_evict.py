@@ -362,3 +362,24 @@ def test_a_budget_past_the_layer_is_refused_ahead_of_its_list():
         with pytest.raises(PaError) as e:
             eng.evict(0, [(0, 0, 10)] * 32, keep)
         assert e.value.code == -1
+
+
+def test_layer_call_right_behind_keys_rotated_into_its_cache():
+    # keys kept unrotated elsewhere, rotated into the cache of one layer of two at their new places
+    eng = AttnEngine(AttnConfig(n_heads=16, n_kv_heads=2, head_dim=256, n_rot=64, rope_theta=1e7, max_seq=1501, n_layers=2, act_dtype=F16, max_cols=64))
+    rot = eng.rotary()
+    g = torch.Generator(device="cuda").manual_seed(8)
+    new = lambda *s: torch.empty(s, device="cuda").normal_(generator=g).half()
+    for turn in range(12):
+        li = turn % 2
+        raw, q, k, v = new(1500, 512), new(1, 4096), new(1, 512), new(1, 512)
+        for w in "kv":
+            eng.cache(li, w).view(F16).copy_(new(1, 1501, 512))
+        rot.apply(raw, 2, pos=0, out=eng.cache(li, "k")[0, :1500].view(F16))
+        got = eng.encode_layer(li, 1500, q, k, v)
+        eng.sync()
+        kk, vv = [eng.cache(li, w)[0].view(F16).view(1501, 2, 256) for w in "kv"]
+        assert torch.equal(kk[:1500].reshape(1500, 512), rot.apply(raw, 2))
+        qr, _ = rotated(q.view(1, 16, 256), [1500], *frequencies(64, 1e7), "half")
+        want, _, delta = attend(torch.from_numpy(qr[0]).cuda(), kk, vv)
+        close(got[0], want, vv, delta, 1501)
