@@ -22,17 +22,21 @@ static uint32_t pad64(uint32_t rows) { return (rows + 63) & ~63u; }
 static uint64_t scores_of(const pa_ctx* ctx, uint32_t rows) { return (uint64_t)ctx->cfg.n_heads * pad64(rows); }
 
 // What a call's units cost, in us on the device (measured: a unit of T tiles takes T * tile + start; start: launch, q, the first
-// scores, the record).  tile: 0.75 at head_dim 256 (the tensor cores), 0.8 below, two CTAs an SM; of wide units 1.17.
-struct UnitCost { float p_tile, p_start, o_tile, o_start; };
-static UnitCost unit_cost(uint32_t hd, bool wide) {
+// scores, the record).  tile: 0.75 at head_dim 256 (the tensor cores), 0.8 below, two CTAs an SM; of wide units 1.17.  A record ahead of a
+// unit's last one: 3 of 64 query rows.
+struct UnitCost { float p_tile, p_start, p_record, o_tile, o_start; };
+static UnitCost unit_cost(uint32_t hd, bool wide, uint32_t p_rows) {
   const float tile = hd == 256 ? 0.75f : 0.8f;
-  return wide ? UnitCost{1.17f, 10.5f, tile, 5.5f} : UnitCost{tile, 5.5f, tile, 5.5f};
+  return UnitCost{wide ? 1.17f : tile, wide ? 10.5f : 5.5f, 3.f * (float)p_rows / 64, tile, 5.5f};
 }
+// tiles of a record for a unit of T: all of it, or with f32 outputs (`cap`) at most that many, the unit's shared out evenly
+static uint32_t record_tiles(uint32_t T, uint32_t cap) { return cap ? ceil_div(T, ceil_div(T, cap)) : T; }
 
 // Tiles per unit (T) and the time the call takes with them.  The units run one CTA an SM at a time (two of head_dim 128 and 64), in the grid's order: the shared
 // rows' units, all equal, then those of own rows, which fill what the last wave of the others leaves.  Tried: every number of splits
 // of the longest of the shared rows and the items' own (beyond 24 in steps of 4 %).
-static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_items, uint32_t p_tiles, uint32_t row_tiles, const UnitCost& c, uint32_t most_records, float* us) {
+static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_items, uint32_t p_tiles, uint32_t row_tiles, const UnitCost& c, uint32_t cap, uint32_t most_records,
+                           float* us) {
   const uint32_t n_kv = ctx->cfg.n_kv_heads;
   const float sms = (float)(ctx->sm_count * (ctx->cfg.head_dim == 256 ? 1 : 2));      // CTAs at a time
   float tiles[kMaxShared], own_tiles = 0.f, own_longest = 0.f;
@@ -49,7 +53,9 @@ static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_i
     const uint32_t T = ceil_div(longest, n);
     // records of a row: the shared rows' and the longest item's
     if (ceil_div(p_tiles, T) + ceil_div((uint32_t)own_longest, T) > most_records) break;
-    const float inv = 1.0f / (float)T, tp = (float)std::min(T, p_tiles) * c.p_tile + c.p_start, to = std::min((float)T, own_longest) * c.o_tile + c.o_start;
+    const uint32_t p_do = std::min(T, p_tiles), records = p_do ? ceil_div(p_do, record_tiles(T, cap)) : 1;       // of a unit of shared rows
+    const float inv = 1.0f / (float)T, tp = (float)p_do * c.p_tile + c.p_start + (float)(records - 1) * c.p_record;
+    const float to = std::min((float)T, own_longest) * c.o_tile + c.o_start;
     float own_units = 0.f;
     for (uint32_t i = 0; i < n_items; ++i) own_units += (float)(int)(tiles[i] * inv + 0.999f);
     own_units *= n_kv;
@@ -98,19 +104,22 @@ static int shared_launch(const SharedCall& c, const pa_item* items, const uint32
   // row tiles of the shared rows: of 64 query rows, or of 128 where that promises less time
   p.items_per_tile = 64 / G; p.row_tiles = ceil_div(n, p.items_per_tile);
   float us = 0.f, wide_us = 0.f;
-  uint32_t T = plan_units(ctx, rows + first, n, p_tiles, p.row_tiles, unit_cost(hd, false), most, &us);
+  const uint32_t cap = ctx->cfg.act_dtype == PA_F16 ? 0u : p.row_tiles > 1 && p_tiles ? 16u : 4u;
+  uint32_t T = plan_units(ctx, rows + first, n, p_tiles, p.row_tiles, unit_cost(hd, false, std::min(n, p.items_per_tile) * G), cap, most, &us);
   if (hd == 256 && p_tiles && p.row_tiles > 1 && c.q_f16 && ctx->cfg.act_dtype == PA_F16) {
-    const uint32_t tiles128 = ceil_div(n, 128 / G), T128 = plan_units(ctx, rows + first, n, p_tiles, tiles128, unit_cost(hd, true), most, &wide_us);
+    const uint32_t tiles128 = ceil_div(n, 128 / G), T128 = plan_units(ctx, rows + first, n, p_tiles, tiles128, unit_cost(hd, true, 128), 0, most, &wide_us);
     if (wide_us < us) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }
   }
-  // tiles of a record: those of a unit, or with f32 outputs four (which HBM hides), sixteen where the tensor cores bound it
+  // tiles of a record: those of a unit, or with f32 outputs at most four (which HBM hides), sixteen where the tensor cores bound it: a
+  // unit's shared out evenly (17 as two of 9, not as one of 16 and a unit of 32: 13 items behind 11633 rows, 24/4 heads, 37 us for 23)
   uint32_t own_longest = 0;
   for (uint32_t i = 0; i < n; ++i) own_longest = std::max(own_longest, ceil_div(rows[first + i], 64));
   p.seg = T;
-  if (ctx->cfg.act_dtype == PA_F32) {
-    p.seg = std::min(T, p.row_tiles > 1 && p_tiles ? 16u : 4u);
-    while (p.seg < T && ceil_div(p_tiles, p.seg) + ceil_div(own_longest, p.seg) > most) p.seg = std::min(T, 2 * p.seg);
-    T = ceil_div(T, p.seg) * p.seg;
+  if (cap) {
+    uint32_t records = ceil_div(T, cap);
+    while (records > 1 && ceil_div(p_tiles, ceil_div(T, records)) + ceil_div(own_longest, ceil_div(T, records)) > most) --records;
+    p.seg = ceil_div(T, records);
+    T = records * p.seg;
   }
   if (c.prefix) { p.p_row0 = c.prefix_seq * c.prefix->max_seq; p.p_rows = c.prefix_len; p.p_tps = T; p.p_splits = ceil_div(p_tiles, T); }
   p.p_recs = ceil_div(p_tiles, p.seg);

@@ -158,7 +158,7 @@ def test_long_prefix_in_many_splits():
         close(got[i], want, vv, delta, 20011 + n)
 
 
-@pytest.mark.parametrize("nH,nKV,hd,n,prefix_len", [(24, 4, 256, 11, 9001), (16, 2, 256, 5, 16000), (16, 8, 128, 40, 5000), (8, 8, 64, 70, 7000)])
+@pytest.mark.parametrize("nH,nKV,hd,n,prefix_len", [(24, 4, 256, 11, 9001), (24, 4, 256, 13, 11633), (24, 4, 256, 45, 4878), (16, 2, 256, 5, 16000), (16, 8, 128, 40, 5000), (8, 8, 64, 70, 7000)])
 def test_f32_records_of_a_few_tiles(nH, nKV, hd, n, prefix_len):
     # f32 outputs: a unit of many tiles leaves several records, whatever its last one holds.  What the tensor cores' sums lose by rounding
     # towards zero stays below that of 16 tiles: 2^-24 of the running sum at each of 64 additions, half of them at half of it
