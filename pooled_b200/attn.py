@@ -441,7 +441,7 @@ class AttnEngine:
         """rope_append with `rot`, for one or many sequences: items = [(seq, pos, n_cols)] own consecutive rows of q, k and v.  Item i's k and v go to
         cache rows rows[i] .. (None: the rows of their positions).  Returns the rotated q, [n_cols, q_dim] of q_dtype (None without q)."""
         total = sum([it[2] for it in items])
-        self._columns(total, q, k, v, q_out)
+        self._columns(total, q, q_head_stride, k, v, q_out)
         if q is not None and q_out is None:
             q_out = torch.empty_strided((total, self._q_dim), (self._q_dim, 1), dtype=q_dtype, device=self._dev)
         if k.stride(0) != v.stride(0) and total > 1:
@@ -457,15 +457,15 @@ class AttnEngine:
             if t is not None and (t.get_device() != self.device or not (t.is_contiguous() or t.stride(-1) == 1)):
                 raise _l.PaError(-1, f"a tensor on {t.device} with strides {t.stride()}: the engine takes rows of consecutive values on cuda:{self.device}")
 
-    def _columns(self, n: int, q, k, v, out):
-        """Columns of the engine's own types: q, k, v of act_dtype, n of each."""
+    def _columns(self, n: int, q, q_head_stride, k, v, out):
+        """Columns of the engine's own types: q, k, v of act_dtype, n of each, q with all its heads."""
         c = self.cfg
         self._on_device(q, k, v, out)
-        for t, width in ((q, c.head_dim), (k, self._kv_dim), (v, self._kv_dim)):
+        for t, width in ((q, (c.n_heads - 1) * (q_head_stride or c.head_dim) + c.head_dim), (k, self._kv_dim), (v, self._kv_dim)):
             if t is not None:
                 cols, have = t.shape
                 if t.dtype != c.act_dtype or cols != n or have < width:
-                    raise _l.PaError(-1, f"{t.dtype} {tuple(t.shape)}: {n} columns of {c.act_dtype} are wanted")
+                    raise _l.PaError(-1, f"{t.dtype} {tuple(t.shape)}: {n} columns of {width} values of {c.act_dtype} are wanted")
         if out is not None:
             cols, have = out.shape
             if cols != n or have < self._q_dim:

@@ -117,3 +117,29 @@ def test_the_host_refuses_what_does_not_fit():
         with pytest.raises(PaError):
             call()
     eng.layers = []
+
+
+class NoCalls:
+    def __getattr__(self, name):
+        return lambda *a: pytest.fail(f"{name} was called")
+
+
+@pytest.fixture
+def detached():
+    """An engine of 4/2 heads of 64 and a rotation that have no device (tensors of the host pass for the engine's): nothing may reach the library."""
+    eng = object.__new__(AttnEngine)
+    eng.cfg = AttnConfig(n_heads=4, n_kv_heads=2, head_dim=64, n_rot=64, rope_theta=1e4, max_seq=32, act_dtype=torch.float32)
+    eng.device, eng.layers, eng._call, eng.ctx, eng.slots, eng._xc_keep, eng._q_dim, eng._kv_dim = -1, [C.c_void_p(8)], NoCalls(), None, {}, None, 256, 128
+    eng._f_rot_append = eng._f_shared = eng._f_weights = eng._f_evict = 0
+    rot = object.__new__(Rotary)
+    rot.eng, rot.handle, rot._h, rot._apply, rot._f_apply = eng, C.c_void_p(8), 8, NoCalls(), 0
+    yield eng, rot
+    eng.layers = []
+
+
+@pytest.mark.parametrize("width,head_stride", [(64, None), (128, None), (255, None), (256, 128), (447, 128)])
+def test_a_q_that_does_not_hold_its_heads_is_refused_ahead_of_an_append(detached, width, head_stride):
+    eng, rot = detached
+    kv, out = torch.zeros((2, 128)), torch.zeros((2, 256))
+    with pytest.raises(PaError):
+        eng.rotary_append(0, rot, [(0, 0, 2)], torch.zeros((2, width)), kv, kv, q_head_stride=head_stride, q_out=out)
