@@ -162,7 +162,7 @@ class Rotary:
                 ohs = hs
             if out_cols != cols:
                 raise _l.PaError(-1, f"out has {out_cols} columns for {cols}")
-        if last * hs + hd > have or last * ohs + hd > out_have:
+        if hs < 0 or ohs < 0 or last * hs + hd > have or last * ohs + hd > out_have:
             raise _l.PaError(-1, f"{n_heads} heads do not fit the columns of x or out")
         rc = self._apply(self._f_apply, self._h, x, dt, hs, n_heads, positions, pos, out, out_dt, ohs, eng._raw_st())
         if rc:
@@ -457,11 +457,18 @@ class AttnEngine:
             if t is not None and (t.get_device() != self.device or not (t.is_contiguous() or t.stride(-1) == 1)):
                 raise _l.PaError(-1, f"a tensor on {t.device} with strides {t.stride()}: the engine takes rows of consecutive values on cuda:{self.device}")
 
+    def _heads(self, stride) -> int:
+        """How far a column of n_heads heads reaches; `stride` values (None: head_dim) lie between two of them."""
+        hd = self.cfg.head_dim
+        if stride is not None and stride < 0:
+            raise _l.PaError(-1, f"a head stride of {stride}")
+        return (self.cfg.n_heads - 1) * (stride or hd) + hd
+
     def _columns(self, n: int, q, q_head_stride, k, v, out):
         """Columns of the engine's own types: q, k, v of act_dtype, n of each, q with all its heads."""
         c = self.cfg
         self._on_device(q, k, v, out)
-        for t, width in ((q, (c.n_heads - 1) * (q_head_stride or c.head_dim) + c.head_dim), (k, self._kv_dim), (v, self._kv_dim)):
+        for t, width in ((q, self._heads(q_head_stride)), (k, self._kv_dim), (v, self._kv_dim)):
             if t is not None:
                 cols, have = t.shape
                 if t.dtype != c.act_dtype or cols != n or have < width:
@@ -474,14 +481,14 @@ class AttnEngine:
     def _batch(self, n: int, q, q_head_stride, gate, gate_head_stride, out):
         """The tensors of a decode of n single tokens; returns out, made where it is None."""
         c = self.cfg
-        hd, last, act = c.head_dim, c.n_heads - 1, c.act_dtype
+        act = c.act_dtype
         self._on_device(q, gate)
         cols, have = q.shape
-        if cols != n or last * (q_head_stride or hd) + hd > have:
+        if cols != n or self._heads(q_head_stride) > have:
             raise _l.PaError(-1, f"q of shape {tuple(q.shape)} for {n} items of {c.n_heads} heads")
         if gate is not None:
             cols, have = gate.shape
-            if gate.dtype != act or cols != n or last * (gate_head_stride or hd) + hd > have:
+            if gate.dtype != act or cols != n or self._heads(gate_head_stride) > have:
                 raise _l.PaError(-1, f"{gate.dtype} gate of shape {tuple(gate.shape)} for {n} items of {c.n_heads} heads")
         if out is None:
             return torch.empty_strided((n, self._q_dim), (self._q_dim, 1), dtype=act, device=self._dev)

@@ -143,3 +143,17 @@ def test_a_q_that_does_not_hold_its_heads_is_refused_ahead_of_an_append(detached
     kv, out = torch.zeros((2, 128)), torch.zeros((2, 256))
     with pytest.raises(PaError):
         eng.rotary_append(0, rot, [(0, 0, 2)], torch.zeros((2, width)), kv, kv, q_head_stride=head_stride, q_out=out)
+
+
+@pytest.mark.parametrize("stride", [-1, -64, -2 ** 40])
+def test_heads_ahead_of_their_column_are_refused(detached, stride):
+    # a negative stride would pass for one that fits and become an address ahead of the tensor
+    eng, rot = detached
+    q, kv, out = torch.zeros((2, 256)), torch.zeros((2, 128)), torch.zeros((2, 256))
+    pairs = [(0, 1), (0, 2)]
+    for call in (lambda: rot.apply(q, 4, head_stride=stride, out=out), lambda: rot.apply(q, 4, out=out, out_head_stride=stride), lambda: rot.apply(q, 4, head_stride=stride, out=q),
+                 lambda: eng.rotary_append(0, rot, [(0, 0, 2)], q, kv, kv, q_head_stride=stride, q_out=out), lambda: eng.decode_shared(0, None, 0, 0, pairs, q, out=out, q_head_stride=stride),
+                 lambda: eng.decode_shared(0, None, 0, 0, pairs, q, gate=q, out=out, gate_head_stride=stride), lambda: eng.decode_weights(0, pairs, q, out=out, q_head_stride=stride),
+                 lambda: eng.decode_weights(0, pairs, q, gate=q, out=out, gate_head_stride=stride)):
+        with pytest.raises(PaError):
+            call()
