@@ -339,7 +339,7 @@ class AttnEngine:
     def _items(self, items):
         arr = (_l.PaItem * len(items))()
         for i, (seq, pos, n_cols) in enumerate(items):
-            arr[i].seq, arr[i].pos, arr[i].n_cols = seq, pos, n_cols
+            arr[i].seq, arr[i].pos, arr[i].n_cols = _l.u32(seq), _l.u32(pos), _l.u32(n_cols)
         return arr
 
     def _gate(self, gate, gate_head_stride):
@@ -433,7 +433,7 @@ class AttnEngine:
         "linear", "ntk", "yarn" (beta_fast, beta_slow: 32 and 1 unless given) or "bands" (high, low: 4 and 1) for a context `factor` times the
         `original` one; mscale 0: the scaling's own factor on cos and sin.  The formulas stand in include/pooled_attn.h."""
         fast, slow = (high, low) if scaling == "bands" else (beta_fast, beta_slow)
-        return Rotary(self, _l.PaRotaryConfig(n_rot=self.cfg.n_rot if n_rot is None else n_rot, layout=_LAYOUT[layout], scaling=_SCALING[scaling], original=original,
+        return Rotary(self, _l.PaRotaryConfig(n_rot=_l.u32(self.cfg.n_rot if n_rot is None else n_rot), layout=_LAYOUT[layout], scaling=_SCALING[scaling], original=_l.u32(original),
                                               theta=self.cfg.rope_theta if theta is None else theta, factor=factor, fast=fast, slow=slow, mscale=mscale))
 
     def rotary_append(self, li: int, rot: Rotary, items, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, rows=None, q_head_stride: int | None = None,
@@ -527,7 +527,7 @@ class AttnEngine:
         return self._view((li, "w"), ptr, (self.cfg.n_seqs, self.cfg.n_kv_heads, self.cfg.max_seq), "<f4")
 
     def clear_weights(self, li: int, seq: int):
-        self._ck(self.L.pa_weights_clear(self.layers[li], seq, self._st()))
+        self._ck(self.L.pa_weights_clear(self.layers[li], _l.u32(seq), self._st()))
 
     def decode_weights(self, li: int, seqs_pos, q: torch.Tensor, gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
                        q_head_stride: int | None = None, gate_head_stride: int | None = None) -> torch.Tensor:

@@ -3,7 +3,7 @@
  * A decode step is one call per layer, and while the GPU spends 6 to 10 us on a layer of a short context, ctypes' conversion of
  * 18 arguments, the tensors' accessors as Python calls and the stream object took 7 us of host time before the library
  * was entered.  Here the accessors are vectorcalls on interned names and the arguments plain C values.
- * Conversions are ctypes': integers wrap to their width, the GIL is released for the call. */
+ * An integer that does not fit its parameter is refused with the package's PaError (ctypes would wrap it); the GIL is released for the call. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stdint.h>
@@ -46,15 +46,48 @@ static int stride0(PyObject* t, uint64_t* s) {
   Py_DECREF(r);
   return PyErr_Occurred() ? -1 : 0;
 }
-static int u64_of(PyObject* o, uint64_t* v) { *v = PyLong_AsUnsignedLongLongMask(o); return PyErr_Occurred() ? -1 : 0; }
-static int u32_of(PyObject* o, uint32_t* v) { *v = (uint32_t)PyLong_AsUnsignedLongMask(o); return PyErr_Occurred() ? -1 : 0; }
+/* PaError(-1, ...) of pooled_b200.lib, as a refused call raises */
+static int does_not_fit(PyObject* o, const char* what) {
+  PyErr_Clear();
+  PyObject *lib = PyImport_ImportModule("pooled_b200.lib"), *cls = lib ? PyObject_GetAttrString(lib, "PaError") : NULL;
+  PyObject *msg = cls ? PyUnicode_FromFormat("%R is no %s", o, what) : NULL, *err = msg ? PyObject_CallFunction(cls, "iO", -1, msg) : NULL;
+  if (err) PyErr_SetObject(cls, err);
+  Py_XDECREF(err); Py_XDECREF(msg); Py_XDECREF(cls); Py_XDECREF(lib);
+  return -1;
+}
+/* an integer of [lo, hi] */
+static int int_of(PyObject* o, int64_t lo, int64_t hi, const char* what, int64_t* v) {
+  int over;
+  *v = PyLong_AsLongLongAndOverflow(o, &over);
+  if (over || *v < lo || *v > hi) return !over && *v == -1 && PyErr_Occurred() ? -1 : does_not_fit(o, what);
+  return *v == -1 && PyErr_Occurred() ? -1 : 0;
+}
+static int u64_of(PyObject* o, uint64_t* v) {
+  int over;
+  const long long x = PyLong_AsLongLongAndOverflow(o, &over);
+  if (over <= 0 && x < 0) return !over && PyErr_Occurred() ? -1 : does_not_fit(o, "unsigned 64-bit integer");
+  *v = over ? PyLong_AsUnsignedLongLong(o) : (uint64_t)x;
+  return over && PyErr_Occurred() ? does_not_fit(o, "unsigned 64-bit integer") : 0;
+}
+static int u32_of(PyObject* o, uint32_t* v) {
+  int64_t x;
+  if (int_of(o, 0, UINT32_MAX, "unsigned 32-bit integer", &x)) return -1;
+  *v = (uint32_t)x;
+  return 0;
+}
+static int i32_of(PyObject* o, int32_t* v) {
+  int64_t x;
+  if (int_of(o, INT32_MIN, INT32_MAX, "32-bit integer", &x)) return -1;
+  *v = (int32_t)x;
+  return 0;
+}
 static int rows_of(PyObject* t, uint32_t* n) {
   PyObject* a[2] = {t, i_zero};
   PyObject* r = PyObject_VectorcallMethod(s_size, a, 2 | PY_VECTORCALL_ARGUMENTS_OFFSET, NULL);
   if (!r) return -1;
-  *n = (uint32_t)PyLong_AsUnsignedLongMask(r);
+  const int bad = u32_of(r, n);
   Py_DECREF(r);
-  return PyErr_Occurred() ? -1 : 0;
+  return bad;
 }
 static int args_are(Py_ssize_t n, Py_ssize_t want, const char* who) {
   if (n == want) return 0;
@@ -174,16 +207,17 @@ static const char* const kTriples = "the items are a sequence of triples";
 /* rotary_apply(entry, rotary, x, x_dtype, head_stride, n_heads, positions, pos, y, y_dtype, y_head_stride, stream) -> status */
 static PyObject* rotary_apply(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   uint64_t fn, rot, xcs, xhs, ycs, yhs, stream;
-  uint32_t xdt, ydt, heads, pos, cols;
+  uint32_t xdt, ydt, heads, cols;
+  int32_t pos;
   void *x, *ps, *y;
   (void)self;
   if (args_are(n, 12, "rotary_apply") || u64_of(a[0], &fn) || u64_of(a[1], &rot) || ptr_of(a[2], &x) || stride0(a[2], &xcs) || rows_of(a[2], &cols) || u32_of(a[3], &xdt) ||
-      u64_of(a[4], &xhs) || u32_of(a[5], &heads) || ptr_of(a[6], &ps) || u32_of(a[7], &pos) || ptr_of(a[8], &y) || stride0(a[8], &ycs) || u32_of(a[9], &ydt) ||
+      u64_of(a[4], &xhs) || u32_of(a[5], &heads) || ptr_of(a[6], &ps) || i32_of(a[7], &pos) || ptr_of(a[8], &y) || stride0(a[8], &ycs) || u32_of(a[9], &ydt) ||
       u64_of(a[10], &yhs) || u64_of(a[11], &stream))
     return NULL;
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = ((fn_rotary_apply)(uintptr_t)fn)((pa_rotary*)(uintptr_t)rot, x, (int)xdt, xcs, xhs, heads, (const int32_t*)ps, (int32_t)pos, cols, y, (int)ydt, ycs, yhs,
+  rc = ((fn_rotary_apply)(uintptr_t)fn)((pa_rotary*)(uintptr_t)rot, x, (int)xdt, xcs, xhs, heads, (const int32_t*)ps, pos, cols, y, (int)ydt, ycs, yhs,
                     (void*)(uintptr_t)stream);
   Py_END_ALLOW_THREADS
   return PyLong_FromLong(rc);

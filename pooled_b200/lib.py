@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes as C
 import importlib.machinery
 import importlib.util
+import operator
 import os
 import sysconfig
 
@@ -131,8 +132,28 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _fit(v, lo, hi, what):
+    v = operator.index(v)
+    if not lo <= v <= hi:
+        raise PaError(-1, f"{v} is no {what}")
+    return v
+
+
+def u32(v) -> int:
+    """v as a parameter of 32 bits: ctypes would wrap what does not fit."""
+    return _fit(v, 0, 2 ** 32 - 1, "unsigned 32-bit integer")
+
+
+def i32(v) -> int:
+    return _fit(v, -2 ** 31, 2 ** 31 - 1, "32-bit integer")
+
+
+def u64(v) -> int:
+    return _fit(v, 0, 2 ** 64 - 1, "unsigned 64-bit integer")
+
+
 def _gate(t, head_stride):
-    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), head_stride)
+    return (None, 0, 0) if t is None else (t.data_ptr(), t.stride(0), u64(head_stride))
 
 
 class CtypesCalls:
@@ -142,48 +163,46 @@ class CtypesCalls:
         self.lib = lib
 
     def attn_layer(self, entry, layer, seq, pos, mode, q, q_head_stride, k, v, gate, gate_head_stride, cs_table, out, stream):
-        return self.lib.pa_attn_layer(layer, seq, pos, q.shape[0], mode, _ptr(q), q.stride(0), q_head_stride, _ptr(k), _ptr(v), k.stride(0),
+        return self.lib.pa_attn_layer(layer, u32(seq), u32(pos), u32(q.shape[0]), u32(mode), _ptr(q), q.stride(0), u64(q_head_stride), _ptr(k), _ptr(v), k.stride(0),
                                       *_gate(gate, gate_head_stride), _ptr(cs_table), _ptr(out), out.stride(0), stream)
 
     def attn_items(self, entry, layer, seqs_pos, q, q_head_stride, k, v, gate, gate_head_stride, out, exchange, stream):
-        items = (PaItem * max(1, len(seqs_pos)))(*[PaItem(s, p, 1, 0) for s, p in seqs_pos])
-        return self.lib.pa_attn_items(layer, items, len(seqs_pos), _ptr(q), q.stride(0), q_head_stride, _ptr(k), _ptr(v), k.stride(0),
+        return self.lib.pa_attn_items(layer, self._items(seqs_pos, False), len(seqs_pos), _ptr(q), q.stride(0), u64(q_head_stride), _ptr(k), _ptr(v), k.stride(0),
                                       *_gate(gate, gate_head_stride), _ptr(out), out.stride(0), exchange, stream)
 
     def rope_append(self, entry, layer, seq, pos, q, q_head_stride, k, v, cs_table, q_rot, stream):
-        return self.lib.pa_rope_append(layer, seq, pos, q.shape[0], _ptr(q), q.stride(0), q_head_stride, _ptr(k), _ptr(v), k.stride(0), _ptr(cs_table),
+        return self.lib.pa_rope_append(layer, u32(seq), u32(pos), u32(q.shape[0]), _ptr(q), q.stride(0), u64(q_head_stride), _ptr(k), _ptr(v), k.stride(0), _ptr(cs_table),
                                        _ptr(q_rot), stream)
 
     def decode_gather(self, entry, layer, seq, lists, list_stride, q, q_dtype, q_head_stride, gate, gate_head_stride, out, stream):
-        return self.lib.pa_decode_gather(layer, seq, q.shape[0], _ptr(lists), list_stride, _ptr(q), q_dtype, q.stride(0), q_head_stride,
+        return self.lib.pa_decode_gather(layer, u32(seq), u32(q.shape[0]), _ptr(lists), u32(list_stride), _ptr(q), q_dtype, q.stride(0), u64(q_head_stride),
                                          *_gate(gate, gate_head_stride), _ptr(out), out.stride(0), stream)
 
-
     def _items(self, items, n_cols=True):
-        return (PaItem * max(1, len(items)))(*[PaItem(*it, 0) if n_cols else PaItem(*it, 1, 0) for it in items])
+        return (PaItem * max(1, len(items)))(*[PaItem(*map(u32, it), 0) if n_cols else PaItem(*map(u32, it), 1, 0) for it in items])
 
     def rotary_apply(self, entry, rotary, x, x_dtype, head_stride, n_heads, positions, pos, y, y_dtype, y_head_stride, stream):
-        return self.lib.pa_rotary_apply(rotary, _ptr(x), x_dtype, x.stride(0), head_stride, n_heads, _ptr(positions), pos, x.shape[0], _ptr(y), y_dtype, y.stride(0),
-                                        y_head_stride, stream)
+        return self.lib.pa_rotary_apply(rotary, _ptr(x), x_dtype, x.stride(0), u64(head_stride), u32(n_heads), _ptr(positions), i32(pos), u32(x.shape[0]), _ptr(y), y_dtype,
+                                        y.stride(0), u64(y_head_stride), stream)
 
     def rotary_append(self, entry, rotary, layer, items, rows, q, q_head_stride, k, v, q_out, q_out_dtype, stream):
         if rows is not None and len(rows) != len(items):
             raise ValueError("one row per item")
-        r = None if rows is None else (C.c_uint32 * max(1, len(rows)))(*rows)
+        r = None if rows is None else (C.c_uint32 * max(1, len(rows)))(*map(u32, rows))
         return self.lib.pa_rotary_append(rotary, layer, self._items(items), len(items), r, *_gate(q, q_head_stride), _ptr(k), _ptr(v), k.stride(0), _ptr(q_out),
                                          q_out_dtype, 0 if q_out is None else q_out.stride(0), stream)
 
     def decode_shared(self, entry, layer, prefix_layer, prefix_seq, prefix_len, own_base, seqs_pos, q, q_dtype, q_head_stride, gate, gate_head_stride, out, stream):
-        return self.lib.pa_decode_shared(layer, prefix_layer, prefix_seq, prefix_len, own_base, self._items(seqs_pos, False), len(seqs_pos), _ptr(q), q_dtype, q.stride(0),
-                                         q_head_stride, *_gate(gate, gate_head_stride), _ptr(out), out.stride(0), stream)
+        return self.lib.pa_decode_shared(layer, prefix_layer, u32(prefix_seq), u32(prefix_len), u32(own_base), self._items(seqs_pos, False), len(seqs_pos), _ptr(q), q_dtype,
+                                         q.stride(0), u64(q_head_stride), *_gate(gate, gate_head_stride), _ptr(out), out.stride(0), stream)
 
     def decode_weights(self, entry, layer, seqs_pos, q, q_dtype, q_head_stride, gate, gate_head_stride, out, stream):
-        return self.lib.pa_decode_weights(layer, self._items(seqs_pos, False), len(seqs_pos), _ptr(q), q_dtype, q.stride(0), q_head_stride,
+        return self.lib.pa_decode_weights(layer, self._items(seqs_pos, False), len(seqs_pos), _ptr(q), q_dtype, q.stride(0), u64(q_head_stride),
                                           *_gate(gate, gate_head_stride), _ptr(out), out.stride(0), stream)
 
     def evict(self, entry, layer, items, n_keep, n_first, n_recent, kept, stream):
-        arr = (PaEvictItem * max(1, len(items)))(*[PaEvictItem(*it, 0) for it in items])
-        return self.lib.pa_evict(layer, arr, len(items), n_keep, n_first, n_recent, _ptr(kept), stream)
+        arr = (PaEvictItem * max(1, len(items)))(*[PaEvictItem(*map(u32, it), 0) for it in items])
+        return self.lib.pa_evict(layer, arr, len(items), u32(n_keep), u32(n_first), u32(n_recent), _ptr(kept), stream)
 
 
 class Lib:

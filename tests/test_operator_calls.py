@@ -131,6 +131,7 @@ def detached():
     eng.cfg = AttnConfig(n_heads=4, n_kv_heads=2, head_dim=64, n_rot=64, rope_theta=1e4, max_seq=32, act_dtype=torch.float32)
     eng.device, eng.layers, eng._call, eng.ctx, eng.slots, eng._xc_keep, eng._q_dim, eng._kv_dim = -1, [C.c_void_p(8)], NoCalls(), None, {}, None, 256, 128
     eng._f_rot_append = eng._f_shared = eng._f_weights = eng._f_evict = 0
+    eng._raw_st = lambda: 0
     rot = object.__new__(Rotary)
     rot.eng, rot.handle, rot._h, rot._apply, rot._f_apply = eng, C.c_void_p(8), 8, NoCalls(), 0
     yield eng, rot
@@ -155,5 +156,56 @@ def test_heads_ahead_of_their_column_are_refused(detached, stride):
                  lambda: eng.rotary_append(0, rot, [(0, 0, 2)], q, kv, kv, q_head_stride=stride, q_out=out), lambda: eng.decode_shared(0, None, 0, 0, pairs, q, out=out, q_head_stride=stride),
                  lambda: eng.decode_shared(0, None, 0, 0, pairs, q, gate=q, out=out, gate_head_stride=stride), lambda: eng.decode_weights(0, pairs, q, out=out, q_head_stride=stride),
                  lambda: eng.decode_weights(0, pairs, q, gate=q, out=out, gate_head_stride=stride)):
+        with pytest.raises(PaError):
+            call()
+
+
+@pytest.mark.parametrize("by_module", [True, False])
+def test_integers_past_their_width_are_refused(pa, by_module):
+    # wrapped, 2^32 + 5 rows to keep would be 5, position 2^31 would turn the other way
+    calls = pa.call if by_module else L.CtypesCalls(NoCalls())
+    never = C.CFUNCTYPE(C.c_int)(lambda: pytest.fail("the library was called"))
+    fn = C.cast(never, C.c_void_p).value
+    q, k, o, p = torch.zeros((3, 64)), torch.zeros((3, 16)), torch.zeros((3, 64)), torch.zeros((2, 2, 5), dtype=torch.int32)
+    pairs, triples = [(0, 5), (2, 6), (1, 0)], [(3, 7, 1), (0, 9, 2)]
+    good = {
+        "rotary_apply": (4096, q, 0, 16, 4, None, 0, o, 1, 16, 7), "rotary_append": (4096, 8192, triples, [1, 2], q, 16, k, k, o, 1, 7),
+        "decode_shared": (4096, 8192, 2, 100, 50, pairs, q, 1, 16, q, 32, o, 7), "decode_weights": (4096, pairs, q, 1, 16, q, 32, o, 7),
+        "evict": (4096, triples, 5, 1, 2, p, 7), "attn_layer": (4096, 1, 77, 2, q, 32, k, k, q, 32, None, o, 5), "attn_items": (4096, pairs, q, 32, k, k, q, 64, o, 0, 5),
+        "rope_append": (4096, 1, 77, q, 32, k, k, None, o, 5), "decode_gather": (4096, 1, p, 9, q, 1, 32, q, 64, o, 5)}
+    wide = {"rotary_apply": (3, 8 + 1), "rotary_append": (5,), "decode_shared": (8, 10), "decode_weights": (4, 6), "evict": (), "attn_layer": (5, 9), "attn_items": (3, 7), "rope_append": (4,),
+            "decode_gather": (6, 8)}                               # places of head strides, 64 bits
+    narrow = {"rotary_apply": (4,), "rotary_append": (), "decode_shared": (2, 3, 4), "decode_weights": (), "evict": (2, 3, 4), "attn_layer": (1, 2, 3), "attn_items": (),
+              "rope_append": (1, 2), "decode_gather": (1, 3)}
+    places = {"rotary_append": 2, "decode_shared": 5, "decode_weights": 1, "evict": 1, "attn_items": 1}       # of the items
+
+    def refused(method, args):
+        with pytest.raises(L.PaError) as e:
+            getattr(calls, method)(fn, *args)
+        assert e.value.code == -1
+
+    for method, args in good.items():
+        for places_of, values in ((wide, (-1, -64, 2 ** 64, 2 ** 64 + 16)), (narrow, (-1, 2 ** 32, 2 ** 32 + 5, -2 ** 40, 2 ** 70))):
+            for i in places_of[method]:
+                for bad in values:
+                    refused(method, (*args[:i], bad, *args[i + 1:]))
+        if method in places:
+            i = places[method]
+            for k_ in range(len(args[i][0])):
+                for bad in (-1, 2 ** 32, 2 ** 32 + 1):
+                    item = list(args[i][0])
+                    item[k_] = bad
+                    refused(method, (*args[:i], [tuple(item), *args[i][1:]], *args[i + 1:]))
+    for bad in (2 ** 31, -2 ** 31 - 1, 2 ** 32, 2 ** 64):
+        refused("rotary_apply", (*good["rotary_apply"][:6], bad, *good["rotary_apply"][7:]))
+    for bad in ([1, 2 ** 32], [-1, 2]):
+        refused("rotary_append", (4096, 8192, triples, bad, q, 16, k, k, o, 1, 7))
+
+
+def test_integers_of_the_other_calls_are_refused_too(detached):
+    eng, _ = detached
+    eng.L = NoCalls()
+    for call in (lambda: eng.clear_weights(0, 2 ** 32), lambda: eng.clear_weights(0, -1), lambda: eng.rotary(n_rot=2 ** 32 + 64), lambda: eng.rotary(original=-1),
+                 lambda: eng.decode(0, [(0, 2 ** 32 + 5, 1)], torch.zeros((1, 256)), out=torch.zeros((1, 256)))):
         with pytest.raises(PaError):
             call()
