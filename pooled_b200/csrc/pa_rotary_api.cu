@@ -111,7 +111,8 @@ extern "C" int pa_rotary_apply(pa_rotary* r, const void* x, int x_dtype, uint64_
   if (n_heads < 1 || n_cols < 1 || n_heads > 65536 || n_cols > 0x7fffffffu) return fail(ctx, PA_EINVAL, "pa_rotary_apply: %u heads, %u columns", n_heads, n_cols);
   if (!positions && (int64_t)pos + n_cols - 1 > INT32_MAX) return fail(ctx, PA_EINVAL, "pa_rotary_apply: position %d + %u columns passes 2^31", pos, n_cols);
   if ((uintptr_t)x % esize(x_dtype) || (uintptr_t)y % esize(y_dtype) || ((uintptr_t)positions & 3)) return fail(ctx, PA_EINVAL, "pa_rotary_apply: a pointer is not aligned to its type");
-  if ((n_heads > 1 && yhs < hd) || (n_cols > 1 && ycs < hd)) return fail(ctx, PA_EINVAL, "pa_rotary_apply: strides of y below head_dim %u: heads would overlap", hd);
+  if (pieces_overlap(n_cols, ycs, n_heads, yhs, hd))
+    return fail(ctx, PA_EINVAL, "pa_rotary_apply: heads of %u values at column stride %llu and head stride %llu of y overlap", hd, (unsigned long long)ycs, (unsigned long long)yhs);
   if (x == y && (x_dtype != y_dtype || (n_heads > 1 && xhs != yhs) || (n_cols > 1 && xcs != ycs)))
     return fail(ctx, PA_EINVAL, "pa_rotary_apply: y may be x with the same type and strides only");
   RotaryParams p{};

@@ -263,3 +263,22 @@ def test_refused_calls():
     refused(lambda: q8.rotary_append(0, q8.rotary(), [(0, 0, 4)], x, kv, kv), -2)
     eng.rotary_append(0, rot, [(0, 0, 4)], x, kv, kv)                 # nothing of the above has latched the context
     eng.sync()
+
+
+def test_columns_that_would_overlap_are_refused():
+    # one stride at a time each layout below looks possible; heads of one column and of another are the same addresses
+    eng = engine()
+    rot = eng.rotary()
+    x = torch.randn((3, 4 * 128), device="cuda").half()
+    room = torch.zeros(8192, dtype=F16, device="cuda")
+    y, r = rotated(x.view(3, 4, 128), np.arange(7, 10), *frequencies(128, 1e6), "half")
+    for col, head in [(128, 128), (128, 256), (256, 128), (511, 128), (128, 383), (130, 256), (512, 513), (300, 200)]:
+        with pytest.raises(PaError) as e:
+            rot.apply(x, 4, pos=7, out=room.as_strided((3, 3 * head + 128), (col, 1)), out_head_stride=head)
+        assert e.value.code == -1 and not room.any()
+    # columns outermost, heads outermost, and heads of a column on both sides of the next column's first
+    for cols, heads, col, head in [(3, 4, 512, 128), (3, 4, 128, 384), (3, 4, 130, 400), (3, 4, 1000, 200), (3, 4, 384, 1152), (2, 2, 256, 384)]:
+        room.zero_()
+        rot.apply(x[:cols], heads, pos=7, out=room.as_strided((cols, (heads - 1) * head + 128), (col, 1)), out_head_stride=head)
+        check(torch.as_strided(room, (cols, heads, 128), (col, head, 1)), y[:cols, :heads], r[:cols, :heads])
+        assert int((room != 0).sum()) <= cols * heads * 128
