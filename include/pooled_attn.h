@@ -379,8 +379,8 @@ PA_API int pa_rotary_apply(pa_rotary* rotary, const void* x, int x_dtype, uint64
                            const int32_t* positions, int32_t pos, uint32_t n_cols, void* y, int y_dtype, uint64_t y_col_stride,
                            uint64_t y_head_stride, void* stream);
 /* The front of a layer call with this rotation, for one or many sequences: items[i] = (seq, pos, n_cols) owns the next n_cols
- * rows of q, k, v (act_dtype) and q_out.  q is rotated into q_out (q_out_dtype, heads packed, no overlap with q; q = NULL: k and v only); k is
- * rotated, k and v are rounded to f16 (as pa_kv_append rounds) and stored in rows rows[i] .. rows[i] + n_cols - 1 of the sequence, or, with
+ * rows of q, k, v (act_dtype) and q_out.  q is rotated into q_out (q_out_dtype, heads packed; q_out may be q with that type, packed heads and
+ * its column stride, and otherwise overlaps none of q, k and v; q = NULL: k and v only); k is rotated, k and v are rounded to f16 (as pa_kv_append rounds) and stored in rows rows[i] .. rows[i] + n_cols - 1 of the sequence, or, with
  * rows = NULL, in the rows of their positions.  Rows and positions part when a cache holds only some of the positions
  * (pa_evict) or begins behind a shared prefix (pa_decode_shared).  At most 128 items; two items may not store the same row.  f16 caches. */
 PA_API int pa_rotary_append(pa_rotary* rotary, pa_layer* layer, const pa_item* items, uint32_t n_items, const uint32_t* rows, const void* q,

@@ -168,6 +168,8 @@ extern "C" int pa_rotary_append(pa_rotary* r, pa_layer* L, const pa_item* items,
     total += it.n_cols;
   }
   if (total > ctx->cfg.max_cols) return fail(ctx, PA_EINVAL, "pa_rotary_append: %llu columns, the context was created for at most %u", (unsigned long long)total, ctx->cfg.max_cols);
+  if (q == q_out && q && ((int)ctx->cfg.act_dtype != q_out_dtype || (ctx->cfg.n_heads > 1 && qhs != hd) || (total > 1 && qcs != q_out_cs)))
+    return fail(ctx, PA_EINVAL, "pa_rotary_append: q_out may be q with its type and strides only (heads packed)");
   if (q && total > 1 && q_out_cs < ctx->q_dim) return fail(ctx, PA_EINVAL, "pa_rotary_append: the column stride of q_out is below %u", ctx->q_dim);
   p.turns = r->turns; p.mscale = (float)r->mscale; p.hd = hd; p.n_rot = r->cfg.n_rot; p.layout = r->cfg.layout; p.n_cols = (uint32_t)total; p.n_items = n_items;
   p.q = q; p.q_col_stride = qcs; p.q_head_stride = qhs; p.q_heads = ctx->cfg.n_heads;

@@ -282,3 +282,23 @@ def test_columns_that_would_overlap_are_refused():
         rot.apply(x[:cols], heads, pos=7, out=room.as_strided((cols, (heads - 1) * head + 128), (col, 1)), out_head_stride=head)
         check(torch.as_strided(room, (cols, heads, 128), (col, head, 1)), y[:cols, :heads], r[:cols, :heads])
         assert int((room != 0).sum()) <= cols * heads * 128
+
+
+@pytest.mark.parametrize("act", [F16, F32])
+def test_append_rotates_q_in_place_with_its_own_layout_only(act):
+    eng = engine(nH=16, nKV=2, hd=256, act=act, max_seq=64, max_cols=64)
+    rot = eng.rotary(n_rot=64, layout="interleaved")
+    full = torch.randn((40, 16 * 512), device="cuda").to(act)                # q and gate of a head side by side
+    k, v = [torch.randn((40, 512), device="cuda").to(act) for _ in "kv"]
+    other = F32 if act == F16 else F16
+    before = full.clone()
+    for cols, bad in [(40, dict(q=full, q_head_stride=512, q_out=full)), (40, dict(q=full[:, :4096], q_out=full.view(-1)[:40 * 4096].view(40, 4096))),
+                      (1, dict(q=full[:1], q_head_stride=512, q_out=full[:1])), (1, dict(q=full[:1, :4096], q_out=full.view(other).view(-1)[:4096].view(1, 4096)))]:
+        with pytest.raises(PaError) as e:
+            eng.rotary_append(0, rot, [(0, 3, cols)], bad.pop("q"), k[:cols], v[:cols], **bad)
+        assert e.value.code == -1 and torch.equal(full, before)
+    for q in (full[:, :4096], full[:1, 4096:]):
+        n = q.shape[0]
+        want = eng.rotary_append(0, rot, [(0, 3, n)], q, k[:n], v[:n], q_dtype=act)
+        assert eng.rotary_append(0, rot, [(0, 3, n)], q, k[:n], v[:n], q_out=q) is q
+        assert torch.equal(q, want)
