@@ -288,8 +288,9 @@ class AttnEngine:
     def _view(self, key, ptr, shape, typestr) -> torch.Tensor:
         t = self._views.get(key)
         if t is None:
-            t = self._views[key] = torch.as_tensor(_DevArray(ptr(), shape, typestr), device=self._dev)
-        return t.detach()                       # a tensor of the caller's own over the same memory
+            with torch.inference_mode(False):
+                t = self._views[key] = torch.as_tensor(_DevArray(ptr(), shape, typestr), device=self._dev)
+        return t.data                           # a tensor of the caller's own over the same memory
 
     # ---- the path, step by step ----
     def rope(self, x: torch.Tensor, n_heads: int, pos: int, head_stride: int | None = None, cs_table: torch.Tensor | None = None) -> torch.Tensor:

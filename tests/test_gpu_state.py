@@ -141,3 +141,25 @@ def test_block_straddling_a_shard_boundary_is_appended_by_both_owners():
                 continue
             ref = po.attn_f64(q_rot[c:c + 1], Kf[r * chunk:r * chunk + n_vis], Vf[r * chunk:r * chunk + n_vis], nH, nKV, hd, n_vis - 1, 1, None)
             util.assert_close(out[c][None], ref, f"shard {r} column {c}")
+
+
+def test_views_of_the_caches_are_the_callers_own():
+    import torch
+    from pooled_b200 import AttnConfig, AttnEngine
+    # whatever the first view of a cache was made or used for: inference mode, a graph of gradients that another view's values change under
+    for first in (torch.inference_mode, torch.no_grad, torch.enable_grad):
+        eng = AttnEngine(AttnConfig(n_heads=2, n_kv_heads=1, head_dim=64, n_rot=64, rope_theta=1e4, max_seq=16, kv_format="f32"))
+        eng_w = AttnEngine(AttnConfig(n_heads=2, n_kv_heads=1, head_dim=64, n_rot=64, rope_theta=1e4, max_seq=16))
+        eng_w.track_weights(0)
+        with first():
+            views = [eng.cache(0, "k"), eng_w.cache(0, "v"), eng_w.weights(0)]
+        for view, again in zip(views, (lambda: eng.cache(0, "k"), lambda: eng_w.cache(0, "v"), lambda: eng_w.weights(0))):
+            again().zero_()
+            again()[..., 3] = 5
+            assert view.data_ptr() == again().data_ptr() and int(again().sum()) == 5 * again()[..., 3].numel()
+        eng.cache(0, "k").fill_(2.0)
+        w = torch.ones(64, device="cuda", requires_grad=True)
+        loss = (eng.cache(0, "k") * w).sum()
+        eng.cache(0, "k")[0, 3] = 1.0
+        loss.backward()
+        assert torch.isfinite(w.grad).all() and not eng.cache(0, "k").requires_grad
