@@ -360,7 +360,7 @@ typedef struct pa_rotary_config {
   uint32_t scaling;   /* pa_rope_scaling */
   uint32_t original;  /* trained positions (YARN, BANDS) */
   double theta;       /* above 1 */
-  double factor;      /* above 0; ignored without scaling */
+  double factor;      /* above 0; ignored without scaling; one that leaves frequencies which are no finite numbers is refused */
   double fast, slow;  /* YARN (0: 32 and 1), BANDS (0: 4 and 1); fast > slow > 0 */
   double mscale;      /* factor on cos and sin; 0: the scaling's own (1 but for YARN) */
   uint32_t reserved[4];

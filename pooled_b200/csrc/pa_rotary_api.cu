@@ -68,7 +68,12 @@ extern "C" int pa_rotary_create(pa_ctx* ctx, const pa_rotary_config* cfg, pa_rot
   rotary_frequencies(c, r->freq, &r->mscale);
   double turns[128];
   const uint32_t half = c.n_rot / 2;
-  for (uint32_t i = 0; i < half; ++i) turns[i] = r->freq[i] / kTwoPi;
+  bool finite = isfinite((float)r->mscale);
+  for (uint32_t i = 0; i < half; ++i) { turns[i] = r->freq[i] / kTwoPi; finite = finite && isfinite(turns[i] * 2147483648.0); }
+  if (!finite) {
+    delete r;
+    return fail(ctx, PA_EINVAL, "pa_rotary_create: this scaling leaves frequencies or a factor on cos and sin that are not finite");
+  }
   DeviceScope on(ctx->device);
   cudaError_t e = cudaMalloc(&r->turns, half * sizeof(double));
   if (e == cudaSuccess) e = cudaMemcpy(r->turns, turns, half * sizeof(double), cudaMemcpyHostToDevice);

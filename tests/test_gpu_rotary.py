@@ -302,3 +302,15 @@ def test_append_rotates_q_in_place_with_its_own_layout_only(act):
         want = eng.rotary_append(0, rot, [(0, 3, n)], q, k[:n], v[:n], q_dtype=act)
         assert eng.rotary_append(0, rot, [(0, 3, n)], q, k[:n], v[:n], q_out=q) is q
         assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("kw", [dict(scaling="ntk", factor=1e-320), dict(scaling="ntk", factor=1e-300, n_rot=4), dict(scaling="linear", factor=5e-324), dict(scaling="yarn", factor=1e-310, original=10),
+                                dict(scaling="bands", factor=1e-310, original=10), dict(mscale=1e39), dict(scaling="yarn", factor=4.0, original=100, mscale=-1e300)])
+def test_scalings_past_the_range_of_numbers_are_refused(kw):
+    eng = engine()
+    with pytest.raises(PaError) as e:
+        eng.rotary(**kw)
+    assert e.value.code == -1
+    rot = eng.rotary(scaling="linear", factor=1e-30, mscale=1e30)              # far, but numbers
+    assert all(math.isfinite(f) for f in rot.freqs()[0])
+    assert torch.isfinite(rot.apply(torch.full((3, 128), 1e-3, device="cuda"), 1, pos=2 ** 31 - 4)).all()
