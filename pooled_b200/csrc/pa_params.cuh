@@ -227,7 +227,7 @@ struct SharedParams {
   uint32_t n_items, n_heads, G;
   float scale_log2;
   float* part_o; float* part_ml; uint32_t n_rec;                            // records of a row (column, head): n_rec apart; m in log2 units
-  uint32_t seg, p_recs;                                                     // tiles of a record; records of the shared rows, ahead of the own rows'
+  uint32_t seg, fold, p_recs;                                               // tiles of a run, runs of a record; records of the shared rows, ahead of the own rows'
   // the shared rows [0, p_rows) from row p_row0 of their cache on: units 0 .. p_splits * row_tiles - 1, a row tile being the
   // heads of items_per_tile items
   uint32_t p_row0, p_rows, p_tps, p_splits, row_tiles, items_per_tile, wide;   // wide: 128 query rows a tile, else up to 64

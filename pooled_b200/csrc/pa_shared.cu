@@ -7,7 +7,8 @@
 // several items (so that a shared byte is read once for all of these, from HBM once in all), for own rows the heads of one.
 // A CTA per unit walks its tiles on the 5th-generation tensor cores and leaves an unnormalised (o, m, l) record per query
 // row (with f32 outputs one every p.seg tiles: the tensor cores' sums round towards zero, which after 32 tiles has cost 2.3e-6
-// of the result, after four 6e-7); the second kernel merges a row's records, gates and stores.  All units have the same number
+// of the result, after four 6e-7; where there is no room for that many, p.fold runs of p.seg tiles are added up in one, in f32); the second
+// kernel merges a row's records, gates and stores.  All units have the same number
 // of tiles, whatever they are units of (plan_units), so that a batch of long shared rows and short own ones fills the machine
 // like one long conversation.
 //
@@ -111,8 +112,8 @@ __device__ __forceinline__ void shared_producer(const ShUnit& un, bool is_v, uin
   }
 }
 
-// the other warps.  DIRECT: records of few rows may leave the lanes as they are
-template <int HD, bool WIDE, bool DIRECT>
+// the other warps.  DIRECT: records of few rows may leave the lanes as they are; FOLD: all do, p.fold runs added up in each
+template <int HD, bool WIDE, bool DIRECT, bool FOLD>
 __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit& un, uint8_t* base, uint32_t bar0, volatile uint32_t* s_err, uint32_t tmem) {
   using L = ShSmem<HD>;
   using T = ShLay<HD, WIDE>;
@@ -253,17 +254,23 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
       return fmaxf(m, at[(wg ^ 1) * 128]);
     };
     // The record of the tiles since the last one.  Of up to 16 query rows, or while the rings are in use, the lanes store what they have, 64
-    // bytes of a chunk of 32 dims; else a unit's only or last record goes through the rings, idle by then, so that whole lines leave
+    // bytes of a chunk of 32 dims (or add it to what they stored there before); else a unit's only or last record goes through the rings, idle by then, so that whole lines leave
     // (a lane has a row: its own stores are 16 bytes each in 32 records 1 KB apart).
     float* s_rl = s_max + 512;
+    float m_rec = 0.f;                                    // the reference of what the lane has stored so far in a record of several runs
     auto record = [&](uint32_t seg, float m, float l, bool last) {
+      const bool adds = FOLD && seg % p.fold != 0;
+      const float kept = adds ? ex2_approx(m_rec - m) : 0.f;
       const uint32_t threads = 32 * un.live_warps, gt = (tid - 128) & 127;
-      auto slot_of = [&](uint32_t pr) { const uint32_t it = row_item(pr); return ((uint64_t)(un.item0 + it) * p.n_heads + g * G + pr - it * G) * p.n_rec + un.slot + seg; };
+      auto slot_of = [&](uint32_t pr) { const uint32_t it = row_item(pr); return ((uint64_t)(un.item0 + it) * p.n_heads + g * G + pr - it * G) * p.n_rec + un.slot + (FOLD ? seg / p.fold : seg); };
       if (!WIDE) l += __shfl_xor_sync(0xffffffffu, l, 1);
       float* sums = s_rl + (seg & 1) * 128 + row;          // two in turn: nothing else may come between two records
       if (wg) *sums = l;
       named_bar_sync(3 + qd, 64);
-      if (!wg && live && !is_lo) reinterpret_cast<float2*>(p.part_ml)[slot_of(lr)] = make_float2(m, l + *sums);
+      if (!wg && live && !is_lo) {
+        float2* ml = reinterpret_cast<float2*>(p.part_ml) + slot_of(lr);
+        *ml = make_float2(m, FOLD && adds ? fmaf(ml->y, kept, l + *sums) : l + *sums);
+      }
       constexpr uint32_t XW = WIDE ? 2 * L::X_BYTES : L::X_BYTES;
       static_assert(HD / 32 * XW <= (NK + NV) * L::KV_BYTES, "a place in the rings for every chunk");
       mbar_wait(BAR(SH_O_DONE, 0), seg & 1, s_err, WAIT_MMA);
@@ -276,7 +283,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
           t[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
         }
       };
-      if (DIRECT && (un.live_warps == 1 || !last)) {
+      if (DIRECT && (FOLD || un.live_warps == 1 || !last)) {
         constexpr int N = HD == 256 ? 2 : 1;              // chunks at a time
         float* to = p.part_o + slot_of(live ? lr : 0) * HD + (is_lo ? 16 : 0);
 #pragma unroll 1
@@ -288,12 +295,20 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
 #pragma unroll
           for (int k = 0; k < N; ++k) {
             add_rows(o + 32 * k, t);
+            if (FOLD && live && adds) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(to + (c + k * GRP) * 32 + 4 * i);
+                t[4 * i] = fmaf(x.x, kept, t[4 * i]); t[4 * i + 1] = fmaf(x.y, kept, t[4 * i + 1]); t[4 * i + 2] = fmaf(x.z, kept, t[4 * i + 2]); t[4 * i + 3] = fmaf(x.w, kept, t[4 * i + 3]);
+              }
+            }
             if (live) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(to + (c + k * GRP) * 32 + 4 * i) = make_float4(t[4 * i], t[4 * i + 1], t[4 * i + 2], t[4 * i + 3]);
             }
           }
         }
+        m_rec = m;
         tc_fence_before();
         mbar_arrive(BAR(SH_O_FREE, 0));
         return;
@@ -408,8 +423,9 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
 }
 
 // grid (kv heads, units): the shared rows' units of all heads first.  MIXED: they are wide (an instantiation of its own: calls without wide
-// units run a kernel of half the code, most of whose time at short rows is fetching it)
-template <int HD, bool MIXED>
+// units run a kernel of half the code, most of whose time at short rows is fetching it).  FOLD: records of several runs (likewise: as a
+// branch it made calls that have none 0.1 to 0.3 us slower)
+template <int HD, bool MIXED, bool FOLD>
 __global__ void __launch_bounds__(384, ShSmem<HD>::CTAS)
 pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ SharedParams p) {
@@ -439,7 +455,7 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
     un.mk = &tm_k; un.mv = &tm_v;
   }
   un.tile0 = split * tps;
-  un.slot += un.tile0 / p.seg;                                        // (tiles per unit: a multiple of seg)
+  un.slot += un.tile0 / (FOLD ? p.seg * p.fold : p.seg);                // (tiles per unit: a multiple of a record's)
   un.n_tiles = min((un.n_rows + 63) / 64, un.tile0 + tps) - un.tile0;
   un.pairs = n_q * p.G;
   const bool wide = MIXED && un.shared;
@@ -469,9 +485,9 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
     shared_producer<HD>(un, warp == 3, base, bar0, s_err);
   } else {
     if constexpr (MIXED) {
-      if (wide) shared_roles<HD, true, false>(p, un, base, bar0, s_err, tmem);
+      if (wide) shared_roles<HD, true, false, false>(p, un, base, bar0, s_err, tmem);
     }
-    if (!wide) shared_roles<HD, false, !MIXED>(p, un, base, bar0, s_err, tmem);
+    if (!wide) shared_roles<HD, false, !MIXED, FOLD>(p, un, base, bar0, s_err, tmem);
   }
   __syncthreads();
   if (warp == 2) {
@@ -617,24 +633,25 @@ __global__ void __launch_bounds__(256, SUMS ? 3 : 4) pa_shared_finish_kernel(con
   }
 }
 
-template <int HD, bool MIXED>
+template <int HD, bool MIXED, bool FOLD>
 static cudaError_t launch_shared_t(const SharedParams& p, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v, uint32_t n_kv,
                                    int dev, cudaStream_t st) {
   using S = ShSmem<HD>;
   static std::atomic<bool> attr_set[64];
   if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(pa_shared_kernel<HD, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
+    cudaError_t e = cudaFuncSetAttribute(pa_shared_kernel<HD, MIXED, FOLD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
     if (e != cudaSuccess) return e;
     attr_set[dev & 63].store(true, std::memory_order_release);
   }
-  return launch_pdl(pa_shared_kernel<HD, MIXED>, dim3(n_kv, p.units), dim3(S::THREADS), (size_t)S::TOTAL, st, pk, pv, k, v, p);
+  return launch_pdl(pa_shared_kernel<HD, MIXED, FOLD>, dim3(n_kv, p.units), dim3(S::THREADS), (size_t)S::TOTAL, st, pk, pv, k, v, p);
 }
 cudaError_t launch_shared(const SharedParams& p, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v, uint32_t hd, uint32_t n_kv,
                           int dev, cudaStream_t st) {
-  const bool mixed = p.wide && p.p_splits;
-  if (hd == 256) return mixed ? launch_shared_t<256, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<256, false>(p, pk, pv, k, v, n_kv, dev, st);
-  if (hd == 128 && !mixed) return launch_shared_t<128, false>(p, pk, pv, k, v, n_kv, dev, st);
-  if (hd == 64 && !mixed) return launch_shared_t<64, false>(p, pk, pv, k, v, n_kv, dev, st);
+  const bool mixed = p.wide && p.p_splits, fold = p.fold > 1;
+  if (mixed) return hd == 256 && !fold ? launch_shared_t<256, true, false>(p, pk, pv, k, v, n_kv, dev, st) : cudaErrorInvalidValue;
+  if (hd == 256) return fold ? launch_shared_t<256, false, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<256, false, false>(p, pk, pv, k, v, n_kv, dev, st);
+  if (hd == 128) return fold ? launch_shared_t<128, false, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<128, false, false>(p, pk, pv, k, v, n_kv, dev, st);
+  if (hd == 64) return fold ? launch_shared_t<64, false, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<64, false, false>(p, pk, pv, k, v, n_kv, dev, st);
   return cudaErrorInvalidValue;
 }
 cudaError_t launch_shared_finish(const SharedFinishParams& p, uint32_t hd, uint32_t sum_ctas, cudaStream_t st) {

@@ -111,30 +111,35 @@ static int shared_launch(const SharedCall& c, const pa_item* items, const uint32
     if (wide_us < us) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }
   }
   // tiles of a record: those of a unit, or with f32 outputs at most four (which HBM hides), sixteen where the tensor cores bound it: a
-  // unit's shared out evenly (17 as two of 9, not as one of 16 and a unit of 32: 13 items behind 11633 rows, 24/4 heads, 37 us for 23)
+  // unit's shared out evenly (17 as two of 9, not as one of 16 and a unit of 32: 13 items behind 11633 rows, 24/4 heads, 37 us for 23).
+  // Where that is more records than there is room for, a record holds several such runs.
   uint32_t own_longest = 0;
   for (uint32_t i = 0; i < n; ++i) own_longest = std::max(own_longest, ceil_div(rows[first + i], 64));
-  p.seg = T;
+  uint32_t rec = T;
+  p.fold = 1;
   if (cap) {
     uint32_t records = ceil_div(T, cap);
     while (records > 1 && ceil_div(p_tiles, ceil_div(T, records)) + ceil_div(own_longest, ceil_div(T, records)) > most) --records;
-    p.seg = ceil_div(T, records);
-    T = records * p.seg;
+    rec = ceil_div(T, records);
+    p.fold = ceil_div(rec, cap);
+    rec = ceil_div(rec, p.fold) * p.fold;
+    T = records * rec;
   }
+  p.seg = rec / p.fold;
   if (c.prefix) { p.p_row0 = c.prefix_seq * c.prefix->max_seq; p.p_rows = c.prefix_len; p.p_tps = T; p.p_splits = ceil_div(p_tiles, T); }
-  p.p_recs = ceil_div(p_tiles, p.seg);
+  p.p_recs = ceil_div(p_tiles, rec);
   p.tps = T; p.own_row0 = c.own_row0;
   uint32_t units = p.p_splits * p.row_tiles;
   uint64_t floats = 0;
   for (uint32_t i = 0; i < n; ++i) {
     const uint32_t r = rows[first + i], tiles = ceil_div(r, 64);
-    p.seq[i] = f.seq[i] = items[first + i].seq; p.rows[i] = f.rows[i] = r; p.cta0[i] = units; f.n_own[i] = (uint16_t)ceil_div(tiles, p.seg);
+    p.seq[i] = f.seq[i] = items[first + i].seq; p.rows[i] = f.rows[i] = r; p.cta0[i] = units; f.n_own[i] = (uint16_t)ceil_div(tiles, rec);
     p.score0[i] = f.score0[i] = floats;
     floats += scores_of(ctx, r);
     units += ceil_div(tiles, T);
   }
   p.cta0[n] = units; p.units = units;
-  p.n_rec = p.p_recs + ceil_div(own_longest, p.seg);
+  p.n_rec = p.p_recs + ceil_div(own_longest, rec);
   if (c.sums) p.scores = ctx->scores;
   f.part_o = p.part_o; f.part_ml = p.part_ml; f.n_rec = p.n_rec; f.p_recs = p.p_recs; f.n_items = n; f.n_heads = nH; f.G = G; f.n_kv = n_kv;
   f.gate = c.gate ? reinterpret_cast<const uint8_t*>(c.gate) + (uint64_t)first * c.gcs * aes : nullptr; f.gate_col_stride = c.gcs; f.gate_head_stride = c.ghs;

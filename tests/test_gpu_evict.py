@@ -383,3 +383,20 @@ def test_layer_call_right_behind_keys_rotated_into_its_cache():
         qr, _ = rotated(q.view(1, 16, 256), [1500], *frequencies(64, 1e7), "half")
         want, _, delta = attend(torch.from_numpy(qr[0]).cuda(), kk, vv)
         close(got[0], want, vv, delta, 1501)
+
+
+@pytest.mark.parametrize("nH,nKV,hd,n,rows", [(64, 1, 64, 128, 20000), (24, 4, 256, 60, 9000)])
+def test_f32_sums_stay_short_where_records_run_short(nH, nKV, hd, n, rows):
+    # as in test_gpu_shared: no more than four tiles by the tensor cores alone, in batches that have no room for as many records
+    eng = tracked(nH, nKV, hd, rows, n, F32)
+    k, v = fill(eng, 24)
+    g = torch.Generator(device="cuda").manual_seed(25)
+    q = torch.empty((n, nH * hd), device="cuda").normal_(generator=g)
+    lens = [rows - 61 * i for i in range(n)]
+    got = eng.decode_weights(0, [(i, m - 1) for i, m in enumerate(lens)], q)
+    for i in (0, n // 2, n - 1):
+        m = lens[i]
+        want, p, delta = attend(q[i].view(nH, hd), k[i, :m], v[i, :m])
+        close(got[i], want, v[i, :m], delta, m)
+        check_sums(eng.weights(0)[i, :, :m], torch.zeros((nKV, m), device="cuda"), p.view(nKV, nH // nKV, m).sum(1), delta.max())
+        assert (got[i].double().view(want.shape) - want).norm() <= 3e-6 * want.norm()

@@ -289,3 +289,24 @@ def test_refused_calls():
     refused(-2, e=shard)
     eng.decode_shared(0, first, 0, 100, [(0, 100)], q, own_base=100)
     eng.sync()
+
+
+@pytest.mark.parametrize("nH,nKV,hd,n,prefix_len,own_len", [(16, 8, 128, 128, 33001, 70), (64, 8, 64, 128, 33001, 1), (24, 4, 256, 100, 20000, 300), (16, 2, 256, 128, 200, 9000), (64, 4, 64, 1, 133000, 0),
+                                                            (64, 64, 64, 1, 90001, 5)])
+def test_f32_sums_stay_short_where_records_run_short(nH, nKV, hd, n, prefix_len, own_len):
+    # more rows of more tiles than there are records of 16 or 4 tiles for: what the tensor cores' sums lose by rounding towards zero is still that of
+    # at most 16 tiles (test_f32_records_of_a_few_tiles), whatever the length
+    eng, first = engine(nH, nKV, hd, max(1, own_len), n, F32), engine(nH, nKV, hd, prefix_len, 1, F32)
+    k, v = fill(eng, 21)
+    pk, pv = fill(first, 22)
+    own = [own_len - (i % 7) * (own_len // 9) for i in range(n)]
+    g = torch.Generator(device="cuda").manual_seed(23)
+    q = torch.empty((n, nH * hd), device="cuda").normal_(generator=g)
+    got = eng.decode_shared(0, first, 0, prefix_len, [(i, prefix_len - 1 + own[i]) for i in range(n)], q, own_base=prefix_len)
+    for i in sorted({0, n // 3, n // 2, n - 1}):
+        kk, vv = torch.cat([pk[0], k[i, :own[i]]]), torch.cat([pv[0], v[i, :own[i]]])
+        for h0 in range(0, nH, nH // nKV):                                     # a kv head at a time: the 64-bit values of all of them would take too much room
+            h1 = h0 + nH // nKV
+            want, _, delta = attend(q[i].view(nH, hd)[h0:h1], kk[:, h0 * nKV // nH:h1 * nKV // nH], vv[:, h0 * nKV // nH:h1 * nKV // nH])
+            close(got[i].view(nH, hd)[h0:h1], want, vv, delta, prefix_len + own[i])
+            assert (got[i].view(nH, hd)[h0:h1].double() - want).norm() <= 3e-6 * want.norm()
