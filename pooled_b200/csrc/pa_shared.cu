@@ -6,8 +6,9 @@
 // A unit is a run of 64-row K / V tiles of one kv head and the query rows that attend them: for the shared rows the heads of
 // several items (so that a shared byte is read once for all of these, from HBM once in all), for own rows the heads of one.
 // A CTA per unit walks its tiles on the 5th-generation tensor cores and leaves an unnormalised (o, m, l) record per query
-// row (with f32 outputs one every p.seg tiles: the tensor cores' sums round towards zero, which after 32 tiles has cost 2.3e-6
-// of the result, after four 6e-7; where there is no room for that many, p.fold runs of p.seg tiles are added up in one, in f32); the second
+// row, or one for every p.seg tiles: the tensor cores' sums round towards zero, which after 32 tiles has cost 2.3e-6 of the result, after
+// four 6e-7, after 2344 1.5e-4, so with f32 outputs a run has at most 4 tiles (16 where the tensor cores bound the call), with f16 ones 128.
+// Where there is no room for that many records, p.fold runs are added up in one, in f32.  The second
 // kernel merges a row's records, gates and stores.  All units have the same number
 // of tiles, whatever they are units of (plan_units), so that a batch of long shared rows and short own ones fills the machine
 // like one long conversation.

@@ -29,8 +29,10 @@ static UnitCost unit_cost(uint32_t hd, bool wide, uint32_t p_rows) {
   const float tile = hd == 256 ? 0.75f : 0.8f;
   return UnitCost{wide ? 1.17f : tile, wide ? 10.5f : 5.5f, 3.f * (float)p_rows / 64, tile, 5.5f};
 }
-// tiles of a record for a unit of T: all of it, or with f32 outputs (`cap`) at most that many, the unit's shared out evenly
-static uint32_t record_tiles(uint32_t T, uint32_t cap) { return cap ? ceil_div(T, ceil_div(T, cap)) : T; }
+// f16 outputs: the tensor cores' rounding towards zero (2^-24 of the sum at each of four additions a tile) stays below 2^-15 of the result
+static constexpr uint32_t kF16Tiles = 128;
+// tiles of a record for a unit of T: at most `cap`, the unit's shared out evenly
+static uint32_t record_tiles(uint32_t T, uint32_t cap) { return ceil_div(T, ceil_div(T, cap)); }
 
 // Tiles per unit (T) and the time the call takes with them.  The units run one CTA an SM at a time (two of head_dim 128 and 64), in the grid's order: the shared
 // rows' units, all equal, then those of own rows, which fill what the last wave of the others leaves.  Tried: every number of splits
@@ -104,27 +106,23 @@ static int shared_launch(const SharedCall& c, const pa_item* items, const uint32
   // row tiles of the shared rows: of 64 query rows, or of 128 where that promises less time
   p.items_per_tile = 64 / G; p.row_tiles = ceil_div(n, p.items_per_tile);
   float us = 0.f, wide_us = 0.f;
-  const uint32_t cap = ctx->cfg.act_dtype == PA_F16 ? 0u : p.row_tiles > 1 && p_tiles ? 16u : 4u;
+  const uint32_t cap = ctx->cfg.act_dtype == PA_F16 ? kF16Tiles : p.row_tiles > 1 && p_tiles ? 16u : 4u;
   uint32_t T = plan_units(ctx, rows + first, n, p_tiles, p.row_tiles, unit_cost(hd, false, std::min(n, p.items_per_tile) * G), cap, most, &us);
   if (hd == 256 && p_tiles && p.row_tiles > 1 && c.q_f16 && ctx->cfg.act_dtype == PA_F16) {
-    const uint32_t tiles128 = ceil_div(n, 128 / G), T128 = plan_units(ctx, rows + first, n, p_tiles, tiles128, unit_cost(hd, true, 128), 0, most, &wide_us);
-    if (wide_us < us) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }
+    const uint32_t tiles128 = ceil_div(n, 128 / G), T128 = plan_units(ctx, rows + first, n, p_tiles, tiles128, unit_cost(hd, true, 128), kF16Tiles, most, &wide_us);
+    if (wide_us < us && T128 <= kF16Tiles) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }     // (wide units leave one record)
   }
-  // tiles of a record: those of a unit, or with f32 outputs at most four (which HBM hides), sixteen where the tensor cores bound it: a
-  // unit's shared out evenly (17 as two of 9, not as one of 16 and a unit of 32: 13 items behind 11633 rows, 24/4 heads, 37 us for 23).
-  // Where that is more records than there is room for, a record holds several such runs.
+  // tiles of a record: those of a unit of up to kF16Tiles, with f32 outputs at most four (which HBM hides), sixteen where the tensor cores
+  // bound it: a unit's shared out evenly (17 as two of 9, not as one of 16 and a unit of 32: 13 items behind 11633 rows, 24/4 heads, 37 us
+  // for 23).  Where that is more records than there is room for, a record holds several such runs.
   uint32_t own_longest = 0;
   for (uint32_t i = 0; i < n; ++i) own_longest = std::max(own_longest, ceil_div(rows[first + i], 64));
-  uint32_t rec = T;
-  p.fold = 1;
-  if (cap) {
-    uint32_t records = ceil_div(T, cap);
-    while (records > 1 && ceil_div(p_tiles, ceil_div(T, records)) + ceil_div(own_longest, ceil_div(T, records)) > most) --records;
-    rec = ceil_div(T, records);
-    p.fold = ceil_div(rec, cap);
-    rec = ceil_div(rec, p.fold) * p.fold;
-    T = records * rec;
-  }
+  uint32_t records = ceil_div(T, cap);
+  while (records > 1 && ceil_div(p_tiles, ceil_div(T, records)) + ceil_div(own_longest, ceil_div(T, records)) > most) --records;
+  uint32_t rec = ceil_div(T, records);
+  p.fold = ceil_div(rec, cap);
+  rec = ceil_div(rec, p.fold) * p.fold;
+  T = records * rec;
   p.seg = rec / p.fold;
   if (c.prefix) { p.p_row0 = c.prefix_seq * c.prefix->max_seq; p.p_rows = c.prefix_len; p.p_tps = T; p.p_splits = ceil_div(p_tiles, T); }
   p.p_recs = ceil_div(p_tiles, rec);

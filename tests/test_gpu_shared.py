@@ -310,3 +310,28 @@ def test_f32_sums_stay_short_where_records_run_short(nH, nKV, hd, n, prefix_len,
             want, _, delta = attend(q[i].view(nH, hd)[h0:h1], kk[:, h0 * nKV // nH:h1 * nKV // nH], vv[:, h0 * nKV // nH:h1 * nKV // nH])
             close(got[i].view(nH, hd)[h0:h1], want, vv, delta, prefix_len + own[i])
             assert (got[i].view(nH, hd)[h0:h1].double() - want).norm() <= 3e-6 * want.norm()
+
+
+@pytest.mark.parametrize("nH,nKV,hd,n,prefix_len,own_len", [(64, 1, 64, 128, 131072, 0), (64, 1, 64, 128, 300, 60000), (128, 4, 128, 64, 150000, 3), (32, 2, 256, 128, 100003, 0)])
+def test_f16_results_do_not_shrink_with_the_length(nH, nKV, hd, n, prefix_len, own_len):
+    # What rounding towards zero takes from every value alike, over the heads of an item so that the roundings to f16 average out: 2^-24 of the running
+    # sum at each of 4 additions a tile, 128 tiles (wide units: 8 a tile): at most 2^-15 (2^-14); with the roundings' share, 2^-12 / sqrt(nH * hd) of the
+    # norm, four times over
+    eng, first = engine(nH, nKV, hd, max(1, own_len), n if own_len else 1, F16), engine(nH, nKV, hd, prefix_len, 1, F16)
+    k, v = fill(eng, 26)
+    pk, pv = fill(first, 27)
+    g = torch.Generator(device="cuda").manual_seed(28)
+    q = torch.empty((n, nH * hd), device="cuda").normal_(generator=g).half()
+    got = eng.decode_shared(0, first, 0, prefix_len, [(i if own_len else 0, prefix_len - 1 + own_len) for i in range(n)], q, own_base=prefix_len)
+    for i in (0, n // 2, n - 1):
+        s = i if own_len else 0
+        wants = []
+        for h0 in range(0, nH, nH // nKV):
+            c = h0 * nKV // nH
+            kk, vv = torch.cat([pk[0, :, c:c + 1], k[s, :own_len, c:c + 1]]), torch.cat([pv[0, :, c:c + 1], v[s, :own_len, c:c + 1]])
+            want, _, delta = attend(q[i].view(nH, hd)[h0:h0 + nH // nKV], kk, vv)
+            close(got[i].view(nH, hd)[h0:h0 + nH // nKV], want, vv, delta, prefix_len + own_len)
+            wants.append(want)
+        want = torch.cat(wants)
+        shrunk = 1 - float((got[i].double().view(want.shape) * want).sum() / (want * want).sum())
+        assert abs(shrunk) <= (2.0 ** -14 if hd == 256 else 2.0 ** -15) + 4 * 2.0 ** -12 / math.sqrt(nH * hd), shrunk
