@@ -419,6 +419,7 @@ struct pa_ctx {
     bool no_out_tma = false;     // POOLED_ATTN_NO_OUT_TMA=1: ... and its output rows by per-thread stores
     bool kv_evict_first = true;  // POOLED_ATTN_KV_EVICT_FIRST=0: decode / verify K and V tiles enter L2 with the default policy instead of evict-first
     bool no_merge = false;       // POOLED_ATTN_NO_MERGE: always merge the split records in the combine kernel
+    int shared_wide = -1;        // POOLED_ATTN_SHARED_WIDE: wide units of shared rows wherever they can be (1), never (0), by the plan (-1)
     uint32_t wait_polls = 0;     // pa_set_wait_limit: limit of the waits for other CTAs' and other GPUs' records (0: the built-in limits)
   } tune;
   // device: the scores of one pa_decode_weights call, or the lists of a pa_evict call (pa_layer_track_weights makes it as large as

@@ -108,9 +108,9 @@ static int shared_launch(const SharedCall& c, const pa_item* items, const uint32
   float us = 0.f, wide_us = 0.f;
   const uint32_t cap = ctx->cfg.act_dtype == PA_F16 ? kF16Tiles : p.row_tiles > 1 && p_tiles ? 16u : 4u;
   uint32_t T = plan_units(ctx, rows + first, n, p_tiles, p.row_tiles, unit_cost(hd, false, std::min(n, p.items_per_tile) * G), cap, most, &us);
-  if (hd == 256 && p_tiles && p.row_tiles > 1 && c.q_f16 && ctx->cfg.act_dtype == PA_F16) {
+  if (hd == 256 && p_tiles && p.row_tiles > 1 && c.q_f16 && ctx->cfg.act_dtype == PA_F16 && ctx->tune.shared_wide != 0) {
     const uint32_t tiles128 = ceil_div(n, 128 / G), T128 = plan_units(ctx, rows + first, n, p_tiles, tiles128, unit_cost(hd, true, 128), kF16Tiles, most, &wide_us);
-    if (wide_us < us && T128 <= kF16Tiles) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }     // (wide units leave one record)
+    if ((wide_us < us || ctx->tune.shared_wide == 1) && T128 <= kF16Tiles) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }     // (wide units leave one record)
   }
   // tiles of a record: those of a unit of up to kF16Tiles, with f32 outputs at most four (which HBM hides), sixteen where the tensor cores
   // bound it: a unit's shared out evenly (17 as two of 9, not as one of 16 and a unit of 32: 13 items behind 11633 rows, 24/4 heads, 37 us

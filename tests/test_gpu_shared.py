@@ -335,3 +335,57 @@ def test_f16_results_do_not_shrink_with_the_length(nH, nKV, hd, n, prefix_len, o
         want = torch.cat(wants)
         shrunk = 1 - float((got[i].double().view(want.shape) * want).sum() / (want * want).sum())
         assert abs(shrunk) <= (2.0 ** -14 if hd == 256 else 2.0 ** -15) + 4 * 2.0 ** -12 / math.sqrt(nH * hd), shrunk
+
+
+WIDE = [(16, 2, 17), (16, 2, 32), (16, 2, 100), (24, 4, 22), (24, 4, 43), (64, 1, 3), (10, 2, 33)]      # G = 8, 6, 64 and 5; the last row tile full and not
+
+
+@pytest.mark.parametrize("nH,nKV,n", WIDE)
+@pytest.mark.parametrize("prefix_len", [1, 64, 65, 777, 20011])
+@pytest.mark.parametrize("scale", [1.0, 5.0])
+def test_wide_units(monkeypatch, nH, nKV, n, prefix_len, scale):
+    # 128 query rows a tile wherever they can be, and nowhere: one tile to many splits of many (the rings wrap), a ragged end, flat and peaked weights
+    hd, g = 256, torch.Generator(device="cuda").manual_seed(30)
+    q, gate = [torch.empty((n, nH * hd), device="cuda").normal_(generator=g).half() * s for s in (scale, 1.0)]
+    own = [(37 * i * i) % 130 for i in range(n)]
+    got = []
+    for wide in "01":
+        monkeypatch.setenv("POOLED_ATTN_SHARED_WIDE", wide)
+        eng, first = engine(nH, nKV, hd, 131, n, F16), engine(nH, nKV, hd, prefix_len + 70, 2, F16)
+        k, v = fill(eng, 31)
+        pk, pv = fill(first, 32)
+        for s in range(n):
+            poison(eng, s, own[s])
+        poison(first, 1, prefix_len)
+        poison(first, 0, 0)
+        out = torch.full((n, nH * hd + 8), 9.0, dtype=F16, device="cuda")
+        call = lambda: eng.decode_shared(0, first, 1, prefix_len, [(i, prefix_len - 1 + own[i]) for i in range(n)], q, gate, out=out, own_base=prefix_len)
+        call()
+        eng.sync()
+        assert torch.all(out[:, nH * hd:] == 9.0)
+        got.append(out.clone())
+        assert all(torch.equal(call(), got[-1]) for _ in range(5))
+        for i in range(0, n, 1 if n < 20 else 7):
+            kk, vv = torch.cat([pk[1, :prefix_len], k[i, :own[i]]]), torch.cat([pv[1, :prefix_len], v[i, :own[i]]])
+            want, _, delta = attend(q[i].view(nH, hd), kk, vv, gate[i].view(nH, hd))
+            close(got[-1][i, :nH * hd], want, vv, delta, prefix_len + own[i])
+    if prefix_len >= 777:
+        assert not torch.equal(*got)                                  # (two ways of summing: both ran)
+
+
+@pytest.mark.parametrize("nH,nKV,n", [(16, 2, 128), (24, 4, 85)])
+def test_wide_units_of_many_tiles_whose_scores_rise(monkeypatch, nH, nKV, n):
+    # few records for many rows: units of dozens of tiles, whose every tile passes the last one's maximum by far, for some heads, and falls for others
+    monkeypatch.setenv("POOLED_ATTN_SHARED_WIDE", "1")
+    hd, rows = 256, 20011
+    eng, first = engine(nH, nKV, hd, 64, n, F16), engine(nH, nKV, hd, rows, 1, F16)
+    fill(eng, 33)
+    pk, pv = fill(first, 34, 0.1)
+    first.cache(0, "k").view(F16)[0].view(rows, nKV, hd)[:, :, 0] = torch.linspace(-900, 900, rows, device="cuda").half()[:, None]
+    pk[0, :, :, 0] = torch.linspace(-900, 900, rows, device="cuda").half()[:, None]
+    q = torch.zeros((n, nH, hd), dtype=F16, device="cuda")
+    q[:, 0::3, 0], q[:, 1::3, 0], q[:, :, 1] = 20.0, -20.0, 1.0
+    got = eng.decode_shared(0, first, 0, rows, [(i, rows - 1) for i in range(n)], q.view(n, -1), own_base=rows)
+    for i in range(0, n, 13):
+        want, _, delta = attend(q[i], pk[0], pv[0])
+        close(got[i], want, pv[0], delta, rows)
