@@ -187,24 +187,31 @@ export class NativeAttention {
     this.rotaries.push(asPtr(h));
     return this.rotaries.at(-1);
   }
-  // the front of a layer call with it: items = [[seq, pos, nCols], ...], rows = the cache rows to store in (null: those of the positions)
-  rotaryAppend(li, rot, items, rows, q, k, v, qOut, { f16Out = false, stream = null } = {}) {
-    const { hd, qDim, kvDim } = this.dims, it = paItems(items), r = rows && new Uint8Array(Uint32Array.from(rows).buffer);
-    check(this.S.pa_rotary_append(rot, this.layers[li], new Uint8Array(it.buffer), items.length, r, q, BigInt(qDim), BigInt(hd), k, v, BigInt(kvDim), qOut,
+  // the front of a layer call with it: items = [[seq, pos, nCols], ...], rows = the cache rows to store in (null: those of the positions);
+  // gated: q is a q_full, q and gate interleaved as encodeLayer takes them.  qOut: packed, f32 or (f16Out) f16
+  rotaryAppend(li, rot, items, rows, q, k, v, qOut, { gated = false, f16Out = false, stream = null } = {}) {
+    const { hd, qDim, kvDim } = this.dims, it = paItems(items), r = rows && new Uint8Array(Uint32Array.from(rows).buffer), m = gated ? 2 : 1;
+    check(this.S.pa_rotary_append(rot, this.layers[li], new Uint8Array(it.buffer), items.length, r, q, BigInt(m * qDim), BigInt(m * hd), k, v, BigInt(kvDim), qOut,
       f16Out ? PA_F16 : PA_F32, BigInt(qDim), stream), this.ctx);
   }
-  // one token each of sequences that begin with the same prefixLen rows, kept once: items = [[seq, pos], ...], q rotated, of the activations' type
-  decodeShared(li, prefixLayer, prefixSeq, prefixLen, items, q, gate, out, { ownBase = 0, stream = null } = {}) {
-    const { hd, qDim } = this.dims, it = paItems(items.map(([s, p]) => [s, p, 1]));
-    check(this.S.pa_decode_shared(this.layers[li], prefixLayer, prefixSeq, prefixLen, ownBase, new Uint8Array(it.buffer), items.length, q, this.es === 2 ? PA_F16 : PA_F32,
-      BigInt(qDim), BigInt(hd), gate, BigInt(qDim), BigInt(hd), out, BigInt(qDim), stream), this.ctx);
+  // the gate of a call and its strides: packed, or with `qFull` the one that lies between the heads of that projection
+  _gate(gate, qFull) {
+    const { hd, qDim } = this.dims, m = qFull ? 2 : 1;
+    return [qFull ? Deno.UnsafePointer.offset(qFull, hd * this.es) : gate, BigInt(m * qDim), BigInt(m * hd)];
+  }
+  // one token each of sequences that begin with the same prefixLen rows, kept once: items = [[seq, pos], ...], q rotated and packed (qF16: its type,
+  // the activations' unless given); the gate packed, or null, or with qFull that of an interleaved projection
+  decodeShared(li, prefixLayer, prefixSeq, prefixLen, items, q, gate, out, { ownBase = 0, qFull = null, qF16 = this.es === 2, stream = null } = {}) {
+    const { hd, qDim } = this.dims, it = paItems(items.map(([s, p]) => [s, p, 1])), [g, gs, gh] = this._gate(gate, qFull);
+    check(this.S.pa_decode_shared(this.layers[li], prefixLayer, prefixSeq, prefixLen, ownBase, new Uint8Array(it.buffer), items.length, q, qF16 ? PA_F16 : PA_F32,
+      BigInt(qDim), BigInt(hd), g, gs, gh, out, BigInt(qDim), stream), this.ctx);
   }
   // a cache kept to a budget: sums of attention weights per row, and the rows with the largest kept (items = [[srcSeq, dstSeq, nRows], ...])
   trackWeights(li) { check(this.S.pa_layer_track_weights(this.layers[li]), this.ctx); }
-  decodeWeights(li, items, q, gate, out, { stream = null } = {}) {
-    const { hd, qDim } = this.dims, it = paItems(items.map(([s, p]) => [s, p, 1]));
-    check(this.S.pa_decode_weights(this.layers[li], new Uint8Array(it.buffer), items.length, q, this.es === 2 ? PA_F16 : PA_F32, BigInt(qDim), BigInt(hd), gate, BigInt(qDim),
-      BigInt(hd), out, BigInt(qDim), stream), this.ctx);
+  decodeWeights(li, items, q, gate, out, { qFull = null, qF16 = this.es === 2, stream = null } = {}) {
+    const { hd, qDim } = this.dims, it = paItems(items.map(([s, p]) => [s, p, 1])), [g, gs, gh] = this._gate(gate, qFull);
+    check(this.S.pa_decode_weights(this.layers[li], new Uint8Array(it.buffer), items.length, q, qF16 ? PA_F16 : PA_F32, BigInt(qDim), BigInt(hd), g, gs, gh, out, BigInt(qDim),
+      stream), this.ctx);
   }
   evict(li, items, nKeep, { nFirst = 0, nRecent = 0, kept = null, stream = null } = {}) {
     check(this.S.pa_evict(this.layers[li], new Uint8Array(paItems(items).buffer), items.length, nKeep, nFirst, nRecent, kept, stream), this.ctx);

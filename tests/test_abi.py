@@ -159,3 +159,40 @@ def test_call_module_is_of_this_interpreter_and_calls_as_ctypes_does(pa, monkeyp
         seen.clear()
         assert getattr(pa.call, method)(entry[name], *args) == 1 and getattr(by_ctypes, method)(entry[name], *args) == 2
         assert seen[0] == seen[1] and seen[0][0] == name, method
+
+
+def _js_methods():
+    js = open(os.path.join(ROOT, "js", "pooled_attn.js")).read()
+    body = js[js.index("export class NativeAttention"):]
+    return {m.group(1): m.group(0) for m in re.finditer(r"^  (?:async )?(\w+)\(.*?(?=^  (?:async )?\w+\(|^  //|^})", body, flags=re.M | re.S)}
+
+
+def _arguments(text):
+    """The arguments of the call whose opening bracket `text` begins with."""
+    out, depth, at = [], 0, 1
+    for i, c in enumerate(text):
+        depth += c in "([{"
+        depth -= c in ")]}"
+        if (c == "," and depth == 1) or depth == 0:
+            out.append(text[at:i].strip())
+            at = i + 1
+        if depth == 0:
+            return [a for a in out if a]
+
+
+def test_js_methods_pass_every_parameter():
+    js = open(os.path.join(ROOT, "js", "pooled_attn.js")).read()
+    for m in re.finditer(r"S\.(pa_\w+)\(", js):
+        assert len(_arguments(js[m.end() - 1:])) == len(L.SYMBOLS[m.group(1)][1]), m.group(1)
+
+
+def test_js_operators_take_interleaved_projections():
+    # the class's q_full has q and gate side by side: strides twice the packed ones, the gate a head further
+    methods = _js_methods()
+    append = _arguments(methods["rotaryAppend"][methods["rotaryAppend"].index("pa_rotary_append(") + len("pa_rotary_append"):])
+    assert append[6:8] == ["BigInt(m * qDim)", "BigInt(m * hd)"] and "gated ? 2 : 1" in methods["rotaryAppend"] and "gated = false" in methods["rotaryAppend"]
+    assert "offset(qFull, hd * this.es)" in methods["_gate"] and "BigInt(m * qDim), BigInt(m * hd)" in methods["_gate"]
+    for name, sym, gate in (("decodeShared", "pa_decode_shared", 11), ("decodeWeights", "pa_decode_weights", 7)):
+        args = _arguments(methods[name][methods[name].index(sym + "(") + len(sym):])
+        assert args[gate:gate + 3] == ["g", "gs", "gh"] and "this._gate(gate, qFull)" in methods[name]
+        assert "qF16 = this.es === 2" in methods[name]                # the type that rotaryAppend wrote, if another than the activations'
