@@ -141,9 +141,9 @@ extern "C" int pa_rotary_apply(pa_rotary* r, const void* x, int x_dtype, uint64_
 extern "C" int pa_rotary_append(pa_rotary* r, pa_layer* L, const pa_item* items, uint32_t n_items, const uint32_t* rows, const void* q, uint64_t qcs,
                                 uint64_t qhs, const void* k, const void* v, uint64_t kvcs, void* q_out, int q_out_dtype, uint64_t q_out_cs, void* stream) {
   if (!r || !L) return PA_EINVAL;
-  pa_ctx* ctx = r->ctx;
+  pa_ctx* ctx = L->ctx;
   GUARD(ctx);
-  if (L->ctx != ctx) return fail(ctx, PA_EINVAL, "pa_rotary_append: the layer belongs to another context");
+  if (r->ctx != ctx) return fail(ctx, PA_EINVAL, "pa_rotary_append: the rotation belongs to another context");
   if (L->kv_format != PA_KV_F16) return fail(ctx, PA_EUNSUPPORTED, "pa_rotary_append: f16 caches only");
   if (!items || !k || !v || (q && !q_out)) return fail(ctx, PA_EINVAL, "pa_rotary_append: null items, k, v or q_out");
   if (n_items < 1 || n_items > (uint32_t)kMaxShared) return fail(ctx, PA_EINVAL, "pa_rotary_append: 1 to %d items per call", kMaxShared);

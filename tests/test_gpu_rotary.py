@@ -314,3 +314,10 @@ def test_scalings_past_the_range_of_numbers_are_refused(kw):
     rot = eng.rotary(scaling="linear", factor=1e-30, mscale=1e30)              # far, but numbers
     assert all(math.isfinite(f) for f in rot.freqs()[0])
     assert torch.isfinite(rot.apply(torch.full((3, 128), 1e-3, device="cuda"), 1, pos=2 ** 31 - 4)).all()
+
+
+def test_a_rotation_of_another_engine_is_named_in_the_layers_own_error():
+    eng, other = engine(max_cols=32), engine(max_cols=32)
+    x, kv = torch.zeros((4, 512), dtype=F16, device="cuda"), torch.zeros((4, 256), dtype=F16, device="cuda")
+    with pytest.raises(PaError, match="another context"):
+        eng.rotary_append(0, other.rotary(), [(0, 0, 4)], x, kv, kv)
