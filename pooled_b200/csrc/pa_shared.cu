@@ -7,8 +7,8 @@
 // several items (so that a shared byte is read once for all of these, from HBM once in all), for own rows the heads of one.
 // A CTA per unit walks its tiles on the 5th-generation tensor cores and leaves an unnormalised (o, m, l) record per query
 // row, or one for every p.seg tiles: the tensor cores' sums round towards zero, which after 32 tiles has cost 2.3e-6 of the result, after
-// four 6e-7, after 2344 1.5e-4, so with f32 outputs a run has at most 4 tiles (16 where the tensor cores bound the call), with f16 ones 128.
-// Where there is no room for that many records, p.fold runs are added up in one, in f32.  The second
+// four 6e-7, after 2344 1.5e-4, so with f32 outputs a run has at most 4 tiles (16 where the tensor cores bound the call, 24 where there is no room
+// for that many records), with f16 ones 128; longer records are the f32 sum of p.fold runs.  The second
 // kernel merges a row's records, gates and stores.  All units have the same number
 // of tiles, whatever they are units of (plan_units), so that a batch of long shared rows and short own ones fills the machine
 // like one long conversation.
@@ -284,28 +284,35 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
           t[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
         }
       };
-      if (DIRECT && (FOLD || un.live_warps == 1 || !last)) {
-        constexpr int N = HD == 256 ? 2 : 1;              // chunks at a time
+      if (FOLD || (DIRECT && (un.live_warps == 1 || !last))) {
+        constexpr int N = HD == 256 ? 2 : 1, E = WIDE ? 32 : 16;              // chunks at a time; values of a chunk that a lane stores
         float* to = p.part_o + slot_of(live ? lr : 0) * HD + (is_lo ? 16 : 0);
 #pragma unroll 1
         for (int c = wg; c < HD / 32; c += N * GRP) {
-          float o[32 * N], t[16];
+          float o[32 * N];
 #pragma unroll
           for (int k = 0; k < N; ++k) tmem_ld32_async(t_o + (c + k * GRP) * 32 + lane_addr, o + 32 * k);
           tmem_wait_ld(o);
 #pragma unroll
           for (int k = 0; k < N; ++k) {
-            add_rows(o + 32 * k, t);
+            float t[E];
+            if constexpr (WIDE) {
+#pragma unroll
+              for (int i = 0; i < E; ++i) t[i] = o[32 * k + i];
+            } else {
+              add_rows(o + 32 * k, t);
+            }
+            float4* at = reinterpret_cast<float4*>(to + (c + k * GRP) * 32);
             if (FOLD && live && adds) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float4 x = *reinterpret_cast<const float4*>(to + (c + k * GRP) * 32 + 4 * i);
-                t[4 * i] = fmaf(x.x, kept, t[4 * i]); t[4 * i + 1] = fmaf(x.y, kept, t[4 * i + 1]); t[4 * i + 2] = fmaf(x.z, kept, t[4 * i + 2]); t[4 * i + 3] = fmaf(x.w, kept, t[4 * i + 3]);
+              for (int i = 0; i < E; i += 4) {
+                const float4 x = at[i / 4];
+                t[i] = fmaf(x.x, kept, t[i]); t[i + 1] = fmaf(x.y, kept, t[i + 1]); t[i + 2] = fmaf(x.z, kept, t[i + 2]); t[i + 3] = fmaf(x.w, kept, t[i + 3]);
               }
             }
             if (live) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(to + (c + k * GRP) * 32 + 4 * i) = make_float4(t[4 * i], t[4 * i + 1], t[4 * i + 2], t[4 * i + 3]);
+              for (int i = 0; i < E; i += 4) at[i / 4] = make_float4(t[i], t[i + 1], t[i + 2], t[i + 3]);
             }
           }
         }
@@ -424,7 +431,7 @@ __device__ __forceinline__ void shared_roles(const SharedParams& p, const ShUnit
 }
 
 // grid (kv heads, units): the shared rows' units of all heads first.  MIXED: they are wide (an instantiation of its own: calls without wide
-// units run a kernel of half the code, most of whose time at short rows is fetching it).  FOLD: records of several runs (likewise: as a
+// units run a kernel of half the code, most of whose time at short rows is fetching it).  FOLD: records of several runs, wide units of several (likewise: as a
 // branch it made calls that have none 0.1 to 0.3 us slower)
 template <int HD, bool MIXED, bool FOLD>
 __global__ void __launch_bounds__(384, ShSmem<HD>::CTAS)
@@ -486,7 +493,7 @@ pa_shared_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constan
     shared_producer<HD>(un, warp == 3, base, bar0, s_err);
   } else {
     if constexpr (MIXED) {
-      if (wide) shared_roles<HD, true, false, false>(p, un, base, bar0, s_err, tmem);
+      if (wide) shared_roles<HD, true, false, FOLD>(p, un, base, bar0, s_err, tmem);
     }
     if (!wide) shared_roles<HD, false, !MIXED, FOLD>(p, un, base, bar0, s_err, tmem);
   }
@@ -648,8 +655,9 @@ static cudaError_t launch_shared_t(const SharedParams& p, const CUtensorMap& pk,
 }
 cudaError_t launch_shared(const SharedParams& p, const CUtensorMap& pk, const CUtensorMap& pv, const CUtensorMap& k, const CUtensorMap& v, uint32_t hd, uint32_t n_kv,
                           int dev, cudaStream_t st) {
-  const bool mixed = p.wide && p.p_splits, fold = p.fold > 1;
-  if (mixed) return hd == 256 && !fold ? launch_shared_t<256, true, false>(p, pk, pv, k, v, n_kv, dev, st) : cudaErrorInvalidValue;
+  const bool mixed = p.wide && p.p_splits, fold = p.fold > 1 || (mixed && p.p_tps > p.seg);      // (the other wide units leave one record)
+  if (mixed && hd != 256) return cudaErrorInvalidValue;
+  if (mixed) return fold ? launch_shared_t<256, true, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<256, true, false>(p, pk, pv, k, v, n_kv, dev, st);
   if (hd == 256) return fold ? launch_shared_t<256, false, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<256, false, false>(p, pk, pv, k, v, n_kv, dev, st);
   if (hd == 128) return fold ? launch_shared_t<128, false, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<128, false, false>(p, pk, pv, k, v, n_kv, dev, st);
   if (hd == 64) return fold ? launch_shared_t<64, false, true>(p, pk, pv, k, v, n_kv, dev, st) : launch_shared_t<64, false, false>(p, pk, pv, k, v, n_kv, dev, st);

@@ -29,8 +29,12 @@ static UnitCost unit_cost(uint32_t hd, bool wide, uint32_t p_rows) {
   const float tile = hd == 256 ? 0.75f : 0.8f;
   return UnitCost{wide ? 1.17f : tile, wide ? 10.5f : 5.5f, 3.f * (float)p_rows / 64, tile, 5.5f};
 }
-// f16 outputs: the tensor cores' rounding towards zero (2^-24 of the sum at each of four additions a tile) stays below 2^-15 of the result
+// f16 outputs: the tensor cores' rounding towards zero (2^-24 of the sum at each of four additions a tile, of
+// wide units eight) stays below 2^-15 of the result (2^-14)
 static constexpr uint32_t kF16Tiles = 128;
+// f32 outputs: most tiles of a run where records run short (1.8e-6 of the result, as 32 tiles cost 2.3e-6); runs of 16 there, that is two of 9 for
+// one of 17 or 18, took 32 items behind 32768 rows (16/2 heads of 256) from 49 to 57 us
+static constexpr uint32_t kF32Run = 24;
 // tiles of a record for a unit of T: at most `cap`, the unit's shared out evenly
 static uint32_t record_tiles(uint32_t T, uint32_t cap) { return ceil_div(T, ceil_div(T, cap)); }
 
@@ -110,17 +114,18 @@ static int shared_launch(const SharedCall& c, const pa_item* items, const uint32
   uint32_t T = plan_units(ctx, rows + first, n, p_tiles, p.row_tiles, unit_cost(hd, false, std::min(n, p.items_per_tile) * G), cap, most, &us);
   if (hd == 256 && p_tiles && p.row_tiles > 1 && c.q_f16 && ctx->cfg.act_dtype == PA_F16 && ctx->tune.shared_wide != 0) {
     const uint32_t tiles128 = ceil_div(n, 128 / G), T128 = plan_units(ctx, rows + first, n, p_tiles, tiles128, unit_cost(hd, true, 128), kF16Tiles, most, &wide_us);
-    if ((wide_us < us || ctx->tune.shared_wide == 1) && T128 <= kF16Tiles) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }     // (wide units leave one record)
+    if (wide_us < us || ctx->tune.shared_wide == 1) { p.wide = 1; p.items_per_tile = 128 / G; p.row_tiles = tiles128; T = T128; }
   }
   // tiles of a record: those of a unit of up to kF16Tiles, with f32 outputs at most four (which HBM hides), sixteen where the tensor cores
   // bound it: a unit's shared out evenly (17 as two of 9, not as one of 16 and a unit of 32: 13 items behind 11633 rows, 24/4 heads, 37 us
-  // for 23).  Where that is more records than there is room for, a record holds several such runs.
+  // for 23).  Where that is more records than there is room for, a record is of more, and past kF32Run tiles (f16: kF16Tiles) it adds up
+  // several runs.
   uint32_t own_longest = 0;
   for (uint32_t i = 0; i < n; ++i) own_longest = std::max(own_longest, ceil_div(rows[first + i], 64));
   uint32_t records = ceil_div(T, cap);
   while (records > 1 && ceil_div(p_tiles, ceil_div(T, records)) + ceil_div(own_longest, ceil_div(T, records)) > most) --records;
   uint32_t rec = ceil_div(T, records);
-  p.fold = ceil_div(rec, cap);
+  p.fold = ceil_div(rec, std::max(cap, kF32Run));
   rec = ceil_div(rec, p.fold) * p.fold;
   T = records * rec;
   p.seg = rec / p.fold;

@@ -387,7 +387,7 @@ def test_layer_call_right_behind_keys_rotated_into_its_cache():
 
 @pytest.mark.parametrize("nH,nKV,hd,n,rows", [(64, 1, 64, 128, 20000), (24, 4, 256, 60, 9000)])
 def test_f32_sums_stay_short_where_records_run_short(nH, nKV, hd, n, rows):
-    # as in test_gpu_shared: no more than four tiles by the tensor cores alone, in batches that have no room for as many records
+    # as in test_gpu_shared: no more than 24 tiles by the tensor cores alone, in batches that have no room for as many records
     eng = tracked(nH, nKV, hd, rows, n, F32)
     k, v = fill(eng, 24)
     g = torch.Generator(device="cuda").manual_seed(25)

@@ -294,8 +294,9 @@ def test_refused_calls():
 @pytest.mark.parametrize("nH,nKV,hd,n,prefix_len,own_len", [(16, 8, 128, 128, 33001, 70), (64, 8, 64, 128, 33001, 1), (24, 4, 256, 100, 20000, 300), (16, 2, 256, 128, 200, 9000), (64, 4, 64, 1, 133000, 0),
                                                             (64, 64, 64, 1, 90001, 5)])
 def test_f32_sums_stay_short_where_records_run_short(nH, nKV, hd, n, prefix_len, own_len):
-    # more rows of more tiles than there are records of 16 or 4 tiles for: what the tensor cores' sums lose by rounding towards zero is still that of
-    # at most 16 tiles (test_f32_records_of_a_few_tiles), whatever the length
+    # More rows of more tiles than there are records of 16 or 4 tiles for: what the tensor cores' sums lose by rounding towards zero is still that of
+    # at most 24, whatever the length.  At each of 96 additions at most an f32 unit of the running sum, 2^-24 to 2^-23 of it and half of that on
+    # average, the running sum 3/4 of the last on average: 96 * 0.75 * (2^-25 to 2^-24), at 1.4 units 2^-24.5 = 3.0e-6
     eng, first = engine(nH, nKV, hd, max(1, own_len), n, F32), engine(nH, nKV, hd, prefix_len, 1, F32)
     k, v = fill(eng, 21)
     pk, pv = fill(first, 22)
@@ -312,7 +313,7 @@ def test_f32_sums_stay_short_where_records_run_short(nH, nKV, hd, n, prefix_len,
             assert (got[i].view(nH, hd)[h0:h1].double() - want).norm() <= 3e-6 * want.norm()
 
 
-@pytest.mark.parametrize("nH,nKV,hd,n,prefix_len,own_len", [(64, 1, 64, 128, 131072, 0), (64, 1, 64, 128, 300, 60000), (128, 4, 128, 64, 150000, 3), (32, 2, 256, 128, 100003, 0)])
+@pytest.mark.parametrize("nH,nKV,hd,n,prefix_len,own_len", [(64, 1, 64, 128, 131072, 0), (64, 1, 64, 128, 300, 60000), (128, 4, 128, 64, 150000, 3), (32, 2, 256, 128, 100003, 0), (24, 4, 256, 128, 66001, 1)])
 def test_f16_results_do_not_shrink_with_the_length(nH, nKV, hd, n, prefix_len, own_len):
     # What rounding towards zero takes from every value alike, over the heads of an item so that the roundings to f16 average out: 2^-24 of the running
     # sum at each of 4 additions a tile, 128 tiles (wide units: 8 a tile): at most 2^-15 (2^-14); with the roundings' share, 2^-12 / sqrt(nH * hd) of the
@@ -389,3 +390,31 @@ def test_wide_units_of_many_tiles_whose_scores_rise(monkeypatch, nH, nKV, n):
     for i in range(0, n, 13):
         want, _, delta = attend(q[i], pk[0], pv[0])
         close(got[i], want, pv[0], delta, rows)
+
+
+@pytest.mark.parametrize("nH,nKV,n,rows", [(16, 2, 128, 70003), (24, 4, 128, 131075), (64, 2, 128, 40001)])
+def test_wide_units_of_several_runs(monkeypatch, nH, nKV, n, rows):
+    # units of more than 128 tiles: runs added up in one record, or one after another, under a reference that moves
+    monkeypatch.setenv("POOLED_ATTN_SHARED_WIDE", "1")
+    hd = 256
+    eng, first = engine(nH, nKV, hd, 200, 2, F16), engine(nH, nKV, hd, rows, 1, F16)
+    k, v = fill(eng, 35)
+    pk, pv = fill(first, 36, 0.1)
+    for c in (first.cache(0, "k").view(F16)[0].view(rows, nKV, hd), pk[0]):
+        c[:, :, 0] = torch.linspace(-900, 900, rows, device="cuda").half()[:, None]
+    g = torch.Generator(device="cuda").manual_seed(37)
+    q = torch.empty((n, nH, hd), device="cuda").normal_(generator=g).half()
+    q[:, 0::3], q[:, 1::3], q[:, 2::3, 0] = 0.0, 0.0, 0.0
+    q[:, 0::3, 0], q[:, 1::3, 0], q[:, :, 1] = 20.0, -20.0, 1.0
+    got = eng.decode_shared(0, first, 0, rows, [(i % 2, rows - 1 + (0, 130)[i % 2]) for i in range(n)], q.view(n, -1), own_base=rows)
+    for i in range(0, n, 31):
+        m = (0, 130)[i % 2]
+        for h0 in range(0, nH, nH // nKV):
+            c, h1 = h0 * nKV // nH, h0 + nH // nKV
+            vv = torch.cat([pv[0, :, c:c + 1], v[i % 2, :m, c:c + 1]])
+            want, _, delta = attend(q[i, h0:h1], torch.cat([pk[0, :, c:c + 1], k[i % 2, :m, c:c + 1]]), vv)
+            close(got[i].view(nH, hd)[h0:h1], want, vv, delta, rows + m)
+            flat = (torch.arange(h0, h1) % 3 == 2).to(want.device)              # weights of all rows alike: the bound of test_f16_results_do_not_shrink_with_the_length
+            w, o = want[flat], got[i].view(nH, hd)[h0:h1][flat].double()
+            if rows > 60000:
+                assert abs(1 - float((o * w).sum() / (w * w).sum())) <= 2.0 ** -14 + 4 * 2.0 ** -12 / math.sqrt(w.numel())
