@@ -371,7 +371,8 @@ PA_API int pa_rotary_destroy(pa_rotary* rotary);   /* before its context */
 /* The frequencies in use, radians per position: n_rot / 2 values, and mscale (either may be NULL).  Host arithmetic only. */
 PA_API int pa_rotary_freqs(const pa_rotary* rotary, double* freqs, double* mscale);
 /* Rotates x into y.  x: x_dtype [n_cols][x_col_stride], head h at h * x_head_stride; y: y_dtype, the same with its own strides;
- * y may be x with equal type and strides (rows of a cache of the rotary's context too), and otherwise does not overlap it.  Column c is at position positions[c] (int32 on
+ * y may be x with equal type and strides (rows of a cache of the rotary's context too), and otherwise does not overlap it; its own heads and columns do not
+ * overlap one another.  Column c is at position positions[c] (int32 on
  * the device, read when the kernel runs), or, without positions, at pos + c.  A negative position turns back: with mscale 1
  * the rotation by -p undoes the rotation by p.  Any number of columns and heads; beside pa_rope, which keeps the context's
  * own rotation bit for bit. */

@@ -11,7 +11,10 @@
 // Moving.  A row that stays never moves up, so a CTA that walks a column slice of the kept rows in order may read a batch
 // of rows, wait for all its threads and store it: what it stores lies below everything that is still to be read.  In place a
 // CTA owns 64 bytes of a head's rows, of K or of V, and all of its rows; into another sequence nothing can be overwritten, and
-// CTAs share the rows out and take whole ones.  What bounds it: HBM, 4 * kv_dim bytes a row read and written.
+// CTAs share the rows out and take whole ones.  What bounds it into another sequence: HBM, 4 * kv_dim bytes a row read and written (4 x 32768 ->
+// 30000 rows, 8 heads of 128: 187 us with the selection, 152 of them bytes).  In place 2 * hd / 32 CTAs a head work, a chain of batches of 512
+// rows with a load and a barrier each: latency, until there are heads and sequences enough (the same 215 us; one sequence 113 us for 65,
+// with 24 % of DRAM's rate; 32768 -> 4096 rows of 2 heads of 256 23 us for 16).
 #include <algorithm>
 
 #include "pa_params.cuh"

@@ -29,11 +29,12 @@
 //               CTAs an SM
 //   wide (head_dim 256, f16 queries and outputs, shared rows of more than 64 query rows, where the plan finds it faster)   128 query
 //               rows without low parts of q; the low parts of the weights are multiplied behind the high ones into the same
-//               accumulator.  1.17 us a tile and a start 5 us longer: 32 items of 8 heads behind 32768 rows 35 us, narrow 42, and
+//               accumulator.  1.17 us a tile and a start 5 us longer: 32 items of 8 heads behind 32768 rows 35 us, narrow 39, and
 //               32 with weights of one f16 value, whose rounding would add as much error as the output's own.  (With f32
 //               queries and the products of their low parts 1.43 us and 13 us of start, slower than two narrow tiles at every size
 //               tried; at head_dim 128 0.64 us, slower than two narrow CTAs an SM.)
-// What bounds it: HBM, one query tile per kv head and long rows; the tensor cores, several; short calls the chain of launch, q,
+// What bounds it: HBM, one query tile per kv head and long rows; several, the tensor cores within a unit (33 % of a launch at 32 items: the
+// rest is starts, ends and records); short calls the chain of launch, q,
 // scores, weights, products and records, and fetching the code for it: without wide units a kernel of half the code runs.
 #include <algorithm>
 

@@ -21,7 +21,7 @@ static uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 static uint32_t pad64(uint32_t rows) { return (rows + 63) & ~63u; }
 static uint64_t scores_of(const pa_ctx* ctx, uint32_t rows) { return (uint64_t)ctx->cfg.n_heads * pad64(rows); }
 
-// What a call's units cost, in us on the device (measured: a unit of T tiles takes T * tile + start; start: launch, q, the first
+// What a call's units cost, in us on the device (a model of measurements: a unit of T tiles takes T * tile + start; start: launch, q, the first
 // scores, the record).  tile: 0.75 at head_dim 256 (the tensor cores), 0.8 below, two CTAs an SM; of wide units 1.17.  A record ahead of a
 // unit's last one: 3 of 64 query rows.
 struct UnitCost { float p_tile, p_start, p_record, o_tile, o_start; };
@@ -40,7 +40,9 @@ static uint32_t record_tiles(uint32_t T, uint32_t cap) { return ceil_div(T, ceil
 
 // Tiles per unit (T) and the time the call takes with them.  The units run one CTA an SM at a time (two of head_dim 128 and 64), in the grid's order: the shared
 // rows' units, all equal, then those of own rows, which fill what the last wave of the others leaves.  Tried: every number of splits
-// of the longest of the shared rows and the items' own (beyond 24 in steps of 4 %).
+// of the longest of the shared rows and the items' own (beyond 24 in steps of 4 %).  Between narrow and wide units this chooses within 1.2 % of
+// the faster on average over 168 calls (12 to 128 items of 6 or 8 heads, 1 to 65536 shared and 40 to 777 own rows), 12 of them more
+// than 5 % off and the worst 28 % (34 items of 6 heads behind 700 rows, own rows up to 777: 31.5 us, wide 24.7).
 static uint32_t plan_units(const pa_ctx* ctx, const uint32_t* rows, uint32_t n_items, uint32_t p_tiles, uint32_t row_tiles, const UnitCost& c, uint32_t cap, uint32_t most_records,
                            float* us) {
   const uint32_t n_kv = ctx->cfg.n_kv_heads;
