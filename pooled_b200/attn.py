@@ -340,7 +340,9 @@ class AttnEngine:
     def _items(self, items):
         arr = (_l.PaItem * len(items))()
         for i, (seq, pos, n_cols) in enumerate(items):
-            arr[i].seq, arr[i].pos, arr[i].n_cols = _l.u32(seq), _l.u32(pos), _l.u32(n_cols)
+            if (seq | pos | n_cols) >> 32:                     # negative, or past 32 bits: ctypes would wrap it
+                raise _l.PaError(-1, f"item {i}: sequence {seq}, position {pos}, {n_cols} columns")
+            arr[i].seq, arr[i].pos, arr[i].n_cols = seq, pos, n_cols
         return arr
 
     def _gate(self, gate, gate_head_stride):

@@ -141,7 +141,7 @@ def _fit(v, lo, hi, what):
 
 def u32(v) -> int:
     """v as a parameter of 32 bits: ctypes would wrap what does not fit."""
-    return _fit(v, 0, 2 ** 32 - 1, "unsigned 32-bit integer")
+    return v if type(v) is int and 0 <= v <= 0xffffffff else _fit(v, 0, 0xffffffff, "unsigned 32-bit integer")
 
 
 def i32(v) -> int:
