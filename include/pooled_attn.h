@@ -370,10 +370,26 @@ PA_API int pa_rotary_create(pa_ctx* ctx, const pa_rotary_config* cfg, pa_rotary*
 PA_API int pa_rotary_destroy(pa_rotary* rotary);   /* before its context */
 /* The frequencies in use, radians per position: n_rot / 2 values, and mscale (either may be NULL).  Host arithmetic only. */
 PA_API int pa_rotary_freqs(const pa_rotary* rotary, double* freqs, double* mscale);
+/* Rotations of several axes (images and video: time, height, width): a pair turns by the position of its axis.  pairs[a] of the n_rot / 2
+ * pairs belong to axis a (n_axes of 1 to 4; together all of them):
+ *   PA_ROPE_AXES_BLOCKS  the first pairs[0] to axis 0, the next pairs[1] to axis 1, and so on
+ *   PA_ROPE_AXES_CYCLED  pair i to axis i mod n_axes while i < n_axes * pairs[i mod n_axes], all others to axis 0 (an axis with more pairs
+ *                        than it has turns is refused)
+ *   PA_ROPE_AXES_OWN     blocks, each with the frequencies of a rotation of its own: f_j = theta^(-2j / (2 pairs[a])), j < pairs[a], scaled as such
+ * In the first two f_i and its scaling are the configuration's, as if there was one axis.  pa_rotary_apply and pa_rotary_append_at take
+ * a position of every axis for every column: positions is [n_axes][n_cols].  Where the host gives positions (no array; pa_rotary_append)
+ * all axes have the same, as text has.  axes = NULL: pa_rotary_create. */
+typedef enum pa_rope_axes { PA_ROPE_AXES_BLOCKS = 0, PA_ROPE_AXES_CYCLED = 1, PA_ROPE_AXES_OWN = 2 } pa_rope_axes;
+typedef struct pa_rotary_axes {
+  uint32_t n_axes, order; /* order: pa_rope_axes */
+  uint32_t pairs[4];
+  uint32_t reserved[2];
+} pa_rotary_axes;
+PA_API int pa_rotary_create_axes(pa_ctx* ctx, const pa_rotary_config* cfg, const pa_rotary_axes* axes, pa_rotary** out);
 /* Rotates x into y.  x: x_dtype [n_cols][x_col_stride], head h at h * x_head_stride; y: y_dtype, the same with its own strides;
  * y may be x with equal type and strides (rows of a cache of the rotary's context too), and otherwise does not overlap it; its own heads and columns do not
  * overlap one another.  Column c is at position positions[c] (int32 on
- * the device, read when the kernel runs), or, without positions, at pos + c.  A negative position turns back: with mscale 1
+ * the device, read when the kernel runs; of several axes [n_axes][n_cols]), or, without positions, at pos + c.  A negative position turns back: with mscale 1
  * the rotation by -p undoes the rotation by p.  Any number of columns and heads; beside pa_rope, which keeps the context's
  * own rotation bit for bit. */
 PA_API int pa_rotary_apply(pa_rotary* rotary, const void* x, int x_dtype, uint64_t x_col_stride, uint64_t x_head_stride, uint32_t n_heads_x,
@@ -387,6 +403,45 @@ PA_API int pa_rotary_apply(pa_rotary* rotary, const void* x, int x_dtype, uint64
 PA_API int pa_rotary_append(pa_rotary* rotary, pa_layer* layer, const pa_item* items, uint32_t n_items, const uint32_t* rows, const void* q,
                             uint64_t q_col_stride, uint64_t q_head_stride, const void* k, const void* v, uint64_t kv_col_stride,
                             void* q_out, int q_out_dtype, uint64_t q_out_col_stride, void* stream);
+
+/* The same at positions that the device holds: column c (of all items together) is at positions[c], of several axes at positions[a][c] ([n_axes]
+ * [total columns], int32, read when the kernel runs).  The tokens of a drafted tree (each at its depth, in rows of their own), columns
+ * of images.  items[i].pos names rows only, those of pa_rotary_append where rows = NULL. */
+PA_API int pa_rotary_append_at(pa_rotary* rotary, pa_layer* layer, const pa_item* items, uint32_t n_items, const uint32_t* rows, const int32_t* positions, const void* q,
+                               uint64_t q_col_stride, uint64_t q_head_stride, const void* k, const void* v, uint64_t kv_col_stride, void* q_out, int q_out_dtype,
+                               uint64_t q_out_col_stride, void* stream);
+
+/* ---- trees of drafted tokens -------------------------------------------------------------------------------------- */
+
+/* pa_decode for trees of drafted tokens, one of each of several sequences: items[i] = (seq, base, n) is a tree of n tokens (1 to 256; their q
+ * rotated, their K and V in rows base .. base + n - 1 of the sequence) behind its committed rows [0, base).  parents (int32, on the
+ * device, read when the kernels run): for every column of the call the number within its tree of the token that it follows, an earlier one;
+ * any other value: it follows the committed rows.  A token attends the committed rows, its ancestors and itself, whatever the other
+ * tokens' rows hold (infinities and NaN too).  parents = NULL: chains, every token follows the one before it.  n_cols = 1: a single
+ * token.  Items may repeat a sequence.  q, gate, out and their limits as pa_decode_shared's.  At most 32 items; f16 caches, origin 0. */
+PA_API int pa_decode_tree(pa_layer* layer, const pa_item* items, uint32_t n_items, const int32_t* parents, const void* q, int q_dtype, uint64_t q_col_stride,
+                          uint64_t q_head_stride, const void* gate, uint64_t gate_col_stride, uint64_t gate_head_stride, void* out, uint64_t out_col_stride,
+                          void* stream);
+
+/* ---- rows copied, forked and moved together ------------------------------------------------------------------------ */
+
+/* Moves rows of the caches of several layers (of one context, cache format, number of sequences and rows; any format) in one call: item i copies rows
+ * src_row .. src_row + n_rows - 1 of sequence src_seq to rows dst_row .. of sequence dst_seq, K, V, the scales of int8 caches and the
+ * sums of layers whose weights are tracked.  Rows are cache rows, whatever the layer's origin.
+ *   - a prompt forked to many sequences: items with the same source read it once
+ *   - source and destination of one item may overlap: the destination ends up with the rows that the source held (rows that follow an
+ *     evicted stretch move up to it, or down from it); n_rows = 0 moves nothing
+ *   - lists (u32 on the device, list_stride words an item, as pa_decode_gather's): [0] = n, then n offsets into the item's rows; row j of the
+ *     destination gets row src_row + offset j: the accepted path of a drafted tree (dst_row = src_row = base), a selection.  At most
+ *     min(n_rows, list_stride - 1) rows of an item are moved; offsets that are not below n_rows move nothing.  Where source and
+ *     destination overlap, the offsets ascend and dst_row <= src_row.  Other lists may repeat offsets.
+ * Everything else is left as it was.  No item may store rows that another one reads or stores (for lists: the rows it may reach).
+ * At most 64 items; the call writes nothing when it is refused. */
+typedef struct pa_move_item {
+  uint32_t src_seq, src_row, dst_seq, dst_row, n_rows, reserved;
+} pa_move_item;
+PA_API int pa_cache_move(pa_layer* const* layers, uint32_t n_layers, const pa_move_item* items, uint32_t n_items, const uint32_t* lists, uint32_t list_stride,
+                         void* stream);
 
 /* ---- batches that share a prefix ------------------------------------------------------------------------------ */
 

@@ -68,10 +68,14 @@ export const SYMBOLS = {
   pa_decode_static: { parameters: [I32, P, P, U32, U32, U32, U32, U32, U32, P, P, P, P, BUF, U64], result: I32 },
   pa_decode_static_status: { parameters: [I32, P, BUF], result: I32, nonblocking: true },
   pa_rotary_create: { parameters: [P, BUF, BUF], result: I32 },
+  pa_rotary_create_axes: { parameters: [P, BUF, BUF, BUF], result: I32 },
   pa_rotary_destroy: { parameters: [P], result: I32 },
   pa_rotary_freqs: { parameters: [P, BUF, BUF], result: I32 },
   pa_rotary_apply: { parameters: [P, P, I32, U64, U64, U32, P, I32, U32, P, I32, U64, U64, P], result: I32 },
   pa_rotary_append: { parameters: [P, P, BUF, U32, BUF, P, U64, U64, P, P, U64, P, I32, U64, P], result: I32 },
+  pa_rotary_append_at: { parameters: [P, P, BUF, U32, BUF, P, P, U64, U64, P, P, U64, P, I32, U64, P], result: I32 },
+  pa_decode_tree: { parameters: [P, BUF, U32, P, P, I32, U64, U64, P, U64, U64, P, U64, P], result: I32 },
+  pa_cache_move: { parameters: [BUF, U32, BUF, U32, P, U32, P], result: I32 },
   pa_decode_shared: { parameters: [P, P, U32, U32, U32, BUF, U32, P, I32, U64, U64, P, U64, U64, P, U64, P], result: I32 },
   pa_layer_track_weights: { parameters: [P], result: I32 },
   pa_weights_ptr: { parameters: [P], result: P },
@@ -179,11 +183,15 @@ export class NativeAttention {
       out, BigInt(qDim), sharded ? 1 : 0, stream), this.ctx);
   }
   // A rotation beside the context's own (include/pooled_attn.h, pa_rotary_config): layout 0 half, 1 interleaved; scaling 0 none, 1 linear,
-  // 2 ntk, 3 yarn, 4 bands.  u32 n_rot, layout, scaling, original; f64 theta, factor, fast, slow, mscale; u32 reserved[4]
-  rotary({ nRot, theta, layout = 0, scaling = 0, original = 0, factor = 1, fast = 0, slow = 0, mscale = 0 }) {
+  // 2 ntk, 3 yarn, 4 bands.  u32 n_rot, layout, scaling, original; f64 theta, factor, fast, slow, mscale; u32 reserved[4].  axes: the pairs of
+  // every axis (pa_rotary_axes: u32 n_axes, order, pairs[4], reserved[2]), axesOrder 0 blocks, 1 cycled, 2 blocks with frequencies of their own
+  rotary({ nRot, theta, layout = 0, scaling = 0, original = 0, factor = 1, fast = 0, slow = 0, mscale = 0, axes = null, axesOrder = 0 }) {
     const b = new ArrayBuffer(72), u = new Uint32Array(b), f = new Float64Array(b), h = outPtr();
     u.set([nRot, layout, scaling, original]); f.set([theta, factor, fast, slow, mscale], 2);
-    check(this.S.pa_rotary_create(this.ctx, new Uint8Array(b), new Uint8Array(h.buffer)), this.ctx);
+    if (axes && axes.length > 4) throw new Error("pooled_attn: 1 to 4 axes are possible");
+    const many = axes && Uint32Array.from([axes.length, axesOrder, ...axes, ...Array(6 - axes.length).fill(0)]);
+    if (many) check(this.S.pa_rotary_create_axes(this.ctx, new Uint8Array(b), new Uint8Array(many.buffer), new Uint8Array(h.buffer)), this.ctx);
+    else check(this.S.pa_rotary_create(this.ctx, new Uint8Array(b), new Uint8Array(h.buffer)), this.ctx);
     this.rotaries.push(asPtr(h));
     return this.rotaries.at(-1);
   }
@@ -193,6 +201,25 @@ export class NativeAttention {
     const { hd, qDim, kvDim } = this.dims, it = paItems(items), r = rows && new Uint8Array(Uint32Array.from(rows).buffer), m = gated ? 2 : 1;
     check(this.S.pa_rotary_append(rot, this.layers[li], new Uint8Array(it.buffer), items.length, r, q, BigInt(m * qDim), BigInt(m * hd), k, v, BigInt(kvDim), qOut,
       f16Out ? PA_F16 : PA_F32, BigInt(qDim), stream), this.ctx);
+  }
+  // the same at positions that the device holds: i32 [nCols], of a rotation of several axes [axes][nCols]
+  rotaryAppendAt(li, rot, items, rows, positions, q, k, v, qOut, { gated = false, f16Out = false, stream = null } = {}) {
+    const { hd, qDim, kvDim } = this.dims, it = paItems(items), r = rows && new Uint8Array(Uint32Array.from(rows).buffer), m = gated ? 2 : 1;
+    check(this.S.pa_rotary_append_at(rot, this.layers[li], new Uint8Array(it.buffer), items.length, r, positions, q, BigInt(m * qDim), BigInt(m * hd), k, v, BigInt(kvDim), qOut,
+      f16Out ? PA_F16 : PA_F32, BigInt(qDim), stream), this.ctx);
+  }
+  // trees of drafted tokens: items = [[seq, base, n], ...], parents i32 on the device (null: chains), q rotated and packed; the gate as decodeShared takes it
+  decodeTree(li, items, parents, q, gate, out, { qFull = null, qF16 = this.es === 2, stream = null } = {}) {
+    const { hd, qDim } = this.dims, it = paItems(items), [g, gs, gh] = this._gate(gate, qFull);
+    check(this.S.pa_decode_tree(this.layers[li], new Uint8Array(it.buffer), items.length, parents, q, qF16 ? PA_F16 : PA_F32, BigInt(qDim), BigInt(hd), g, gs, gh, out,
+      BigInt(qDim), stream), this.ctx);
+  }
+  // rows of all layers' caches copied, forked or moved together: items = [[srcSeq, srcRow, dstSeq, dstRow, nRows], ...]; lists (u32 on the device,
+  // listStride words an item): [n, offsets ...] of the rows to move, the accepted path of a tree
+  move(items, { lists = null, listStride = 0, stream = null } = {}) {
+    const lp = new BigUint64Array(this.layers.map((L) => BigInt(Deno.UnsafePointer.value(L)))), u = new Uint32Array(6 * items.length);
+    items.forEach((it, i) => u.set([...it, 0], 6 * i));
+    check(this.S.pa_cache_move(new Uint8Array(lp.buffer), this.layers.length, new Uint8Array(u.buffer), items.length, lists, listStride, stream), this.ctx);
   }
   // the gate of a call and its strides: packed, or with `qFull` the one that lies between the heads of that projection
   _gate(gate, qFull) {

@@ -114,13 +114,21 @@ _SCALING = {"none": _l.PA_ROPE_SCALE_NONE, "linear": _l.PA_ROPE_SCALE_LINEAR, "n
             "bands": _l.PA_ROPE_SCALE_BANDS}
 
 
-class Rotary:
-    """A rotation of its own layout and scaling (pa_rotary), made by AttnEngine.rotary."""
+_AXES = {"blocks": _l.PA_ROPE_AXES_BLOCKS, "cycled": _l.PA_ROPE_AXES_CYCLED, "own": _l.PA_ROPE_AXES_OWN}
 
-    def __init__(self, eng: "AttnEngine", cfg: "_l.PaRotaryConfig"):
+
+class Rotary:
+    """A rotation of its own layout, scaling and number of axes (pa_rotary), made by AttnEngine.rotary."""
+    n_axes = 1
+
+    def __init__(self, eng: "AttnEngine", cfg: "_l.PaRotaryConfig", axes: "_l.PaRotaryAxes | None" = None):
         self.eng, self.n_rot, self.handle = eng, cfg.n_rot, None
         h = C.c_void_p()
-        eng._ck(eng.L.pa_rotary_create(eng.ctx, C.byref(cfg), C.byref(h)))
+        if axes is None:
+            eng._ck(eng.L.pa_rotary_create(eng.ctx, C.byref(cfg), C.byref(h)))
+        else:
+            self.n_axes = axes.n_axes
+            eng._ck(eng.L.pa_rotary_create_axes(eng.ctx, C.byref(cfg), C.byref(axes), C.byref(h)))
         self.handle, self._h = h, h.value
         eng._rotaries.add(self)
         self._apply, self._f_apply = eng._call.rotary_apply, eng.L.entry["pa_rotary_apply"]
@@ -142,15 +150,21 @@ class Rotary:
         self.eng._ck(self.eng.L.pa_rotary_freqs(self.handle, f, C.byref(m)))
         return list(f), m.value
 
+    def _places(self, positions, cols):
+        """Positions of the device: one per axis and column."""
+        if positions.dtype != torch.int32 or not positions.is_contiguous() or (tuple(positions.shape) != (cols,) if positions.dim() == 1 and self.n_axes == 1
+                                                                               else tuple(positions.shape) != (self.n_axes, cols)):
+            raise _l.PaError(-1, f"positions are a contiguous int32 tensor of one value per column, [{self.n_axes}, {cols}] of several axes")
+
     def apply(self, x: torch.Tensor, n_heads: int, pos: int = 0, positions: torch.Tensor | None = None, head_stride: int | None = None,
               out: torch.Tensor | None = None, out_head_stride: int | None = None) -> torch.Tensor:
-        """x [n_cols, stride] (float16 or float32) rotated: column c at pos + c, or at positions[c] (int32 on the device).  Into a
-        new [n_cols, n_heads * head_dim] of x's type, or `out`, which may be x itself (with x's head_stride)."""
+        """x [n_cols, stride] (float16 or float32) rotated: column c at pos + c, or at positions[c] (int32 on the device; of several axes
+        [axes, n_cols]).  Into a new [n_cols, n_heads * head_dim] of x's type, or `out`, which may be x itself (with x's head_stride)."""
         eng = self.eng
         hd = eng.cfg.head_dim
         eng._on_device(x, out, positions)
-        if positions is not None and (positions.dtype != torch.int32 or positions.dim() != 1 or positions.shape[0] != x.shape[0] or positions.stride(0) != 1):
-            raise _l.PaError(-1, "positions are a contiguous int32 tensor of one value per column")
+        if positions is not None:
+            self._places(positions, x.shape[0])
         cols, have = x.shape
         hs, ohs, last, dt = head_stride or hd, out_head_stride or hd, n_heads - 1, _dt(x.dtype)
         if out is None:
@@ -179,6 +193,7 @@ class AttnEngine:
         self._call, e = self.L.call, self.L.entry
         self._f_layer, self._f_items, self._f_rope, self._f_gather = e["pa_attn_layer"], e["pa_attn_items"], e["pa_rope_append"], e["pa_decode_gather"]
         self._f_rot_append, self._f_shared, self._f_weights, self._f_evict = e["pa_rotary_append"], e["pa_decode_shared"], e["pa_decode_weights"], e["pa_evict"]
+        self._f_rot_at, self._f_tree, self._f_move = e["pa_rotary_append_at"], e["pa_decode_tree"], e["pa_cache_move"]
         pc = _l.PaConfig(n_heads=cfg.n_heads, n_kv_heads=cfg.n_kv_heads, head_dim=cfg.head_dim, n_rot=cfg.n_rot, rope_theta=cfg.rope_theta,
                          rope_mode=_ROPE[cfg.rope_mode], act_dtype=_dt(cfg.act_dtype), max_cols=cfg.max_cols, splits=cfg.splits,
                          flags=_l.PA_FLAG_FAST if cfg.fast else 0)
@@ -191,6 +206,7 @@ class AttnEngine:
         self._dev = torch.device("cuda", device)
         self._views: dict = {}                  # cache() and the like: the device arrays as tensors, made once
         self._rotaries = weakref.WeakSet()      # destroyed ahead of the context
+        self._all_layers = None                 # move(): the layers' handles as an array, made once
         self.L.check(self.L.pa_create(device, C.byref(pc), C.byref(h)))
         self.ctx = h
         try:
@@ -230,7 +246,7 @@ class AttnEngine:
         self._views = {}
         for lh in self.layers:
             self.L.pa_layer_destroy(lh)
-        self.layers = []
+        self.layers, self._all_layers = [], None
         for r in list(getattr(self, "_rotaries", ())):
             r.destroy()
         if self.ctx:
@@ -431,24 +447,40 @@ class AttnEngine:
 
     # ---- rotations of other layouts and scalings ----
     def rotary(self, n_rot: int | None = None, theta: float | None = None, layout: str = "half", scaling: str = "none", factor: float = 1.0, original: int = 0,
-               beta_fast: float = 0.0, beta_slow: float = 0.0, high: float = 0.0, low: float = 0.0, mscale: float = 0.0) -> Rotary:
+               beta_fast: float = 0.0, beta_slow: float = 0.0, high: float = 0.0, low: float = 0.0, mscale: float = 0.0, axes=None, axes_order: str = "blocks") -> Rotary:
         """A rotation beside the engine's own: pairs of dims "half" a rotation apart or "interleaved", frequencies unscaled ("none"),
         "linear", "ntk", "yarn" (beta_fast, beta_slow: 32 and 1 unless given) or "bands" (high, low: 4 and 1) for a context `factor` times the
-        `original` one; mscale 0: the scaling's own factor on cos and sin.  The formulas stand in include/pooled_attn.h."""
+        `original` one; mscale 0: the scaling's own factor on cos and sin.  axes: the pairs of every axis of positions (time, height, width), in "blocks",
+        "cycled" through the pairs, or in blocks with frequencies of their "own".  The formulas stand in include/pooled_attn.h."""
         fast, slow = (high, low) if scaling == "bands" else (beta_fast, beta_slow)
+        many = None
+        if axes is not None:
+            pairs = [_l.u32(n) for n in axes]
+            if not 1 <= len(pairs) <= 4:
+                raise _l.PaError(-1, f"{len(pairs)} axes: 1 to 4 are possible")
+            many = _l.PaRotaryAxes(n_axes=len(pairs), order=_AXES[axes_order], pairs=(C.c_uint32 * 4)(*pairs))
         return Rotary(self, _l.PaRotaryConfig(n_rot=_l.u32(self.cfg.n_rot if n_rot is None else n_rot), layout=_LAYOUT[layout], scaling=_SCALING[scaling], original=_l.u32(original),
-                                              theta=self.cfg.rope_theta if theta is None else theta, factor=factor, fast=fast, slow=slow, mscale=mscale))
+                                              theta=self.cfg.rope_theta if theta is None else theta, factor=factor, fast=fast, slow=slow, mscale=mscale), many)
 
     def rotary_append(self, li: int, rot: Rotary, items, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, rows=None, q_head_stride: int | None = None,
-                      q_dtype: torch.dtype = torch.float32, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+                      q_dtype: torch.dtype = torch.float32, q_out: torch.Tensor | None = None, positions: torch.Tensor | None = None) -> torch.Tensor | None:
         """rope_append with `rot`, for one or many sequences: items = [(seq, pos, n_cols)] own consecutive rows of q, k and v.  Item i's k and v go to
-        cache rows rows[i] .. (None: the rows of their positions).  Returns the rotated q, [n_cols, q_dim] of q_dtype (None without q)."""
+        cache rows rows[i] .. (None: the rows of their positions).  positions (int32 on the device, [n_cols] or [axes, n_cols]): where the columns are,
+        instead of the items' positions, which then name rows only.  Returns the rotated q, [n_cols, q_dim] of q_dtype (None without q)."""
         total = sum([it[2] for it in items])
         self._columns(total, q, q_head_stride, k, v, q_out)
         if q is not None and q_out is None:
             q_out = torch.empty_strided((total, self._q_dim), (self._q_dim, 1), dtype=q_dtype, device=self._dev)
         if k.stride(0) != v.stride(0) and total > 1:
             raise _l.PaError(-1, "k and v have different column strides")
+        if positions is not None:
+            self._on_device(positions)
+            rot._places(positions, total)
+            rc = self._call.rotary_append_at(self._f_rot_at, rot._h, self.layers[li].value, items, rows, positions, q, q_head_stride or self.cfg.head_dim, k, v, q_out,
+                                             _l.PA_F32 if q is None else _dt(q_out.dtype), self._raw_st())
+            if rc:
+                self._ck(rc)
+            return q_out
         rc = self._call.rotary_append(self._f_rot_append, rot._h, self.layers[li].value, items, rows, q, q_head_stride or self.cfg.head_dim, k, v, q_out,
                                       _l.PA_F32 if q is None else _dt(q_out.dtype), self._raw_st())
         if rc:
@@ -500,6 +532,50 @@ class AttnEngine:
         if out.dtype != act or cols != n or have < self._q_dim:
             raise _l.PaError(-1, f"{out.dtype} output of shape {tuple(out.shape)} for {n} columns of {self._q_dim}")
         return out
+
+    # ---- trees of drafted tokens ----
+    def decode_tree(self, li: int, items, q: torch.Tensor, parents: torch.Tensor | None = None, gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    q_head_stride: int | None = None, gate_head_stride: int | None = None) -> torch.Tensor:
+        """Trees of drafted tokens: items = [(seq, base, n)], n tokens (q rotated; their rows base .. base + n - 1 appended) behind rows [0, base) of their
+        sequence.  parents (int32 on the device, [total tokens]): the number within its tree of the token that a token follows, -1: the committed
+        rows; None: chains.  A token attends the committed rows, its ancestors and itself."""
+        total = sum([it[2] for it in items])
+        out = self._batch(total, q, q_head_stride, gate, gate_head_stride, out)
+        if parents is not None:
+            self._on_device(parents)
+            if parents.dtype != torch.int32 or parents.shape != (total,):
+                raise _l.PaError(-1, f"{parents.dtype} parents of shape {tuple(parents.shape)}: int32, one per token of {total}, are wanted")
+        hd = self.cfg.head_dim
+        rc = self._call.decode_tree(self._f_tree, self.layers[li].value, items, parents, q, _dt(q.dtype), q_head_stride or hd, gate, gate_head_stride or hd, out, self._raw_st())
+        if rc:
+            self._ck(rc)
+        return out
+
+    # ---- rows copied, forked and moved together ----
+    def move(self, items, lists: torch.Tensor | None = None, layers=None):
+        """Moves cache rows of all layers (or those numbered in `layers`) in one call: items = [(src_seq, src_row, dst_seq, dst_row, n_rows)], K, V, scales
+        and tracked sums.  An item may overlap itself; items with one source are forks of it.  lists (int32 on the device, [n_items, stride], as
+        decode_gather's): per item how many rows and their offsets into the item's n_rows source rows, which go to dst_row, dst_row + 1, ..: the accepted
+        path of a tree."""
+        if layers is None:
+            if self._all_layers is None:
+                self._all_layers = self._handles(range(len(self.layers)))
+            arr, n = self._all_layers
+        else:
+            arr, n = self._handles(layers)
+        stride = 0
+        if lists is not None:
+            self._on_device(lists)
+            if lists.dtype != torch.int32 or lists.dim() != 2 or lists.shape[0] != len(items) or not lists.is_contiguous():
+                raise _l.PaError(-1, f"{lists.dtype} lists of shape {tuple(lists.shape)}: contiguous int32, one row per item of {len(items)}, are wanted")
+            stride = lists.shape[1]
+        rc = self._call.cache_move(self._f_move, C.addressof(arr), n, items, lists, stride, self._raw_st())
+        if rc:
+            self._ck(rc)
+
+    def _handles(self, layers):
+        hs = [self.layers[li].value for li in layers]
+        return (C.c_void_p * max(1, len(hs)))(*hs), len(hs)
 
     # ---- batches that share a prefix ----
     def decode_shared(self, li: int, prefix: "AttnEngine | None", prefix_seq: int, prefix_len: int, seqs_pos, q: torch.Tensor, gate: torch.Tensor | None = None,

@@ -12,7 +12,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libpooled_attn.so")
 CALL_OUT = os.path.join(HERE, "_pa_call" + sysconfig.get_config_var("EXT_SUFFIX"))   # CPython module: the per-layer calls without ctypes
 SOURCES = ["pa_api.cu", "pa_rope_append.cu", "pa_decode.cu", "pa_prefill.cu", "pa_verify.cu", "pa_kvfmt.cu", "pa_q8.cu", "pa_front.cu", "pa_noalloc.cu",
-           "pa_rotary.cu", "pa_rotary_api.cu", "pa_shared.cu", "pa_shared_api.cu", "pa_evict.cu"]
+           "pa_rotary.cu", "pa_rotary_api.cu", "pa_shared.cu", "pa_shared_api.cu", "pa_evict.cu",
+           "pa_tree.cu", "pa_tree_api.cu", "pa_move.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "--use_fast_math=false",
          "-Xcompiler", "-fPIC,-fvisibility=hidden", "--expt-relaxed-constexpr"]
 

@@ -201,6 +201,8 @@ extern "C" int pa_create(int device, const pa_config* cfg, pa_ctx** out) {
   if ((e = cudaMemset(ctx->merge_rec, 0xff, ctx->merge_bytes)) != cudaSuccess) return bail(PA_ECUDA, "cudaMemset(merge records)", e);
   if ((e = cudaMalloc(&ctx->merge_ctr, ctx->sm_count * 8)) != cudaSuccess) return bail(PA_ENOMEM, "cudaMalloc(merge counters)", e);
   if ((e = cudaMemset(ctx->merge_ctr, 0, ctx->sm_count * 8)) != cudaSuccess) return bail(PA_ECUDA, "cudaMemset(merge counters)", e);
+  if ((e = cudaMalloc(&ctx->move_words, kMoveHead * 4 + kMoveTiles)) != cudaSuccess) return bail(PA_ENOMEM, "cudaMalloc(order of moves)", e);
+  if ((e = cudaMemset(ctx->move_words, 0, kMoveHead * 4 + kMoveTiles)) != cudaSuccess) return bail(PA_ECUDA, "cudaMemset(order of moves)", e);
   if ((e = cudaMalloc(&ctx->dev_err, 4)) != cudaSuccess) return bail(PA_ENOMEM, "cudaMalloc(err)", e);
   if ((e = cudaMemset(ctx->dev_err, 0, 4)) != cudaSuccess) return bail(PA_ECUDA, "cudaMemset(err)", e);
   if ((e = cudaMallocHost(&ctx->host_err, 4)) != cudaSuccess) return bail(PA_ENOMEM, "cudaMallocHost(err)", e);
@@ -216,7 +218,7 @@ extern "C" int pa_create(int device, const pa_config* cfg, pa_ctx** out) {
 extern "C" int pa_destroy(pa_ctx* ctx) {
   if (!ctx) return PA_OK;
   cudaSetDevice(ctx->device);
-  cudaFree(ctx->inv_freq); cudaFree(ctx->angles); cudaFree(ctx->norm_q); cudaFree(ctx->norm_k); cudaFree(ctx->q_rot); cudaFree(ctx->k_rot); cudaFree(ctx->part_o); cudaFree(ctx->part_ml); cudaFree(ctx->dev_err); cudaFree(ctx->merge_rec); cudaFree(ctx->merge_ctr);
+  cudaFree(ctx->inv_freq); cudaFree(ctx->angles); cudaFree(ctx->norm_q); cudaFree(ctx->norm_k); cudaFree(ctx->q_rot); cudaFree(ctx->k_rot); cudaFree(ctx->part_o); cudaFree(ctx->part_ml); cudaFree(ctx->dev_err); cudaFree(ctx->merge_rec); cudaFree(ctx->merge_ctr); cudaFree(ctx->move_words);
   cudaFree(ctx->stage_dev);
   cudaFree(ctx->scores);
   for (void* p : ctx->outgrown) cudaFree(p);
@@ -345,7 +347,7 @@ extern "C" int pa_reset(pa_ctx* ctx) {
   cudaGetLastError();
   if (cudaDeviceSynchronize() != cudaSuccess || cudaMemset(ctx->dev_err, 0, 4) != cudaSuccess ||
       cudaMemset(ctx->merge_rec, 0xff, ctx->merge_bytes) != cudaSuccess || cudaMemset(ctx->merge_ctr, 0, ctx->sm_count * 8) != cudaSuccess ||
-      cudaDeviceSynchronize() != cudaSuccess)
+      cudaMemset(ctx->move_words, 0, kMoveHead * 4 + kMoveTiles) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess)
     return fail(ctx, PA_ECUDA, "pa_reset: the device does not answer");
   *ctx->host_err = 0;
   ctx->failed = false;
@@ -483,7 +485,7 @@ static bool front_supports(const pa_ctx* ctx, int mode) {
 static void rows_in_flight(pa_layer* L, uint32_t pos) {
   pa_ctx* ctx = L->ctx;
   uint32_t r0 = pos - L->origin;
-  if (ctx->inflight_layer == L && ctx->inflight_row0 < r0) r0 = ctx->inflight_row0;
+  if (rows_may_be_in_flight(ctx, L) && ctx->inflight_row0 < r0) r0 = ctx->inflight_row0;
   ctx->inflight_layer = L; ctx->inflight_row0 = r0;
 }
 static int front_impl(pa_layer* L, uint32_t seq, uint32_t pos, uint32_t n_cols, const void* q, uint64_t qcs, uint64_t qhs, void* q_out, uint64_t q_out_cs,
@@ -650,7 +652,7 @@ static int rope_append_items_impl(pa_layer* L, const pa_item* items, uint32_t n_
   CU_TRY(ctx, launch_rope_append(p, n_items, (cudaStream_t)stream));
   ctx->stats.kernel_launches++;
   // what the kernel just launched may still be writing: rows from row0 on (none on a shard that owns no item's row)
-  if (ctx->inflight_layer == L && ctx->inflight_row0 < row0) row0 = ctx->inflight_row0;
+  if (rows_may_be_in_flight(ctx, L) && ctx->inflight_row0 < row0) row0 = ctx->inflight_row0;
   ctx->inflight_layer = L; ctx->inflight_row0 = row0;
   return PA_OK;
 }
@@ -869,7 +871,7 @@ static int decode_any_impl(pa_layer* L, const pa_item* items, uint32_t n_items, 
         f.early = after_front && c0 == 0 ? 1u : 0u;   // (a later block of a wide call follows a merge, not the front)
         if (fz) {
           f.k_new = fz->k; f.v_new = fz->v; f.half = ctx->cfg.n_rot / 2; f.early = 1;
-          f.early_limit = ctx->inflight_layer == L ? ctx->inflight_row0 : 0xffffffffu;
+          f.early_limit = rows_may_be_in_flight(ctx, L) ? ctx->inflight_row0 : 0xffffffffu;
           memcpy(f.ang, host_angles(ctx, fz->pos, 1), (size_t)f.half * sizeof(Angle));
         }
         f.scale_log2 = (float)(1.4426950408889634 / sqrt((double)hd));
@@ -1006,7 +1008,7 @@ static int decode_impl(pa_layer* L, const pa_item* items, uint32_t n_items, cons
   // after this library's own RoPE/append kernel the only rows in flux are the call's new ones: older rows may be
   // fetched while that kernel still runs
   p.prefetch_old_rows = after_own_append ? 1u : 0u;
-  p.early_limit = (after_own_append && ctx->inflight_layer == L) ? ctx->inflight_row0 : 0xffffffffu;
+  p.early_limit = (after_own_append && rows_may_be_in_flight(ctx, L)) ? ctx->inflight_row0 : 0xffffffffu;
   p.pre_stages = (uint32_t)ctx->tune.pre_stages;
   p.kv_evict_first = ctx->tune.kv_evict_first ? 1u : 0u;
   // tiles beyond the ring asked into L2 ahead of the wait: on a shard the wait spans the cross-GPU exchange of the call
@@ -1099,7 +1101,7 @@ extern "C" int pa_decode(pa_layer* L, const pa_item* items, uint32_t n_items, co
   // straight after this library's own append into the layer (the kernel before this one on the stream), rows older
   // than the appended ones may be fetched while that kernel still runs
   return decode_impl(L, items, n_items, q, q_dtype, q_col_stride, q_head_stride, gate, gate_col_stride, gate_head_stride, out, out_col_stride, nullptr,
-                     (cudaStream_t)stream, "pa_decode", L->ctx->inflight_layer == L);
+                     (cudaStream_t)stream, "pa_decode", rows_may_be_in_flight(L->ctx, L));
 }
 
 extern "C" int pa_decode_gather(pa_layer* L, uint32_t seq, uint32_t n_cols, const uint32_t* row_lists, uint32_t list_stride, const void* q, int q_dtype,
@@ -1753,7 +1755,7 @@ extern "C" int pa_decode_exchange(pa_layer* L, const pa_item* items, uint32_t n_
   if (!out) return fail(L->ctx, PA_EINVAL, "pa_decode_exchange: null out");
   if (L->kv_format != PA_KV_F16) return fail(L->ctx, PA_EUNSUPPORTED, "pa_decode_exchange: the peer exchange is for f16 caches");
   return decode_impl(L, items, n_items, q, q_dtype, q_col_stride, q_head_stride, gate, gate_col_stride, gate_head_stride, out, out_col_stride, nullptr,
-                     (cudaStream_t)stream, "pa_decode_exchange", L->ctx->inflight_layer == L, true);
+                     (cudaStream_t)stream, "pa_decode_exchange", rows_may_be_in_flight(L->ctx, L), true);
 }
 
 // One token of each of several sequences through a whole layer: the fused front of the decode kernel for every item

@@ -22,6 +22,11 @@ typedef int (*fn_decode_gather)(pa_layer*, uint32_t, uint32_t, const uint32_t*, 
 typedef int (*fn_rotary_apply)(pa_rotary*, const void*, int, uint64_t, uint64_t, uint32_t, const int32_t*, int32_t, uint32_t, void*, int, uint64_t, uint64_t, void*);
 typedef int (*fn_rotary_append)(pa_rotary*, pa_layer*, const pa_item*, uint32_t, const uint32_t*, const void*, uint64_t, uint64_t, const void*, const void*, uint64_t,
                                 void*, int, uint64_t, void*);
+typedef int (*fn_rotary_append_at)(pa_rotary*, pa_layer*, const pa_item*, uint32_t, const uint32_t*, const int32_t*, const void*, uint64_t, uint64_t, const void*,
+                                   const void*, uint64_t, void*, int, uint64_t, void*);
+typedef int (*fn_decode_tree)(pa_layer*, const pa_item*, uint32_t, const int32_t*, const void*, int, uint64_t, uint64_t, const void*, uint64_t, uint64_t, void*, uint64_t,
+                              void*);
+typedef int (*fn_cache_move)(pa_layer* const*, uint32_t, const pa_move_item*, uint32_t, const uint32_t*, uint32_t, void*);
 typedef int (*fn_decode_shared)(pa_layer*, pa_layer*, uint32_t, uint32_t, uint32_t, const pa_item*, uint32_t, const void*, int, uint64_t, uint64_t, const void*,
                                 uint64_t, uint64_t, void*, uint64_t, void*);
 typedef int (*fn_decode_weights)(pa_layer*, const pa_item*, uint32_t, const void*, int, uint64_t, uint64_t, const void*, uint64_t, uint64_t, void*, uint64_t, void*);
@@ -182,25 +187,27 @@ static PyObject* decode_gather(PyObject* self, PyObject* const* a, Py_ssize_t n)
   return PyLong_FromLong(rc);
 }
 
-/* a sequence of `width`-tuples of integers as `width` words each of a four-word struct, the others `rest`; NULL with an error set.  Freed by the caller. */
-static uint32_t* words_of(PyObject* o, Py_ssize_t width, uint32_t rest, const char* what, Py_ssize_t* cnt) {
+/* a sequence of `width`-tuples of integers as `width` words each of a struct of `size`, the third of a pair `rest`, the others 0; NULL with an
+ * error set.  Freed by the caller. */
+static uint32_t* words_in(PyObject* o, Py_ssize_t width, Py_ssize_t size, uint32_t rest, const char* what, Py_ssize_t* cnt) {
   PyObject* list = PySequence_Fast(o, what);
   if (!list) return NULL;
   *cnt = PySequence_Fast_GET_SIZE(list);
-  uint32_t* w = (uint32_t*)calloc((size_t)(*cnt ? *cnt : 1) * 4, sizeof(uint32_t));
+  uint32_t* w = (uint32_t*)calloc((size_t)(*cnt ? *cnt : 1) * (size_t)size, sizeof(uint32_t));
   if (!w) { Py_DECREF(list); PyErr_NoMemory(); return NULL; }
   for (Py_ssize_t i = 0; i < *cnt; ++i) {
     PyObject* t = PySequence_Fast(PySequence_Fast_GET_ITEM(list, i), what);
     int bad = !t;
     if (t && PySequence_Fast_GET_SIZE(t) != width) { PyErr_SetString(PyExc_ValueError, what); bad = 1; }
-    for (Py_ssize_t k = 0; !bad && k < width; ++k) bad = u32_of(PySequence_Fast_GET_ITEM(t, k), &w[4 * i + k]);
+    for (Py_ssize_t k = 0; !bad && k < width; ++k) bad = u32_of(PySequence_Fast_GET_ITEM(t, k), &w[size * i + k]);
     Py_XDECREF(t);
     if (bad) { free(w); Py_DECREF(list); return NULL; }
-    if (width == 2) w[4 * i + 2] = rest;
+    if (width == 2) w[size * i + 2] = rest;
   }
   Py_DECREF(list);
   return w;
 }
+static uint32_t* words_of(PyObject* o, Py_ssize_t width, uint32_t rest, const char* what, Py_ssize_t* cnt) { return words_in(o, width, 4, rest, what, cnt); }
 static const char* const kPairs = "the items are a sequence of (seq, pos) pairs";
 static const char* const kTriples = "the items are a sequence of triples";
 
@@ -223,6 +230,22 @@ static PyObject* rotary_apply(PyObject* self, PyObject* const* a, Py_ssize_t n) 
   return PyLong_FromLong(rc);
 }
 
+/* the rows of an append, one for each of `cnt` items (None: NULL); -1 with an error set.  Freed by the caller. */
+static int rows_list(PyObject* o, Py_ssize_t cnt, uint32_t** rows) {
+  *rows = NULL;
+  if (o == Py_None) return 0;
+  PyObject* list = PySequence_Fast(o, "the rows are a sequence of integers");
+  if (!list) return -1;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(list);
+  int bad = n != cnt;
+  if (bad) PyErr_SetString(PyExc_ValueError, "one row per item");
+  else if (!(*rows = (uint32_t*)calloc((size_t)(n ? n : 1), sizeof(uint32_t)))) { PyErr_NoMemory(); bad = 1; }
+  for (Py_ssize_t i = 0; !bad && i < n; ++i) bad = u32_of(PySequence_Fast_GET_ITEM(list, i), &(*rows)[i]);
+  Py_DECREF(list);
+  if (bad) { free(*rows); *rows = NULL; return -1; }
+  return 0;
+}
+
 /* rotary_append(entry, rotary, layer, [(seq, pos, n_cols)], rows, q, q_head_stride, k, v, q_out, q_out_dtype, stream) -> status */
 static PyObject* rotary_append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   uint64_t fn, rot, layer, qcs = 0, qhs = 0, kcs, ocs = 0, stream;
@@ -233,28 +256,82 @@ static PyObject* rotary_append(PyObject* self, PyObject* const* a, Py_ssize_t n)
       (a[5] != Py_None && (stride0(a[5], &qcs) || u64_of(a[6], &qhs))) || ptr_of(a[7], &k) || stride0(a[7], &kcs) || ptr_of(a[8], &v) || ptr_of(a[9], &o) ||
       (a[9] != Py_None && stride0(a[9], &ocs)) || u32_of(a[10], &odt) || u64_of(a[11], &stream))
     return NULL;
-  Py_ssize_t cnt, nr = 0;
-  uint32_t *items = words_of(a[3], 3, 0, kTriples, &cnt), *rows = NULL;
+  Py_ssize_t cnt;
+  uint32_t *items = words_of(a[3], 3, 0, kTriples, &cnt), *rows;
   if (!items) return NULL;
-  if (a[4] != Py_None) {
-    PyObject* list = PySequence_Fast(a[4], "the rows are a sequence of integers");
-    int bad = !list;
-    if (list) {
-      nr = PySequence_Fast_GET_SIZE(list);
-      if (nr != cnt) { PyErr_SetString(PyExc_ValueError, "one row per item"); bad = 1; }
-      rows = bad ? NULL : (uint32_t*)calloc((size_t)(nr ? nr : 1), sizeof(uint32_t));
-      if (!bad && !rows) { PyErr_NoMemory(); bad = 1; }
-      for (Py_ssize_t i = 0; !bad && i < nr; ++i) bad = u32_of(PySequence_Fast_GET_ITEM(list, i), &rows[i]);
-      Py_DECREF(list);
-    }
-    if (bad) { free(rows); free(items); return NULL; }
-  }
+  if (rows_list(a[4], cnt, &rows)) { free(items); return NULL; }
   int rc;
   Py_BEGIN_ALLOW_THREADS
   rc = ((fn_rotary_append)(uintptr_t)fn)((pa_rotary*)(uintptr_t)rot, (pa_layer*)(uintptr_t)layer, (const pa_item*)items, (uint32_t)cnt, rows, q, qcs, qhs, k, v, kcs, o,
                     (int)odt, ocs, (void*)(uintptr_t)stream);
   Py_END_ALLOW_THREADS
   free(rows); free(items);
+  return PyLong_FromLong(rc);
+}
+
+/* rotary_append_at(entry, rotary, layer, [(seq, pos, n_cols)], rows, positions, q, q_head_stride, k, v, q_out, q_out_dtype, stream) -> status */
+static PyObject* rotary_append_at(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  uint64_t fn, rot, layer, qcs = 0, qhs = 0, kcs, ocs = 0, stream;
+  uint32_t odt;
+  void *ps, *q, *k, *v, *o;
+  (void)self;
+  if (args_are(n, 13, "rotary_append_at") || u64_of(a[0], &fn) || u64_of(a[1], &rot) || u64_of(a[2], &layer) || ptr_of(a[5], &ps) || ptr_of(a[6], &q) ||
+      (a[6] != Py_None && (stride0(a[6], &qcs) || u64_of(a[7], &qhs))) || ptr_of(a[8], &k) || stride0(a[8], &kcs) || ptr_of(a[9], &v) || ptr_of(a[10], &o) ||
+      (a[10] != Py_None && stride0(a[10], &ocs)) || u32_of(a[11], &odt) || u64_of(a[12], &stream))
+    return NULL;
+  Py_ssize_t cnt;
+  uint32_t *items = words_of(a[3], 3, 0, kTriples, &cnt), *rows;
+  if (!items) return NULL;
+  if (rows_list(a[4], cnt, &rows)) { free(items); return NULL; }
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = ((fn_rotary_append_at)(uintptr_t)fn)((pa_rotary*)(uintptr_t)rot, (pa_layer*)(uintptr_t)layer, (const pa_item*)items, (uint32_t)cnt, rows, (const int32_t*)ps, q, qcs,
+                    qhs, k, v, kcs, o, (int)odt, ocs, (void*)(uintptr_t)stream);
+  Py_END_ALLOW_THREADS
+  free(rows); free(items);
+  return PyLong_FromLong(rc);
+}
+
+/* decode_tree(entry, layer, [(seq, base, n_tokens)], parents, q, q_dtype, q_head_stride, gate, gate_head_stride, out, stream) -> status */
+static PyObject* decode_tree(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  uint64_t fn, layer, qcs, qhs, gcs = 0, ghs = 0, ocs, stream;
+  uint32_t qdt;
+  void *ps, *q, *g, *out;
+  (void)self;
+  if (args_are(n, 11, "decode_tree") || u64_of(a[0], &fn) || u64_of(a[1], &layer) || ptr_of(a[3], &ps) || ptr_of(a[4], &q) || stride0(a[4], &qcs) || u32_of(a[5], &qdt) ||
+      u64_of(a[6], &qhs) || ptr_of(a[7], &g) || (a[7] != Py_None && (stride0(a[7], &gcs) || u64_of(a[8], &ghs))) || ptr_of(a[9], &out) || stride0(a[9], &ocs) ||
+      u64_of(a[10], &stream))
+    return NULL;
+  Py_ssize_t cnt;
+  uint32_t* items = words_of(a[2], 3, 0, kTriples, &cnt);
+  if (!items) return NULL;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = ((fn_decode_tree)(uintptr_t)fn)((pa_layer*)(uintptr_t)layer, (const pa_item*)items, (uint32_t)cnt, (const int32_t*)ps, q, (int)qdt, qcs, qhs, g, gcs, ghs, out, ocs,
+                    (void*)(uintptr_t)stream);
+  Py_END_ALLOW_THREADS
+  free(items);
+  return PyLong_FromLong(rc);
+}
+
+/* cache_move(entry, layers (address of an array of them), n_layers, [(src_seq, src_row, dst_seq, dst_row, n_rows)], lists, list_stride, stream) -> status */
+static PyObject* cache_move(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  uint64_t fn, layers, stream;
+  uint32_t n_layers, list_stride;
+  void* lists;
+  (void)self;
+  if (args_are(n, 7, "cache_move") || u64_of(a[0], &fn) || u64_of(a[1], &layers) || u32_of(a[2], &n_layers) || ptr_of(a[4], &lists) || u32_of(a[5], &list_stride) ||
+      u64_of(a[6], &stream))
+    return NULL;
+  Py_ssize_t cnt;
+  uint32_t* items = words_in(a[3], 5, 6, 0, "the items are a sequence of (src_seq, src_row, dst_seq, dst_row, n_rows)", &cnt);
+  if (!items) return NULL;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = ((fn_cache_move)(uintptr_t)fn)((pa_layer* const*)(uintptr_t)layers, n_layers, (const pa_move_item*)items, (uint32_t)cnt, (const uint32_t*)lists, list_stride,
+                    (void*)(uintptr_t)stream);
+  Py_END_ALLOW_THREADS
+  free(items);
   return PyLong_FromLong(rc);
 }
 
@@ -328,6 +405,9 @@ static PyMethodDef methods[] = {
     {"decode_gather", (PyCFunction)(void (*)(void))decode_gather, METH_FASTCALL, "pa_decode_gather on tensors"},
     {"rotary_apply", (PyCFunction)(void (*)(void))rotary_apply, METH_FASTCALL, "pa_rotary_apply on tensors"},
     {"rotary_append", (PyCFunction)(void (*)(void))rotary_append, METH_FASTCALL, "pa_rotary_append on tensors"},
+    {"rotary_append_at", (PyCFunction)(void (*)(void))rotary_append_at, METH_FASTCALL, "pa_rotary_append_at on tensors"},
+    {"decode_tree", (PyCFunction)(void (*)(void))decode_tree, METH_FASTCALL, "pa_decode_tree on tensors"},
+    {"cache_move", (PyCFunction)(void (*)(void))cache_move, METH_FASTCALL, "pa_cache_move on tensors"},
     {"decode_shared", (PyCFunction)(void (*)(void))decode_shared, METH_FASTCALL, "pa_decode_shared on tensors"},
     {"decode_weights", (PyCFunction)(void (*)(void))decode_weights, METH_FASTCALL, "pa_decode_weights on tensors"},
     {"evict", (PyCFunction)(void (*)(void))evict, METH_FASTCALL, "pa_evict on tensors"},

@@ -23,7 +23,7 @@ constexpr uint32_t kWaitPolls = 1u << 24;  // with 32..64 ns back-off: well unde
 constexpr uint32_t kMergePolls = 1u << 20; // looks for another CTA's record: about a second
 constexpr uint32_t kMergeLeave = 1u << 12; // ... before a unit is left to the CTA that comes last (f32 tokens): some milliseconds
 
-enum : uint32_t { WAIT_KFULL = 1, WAIT_VFULL = 2, WAIT_EMPTY = 3, WAIT_MMA = 4, WAIT_TMEM = 5, WAIT_QFULL = 6, WAIT_PEER = 7, WAIT_MERGE = 8 };
+enum : uint32_t { WAIT_KFULL = 1, WAIT_VFULL = 2, WAIT_EMPTY = 3, WAIT_MMA = 4, WAIT_TMEM = 5, WAIT_QFULL = 6, WAIT_PEER = 7, WAIT_MERGE = 8, WAIT_MOVE = 9 };
 
 // Most splits of a decode call over `tiles` 64-row tiles.  Up to eight tiles one each: their records are merged through
 // cluster shared memory (see the end of pa_decode_kernel), so another split costs little and a tile is 0.7 to 1.2 us of a chain
@@ -427,6 +427,9 @@ struct pa_ctx {
   float* scores = nullptr;
   size_t scores_floats = 0;
   std::vector<void*> outgrown;
+  // device: what a pa_cache_move whose rows lie over one another needs to keep its order: [0] tiles begun, [1] CTAs done, a byte for
+  // every tile from kMoveHead words on; zero between calls
+  unsigned int* move_words = nullptr;
   bool failed = false;
   std::string err;
   pa_stats stats{};
@@ -451,3 +454,9 @@ struct pa_layer {
   double norm_eps = 0.0;
   float* sums = nullptr;            // summed attention weights, f32 [n_seqs][n_kv_heads][max_seq] (pa_layer_track_weights)
 };
+
+namespace pa {
+// inflight_layer after a call that wrote rows of several layers: nothing of any layer may be fetched early
+inline const pa_layer* const kEveryLayer = reinterpret_cast<const pa_layer*>(1);
+inline bool rows_may_be_in_flight(const pa_ctx* ctx, const pa_layer* L) { return ctx->inflight_layer == L || ctx->inflight_layer == kEveryLayer; }
+}  // namespace pa

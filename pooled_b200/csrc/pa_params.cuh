@@ -210,7 +210,8 @@ struct RotaryParams {
   const void* q; uint64_t q_col_stride, q_head_stride; uint32_t q_heads;    // q == nullptr: k and v only
   void* q_out; uint64_t q_out_col_stride, q_out_head_stride;
   int in_f16, out_f16;
-  const int32_t* positions;                                                 // no append: per column, or nullptr: pos[0] + column
+  const int32_t* positions;                                                 // [n_axes][n_cols], or nullptr: pos[item] + its column
+  uint32_t n_axes, axes_cycled, axis_pairs[4];                              // several axes: pairs of each
   // append: rows of f16 caches; item i owns columns col0[i] .., at positions pos[i] .. and cache rows row[i] .. (over all sequences)
   const void* k; const void* v; uint64_t kv_col_stride; uint32_t kv_heads;
   __half* k_cache; __half* v_cache;
@@ -257,6 +258,31 @@ struct SharedFinishParams {
 };
 constexpr uint32_t kSumRows = 256;    // rows of one CTA's sums
 
+// attention of trees of drafted tokens (pa_tree_kernel) and the merge of its records (pa_tree_finish_kernel); an item may come in parts
+constexpr int kMaxTrees = 32;         // items of one pa_decode_tree call, parts of one launch
+struct TreeParams {
+  const void* q; int q_f16; uint64_t q_col_stride, q_head_stride;           // rotated queries of the launch's columns
+  uint32_t n_heads, G;
+  float scale_log2;
+  float* part_o; float* part_ml; uint32_t n_rec, seg, fold;                 // as in SharedParams
+  const int32_t* parents;                                                   // of all the call's columns, or nullptr: chains
+  const __half* v;                                                          // the V cache, whose values tree_restore looks up
+  uint32_t kv_dim, max_seq, n_items, tps, units;
+  uint32_t seq[kMaxTrees], base[kMaxTrees], rows[kMaxTrees];                // a part's sequence, its committed rows, and those with its last token
+  uint32_t col0[kMaxTrees + 1], node0[kMaxTrees], parent0[kMaxTrees];       // first column in the launch, which token of the tree that is, where the tree's parents begin
+  uint32_t unit0[kMaxTrees + 1];                                            // first unit: row tiles fastest, then splits of tps tiles
+  uint16_t tile_cols[kMaxTrees], row_tiles[kMaxTrees];                      // columns of a row tile
+  uint32_t* err;
+};
+struct TreeFinishParams {
+  const float* part_o; const float* part_ml; uint32_t n_rec;
+  uint32_t n_items, n_heads, n_rows, lanes;                                 // lanes: as in SharedFinishParams; 0: a warp a row
+  const void* gate; uint64_t gate_col_stride, gate_head_stride;
+  void* out; uint64_t out_col_stride; int act_f16, vec;                     // vec: four values of gate and out lie on whole vectors
+  uint32_t col0[kMaxTrees + 1];
+  uint16_t n_own[kMaxTrees];                                                // records of an item's rows
+};
+
 // eviction by summed weights (pa_evict_select_kernel, pa_evict_move_kernel)
 constexpr int kMaxEvict = 32;                       // items of one pa_evict call
 constexpr uint32_t kEvictKeys = 49152;              // rows of one CTA where eight share them out
@@ -267,6 +293,32 @@ struct EvictParams {
   uint32_t* list;                                   // [n_items][n_kv][n_keep]: the rows that stay
   uint32_t chunks;                                  // CTAs that share the rows of an item that goes to another sequence (the launcher sets it)
   uint32_t src[kMaxEvict], dst[kMaxEvict], rows[kMaxEvict];
+};
+
+// rows moved within and between the sequences of several layers (pa_move_kernel)
+constexpr int kMaxMoves = 64;                       // items of one pa_cache_move call
+constexpr int kMoveLayers = 64;                     // layers of one launch
+constexpr uint32_t kMoveUnits = 2048;               // units (16 bytes of a row, 4 of scales and sums) of a tile: eight of each thread
+constexpr uint32_t kMoveColumnRows = 512;           // most rows over one another that a tile holds all of
+constexpr uint32_t kMoveHead = 4, kMoveTiles = 1u << 20;   // words ahead of the tiles' bytes; tiles of a launch that keeps an order
+enum : uint8_t { MOVE_OVER = 1, MOVE_UP = 2, MOVE_COLUMNS = 4 };
+struct MoveParams {
+  void* rows[kMoveLayers][2];                       // K and V caches,
+  float* scales[kMoveLayers][2];                    // their scales (int8 caches),
+  float* sums[kMoveLayers];                         // summed weights (layers that have them)
+  uint32_t per[2], inv[2];                          // units of a row and of a row of scales, ceil(2^32 / them)
+  uint32_t max_seq, n_kv, n_groups;
+  // tiles: of a layer first K, then V (tiles[0] each), scales of K and of V (tiles[1]), sums head by head (tiles[2]); first[kind][g]: a
+  // group's first among them
+  uint32_t tiles[3], layer_tiles, first[3][kMaxMoves + 1];
+  // groups: source rows that go to one place, or to those of several items
+  uint32_t seq[kMaxMoves], row[kMaxMoves], n[kMaxMoves], item0[kMaxMoves + 1];
+  uint32_t dst_seq[kMaxMoves], dst_row[kMaxMoves];  // of the items, groups' items together
+  uint32_t list[kMaxMoves];                         // of the items: which list
+  uint8_t flags[kMaxMoves];                         // MOVE_* of a group
+  const uint32_t* lists; uint32_t list_stride;
+  unsigned int* words;                              // != nullptr: tiles of MOVE_OVER groups that are not MOVE_COLUMNS keep their order
+  uint32_t* err;
 };
 
 }  // namespace pa

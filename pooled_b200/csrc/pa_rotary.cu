@@ -1,4 +1,4 @@
-// Rotary positions of any layout and scaling (pa_rotary): q or k of any number of columns rotated from one buffer into
+// Rotary positions of any layout, scaling and number of axes (pa_rotary): q or k of any number of columns rotated from one buffer into
 // another, or the front of a layer call -- q rotated, k rotated and v converted into rows of an f16 cache -- in one launch.
 //
 // A pair (a, b) at position p turns to m (a cos t - b sin t, b cos t + a sin t), t = p f_i.  The host keeps f_i / 2 pi in
@@ -131,6 +131,15 @@ __device__ __forceinline__ uint32_t rot_item(const RotaryParams& p, uint32_t col
   return lo;
 }
 
+// the axis whose position turns pair k: blocks of pairs, or the axes in turn for as long as they have pairs left, then the first
+__device__ __forceinline__ uint32_t rot_axis(const RotaryParams& p, uint32_t k) {
+  if (p.n_axes < 2) return 0;
+  const uint32_t n0 = p.axis_pairs[0], n1 = p.axis_pairs[1], n2 = p.axis_pairs[2];
+  if (!p.axes_cycled) return (k >= n0) + (k >= n0 + n1 && p.n_axes > 2) + (k >= n0 + n1 + n2 && p.n_axes > 3);
+  const uint32_t a = k % p.n_axes, n = a == 1 ? n1 : a == 2 ? n2 : p.axis_pairs[3];
+  return a && k < p.n_axes * n ? a : 0;
+}
+
 // V: 16-byte vectors, or 1: single values (then a unit is one pair, or two copied values), for layouts that vectors do not fit.
 // Threads (units, columns); grid (column groups, unit blocks).
 template <typename TI, typename TO, bool APPEND, int V>
@@ -142,12 +151,13 @@ __global__ void __launch_bounds__(kRotThreads) pa_rotary_kernel(const __grid_con
     for (uint32_t i = tid; i < cols * half; i += threads) {
       const uint32_t c = i / half, k = i - c * half, col = c0 + c;
       int32_t pos;
-      if (APPEND) { const uint32_t it = rot_item(p, col); pos = p.pos[it] + (int32_t)(col - p.col0[it]); }
-      else pos = p.positions ? p.positions[col] : p.pos[0] + (int32_t)col;
+      if (p.positions) pos = p.positions[(uint64_t)rot_axis(p, k) * p.n_cols + col];
+      else if (APPEND) { const uint32_t it = rot_item(p, col); pos = p.pos[it] + (int32_t)(col - p.col0[it]); }
+      else pos = p.pos[0] + (int32_t)col;
       rot_angle(p.turns, k, pos, p.mscale, s_c[c * pitch + k], s_s[c * pitch + k]);
     }
   };
-  const bool early = APPEND || !p.positions, lay = p.layout == PA_ROPE_HALF;
+  const bool early = !p.positions, lay = p.layout == PA_ROPE_HALF;
   if (early) angles();
   // this thread's unit: of q, of k (rotated) or of v (copied: no rotated dims)
   const uint32_t per_head = rot_units<V>(p.hd, p.n_rot, lay), uq = p.q ? p.q_heads * per_head : 0, uk = APPEND ? p.kv_heads * per_head : 0;

@@ -15,6 +15,7 @@ using namespace pa;
 struct pa_rotary {
   pa_ctx* ctx = nullptr;
   pa_rotary_config cfg{};
+  pa_rotary_axes axes{1, PA_ROPE_AXES_BLOCKS, {}, {}};
   double freq[128] = {};          // radians per position
   double mscale = 1.0;
   double* turns = nullptr;        // device: freq / 2 pi
@@ -43,7 +44,26 @@ static void rotary_frequencies(const pa_rotary_config& c, double* f, double* msc
   *mscale = c.mscale != 0.0 ? c.mscale : c.scaling == PA_ROPE_SCALE_YARN && c.factor > 1.0 ? 1.0 + 0.1 * log(c.factor) : 1.0;
 }
 
-extern "C" int pa_rotary_create(pa_ctx* ctx, const pa_rotary_config* cfg, pa_rotary** out) {
+// the pairs of a rotation of several axes, ahead of their frequencies
+static int check_axes(pa_ctx* ctx, const pa_rotary_config& c, const pa_rotary_axes& a) {
+  if (a.n_axes < 1 || a.n_axes > 4) return fail(ctx, PA_EINVAL, "pa_rotary_create_axes: %u axes, 1 to 4 are possible", a.n_axes);
+  if (a.order > PA_ROPE_AXES_OWN) return fail(ctx, PA_EINVAL, "pa_rotary_create_axes: unknown order %u", a.order);
+  const uint32_t half = c.n_rot / 2;
+  uint64_t sum = 0;
+  for (uint32_t i = 0; i < a.n_axes; ++i) sum += a.pairs[i];
+  if (sum != half) return fail(ctx, PA_EINVAL, "pa_rotary_create_axes: the axes have %llu pairs of %u", (unsigned long long)sum, half);
+  for (uint32_t i = 0; i < a.n_axes; ++i) {
+    if (a.order == PA_ROPE_AXES_CYCLED && i && a.pairs[i] && i + a.n_axes * (a.pairs[i] - 1) >= half)
+      return fail(ctx, PA_EINVAL, "pa_rotary_create_axes: axis %u has %u pairs, every %uth of %u are fewer", i, a.pairs[i], a.n_axes, half);
+    if (a.order == PA_ROPE_AXES_OWN && a.pairs[i] == 1 && c.scaling == PA_ROPE_SCALE_NTK)
+      return fail(ctx, PA_EINVAL, "pa_rotary_create_axes: PA_ROPE_SCALE_NTK needs at least 2 pairs of an axis with frequencies of its own");
+  }
+  return PA_OK;
+}
+
+extern "C" int pa_rotary_create(pa_ctx* ctx, const pa_rotary_config* cfg, pa_rotary** out) { return pa_rotary_create_axes(ctx, cfg, nullptr, out); }
+
+extern "C" int pa_rotary_create_axes(pa_ctx* ctx, const pa_rotary_config* cfg, const pa_rotary_axes* axes, pa_rotary** out) {
   GUARD(ctx);
   if (!cfg || !out) return fail(ctx, PA_EINVAL, "pa_rotary_create: null argument");
   *out = nullptr;
@@ -62,10 +82,21 @@ extern "C" int pa_rotary_create(pa_ctx* ctx, const pa_rotary_config* cfg, pa_rot
     if (c.slow == 0.0) c.slow = 1.0;
     if (!(c.slow > 0.0) || !(c.fast > c.slow) || !isfinite(c.fast)) return fail(ctx, PA_EINVAL, "pa_rotary_create: fast must be above slow, and slow above 0");
   }
+  if (axes)
+    if (int rc = check_axes(ctx, c, *axes)) return rc;
   pa_rotary* r = new (std::nothrow) pa_rotary();
   if (!r) return fail(ctx, PA_ENOMEM, "pa_rotary_create: out of host memory");
   r->ctx = ctx; r->cfg = c;
-  rotary_frequencies(c, r->freq, &r->mscale);
+  if (axes) r->axes = *axes;
+  if (r->axes.order == PA_ROPE_AXES_OWN) {
+    for (uint32_t i = 0, first = 0; i < r->axes.n_axes; first += r->axes.pairs[i++]) {
+      pa_rotary_config own = c;
+      own.n_rot = 2 * r->axes.pairs[i];
+      rotary_frequencies(own, r->freq + first, &r->mscale);
+    }
+  } else {
+    rotary_frequencies(c, r->freq, &r->mscale);
+  }
   double turns[128];
   const uint32_t half = c.n_rot / 2;
   bool finite = isfinite((float)r->mscale);
@@ -103,6 +134,11 @@ extern "C" int pa_rotary_freqs(const pa_rotary* r, double* freqs, double* mscale
   return PA_OK;
 }
 
+static void set_axes(RotaryParams& p, const pa_rotary* r) {
+  p.n_axes = r->axes.n_axes; p.axes_cycled = r->axes.order == PA_ROPE_AXES_CYCLED;
+  std::copy(r->axes.pairs, r->axes.pairs + 4, p.axis_pairs);
+}
+
 static uint32_t esize(int dtype) { return dtype == PA_F16 ? 2 : 4; }
 
 extern "C" int pa_rotary_apply(pa_rotary* r, const void* x, int x_dtype, uint64_t xcs, uint64_t xhs, uint32_t n_heads, const int32_t* positions,
@@ -125,6 +161,7 @@ extern "C" int pa_rotary_apply(pa_rotary* r, const void* x, int x_dtype, uint64_
   p.q = x; p.q_col_stride = xcs; p.q_head_stride = xhs; p.q_heads = n_heads;
   p.q_out = y; p.q_out_col_stride = ycs; p.q_out_head_stride = yhs; p.in_f16 = x_dtype == PA_F16; p.out_f16 = y_dtype == PA_F16;
   p.positions = positions; p.pos[0] = pos;
+  set_axes(p, r);
   DeviceScope on(ctx->device);
   CU_TRY(ctx, launch_rotary(p, false, (uint32_t)ctx->sm_count, (cudaStream_t)stream));
   ctx->stats.kernel_launches++; ctx->stats.calls++;
@@ -138,44 +175,46 @@ extern "C" int pa_rotary_apply(pa_rotary* r, const void* x, int x_dtype, uint64_
   return PA_OK;
 }
 
-extern "C" int pa_rotary_append(pa_rotary* r, pa_layer* L, const pa_item* items, uint32_t n_items, const uint32_t* rows, const void* q, uint64_t qcs,
-                                uint64_t qhs, const void* k, const void* v, uint64_t kvcs, void* q_out, int q_out_dtype, uint64_t q_out_cs, void* stream) {
+static int rotary_append(const char* who, pa_rotary* r, pa_layer* L, const pa_item* items, uint32_t n_items, const uint32_t* rows, const int32_t* positions, const void* q,
+                         uint64_t qcs, uint64_t qhs, const void* k, const void* v, uint64_t kvcs, void* q_out, int q_out_dtype, uint64_t q_out_cs, void* stream) {
   if (!r || !L) return PA_EINVAL;
   pa_ctx* ctx = L->ctx;
   GUARD(ctx);
-  if (r->ctx != ctx) return fail(ctx, PA_EINVAL, "pa_rotary_append: the rotation belongs to another context");
-  if (L->kv_format != PA_KV_F16) return fail(ctx, PA_EUNSUPPORTED, "pa_rotary_append: f16 caches only");
-  if (!items || !k || !v || (q && !q_out)) return fail(ctx, PA_EINVAL, "pa_rotary_append: null items, k, v or q_out");
-  if (n_items < 1 || n_items > (uint32_t)kMaxShared) return fail(ctx, PA_EINVAL, "pa_rotary_append: 1 to %d items per call", kMaxShared);
-  if (q_out_dtype != PA_F32 && q_out_dtype != PA_F16) return fail(ctx, PA_EINVAL, "pa_rotary_append: unknown q_out dtype");
+  if (r->ctx != ctx) return fail(ctx, PA_EINVAL, "%s: the rotation belongs to another context", who);
+  if (L->kv_format != PA_KV_F16) return fail(ctx, PA_EUNSUPPORTED, "%s: f16 caches only", who);
+  if (!items || !k || !v || (q && !q_out)) return fail(ctx, PA_EINVAL, "%s: null items, k, v or q_out", who);
+  if (n_items < 1 || n_items > (uint32_t)kMaxShared) return fail(ctx, PA_EINVAL, "%s: 1 to %d items per call", who, kMaxShared);
+  if (q_out_dtype != PA_F32 && q_out_dtype != PA_F16) return fail(ctx, PA_EINVAL, "%s: unknown q_out dtype", who);
   const uint32_t hd = ctx->cfg.head_dim, ae = esize((int)ctx->cfg.act_dtype);
-  if ((uintptr_t)q % ae || (uintptr_t)k % ae || (uintptr_t)v % ae || (q && (uintptr_t)q_out % esize(q_out_dtype)))
-    return fail(ctx, PA_EINVAL, "pa_rotary_append: a pointer is not aligned to its type");
+  if ((uintptr_t)q % ae || (uintptr_t)k % ae || (uintptr_t)v % ae || (q && (uintptr_t)q_out % esize(q_out_dtype)) || ((uintptr_t)positions & 3))
+    return fail(ctx, PA_EINVAL, "%s: a pointer is not aligned to its type", who);
   RotaryParams p{};
   uint64_t total = 0;
   uint32_t row_first[kMaxShared], lowest = 0xffffffffu;
   p.one_each = 1;
   for (uint32_t i = 0; i < n_items; ++i) {
     const pa_item& it = items[i];
-    if (it.seq >= L->n_seqs) return fail(ctx, PA_EINVAL, "pa_rotary_append: sequence %u of %u", it.seq, L->n_seqs);
-    if (it.n_cols < 1 || (uint64_t)it.pos + it.n_cols > (1ull << 31)) return fail(ctx, PA_EINVAL, "pa_rotary_append: item %u has %u columns at position %u", i, it.n_cols, it.pos);
-    if (!rows && it.pos < L->origin) return fail(ctx, PA_EINVAL, "pa_rotary_append: position %u lies ahead of the layer's first, %u", it.pos, L->origin);
+    if (it.seq >= L->n_seqs) return fail(ctx, PA_EINVAL, "%s: sequence %u of %u", who, it.seq, L->n_seqs);
+    if (it.n_cols < 1 || (uint64_t)it.pos + it.n_cols > (1ull << 31)) return fail(ctx, PA_EINVAL, "%s: item %u has %u columns at position %u", who, i, it.n_cols, it.pos);
+    if (!rows && it.pos < L->origin) return fail(ctx, PA_EINVAL, "%s: position %u lies ahead of the layer's first, %u", who, it.pos, L->origin);
     const uint32_t row = rows ? rows[i] : it.pos - L->origin;
     if ((uint64_t)row + it.n_cols > L->max_seq)
-      return fail(ctx, PA_EINVAL, "pa_rotary_append: rows %u..%llu pass the layer's %u", row, (unsigned long long)row + it.n_cols - 1, L->max_seq);
+      return fail(ctx, PA_EINVAL, "%s: rows %u..%llu pass the layer's %u", who, row, (unsigned long long)row + it.n_cols - 1, L->max_seq);
     for (uint32_t j = 0; j < i; ++j)
       if (items[j].seq == it.seq && row < row_first[j] + items[j].n_cols && row_first[j] < row + it.n_cols)
-        return fail(ctx, PA_EINVAL, "pa_rotary_append: items %u and %u store the same row of sequence %u", j, i, it.seq);
+        return fail(ctx, PA_EINVAL, "%s: items %u and %u store the same row of sequence %u", who, j, i, it.seq);
     row_first[i] = row;
     lowest = std::min(lowest, row);
     p.pos[i] = (int32_t)it.pos; p.col0[i] = (uint32_t)total; p.row[i] = (uint64_t)it.seq * L->max_seq + row;
     if (it.n_cols != 1) p.one_each = 0;
     total += it.n_cols;
   }
-  if (total > ctx->cfg.max_cols) return fail(ctx, PA_EINVAL, "pa_rotary_append: %llu columns, the context was created for at most %u", (unsigned long long)total, ctx->cfg.max_cols);
+  if (total > ctx->cfg.max_cols) return fail(ctx, PA_EINVAL, "%s: %llu columns, the context was created for at most %u", who, (unsigned long long)total, ctx->cfg.max_cols);
   if (q == q_out && q && ((int)ctx->cfg.act_dtype != q_out_dtype || (ctx->cfg.n_heads > 1 && qhs != hd) || (total > 1 && qcs != q_out_cs)))
-    return fail(ctx, PA_EINVAL, "pa_rotary_append: q_out may be q with its type and strides only (heads packed)");
-  if (q && total > 1 && q_out_cs < ctx->q_dim) return fail(ctx, PA_EINVAL, "pa_rotary_append: the column stride of q_out is below %u", ctx->q_dim);
+    return fail(ctx, PA_EINVAL, "%s: q_out may be q with its type and strides only (heads packed)", who);
+  if (q && total > 1 && q_out_cs < ctx->q_dim) return fail(ctx, PA_EINVAL, "%s: the column stride of q_out is below %u", who, ctx->q_dim);
+  p.positions = positions;
+  set_axes(p, r);
   p.turns = r->turns; p.mscale = (float)r->mscale; p.hd = hd; p.n_rot = r->cfg.n_rot; p.layout = r->cfg.layout; p.n_cols = (uint32_t)total; p.n_items = n_items;
   p.q = q; p.q_col_stride = qcs; p.q_head_stride = qhs; p.q_heads = ctx->cfg.n_heads;
   p.q_out = q_out; p.q_out_col_stride = q_out_cs; p.q_out_head_stride = hd; p.in_f16 = ctx->cfg.act_dtype == PA_F16; p.out_f16 = q_out_dtype == PA_F16;
@@ -184,7 +223,21 @@ extern "C" int pa_rotary_append(pa_rotary* r, pa_layer* L, const pa_item* items,
   CU_TRY(ctx, launch_rotary(p, true, (uint32_t)ctx->sm_count, (cudaStream_t)stream));
   ctx->stats.kernel_launches++; ctx->stats.calls++;
   // what follows on this layer may start before the rows are stored: it fetches early only below the lowest of them
-  if (ctx->inflight_layer == L) lowest = std::min(lowest, ctx->inflight_row0);
+  if (rows_may_be_in_flight(ctx, L)) lowest = std::min(lowest, ctx->inflight_row0);
   ctx->inflight_layer = L; ctx->inflight_row0 = lowest;
   return PA_OK;
+}
+
+extern "C" int pa_rotary_append(pa_rotary* r, pa_layer* L, const pa_item* items, uint32_t n_items, const uint32_t* rows, const void* q, uint64_t qcs,
+                                uint64_t qhs, const void* k, const void* v, uint64_t kvcs, void* q_out, int q_out_dtype, uint64_t q_out_cs, void* stream) {
+  return rotary_append("pa_rotary_append", r, L, items, n_items, rows, nullptr, q, qcs, qhs, k, v, kvcs, q_out, q_out_dtype, q_out_cs, stream);
+}
+
+extern "C" int pa_rotary_append_at(pa_rotary* r, pa_layer* L, const pa_item* items, uint32_t n_items, const uint32_t* rows, const int32_t* positions, const void* q,
+                                   uint64_t qcs, uint64_t qhs, const void* k, const void* v, uint64_t kvcs, void* q_out, int q_out_dtype, uint64_t q_out_cs,
+                                   void* stream) {
+  if (!L) return PA_EINVAL;
+  GUARD(L->ctx);
+  if (!positions) return fail(L->ctx, PA_EINVAL, "pa_rotary_append_at: null positions");
+  return rotary_append("pa_rotary_append_at", r, L, items, n_items, rows, positions, q, qcs, qhs, k, v, kvcs, q_out, q_out_dtype, q_out_cs, stream);
 }

@@ -1,0 +1,207 @@
+// Attention of trees of drafted tokens over a cache (pa_decode_tree).
+//
+//   o_c = sum_r e^(q_c.k_r / sqrt(hd) - M) v_r / sum_r e^(q_c.k_r / sqrt(hd) - M),   r < base, or r - base one of token c's ancestors or c itself
+//
+// A unit is a run of 64-row K / V tiles of one sequence and kv head, and a row tile: the group's heads of some of the tree's
+// tokens.  Its CTA is the one of the shared-prefix decode (pa_shared.cuh: roles, precision, narrow and wide row tiles, records),
+// and the tree's rows are simply the last of the sequence's, so a small tree costs one tile at most.  What the tree adds:
+//   the mask    in tiles that hold rows of the tree a lane walks its token's parents (in shared memory, 35 cycles each, ahead of
+//               the wait for the scores) and collects a bit for each of the tile's keys; scores of the other keys are -infinity by
+//               selection, so whatever the K of a token that is no ancestor holds stays out
+//   V           a weight of zero does not make up for an infinity or NaN: the V producer looks through the tree's rows of a tile
+//               while the scores are being made, puts zeros in the place of such values and notes their rows; a token that attends
+//               one of them has its values added to its record at the end, so that it ends as the formula does
+// What bounds it: with few tokens HBM; from some 100 query rows a kv head on the tensor cores (a byte of K and V serves all row
+// tiles from L2): 64 tokens of 16 / 2 heads of 256 behind 32768 rows 75 us (0.28 of the measured rate of plain bf16 products), 16 x 60 of
+// 16 / 8 heads of 128 behind up to 4003 rows 75 us.
+#include "pa_shared.cuh"
+
+namespace pa {
+
+// grid (kv heads, units)
+template <int HD, bool WIDE, bool FOLD>
+__global__ void __launch_bounds__(384, ShSmem<HD>::CTAS)
+pa_tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TreeParams p) {
+  using L = ShSmem<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + L::OFF_BAR);
+  volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(bars + 31);
+  volatile uint32_t* s_err = s_tmem + 1;
+  const uint32_t bar0 = smem_u32(bars);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t it = 0, hi = p.n_items - 1, u = blockIdx.y;
+  while (it < hi) { const uint32_t mid = (it + hi + 1) / 2; if (u >= p.unit0[mid]) it = mid; else hi = mid - 1; }
+  u -= p.unit0[it];
+  const uint32_t rts = p.row_tiles[it], split = u / rts, rt = u - split * rts, c0 = rt * p.tile_cols[it], cols = p.col0[it + 1] - p.col0[it];
+  TreeUnit un;
+  un.mk = &tm_k; un.mv = &tm_v;
+  un.shared = un.ragged = false;
+  un.item0 = p.col0[it] + c0;
+  un.pairs = min((uint32_t)p.tile_cols[it], cols - c0) * p.G;
+  un.row0 = p.seq[it] * p.max_seq; un.n_rows = p.rows[it];
+  un.tile0 = split * p.tps;
+  un.n_tiles = min((un.n_rows + 63) / 64, un.tile0 + p.tps) - un.tile0;
+  un.slot = un.tile0 / (FOLD ? p.seg * p.fold : p.seg);
+  un.live_warps = ((WIDE ? 1 : 2) * un.pairs + 31) / 32;
+  un.tree0 = p.base[it]; un.node0 = p.node0[it] + c0; un.parent0 = p.parent0[it];
+  un.tree_tile = min(un.n_tiles, max(un.tree0 / 64, un.tile0) - un.tile0);
+
+  if (warp == 1 && lane == 0) {
+    *s_err = 0;
+    auto init = [&](int which, int n, uint32_t count) { for (int i = 0; i < n; ++i) mbar_init(bar0 + 8u * (uint32_t)(which + i), count); };
+    init(SH_K_FULL, 3, 1); init(SH_K_EMPTY, 3, 1); init(SH_V_FULL, 2, 1); init(SH_V_EMPTY, 2, 1);
+    init(SH_S_FULL, 3, 1); init(SH_P_FULL, 3, 64 * un.live_warps); init(SH_PV_DONE, 3, 1);
+    init(SH_O_DONE, 1, 1); init(SH_O_FREE, 1, 64 * un.live_warps); init(SH_Q_FULL, 1, 256); init(SH_Q_READ, 1, 256); init(SH_V_CLEAN, 2, 1);
+    fence_barrier_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(smem_u32((const void*)s_tmem), sh_tmem_cols<HD>());
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  if (warp == 0 && lane == 0) { prefetch_tmap(un.mk); prefetch_tmap(un.mv); }
+  pdl_wait();
+  pdl_trigger();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  if (warp == 0 || warp == 3) shared_producer<HD, true>(un, warp == 3, base, bar0, s_err);
+  else shared_roles<HD, WIDE, !WIDE, FOLD, true>(p, un, base, bar0, s_err, tmem);
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, sh_tmem_cols<HD>());
+  }
+  if (tid == 0 && *s_err) atomicMax(p.err, *s_err);
+}
+
+__device__ __forceinline__ uint32_t tree_item(const TreeFinishParams& p, uint32_t col) {
+  uint32_t lo = 0, hi = p.n_items - 1;
+  while (lo < hi) { const uint32_t mid = (lo + hi + 1) / 2; if (col >= p.col0[mid]) lo = mid; else hi = mid - 1; }
+  return lo;
+}
+
+// Merge, gate, store.  Few rows: a CTA a row (or slice), as behind a shared prefix.  Many: a warp a row, eight a CTA, so that a row
+// of two or three records does not take a CTA's start and two barriers.
+template <int HD, bool WARPS>
+__global__ void __launch_bounds__(256, 4) pa_tree_finish_kernel(const __grid_constant__ TreeFinishParams p) {
+  pdl_wait();
+  pdl_trigger();
+  if constexpr (!WARPS) {
+    __shared__ float4 s_acc[256];
+    const uint32_t slices = HD / 4 / p.lanes, prow = blockIdx.x / slices, col = prow / p.n_heads;
+    shared_merge_row<HD>(p, s_acc, prow, blockIdx.x % slices, col, prow % p.n_heads, p.n_own[tree_item(p, col)]);
+  } else {
+    const uint32_t prow = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (prow >= p.n_rows) return;
+    const uint32_t col = prow / p.n_heads, h = prow - col * p.n_heads, ns = p.n_own[tree_item(p, col)];
+    constexpr int N = HD == 256 ? 2 : 1, W = HD == 64 ? 2 : 4, U = 4;       // vectors of a lane, 128 dims apart; their values; records at once
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + (uint64_t)prow * p.n_rec;
+    const float* ob = p.part_o + (uint64_t)prow * p.n_rec * HD + lane * W;
+    float x[U][N][W], acc[N][W] = {};
+    auto load = [&](uint32_t s0) {
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float* at = ob + (uint64_t)(s0 + k) * HD + i * 128;
+          if constexpr (W == 4) {
+            const float4 v = s0 + k < ns ? *reinterpret_cast<const float4*>(at) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[k][i][0] = v.x; x[k][i][1] = v.y; x[k][i][2] = v.z; x[k][i][3] = v.w;
+          } else {
+            const float2 v = s0 + k < ns ? *reinterpret_cast<const float2*>(at) : make_float2(0.f, 0.f);
+            x[k][i][0] = v.x; x[k][i][1] = v.y;
+          }
+        }
+    };
+    load(0);
+    const uint64_t go = (uint64_t)col * p.gate_col_stride + (uint64_t)h * p.gate_head_stride + lane * W, oo = (uint64_t)col * p.out_col_stride + (uint64_t)h * HD + lane * W;
+    float gv[N][W];
+    if (p.gate) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (p.vec && W == 4) {
+          if (p.act_f16) {
+            const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.gate) + go + i * 128);
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+            gv[i][0] = a.x; gv[i][1] = a.y; gv[i][W - 2] = b.x; gv[i][W - 1] = b.y;
+          } else {
+            const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.gate) + go + i * 128);
+            gv[i][0] = v.x; gv[i][1] = v.y; gv[i][W - 2] = v.z; gv[i][W - 1] = v.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < W; ++e) gv[i][e] = ld_act(p.gate, go + i * 128 + e, p.act_f16);
+        }
+      }
+    }
+    float M, l;
+    shared_row_ml(ml, ns, M, l);
+    for (uint32_t s0 = 0; s0 < ns; s0 += U) {
+      if (s0) load(s0);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const float w = s0 + k < ns ? ex2_approx(ml[s0 + k].x - M) : 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int e = 0; e < W; ++e) acc[i][e] = fmaf(x[k][i][e], w, acc[i][e]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float t[W];
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        t[e] = __fdiv_rn(acc[i][e], l);
+        if (p.gate) t[e] *= __fdiv_rn(1.0f, 1.0f + __expf(-gv[i][e]));
+      }
+      if (p.vec && W == 4) {
+        if (p.act_f16) {
+          __half2 a = __floats2half2_rn(t[0], t[1]), b = __floats2half2_rn(t[W - 2], t[W - 1]);
+          *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + oo + i * 128) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+        } else {
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + oo + i * 128) = make_float4(t[0], t[1], t[W - 2], t[W - 1]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          if (p.act_f16) reinterpret_cast<__half*>(p.out)[oo + i * 128 + e] = __float2half_rn(t[e]);
+          else reinterpret_cast<float*>(p.out)[oo + i * 128 + e] = t[e];
+        }
+      }
+    }
+  }
+}
+
+template <int HD, bool WIDE, bool FOLD>
+static cudaError_t launch_tree_t(const TreeParams& p, const CUtensorMap& k, const CUtensorMap& v, uint32_t n_kv, int dev, cudaStream_t st) {
+  using S = ShSmem<HD>;
+  static std::atomic<bool> attr_set[64];
+  if (!attr_set[dev & 63].load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(pa_tree_kernel<HD, WIDE, FOLD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
+    if (e != cudaSuccess) return e;
+    attr_set[dev & 63].store(true, std::memory_order_release);
+  }
+  return launch_pdl(pa_tree_kernel<HD, WIDE, FOLD>, dim3(n_kv, p.units), dim3(S::THREADS), (size_t)S::TOTAL, st, k, v, p);
+}
+cudaError_t launch_tree(const TreeParams& p, bool wide, const CUtensorMap& k, const CUtensorMap& v, uint32_t hd, uint32_t n_kv, int dev, cudaStream_t st) {
+  const bool fold = p.fold > 1 || (wide && p.tps > p.seg);      // (wide units leave one record, or the sum of several runs)
+  if (wide && hd != 256) return cudaErrorInvalidValue;
+  if (wide) return fold ? launch_tree_t<256, true, true>(p, k, v, n_kv, dev, st) : launch_tree_t<256, true, false>(p, k, v, n_kv, dev, st);
+  if (hd == 256) return fold ? launch_tree_t<256, false, true>(p, k, v, n_kv, dev, st) : launch_tree_t<256, false, false>(p, k, v, n_kv, dev, st);
+  if (hd == 128) return fold ? launch_tree_t<128, false, true>(p, k, v, n_kv, dev, st) : launch_tree_t<128, false, false>(p, k, v, n_kv, dev, st);
+  if (hd == 64) return fold ? launch_tree_t<64, false, true>(p, k, v, n_kv, dev, st) : launch_tree_t<64, false, false>(p, k, v, n_kv, dev, st);
+  return cudaErrorInvalidValue;
+}
+template <int HD>
+static cudaError_t launch_finish_t(const TreeFinishParams& p, cudaStream_t st) {
+  return p.lanes ? launch_pdl(pa_tree_finish_kernel<HD, false>, dim3(p.n_rows * (HD / 4 / p.lanes)), dim3(256), 0, st, p)
+                 : launch_pdl(pa_tree_finish_kernel<HD, true>, dim3((p.n_rows + 7) / 8), dim3(256), 0, st, p);
+}
+cudaError_t launch_tree_finish(const TreeFinishParams& p, uint32_t hd, cudaStream_t st) {
+  return hd == 256 ? launch_finish_t<256>(p, st) : hd == 128 ? launch_finish_t<128>(p, st) : hd == 64 ? launch_finish_t<64>(p, st) : cudaErrorInvalidValue;
+}
+
+}  // namespace pa

@@ -18,6 +18,7 @@ PA_KV_F16, PA_KV_Q8, PA_KV_F32 = 0, 1, 2
 PA_FLAG_FAST = 1
 PA_ROPE_HALF, PA_ROPE_INTERLEAVED = 0, 1
 PA_ROPE_SCALE_NONE, PA_ROPE_SCALE_LINEAR, PA_ROPE_SCALE_NTK, PA_ROPE_SCALE_YARN, PA_ROPE_SCALE_BANDS = 0, 1, 2, 3, 4
+PA_ROPE_AXES_BLOCKS, PA_ROPE_AXES_CYCLED, PA_ROPE_AXES_OWN = 0, 1, 2
 PA_MODE_AUTO, PA_MODE_DECODE, PA_MODE_PREFILL = 0, 1, 2
 STATUS = {0: "PA_OK", -1: "PA_EINVAL", -2: "PA_EUNSUPPORTED", -3: "PA_ENOMEM", -4: "PA_ECUDA", -5: "PA_ETIMEOUT", -6: "PA_ESTATE"}
 
@@ -41,6 +42,14 @@ class PaItem(C.Structure):
 class PaRotaryConfig(C.Structure):
     _fields_ = [("n_rot", C.c_uint32), ("layout", C.c_uint32), ("scaling", C.c_uint32), ("original", C.c_uint32), ("theta", C.c_double),
                 ("factor", C.c_double), ("fast", C.c_double), ("slow", C.c_double), ("mscale", C.c_double), ("reserved", C.c_uint32 * 4)]
+
+
+class PaRotaryAxes(C.Structure):
+    _fields_ = [("n_axes", C.c_uint32), ("order", C.c_uint32), ("pairs", C.c_uint32 * 4), ("reserved", C.c_uint32 * 2)]
+
+
+class PaMoveItem(C.Structure):
+    _fields_ = [("src_seq", C.c_uint32), ("src_row", C.c_uint32), ("dst_seq", C.c_uint32), ("dst_row", C.c_uint32), ("n_rows", C.c_uint32), ("reserved", C.c_uint32)]
 
 
 class PaEvictItem(C.Structure):
@@ -110,10 +119,14 @@ SYMBOLS = {
     "pa_decode_static": (_i, [_i, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, C.c_char_p, _sz]),
     "pa_decode_static_status": (_i, [_i, _vp, C.POINTER(_u32)]),
     "pa_rotary_create": (_i, [_vp, C.POINTER(PaRotaryConfig), C.POINTER(_vp)]),
+    "pa_rotary_create_axes": (_i, [_vp, C.POINTER(PaRotaryConfig), C.POINTER(PaRotaryAxes), C.POINTER(_vp)]),
     "pa_rotary_destroy": (_i, [_vp]),
     "pa_rotary_freqs": (_i, [_vp, C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     "pa_rotary_apply": (_i, [_vp, _vp, _i, _u64, _u64, _u32, _vp, C.c_int32, _u32, _vp, _i, _u64, _u64, _vp]),
     "pa_rotary_append": (_i, [_vp, _vp, _vp, _u32, _vp, _vp, _u64, _u64, _vp, _vp, _u64, _vp, _i, _u64, _vp]),
+    "pa_rotary_append_at": (_i, [_vp, _vp, _vp, _u32, _vp, _vp, _vp, _u64, _u64, _vp, _vp, _u64, _vp, _i, _u64, _vp]),
+    "pa_decode_tree": (_i, [_vp, _vp, _u32, _vp, _vp, _i, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _vp]),
+    "pa_cache_move": (_i, [_vp, _u32, _vp, _u32, _vp, _u32, _vp]),
     "pa_decode_shared": (_i, [_vp, _vp, _u32, _u32, _u32, _vp, _u32, _vp, _i, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _vp]),
     "pa_layer_track_weights": (_i, [_vp]),
     "pa_weights_ptr": (_vp, [_vp]),
@@ -192,6 +205,21 @@ class CtypesCalls:
         return self.lib.pa_rotary_append(rotary, layer, self._items(items), len(items), r, *_gate(q, q_head_stride), _ptr(k), _ptr(v), k.stride(0), _ptr(q_out),
                                          q_out_dtype, 0 if q_out is None else q_out.stride(0), stream)
 
+    def rotary_append_at(self, entry, rotary, layer, items, rows, positions, q, q_head_stride, k, v, q_out, q_out_dtype, stream):
+        if rows is not None and len(rows) != len(items):
+            raise ValueError("one row per item")
+        r = None if rows is None else (C.c_uint32 * max(1, len(rows)))(*map(u32, rows))
+        return self.lib.pa_rotary_append_at(rotary, layer, self._items(items), len(items), r, _ptr(positions), *_gate(q, q_head_stride), _ptr(k), _ptr(v), k.stride(0),
+                                            _ptr(q_out), q_out_dtype, 0 if q_out is None else q_out.stride(0), stream)
+
+    def decode_tree(self, entry, layer, items, parents, q, q_dtype, q_head_stride, gate, gate_head_stride, out, stream):
+        return self.lib.pa_decode_tree(layer, self._items(items), len(items), _ptr(parents), _ptr(q), q_dtype, q.stride(0), u64(q_head_stride), *_gate(gate, gate_head_stride),
+                                       _ptr(out), out.stride(0), stream)
+
+    def cache_move(self, entry, layers, n_layers, items, lists, list_stride, stream):
+        arr = (PaMoveItem * max(1, len(items)))(*[PaMoveItem(*map(u32, it), 0) for it in items])
+        return self.lib.pa_cache_move(layers, u32(n_layers), arr, len(items), _ptr(lists), u32(list_stride), stream)
+
     def decode_shared(self, entry, layer, prefix_layer, prefix_seq, prefix_len, own_base, seqs_pos, q, q_dtype, q_head_stride, gate, gate_head_stride, out, stream):
         return self.lib.pa_decode_shared(layer, prefix_layer, u32(prefix_seq), u32(prefix_len), u32(own_base), self._items(seqs_pos, False), len(seqs_pos), _ptr(q), q_dtype,
                                          q.stride(0), u64(q_head_stride), *_gate(gate, gate_head_stride), _ptr(out), out.stride(0), stream)
@@ -225,7 +253,7 @@ class Lib:
         `entry`; the same calls through ctypes where it was not built for this interpreter."""
         self.entry = {n: C.cast(getattr(self.dll, n), C.c_void_p).value for n in
                       ("pa_attn_layer", "pa_attn_items", "pa_rope_append", "pa_decode_gather", "pa_rotary_apply", "pa_rotary_append", "pa_decode_shared",
-                       "pa_decode_weights", "pa_evict")}
+                       "pa_decode_weights", "pa_evict", "pa_rotary_append_at", "pa_decode_tree", "pa_cache_move")}
         if not os.path.exists(CALL_PATH):
             return CtypesCalls(self)
         loader = importlib.machinery.ExtensionFileLoader("_pa_call", CALL_PATH)
