@@ -389,7 +389,8 @@ struct pa_ctx {
   float* part_ml = nullptr;    // device: f32 [rows][splits][2]
   uint32_t max_splits = 0;
   size_t part_slots = 0;       // (query row, split) records a decode / verify call may use
-  size_t pf_slots = 0;         // records the partial buffers hold, and a split prefill may use
+  size_t pf_slots = 0;         // ... a split prefill and the shared-prefix and weighing decodes may use
+  size_t tree_slots = 0;       // records the partial buffers hold, and a tree decode may use
   float* merge_rec = nullptr;    // device: the records of a decode call that merges them itself, a block per CTA; all bits set between calls
   size_t merge_bytes = 0;
   unsigned int* merge_ctr = nullptr;   // device: two words for each SM (see pa_decode_f32_kernel), zero between calls

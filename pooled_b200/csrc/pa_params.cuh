@@ -264,23 +264,25 @@ struct TreeParams {
   const void* q; int q_f16; uint64_t q_col_stride, q_head_stride;           // rotated queries of the launch's columns
   uint32_t n_heads, G;
   float scale_log2;
-  float* part_o; float* part_ml; uint32_t n_rec, seg, fold;                 // as in SharedParams
+  float* part_o; float* part_ml; uint32_t seg, fold;                        // as in SharedParams
   const int32_t* parents;                                                   // of all the call's columns, or nullptr: chains
   const __half* v;                                                          // the V cache, whose values tree_restore looks up
   uint32_t kv_dim, max_seq, n_items, tps, units;
+  // the parts, the longest first
   uint32_t seq[kMaxTrees], base[kMaxTrees], rows[kMaxTrees];                // a part's sequence, its committed rows, and those with its last token
-  uint32_t col0[kMaxTrees + 1], node0[kMaxTrees], parent0[kMaxTrees];       // first column in the launch, which token of the tree that is, where the tree's parents begin
+  uint32_t col0[kMaxTrees], cols[kMaxTrees], node0[kMaxTrees], parent0[kMaxTrees];      // its columns in the launch, the first one's place in the tree, where the tree's parents begin
   uint32_t unit0[kMaxTrees + 1];                                            // first unit: row tiles fastest, then splits of tps tiles
-  uint16_t tile_cols[kMaxTrees], row_tiles[kMaxTrees];                      // columns of a row tile
+  uint32_t rec0[kMaxTrees];                                                 // first record: n_rec for every head of every column
+  uint16_t tile_cols[kMaxTrees], row_tiles[kMaxTrees], n_rec[kMaxTrees];    // columns of a row tile; records of a row
   uint32_t* err;
 };
 struct TreeFinishParams {
-  const float* part_o; const float* part_ml; uint32_t n_rec;
-  uint32_t n_items, n_heads, n_rows, lanes;                                 // lanes: as in SharedFinishParams; 0: a warp a row
+  const float* part_o; const float* part_ml;
+  uint32_t n_items, n_heads, n_rows, lanes;                                 // lanes: as in SharedFinishParams; 0: a warp a row (head_dim 256: half of one)
   const void* gate; uint64_t gate_col_stride, gate_head_stride;
   void* out; uint64_t out_col_stride; int act_f16, vec;                     // vec: four values of gate and out lie on whole vectors
-  uint32_t col0[kMaxTrees + 1];
-  uint16_t n_own[kMaxTrees];                                                // records of an item's rows
+  uint32_t col0[kMaxTrees + 1], rec0[kMaxTrees];                            // the parts in their columns' order
+  uint16_t n_rec[kMaxTrees];
 };
 
 // eviction by summed weights (pa_evict_select_kernel, pa_evict_move_kernel)
@@ -307,10 +309,11 @@ struct MoveParams {
   float* scales[kMoveLayers][2];                    // their scales (int8 caches),
   float* sums[kMoveLayers];                         // summed weights (layers that have them)
   uint32_t per[2], inv[2];                          // units of a row and of a row of scales, ceil(2^32 / them)
-  uint32_t max_seq, n_kv, n_groups;
-  // tiles: of a layer first K, then V (tiles[0] each), scales of K and of V (tiles[1]), sums head by head (tiles[2]); first[kind][g]: a
-  // group's first among them
-  uint32_t tiles[3], layer_tiles, first[3][kMaxMoves + 1];
+  uint32_t max_seq, n_kv, n_groups, n_layers, units;   // units: tiles of the launch
+  // tiles of an array: of K or V (tiles[0]), their scales (tiles[1]), the sums of a kv head (tiles[2]); first[kind][g]: a group's first among
+  // them.  at[kind][m], with plain ranges only, the groups by their number of tiles, the most first: how many tiles come before the m groups with
+  // the most are alone
+  uint32_t tiles[3], first[3][kMaxMoves + 1], at[3][kMaxMoves + 1];
   // groups: source rows that go to one place, or to those of several items
   uint32_t seq[kMaxMoves], row[kMaxMoves], n[kMaxMoves], item0[kMaxMoves + 1];
   uint32_t dst_seq[kMaxMoves], dst_row[kMaxMoves];  // of the items, groups' items together

@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256, SUMS ? 3 : 4) pa_shared_finish_kernel(con
   pdl_trigger();
   if (!SUMS || blockIdx.x < p.merge_ctas) {
     const uint32_t slices = HD / 4 / p.lanes, prow = blockIdx.x / slices, slice = blockIdx.x % slices, item = prow / p.n_heads, h = prow % p.n_heads;
-    shared_merge_row<HD>(p, s_acc, prow, slice, item, h, p.p_recs + p.n_own[item]);
+    shared_merge_row<HD>(p, s_acc, (uint64_t)prow * p.n_rec, slice, item, h, p.p_recs + p.n_own[item]);
     return;
   }
   if constexpr (SUMS) {

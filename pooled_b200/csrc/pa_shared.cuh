@@ -25,9 +25,8 @@ struct ShSmem {
 };
 template <int HD, bool WIDE>
 struct ShLay {
-  static_assert(!WIDE || HD == 256, "wide units");
   static constexpr int SB = WIDE || HD == 128 ? 2 : 3;      // tiles of scores in tensor memory; the weights take their scores' place
-  static constexpr int TQC = WIDE ? 4 : HD == 256 ? 2 : 0;     // 64-dim chunks of Q in tensor memory, 32 columns each
+  static constexpr int TQC = HD != 256 ? 0 : WIDE ? 4 : 2;     // 64-dim chunks of Q in tensor memory, 32 columns each
   static constexpr int T_S = TQC * 32, T_O = T_S + SB * 64;
   static_assert(T_O + HD <= (HD == 256 ? 512 : 256), "tensor memory columns");
 };
@@ -53,6 +52,7 @@ struct ShUnit {
 // ... of a tree: the rows from tree0 on are its tokens
 struct TreeUnit : ShUnit {
   uint32_t tree0, node0, tree_tile, parent0;                // first row of the tree; token of the first query row; first tile (of the unit) that holds some; its parents
+  uint32_t n_rec; uint64_t rec0;                            // records of a query row; where those of column 0, head 0 would be
 };
 
 // Warp 3 of a tree's unit: a weight of zero does not make up for an infinity or NaN in the V of a token that is no ancestor, so such values of the
@@ -113,7 +113,7 @@ __device__ __forceinline__ void tree_v_producer(const TreeUnit& un, uint8_t* rin
 }
 
 // the keys of a tile that token `c` of a tree attends: bit i is row kv0 + i
-__device__ __forceinline__ uint64_t tree_sees(const int16_t* parents, uint32_t c, uint32_t tree0, uint32_t kv0) {
+static __device__ __noinline__ uint64_t tree_sees(const int16_t* parents, uint32_t c, uint32_t tree0, uint32_t kv0) {
   uint64_t m = kv0 < tree0 ? (tree0 - kv0 < 64 ? (1ull << (tree0 - kv0)) - 1 : ~0ull) : 0;
   for (int a = (int)c; a >= 0; a = parents[a]) {             // (a parent comes before its token)
     const int at = (int)(tree0 + a - kv0);
@@ -123,16 +123,24 @@ __device__ __forceinline__ uint64_t tree_sees(const int16_t* parents, uint32_t c
   return m;
 }
 
-// t: n dims of a record from dim d of kv head g on, of the query row of token `c`; adds the V values that were no finite numbers
-template <typename P>
-__device__ __noinline__ void tree_restore(const P& p, const TreeUnit& un, const uint32_t* dirty, const int16_t* parents, uint32_t c, uint32_t d, float* t, int n) {
-  for (uint32_t j = un.tree_tile; j < un.n_tiles; ++j) {
-    const uint32_t kv0 = (un.tile0 + j) * 64;
-    uint64_t m = (dirty[2 * (j - un.tree_tile)] | ((uint64_t)dirty[2 * (j - un.tree_tile) + 1] << 32)) & tree_sees(parents, c, un.tree0, kv0);
-    for (; m; m &= m - 1) {
-      const __half* v = p.v + (uint64_t)(un.row0 + kv0 + __ffsll((long long)m) - 1) * p.kv_dim + d;
-      for (int i = 0; i < n; ++i) { const float x = __half2float(v[i]); if (!isfinite(x)) t[i] += x; }
+// Adds the V values that were no finite numbers to the last records of a unit's query rows, record `rec` of each: thread `tid` of `threads`.
+template <int HD, typename P>
+__device__ __noinline__ void tree_restore(const P& p, TreeUnit un, const uint32_t* dirty, const int16_t* parents, uint32_t rec, uint32_t tid, uint32_t threads) {
+  for (uint32_t i = tid; i < un.pairs * (HD / 4); i += threads) {
+    const uint32_t pr = i / (HD / 4), d = i % (HD / 4) * 4, it = pr / p.G;
+    float4* at = reinterpret_cast<float4*>(p.part_o + (un.rec0 + ((uint64_t)(un.item0 + it) * p.n_heads + blockIdx.x * p.G + pr - it * p.G) * un.n_rec + rec) * HD + d);
+    float4 t = *at;
+    for (uint32_t j = un.tree_tile; j < un.n_tiles; ++j) {
+      const uint32_t kv0 = (un.tile0 + j) * 64;
+      uint64_t m = dirty[2 * (j - un.tree_tile)] | ((uint64_t)dirty[2 * (j - un.tree_tile) + 1] << 32);
+      if (m) m &= tree_sees(parents, un.node0 + it, un.tree0, kv0);
+      for (; m; m &= m - 1) {
+        const __half* v = p.v + (uint64_t)(un.row0 + kv0 + __ffsll((long long)m) - 1) * p.kv_dim + blockIdx.x * HD + d;
+        auto value = [&](int e) { const float x = __half2float(v[e]); return isfinite(x) ? 0.f : x; };
+        t.x += value(0); t.y += value(1); t.z += value(2); t.w += value(3);
+      }
     }
+    *at = t;
   }
 }
 
@@ -330,28 +338,17 @@ __device__ __forceinline__ void shared_roles(const P& p, const U& un, uint8_t* b
     // bytes of a chunk of 32 dims (or add it to what they stored there before); else a unit's only or last record goes through the rings, idle by then, so that whole lines leave
     // (a lane has a row: its own stores are 16 bytes each in 32 records 1 KB apart).
     float* s_rl = s_max + 512;
-    auto restore = [&](float* t, int n, uint32_t d) {      // the last record of a tree's unit: values that no product may see
-      if constexpr (TREE) {
-        const uint32_t* dirty = reinterpret_cast<const uint32_t*>(base + L::OFF_BAR + OFF_DIRTY);
-        uint32_t any = 0;
-        for (uint32_t i = un.tree_tile; i < n_tiles; ++i) any |= dirty[2 * (i - un.tree_tile)] | dirty[2 * (i - un.tree_tile) + 1];
-        if (any && live) {
-          float x[32];
-#pragma unroll
-          for (int i = 0; i < n; ++i) x[i] = t[i];
-          const TreeUnit copy = un;                        // (`un` itself stays in registers)
-          tree_restore(p, copy, dirty, parents, un.node0 + row_item(lr), g * HD + d, x, n);
-#pragma unroll
-          for (int i = 0; i < n; ++i) t[i] = x[i];
-        }
-      }
-    };
     float m_rec = 0.f;                                    // the reference of what the lane has stored so far in a record of several runs
     auto record = [&](uint32_t seg, float m, float l, bool last) {
       const bool adds = FOLD && seg % p.fold != 0;
       const float kept = adds ? ex2_approx(m_rec - m) : 0.f;
       const uint32_t threads = 32 * un.live_warps, gt = (tid - 128) & 127;
-      auto slot_of = [&](uint32_t pr) { const uint32_t it = row_item(pr); return ((uint64_t)(un.item0 + it) * p.n_heads + g * G + pr - it * G) * p.n_rec + un.slot + (FOLD ? seg / p.fold : seg); };
+      auto slot_of = [&](uint32_t pr) {
+        const uint32_t it = row_item(pr);
+        const uint64_t row = (uint64_t)(un.item0 + it) * p.n_heads + g * G + pr - it * G;
+        if constexpr (TREE) return un.rec0 + row * un.n_rec + un.slot + (FOLD ? seg / p.fold : seg);
+        else return row * p.n_rec + un.slot + (FOLD ? seg / p.fold : seg);
+      };
       if (!WIDE) l += __shfl_xor_sync(0xffffffffu, l, 1);
       float* sums = s_rl + (seg & 1) * 128 + row;          // two in turn: nothing else may come between two records
       if (wg) *sums = l;
@@ -361,7 +358,8 @@ __device__ __forceinline__ void shared_roles(const P& p, const U& un, uint8_t* b
         *ml = make_float2(m, FOLD && adds ? fmaf(ml->y, kept, l + *sums) : l + *sums);
       }
       constexpr uint32_t XW = WIDE ? 2 * L::X_BYTES : L::X_BYTES;
-      static_assert(HD / 32 * XW <= (NK + NV) * L::KV_BYTES, "a place in the rings for every chunk");
+      constexpr int PLACES = HD / 32 * XW <= (NK + NV) * L::KV_BYTES ? HD / 32 : GRP;      // a place in the rings for every chunk, or one for each group
+      static_assert(PLACES * XW <= (NK + NV) * L::KV_BYTES, "places in the rings");
       mbar_wait(BAR(SH_O_DONE, 0), seg & 1, s_err, WAIT_MMA);
       tc_fence_after();
       // high and low rows of a chunk added, each lane with half of it
@@ -398,7 +396,6 @@ __device__ __forceinline__ void shared_roles(const P& p, const U& un, uint8_t* b
                 t[i] = fmaf(x.x, kept, t[i]); t[i + 1] = fmaf(x.y, kept, t[i + 1]); t[i + 2] = fmaf(x.z, kept, t[i + 2]); t[i + 3] = fmaf(x.w, kept, t[i + 3]);
               }
             }
-            if (last) restore(t, E, (c + k * GRP) * 32 + (is_lo ? 16 : 0));
             if (live) {
 #pragma unroll
               for (int i = 0; i < E; i += 4) at[i / 4] = make_float4(t[i], t[i + 1], t[i + 2], t[i + 3]);
@@ -414,15 +411,14 @@ __device__ __forceinline__ void shared_roles(const P& p, const U& un, uint8_t* b
       for (int c = wg; c < HD / 32; c += GRP) {           // the groups share the chunks out
         float o[32];
         tmem_ld32(t_o + c * 32 + lane_addr, o);
-        float* xs = reinterpret_cast<float*>(base + L::OFF_K + c * XW);
+        float* xs = reinterpret_cast<float*>(base + L::OFF_K + c % PLACES * XW);
+        if (PLACES < HD / 32 && c >= GRP) named_bar_sync(7 + wg, threads);      // the chunk before has left its place
         if constexpr (WIDE) {
-          restore(o, 32, c * 32);
 #pragma unroll
           for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(xs + row * L::XP + 4 * i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         } else {
           float t[16];
           add_rows(o, t);
-          restore(t, 16, c * 32 + (is_lo ? 16 : 0));
 #pragma unroll
           for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(xs + lr * L::XP + (is_lo ? 16 : 0) + 4 * i) = make_float4(t[4 * i], t[4 * i + 1], t[4 * i + 2], t[4 * i + 3]);
         }
@@ -492,6 +488,22 @@ __device__ __forceinline__ void shared_roles(const P& p, const U& un, uint8_t* b
             }
           }
           // weights as f16 pairs, high and low parts
+          if constexpr (WIDE && HD < 256) {                // (16 keys at a time: two CTAs an SM have 80 registers a thread)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float e0 = ex2_approx(fmaf(s[16 * h + 2 * i], p.scale_log2, -m_st)), e1 = ex2_approx(fmaf(s[16 * h + 2 * i + 1], p.scale_log2, -m_st));
+                l_sum += e0 + e1;
+                const __half2 x = __floats2half2_rn(e0, e1);
+                const float2 f = __half22float2(x);
+                hi[i] = *reinterpret_cast<const uint32_t*>(&x); lo[i] = pack_h2(e0 - f.x, e1 - f.y);
+              }
+              tmem_st8u(t_s0 + b * 64 + 16 * wg + 8 * h + lane_addr, hi);
+              tmem_st8u(t_s0 + b * 64 + 32 + 16 * wg + 8 * h + lane_addr, lo);
+            }
+          } else {
           uint32_t hi[NS / 2], lo[NS / 2];
 #pragma unroll
           for (int i = 0; i < NS / 2; ++i) {
@@ -515,6 +527,7 @@ __device__ __forceinline__ void shared_roles(const P& p, const U& un, uint8_t* b
             }
             tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, pw);
           }
+          }
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(BAR(SH_P_FULL, b));
@@ -525,6 +538,16 @@ __device__ __forceinline__ void shared_roles(const P& p, const U& un, uint8_t* b
         if (m_old > -2.0e30f) { record(seg++, m_old, l_old, last); m_old = -3.0e30f; }
         if (last) break;
         if (++in_seg == p.seg && j != n_tiles - 1) { m_old = m_st; l_old = l_sum; l_sum = 0.f; in_seg = 0; }
+      }
+      if constexpr (TREE) {
+        const uint32_t* dirty = reinterpret_cast<const uint32_t*>(base + L::OFF_BAR + OFF_DIRTY);
+        uint32_t any = 0;
+        for (uint32_t i = 2 * un.tree_tile; i < 2 * n_tiles; ++i) any |= dirty[i - 2 * un.tree_tile];
+        if (any) {
+          const uint32_t last = (n_tiles - 1) / p.seg, threads = 64 * un.live_warps;
+          named_bar_sync(1, threads);                       // the records are stored
+          tree_restore<HD>(p, un, dirty, parents, un.slot + (FOLD ? last / p.fold : last), wg * 32 * un.live_warps + qd * 32 + lane, threads);
+        }
       }
     }
   }
@@ -547,12 +570,12 @@ __device__ __forceinline__ void shared_row_ml(const float2* ml, uint32_t ns, flo
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
 }
-// one row (column, head) of `ns` records, or one slice of it, merged, gated and stored by a CTA of 256 threads
+// one row (column, head) of `ns` records from `rec` on, or one slice of it, merged, gated and stored by a CTA of 256 threads
 template <int HD, typename P>
-__device__ __forceinline__ void shared_merge_row(const P& p, float4* s_acc, uint32_t prow, uint32_t slice, uint32_t item, uint32_t h, uint32_t ns) {
+__device__ __forceinline__ void shared_merge_row(const P& p, float4* s_acc, uint64_t rec, uint32_t slice, uint32_t item, uint32_t h, uint32_t ns) {
   const uint32_t tid = threadIdx.x, groups = 256 / p.lanes, grp = tid / p.lanes, ln = tid % p.lanes, dims = p.lanes * 4, d = slice * dims + tid;
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + (uint64_t)prow * p.n_rec;
-  const float* ob = p.part_o + (uint64_t)prow * p.n_rec * HD + slice * dims + ln * 4;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + rec;
+  const float* ob = p.part_o + rec * HD + slice * dims + ln * 4;
   constexpr int U = 4;      // (eight: two CTAs an SM, a second wave for 512 rows)
   float4 x[U];
 #pragma unroll

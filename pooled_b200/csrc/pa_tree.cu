@@ -33,17 +33,18 @@ pa_tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
   uint32_t it = 0, hi = p.n_items - 1, u = blockIdx.y;
   while (it < hi) { const uint32_t mid = (it + hi + 1) / 2; if (u >= p.unit0[mid]) it = mid; else hi = mid - 1; }
   u -= p.unit0[it];
-  const uint32_t rts = p.row_tiles[it], split = u / rts, rt = u - split * rts, c0 = rt * p.tile_cols[it], cols = p.col0[it + 1] - p.col0[it];
+  const uint32_t rts = p.row_tiles[it], split = u / rts, rt = u - split * rts, c0 = rt * p.tile_cols[it];
   TreeUnit un;
   un.mk = &tm_k; un.mv = &tm_v;
   un.shared = un.ragged = false;
   un.item0 = p.col0[it] + c0;
-  un.pairs = min((uint32_t)p.tile_cols[it], cols - c0) * p.G;
+  un.pairs = min((uint32_t)p.tile_cols[it], p.cols[it] - c0) * p.G;
   un.row0 = p.seq[it] * p.max_seq; un.n_rows = p.rows[it];
   un.tile0 = split * p.tps;
   un.n_tiles = min((un.n_rows + 63) / 64, un.tile0 + p.tps) - un.tile0;
   un.slot = un.tile0 / (FOLD ? p.seg * p.fold : p.seg);
   un.live_warps = ((WIDE ? 1 : 2) * un.pairs + 31) / 32;
+  un.n_rec = p.n_rec[it]; un.rec0 = p.rec0[it] - (uint64_t)p.col0[it] * p.n_heads * un.n_rec;
   un.tree0 = p.base[it]; un.node0 = p.node0[it] + c0; un.parent0 = p.parent0[it];
   un.tree_tile = min(un.n_tiles, max(un.tree0 / 64, un.tile0) - un.tile0);
 
@@ -82,58 +83,54 @@ __device__ __forceinline__ uint32_t tree_item(const TreeFinishParams& p, uint32_
   return lo;
 }
 
-// Merge, gate, store.  Few rows: a CTA a row (or slice), as behind a shared prefix.  Many: a warp a row, eight a CTA, so that a row
-// of two or three records does not take a CTA's start and two barriers.
+// Merge, gate, store.  Few rows: a CTA a row (or slice), as behind a shared prefix.  Many: a warp a row (head_dim 256: half of one), eight a
+// CTA, so that a row of two or three records does not take a CTA's start and two barriers.
 template <int HD, bool WARPS>
 __global__ void __launch_bounds__(256, 4) pa_tree_finish_kernel(const __grid_constant__ TreeFinishParams p) {
   pdl_wait();
   pdl_trigger();
   if constexpr (!WARPS) {
     __shared__ float4 s_acc[256];
-    const uint32_t slices = HD / 4 / p.lanes, prow = blockIdx.x / slices, col = prow / p.n_heads;
-    shared_merge_row<HD>(p, s_acc, prow, blockIdx.x % slices, col, prow % p.n_heads, p.n_own[tree_item(p, col)]);
+    const uint32_t slices = HD / 4 / p.lanes, prow = blockIdx.x / slices, col = prow / p.n_heads, it = tree_item(p, col);
+    shared_merge_row<HD>(p, s_acc, p.rec0[it] + (uint64_t)(prow - p.col0[it] * p.n_heads) * p.n_rec[it], blockIdx.x % slices, col, prow % p.n_heads, p.n_rec[it]);
   } else {
-    const uint32_t prow = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    constexpr int PIECES = HD == 256 ? 2 : 1, W = HD == 64 ? 2 : 4, U = 8;       // warps of a row; values of a lane; records at once
+    const uint32_t w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, prow = w / PIECES, d = w % PIECES * 128 + lane * W;
     if (prow >= p.n_rows) return;
-    const uint32_t col = prow / p.n_heads, h = prow - col * p.n_heads, ns = p.n_own[tree_item(p, col)];
-    constexpr int N = HD == 256 ? 2 : 1, W = HD == 64 ? 2 : 4, U = 4;       // vectors of a lane, 128 dims apart; their values; records at once
-    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + (uint64_t)prow * p.n_rec;
-    const float* ob = p.part_o + (uint64_t)prow * p.n_rec * HD + lane * W;
-    float x[U][N][W], acc[N][W] = {};
+    const uint32_t col = prow / p.n_heads, h = prow - col * p.n_heads, it = tree_item(p, col), ns = p.n_rec[it];
+    const uint64_t rec = p.rec0[it] + (uint64_t)(prow - p.col0[it] * p.n_heads) * ns;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + rec;
+    const float* ob = p.part_o + rec * HD + d;
+    float x[U][W], acc[W] = {};
     auto load = [&](uint32_t s0) {
 #pragma unroll
-      for (int k = 0; k < U; ++k)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float* at = ob + (uint64_t)(s0 + k) * HD + i * 128;
-          if constexpr (W == 4) {
-            const float4 v = s0 + k < ns ? *reinterpret_cast<const float4*>(at) : make_float4(0.f, 0.f, 0.f, 0.f);
-            x[k][i][0] = v.x; x[k][i][1] = v.y; x[k][i][2] = v.z; x[k][i][3] = v.w;
-          } else {
-            const float2 v = s0 + k < ns ? *reinterpret_cast<const float2*>(at) : make_float2(0.f, 0.f);
-            x[k][i][0] = v.x; x[k][i][1] = v.y;
-          }
+      for (int k = 0; k < U; ++k) {
+        const float* at = ob + (uint64_t)(s0 + k) * HD;
+        if constexpr (W == 4) {
+          const float4 v = s0 + k < ns ? *reinterpret_cast<const float4*>(at) : make_float4(0.f, 0.f, 0.f, 0.f);
+          x[k][0] = v.x; x[k][1] = v.y; x[k][W - 2] = v.z; x[k][W - 1] = v.w;
+        } else {
+          const float2 v = s0 + k < ns ? *reinterpret_cast<const float2*>(at) : make_float2(0.f, 0.f);
+          x[k][0] = v.x; x[k][1] = v.y;
         }
+      }
     };
     load(0);
-    const uint64_t go = (uint64_t)col * p.gate_col_stride + (uint64_t)h * p.gate_head_stride + lane * W, oo = (uint64_t)col * p.out_col_stride + (uint64_t)h * HD + lane * W;
-    float gv[N][W];
+    const uint64_t go = (uint64_t)col * p.gate_col_stride + (uint64_t)h * p.gate_head_stride + d, oo = (uint64_t)col * p.out_col_stride + (uint64_t)h * HD + d;
+    float gv[W];
     if (p.gate) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (p.vec && W == 4) {
-          if (p.act_f16) {
-            const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.gate) + go + i * 128);
-            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
-            gv[i][0] = a.x; gv[i][1] = a.y; gv[i][W - 2] = b.x; gv[i][W - 1] = b.y;
-          } else {
-            const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.gate) + go + i * 128);
-            gv[i][0] = v.x; gv[i][1] = v.y; gv[i][W - 2] = v.z; gv[i][W - 1] = v.w;
-          }
+      if (p.vec && W == 4) {
+        if (p.act_f16) {
+          const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.gate) + go);
+          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+          gv[0] = a.x; gv[1] = a.y; gv[W - 2] = b.x; gv[W - 1] = b.y;
         } else {
-#pragma unroll
-          for (int e = 0; e < W; ++e) gv[i][e] = ld_act(p.gate, go + i * 128 + e, p.act_f16);
+          const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.gate) + go);
+          gv[0] = v.x; gv[1] = v.y; gv[W - 2] = v.z; gv[W - 1] = v.w;
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) gv[e] = ld_act(p.gate, go + e, p.act_f16);
       }
     }
     float M, l;
@@ -142,34 +139,28 @@ __global__ void __launch_bounds__(256, 4) pa_tree_finish_kernel(const __grid_con
       if (s0) load(s0);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const float w = s0 + k < ns ? ex2_approx(ml[s0 + k].x - M) : 0.f;
+        const float wt = s0 + k < ns ? ex2_approx(ml[s0 + k].x - M) : 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-          for (int e = 0; e < W; ++e) acc[i][e] = fmaf(x[k][i][e], w, acc[i][e]);
+        for (int e = 0; e < W; ++e) acc[e] = fmaf(x[k][e], wt, acc[e]);
       }
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float t[W];
+    for (int e = 0; e < W; ++e) {
+      acc[e] = __fdiv_rn(acc[e], l);
+      if (p.gate) acc[e] *= __fdiv_rn(1.0f, 1.0f + __expf(-gv[e]));
+    }
+    if (p.vec && W == 4) {
+      if (p.act_f16) {
+        const __half2 a = __floats2half2_rn(acc[0], acc[1]), b = __floats2half2_rn(acc[W - 2], acc[W - 1]);
+        *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + oo) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      } else {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + oo) = make_float4(acc[0], acc[1], acc[W - 2], acc[W - 1]);
+      }
+    } else {
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        t[e] = __fdiv_rn(acc[i][e], l);
-        if (p.gate) t[e] *= __fdiv_rn(1.0f, 1.0f + __expf(-gv[i][e]));
-      }
-      if (p.vec && W == 4) {
-        if (p.act_f16) {
-          __half2 a = __floats2half2_rn(t[0], t[1]), b = __floats2half2_rn(t[W - 2], t[W - 1]);
-          *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + oo + i * 128) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
-        } else {
-          *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + oo + i * 128) = make_float4(t[0], t[1], t[W - 2], t[W - 1]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          if (p.act_f16) reinterpret_cast<__half*>(p.out)[oo + i * 128 + e] = __float2half_rn(t[e]);
-          else reinterpret_cast<float*>(p.out)[oo + i * 128 + e] = t[e];
-        }
+        if (p.act_f16) reinterpret_cast<__half*>(p.out)[oo + e] = __float2half_rn(acc[e]);
+        else reinterpret_cast<float*>(p.out)[oo + e] = acc[e];
       }
     }
   }
@@ -186,19 +177,20 @@ static cudaError_t launch_tree_t(const TreeParams& p, const CUtensorMap& k, cons
   }
   return launch_pdl(pa_tree_kernel<HD, WIDE, FOLD>, dim3(n_kv, p.units), dim3(S::THREADS), (size_t)S::TOTAL, st, k, v, p);
 }
-cudaError_t launch_tree(const TreeParams& p, bool wide, const CUtensorMap& k, const CUtensorMap& v, uint32_t hd, uint32_t n_kv, int dev, cudaStream_t st) {
+template <int HD>
+static cudaError_t launch_tree_h(const TreeParams& p, bool wide, const CUtensorMap& k, const CUtensorMap& v, uint32_t n_kv, int dev, cudaStream_t st) {
   const bool fold = p.fold > 1 || (wide && p.tps > p.seg);      // (wide units leave one record, or the sum of several runs)
-  if (wide && hd != 256) return cudaErrorInvalidValue;
-  if (wide) return fold ? launch_tree_t<256, true, true>(p, k, v, n_kv, dev, st) : launch_tree_t<256, true, false>(p, k, v, n_kv, dev, st);
-  if (hd == 256) return fold ? launch_tree_t<256, false, true>(p, k, v, n_kv, dev, st) : launch_tree_t<256, false, false>(p, k, v, n_kv, dev, st);
-  if (hd == 128) return fold ? launch_tree_t<128, false, true>(p, k, v, n_kv, dev, st) : launch_tree_t<128, false, false>(p, k, v, n_kv, dev, st);
-  if (hd == 64) return fold ? launch_tree_t<64, false, true>(p, k, v, n_kv, dev, st) : launch_tree_t<64, false, false>(p, k, v, n_kv, dev, st);
-  return cudaErrorInvalidValue;
+  if (wide) return fold ? launch_tree_t<HD, true, true>(p, k, v, n_kv, dev, st) : launch_tree_t<HD, true, false>(p, k, v, n_kv, dev, st);
+  return fold ? launch_tree_t<HD, false, true>(p, k, v, n_kv, dev, st) : launch_tree_t<HD, false, false>(p, k, v, n_kv, dev, st);
+}
+cudaError_t launch_tree(const TreeParams& p, bool wide, const CUtensorMap& k, const CUtensorMap& v, uint32_t hd, uint32_t n_kv, int dev, cudaStream_t st) {
+  return hd == 256 ? launch_tree_h<256>(p, wide, k, v, n_kv, dev, st) : hd == 128 ? launch_tree_h<128>(p, wide, k, v, n_kv, dev, st)
+       : hd == 64 ? launch_tree_h<64>(p, wide, k, v, n_kv, dev, st) : cudaErrorInvalidValue;
 }
 template <int HD>
 static cudaError_t launch_finish_t(const TreeFinishParams& p, cudaStream_t st) {
   return p.lanes ? launch_pdl(pa_tree_finish_kernel<HD, false>, dim3(p.n_rows * (HD / 4 / p.lanes)), dim3(256), 0, st, p)
-                 : launch_pdl(pa_tree_finish_kernel<HD, true>, dim3((p.n_rows + 7) / 8), dim3(256), 0, st, p);
+                 : launch_pdl(pa_tree_finish_kernel<HD, true>, dim3((p.n_rows * (HD == 256 ? 2 : 1) + 7) / 8), dim3(256), 0, st, p);
 }
 cudaError_t launch_tree_finish(const TreeFinishParams& p, uint32_t hd, cudaStream_t st) {
   return hd == 256 ? launch_finish_t<256>(p, st) : hd == 128 ? launch_finish_t<128>(p, st) : hd == 64 ? launch_finish_t<64>(p, st) : cudaErrorInvalidValue;

@@ -23,34 +23,37 @@ static uint32_t record_tiles(uint32_t T, uint32_t cap) { return ceil_div(T, ceil
 struct TreePart { uint32_t item, first, cols; };
 struct TreePlan { uint32_t T; float us; };
 
-// Tiles a unit (T), and the time that the launch takes with them: units one CTA an SM at a time (two of head_dim 128 and 64), at the
-// costs of the shared decode's (a unit of T tiles T * tile + start), and the records' way through L2.
-static TreePlan plan_tree(const pa_ctx* ctx, const uint32_t* tiles, const uint32_t* row_tiles, uint32_t n, uint32_t cols, bool wide, uint32_t tile_rows, uint32_t cap, uint32_t most) {
+// records of all rows with `T` tiles in each (parts in any order)
+static uint64_t tree_records(const TreePart* parts, const uint32_t* tiles, uint32_t n, uint32_t n_heads, uint32_t T) {
+  uint64_t sum = 0;
+  for (uint32_t i = 0; i < n; ++i) sum += (uint64_t)parts[i].cols * n_heads * ceil_div(tiles[i], T);
+  return sum;
+}
+
+// Tiles a unit (T), and the time that the launch takes with them: units one CTA an SM at a time (two of head_dim 128 and 64), the longest
+// first, at the costs of a unit of T tiles, T * tile + start, and the records' way through L2.
+static TreePlan plan_tree(const pa_ctx* ctx, const TreePart* parts, const uint32_t* tiles, const uint32_t* row_tiles, uint32_t n, bool wide, uint32_t tile_rows, uint32_t cap) {
   const uint32_t hd = ctx->cfg.head_dim, n_kv = ctx->cfg.n_kv_heads, sms = (uint32_t)ctx->sm_count * (hd == 256 ? 1 : 2);
-  const float tile = wide ? 1.17f : hd == 256 ? 0.75f : 0.8f, start = wide ? 10.5f : 5.5f, record = 3.f * (float)tile_rows / 64;
+  const float tile = hd == 256 ? (wide ? 1.22f : 0.77f) : wide ? 1.6f : 1.4f, start = wide ? 10.5f : 5.5f, record = 3.f * (float)tile_rows / 64;
   uint32_t longest = 1;
   float work_tiles = 0.f, hbm = 0.f;
-  bool even = true;
   for (uint32_t i = 0; i < n; ++i) {
     longest = std::max(longest, tiles[i]);
     work_tiles += (float)(tiles[i] * row_tiles[i]);
     hbm += (float)tiles[i];
-    even = even && tiles[i] == tiles[0];
   }
   hbm *= (float)(n_kv * hd * 256) / 6.0e6f;
   TreePlan best{longest, 3.0e38f};
-  const uint32_t most_splits = std::min(longest, std::min(most, 4 * (uint32_t)ctx->sm_count));
-  for (uint32_t s = 1; s <= most_splits; s += 1 + s / 24) {
+  for (uint32_t s = 1; s <= std::min(longest, 512u); s += 1 + s / 24) {
     const uint32_t T = ceil_div(longest, s), own = std::min(T, longest), records = ceil_div(own, record_tiles(T, cap));
+    const uint64_t recs = tree_records(parts, tiles, n, ctx->cfg.n_heads, T);
+    if (recs > ctx->tree_slots) break;
     const float unit = (float)own * tile + start + (float)(records - 1) * record;
     uint32_t units = 0;
     for (uint32_t i = 0; i < n; ++i) units += ceil_div(tiles[i], T) * row_tiles[i];
     units *= n_kv;
-    float us;
-    if (units <= sms) us = unit;
-    else if (even) us = (float)ceil_div(units, sms) * unit;
-    else us = std::max(unit, (work_tiles * n_kv * tile + (float)units * start) / (float)sms + 0.5f * unit);
-    us = std::max(us, hbm + start) + 0.05f * us + (float)cols * ctx->cfg.n_heads * (float)(ceil_div(longest, T) * records * hd * 4) / 4.0e6f;
+    float us = units <= sms ? unit : std::max(unit, (work_tiles * n_kv * tile + (float)units * start) / (float)sms + 0.3f * unit);
+    us = std::max(us, hbm + start) + 0.05f * us + (float)(recs * records * hd * 4) / 4.0e6f;
     if (us < best.us) best = TreePlan{T, us};
   }
   return best;
@@ -74,61 +77,67 @@ static int tree_launch(const TreeCall& c, const TreePart* parts, uint32_t n, uin
   const size_t aes = ctx->cfg.act_dtype == PA_F16 ? 2 : 4;
   TreeParams p{};
   TreeFinishParams f{};
-  const uint32_t most = (uint32_t)std::min<size_t>(512, ctx->pf_slots / ((size_t)cols * nH));
-  uint32_t tiles[kMaxTrees], row_tiles[kMaxTrees], wide_tiles[kMaxTrees], most_row_tiles = 0, rows_of_tile = 0, longest = 0, total = 0;
+  uint32_t tiles[kMaxTrees], row_tiles[kMaxTrees], wide_tiles[kMaxTrees], most_row_tiles = 0, rows_of_tile = 0, total = 0;
   for (uint32_t i = 0; i < n; ++i) {
-    const pa_item& it = c.items[parts[i].item];
-    p.seq[i] = it.seq; p.base[i] = it.pos; p.rows[i] = it.pos + parts[i].first + parts[i].cols;
-    p.node0[i] = parts[i].first; p.parent0[i] = c.item_col0[parts[i].item];
-    p.col0[i] = f.col0[i] = total;
-    total += parts[i].cols;
-    tiles[i] = ceil_div(p.rows[i], 64);
-    longest = std::max(longest, tiles[i]);
+    tiles[i] = ceil_div(c.items[parts[i].item].pos + parts[i].first + parts[i].cols, 64);
     row_tiles[i] = ceil_div(parts[i].cols, 64 / G);
-    wide_tiles[i] = ceil_div(parts[i].cols, std::max(1u, 128 / G));
+    wide_tiles[i] = ceil_div(parts[i].cols, 128 / G);
     most_row_tiles = std::max(most_row_tiles, row_tiles[i]);
     rows_of_tile = std::max(rows_of_tile, std::min(parts[i].cols, 64 / G) * G);
+    f.col0[i] = total;
+    total += parts[i].cols;
   }
-  p.col0[n] = f.col0[n] = total;
+  f.col0[n] = total;
   const bool f16_out = ctx->cfg.act_dtype == PA_F16;
   const uint32_t cap = f16_out ? kF16Tiles : most_row_tiles > 1 ? 16u : 4u;
-  TreePlan plan = plan_tree(ctx, tiles, row_tiles, n, cols, false, rows_of_tile, cap, most);
+  TreePlan plan = plan_tree(ctx, parts, tiles, row_tiles, n, false, rows_of_tile, cap);
   bool wide = false;
-  if (hd == 256 && most_row_tiles > 1 && c.q_f16 && f16_out && ctx->tune.shared_wide != 0) {
-    const TreePlan w = plan_tree(ctx, tiles, wide_tiles, n, cols, true, 128, cap, most);
+  if (most_row_tiles > 1 && c.q_f16 && f16_out && ctx->tune.shared_wide != 0) {
+    const TreePlan w = plan_tree(ctx, parts, tiles, wide_tiles, n, true, 128, cap);
     if (w.us < plan.us || ctx->tune.shared_wide == 1) { plan = w; wide = true; }
   }
   // tiles of a record, as behind a shared prefix: a unit's shared out evenly; more where there is no room for that many, and past the
   // longest run a record adds up several
   uint32_t T = plan.T, records = ceil_div(T, cap);
-  while (records > 1 && ceil_div(longest, ceil_div(T, records)) > most) --records;
+  while (records > 1 && tree_records(parts, tiles, n, nH, ceil_div(T, records)) > ctx->tree_slots) --records;
   uint32_t rec = ceil_div(T, records);
   p.fold = ceil_div(rec, std::max(cap, kF32Run));
   rec = ceil_div(rec, p.fold) * p.fold;
   T = records * rec;
   p.seg = rec / p.fold; p.tps = T;
-  uint64_t read = 0;
+  // the longest first
+  uint32_t order[kMaxTrees], recs = 0;
   for (uint32_t i = 0; i < n; ++i) {
-    const uint32_t rts = wide ? wide_tiles[i] : row_tiles[i];
-    p.row_tiles[i] = (uint16_t)rts; p.tile_cols[i] = (uint16_t)ceil_div(parts[i].cols, rts);      // (evenly)
-    p.row_tiles[i] = (uint16_t)ceil_div(parts[i].cols, p.tile_cols[i]);
-    p.unit0[i] = p.units;
-    p.units += ceil_div(tiles[i], T) * p.row_tiles[i];
-    f.n_own[i] = (uint16_t)ceil_div(tiles[i], rec);
-    read += p.rows[i];
+    uint32_t j = i;
+    for (; j && tiles[order[j - 1]] < tiles[i]; --j) order[j] = order[j - 1];
+    order[j] = i;
+    f.rec0[i] = recs; f.n_rec[i] = (uint16_t)ceil_div(tiles[i], rec);
+    recs += parts[i].cols * nH * f.n_rec[i];
+  }
+  uint64_t read = 0;
+  for (uint32_t k = 0; k < n; ++k) {
+    const uint32_t i = order[k], rts = wide ? wide_tiles[i] : row_tiles[i];
+    const pa_item& it = c.items[parts[i].item];
+    p.seq[k] = it.seq; p.base[k] = it.pos; p.rows[k] = it.pos + parts[i].first + parts[i].cols;
+    p.col0[k] = f.col0[i]; p.cols[k] = parts[i].cols; p.node0[k] = parts[i].first; p.parent0[k] = c.item_col0[parts[i].item];
+    p.rec0[k] = f.rec0[i]; p.n_rec[k] = f.n_rec[i];
+    p.tile_cols[k] = (uint16_t)ceil_div(parts[i].cols, rts);      // (evenly)
+    p.row_tiles[k] = (uint16_t)ceil_div(parts[i].cols, p.tile_cols[k]);
+    p.unit0[k] = p.units;
+    p.units += ceil_div(tiles[i], T) * p.row_tiles[k];
+    read += p.rows[k];
   }
   p.unit0[n] = p.units;
-  p.n_rec = ceil_div(longest, rec);
   p.q = reinterpret_cast<const uint8_t*>(c.q) + (uint64_t)first_col * c.qcs * (c.q_f16 ? 2 : 4); p.q_f16 = c.q_f16; p.q_col_stride = c.qcs; p.q_head_stride = c.qhs;
   p.n_heads = nH; p.G = G; p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)hd));
   p.part_o = ctx->part_o; p.part_ml = ctx->part_ml;
   p.parents = c.parents; p.v = L->v; p.kv_dim = ctx->kv_dim; p.max_seq = L->max_seq; p.n_items = n; p.err = ctx->dev_err;
-  f.part_o = p.part_o; f.part_ml = p.part_ml; f.n_rec = p.n_rec; f.n_items = n; f.n_heads = nH; f.n_rows = cols * nH;
+  f.part_o = p.part_o; f.part_ml = p.part_ml; f.n_items = n; f.n_heads = nH; f.n_rows = cols * nH;
   f.gate = c.gate ? reinterpret_cast<const uint8_t*>(c.gate) + (uint64_t)first_col * c.gcs * aes : nullptr; f.gate_col_stride = c.gcs; f.gate_head_stride = c.ghs;
   f.out = reinterpret_cast<uint8_t*>(c.out) + (uint64_t)first_col * c.ocs * aes; f.out_col_stride = c.ocs; f.act_f16 = f16_out;
   f.vec = !((uintptr_t)f.out % (4 * aes)) && c.ocs % 4 == 0 && (!c.gate || (!((uintptr_t)f.gate % (4 * aes)) && c.gcs % 4 == 0 && c.ghs % 4 == 0));
   // a warp a row where that gives every SM CTAs enough; else a CTA a row, or a 64-dim slice of one with many records
-  f.lanes = f.n_rows >= 4 * (uint32_t)ctx->sm_count ? 0 : f.n_rows * 2 <= (uint32_t)ctx->sm_count * 4 && p.n_rec > 16 ? 16 : hd / 4;
+  f.lanes = f.n_rows >= 4 * (uint32_t)ctx->sm_count ? 0 : f.n_rows * 2 <= (uint32_t)ctx->sm_count * 4 && p.n_rec[0] > 16 ? 16 : hd / 4;
   CU_TRY(ctx, launch_tree(p, wide, L->tm_k64, L->tm_v64, hd, n_kv, ctx->device, st));
   CU_TRY(ctx, launch_tree_finish(f, hd, st));
   ctx->stats.kernel_launches += 2;
@@ -145,7 +154,7 @@ extern "C" int pa_decode_tree(pa_layer* L, const pa_item* items, uint32_t n_item
   if (L->kv_format != PA_KV_F16) return fail(ctx, PA_EUNSUPPORTED, "%s: f16 caches only", who);
   if (L->origin) return fail(ctx, PA_EUNSUPPORTED, "%s: not on a shard of longer sequences", who);
   if (ctx->G > 64) return fail(ctx, PA_EUNSUPPORTED, "%s: more than 64 query heads per kv head", who);
-  if ((size_t)ctx->cfg.n_heads * 2 > ctx->pf_slots) return fail(ctx, PA_EUNSUPPORTED, "%s: more than %zu query heads", who, ctx->pf_slots / 2);
+  if ((size_t)ctx->cfg.n_heads * 2 > ctx->tree_slots) return fail(ctx, PA_EUNSUPPORTED, "%s: more than %zu query heads", who, ctx->tree_slots / 2);
   if (!items || !q || !out) return fail(ctx, PA_EINVAL, "%s: null items, q or out", who);
   if (q_dtype != PA_F32 && q_dtype != PA_F16) return fail(ctx, PA_EINVAL, "%s: unknown q dtype", who);
   if (n_items < 1 || n_items > (uint32_t)kMaxTrees) return fail(ctx, PA_EINVAL, "%s: 1 to %d items per call", who, kMaxTrees);
@@ -167,7 +176,7 @@ extern "C" int pa_decode_tree(pa_layer* L, const pa_item* items, uint32_t n_item
   const TreeCall c{L, items, col0, parents, q, q_dtype == PA_F16, qcs, qhs, gate, gcs, ghs, out, ocs};
   DeviceScope on(ctx->device);
   // columns that fit the records, two a row at least, go in one launch; a tree may be parted
-  const uint32_t most = std::max<uint32_t>(1, (uint32_t)(ctx->pf_slots / (2 * (size_t)ctx->cfg.n_heads)));
+  const uint32_t most = std::max<uint32_t>(1, (uint32_t)(ctx->tree_slots / (2 * (size_t)ctx->cfg.n_heads)));
   for (uint32_t col = 0, item = 0, in = 0; col < total;) {
     TreePart parts[kMaxTrees];
     uint32_t n = 0, cols = 0;
