@@ -152,8 +152,8 @@ class Rotary:
 
     def _places(self, positions, cols):
         """Positions of the device: one per axis and column."""
-        if positions.dtype != torch.int32 or not positions.is_contiguous() or (tuple(positions.shape) != (cols,) if positions.dim() == 1 and self.n_axes == 1
-                                                                               else tuple(positions.shape) != (self.n_axes, cols)):
+        shape, axes = positions.shape, self.n_axes
+        if positions.dtype != torch.int32 or shape != ((cols,) if axes == 1 and len(shape) == 1 else (axes, cols)) or not positions.is_contiguous():
             raise _l.PaError(-1, f"positions are a contiguous int32 tensor of one value per column, [{self.n_axes}, {cols}] of several axes")
 
     def apply(self, x: torch.Tensor, n_heads: int, pos: int = 0, positions: torch.Tensor | None = None, head_stride: int | None = None,
@@ -543,8 +543,8 @@ class AttnEngine:
         out = self._batch(total, q, q_head_stride, gate, gate_head_stride, out)
         if parents is not None:
             self._on_device(parents)
-            if parents.dtype != torch.int32 or parents.shape != (total,):
-                raise _l.PaError(-1, f"{parents.dtype} parents of shape {tuple(parents.shape)}: int32, one per token of {total}, are wanted")
+            if parents.dtype != torch.int32 or parents.shape != (total,) or not parents.is_contiguous():
+                raise _l.PaError(-1, f"{parents.dtype} parents of shape {tuple(parents.shape)}: contiguous int32, one per token of {total}, are wanted")
         hd = self.cfg.head_dim
         rc = self._call.decode_tree(self._f_tree, self.layers[li].value, items, parents, q, _dt(q.dtype), q_head_stride or hd, gate, gate_head_stride or hd, out, self._raw_st())
         if rc:

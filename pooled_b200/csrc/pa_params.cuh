@@ -278,7 +278,7 @@ struct TreeParams {
 };
 struct TreeFinishParams {
   const float* part_o; const float* part_ml;
-  uint32_t n_items, n_heads, n_rows, lanes;                                 // lanes: as in SharedFinishParams; 0: a warp a row (head_dim 256: half of one)
+  uint32_t n_items, n_heads, n_rows, lanes;                                 // lanes: as in SharedFinishParams; 0: a warp a piece of a row
   const void* gate; uint64_t gate_col_stride, gate_head_stride;
   void* out; uint64_t out_col_stride; int act_f16, vec;                     // vec: four values of gate and out lie on whole vectors
   uint32_t col0[kMaxTrees + 1], rec0[kMaxTrees];                            // the parts in their columns' order

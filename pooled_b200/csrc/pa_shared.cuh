@@ -123,6 +123,33 @@ static __device__ __noinline__ uint64_t tree_sees(const int16_t* parents, uint32
   return m;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// The weights of 16 keys as f16 pairs, high and low parts, and their sum, two values an instruction.  The high part is the weight with the bits
+// that f16 lacks cut off (exact but for weights below 2^-14, 2^-21 of the row's largest), the low part what that leaves.
+__device__ __forceinline__ float tree_weights(const float* s, float scale, float m, uint32_t (&hi)[8], uint32_t (&lo)[8]) {
+  const float2 k = make_float2(scale, scale), ref = make_float2(-m, -m);
+  float2 sum = make_float2(0.f, 0.f);
+  auto bits = [](const float2& v) { return *reinterpret_cast<const unsigned long long*>(&v); };
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    unsigned long long x;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(bits(make_float2(s[2 * i], s[2 * i + 1]))), "l"(bits(k)), "l"(bits(ref)));
+    const float2 f = *reinterpret_cast<const float2*>(&x), e = make_float2(ex2_approx(f.x), ex2_approx(f.y));
+    const float2 h = make_float2(__uint_as_float(__float_as_uint(e.x) & 0xffffe000u), __uint_as_float(__float_as_uint(e.y) & 0xffffe000u));
+    unsigned long long t, l;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(t) : "l"(bits(sum)), "l"(bits(e)));
+    sum = *reinterpret_cast<const float2*>(&t);
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(l) : "l"(bits(h)), "l"(bits(make_float2(-1.f, -1.f))), "l"(bits(e)));
+    const float2 rest = *reinterpret_cast<const float2*>(&l);
+    hi[i] = pack_h2(h.x, h.y); lo[i] = pack_h2(rest.x, rest.y);
+  }
+  return sum.x + sum.y;
+}
+
 // Adds the V values that were no finite numbers to the last records of a unit's query rows, record `rec` of each: thread `tid` of `threads`.
 template <int HD, typename P>
 __device__ __noinline__ void tree_restore(const P& p, TreeUnit un, const uint32_t* dirty, const int16_t* parents, uint32_t rec, uint32_t tid, uint32_t threads) {
@@ -467,8 +494,14 @@ __device__ __forceinline__ void shared_roles(const P& p, const U& un, uint8_t* b
             for (int i = 0; i < NS; ++i) if (kv0 + mine + i >= un.n_rows) s[i] = -INFINITY;
           }
           float mt = s[0];
+          if constexpr (TREE) {
+            mt = fmaxf(mt, s[1]);
 #pragma unroll
-          for (int i = 1; i < NS; ++i) mt = fmaxf(mt, s[i]);
+            for (int i = 2; i < NS; i += 2) mt = max3(mt, s[i], s[i + 1]);
+          } else {
+#pragma unroll
+            for (int i = 1; i < NS; ++i) mt = fmaxf(mt, s[i]);
+          }
           if (!WIDE) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
           mt = row_max(mt, j) * p.scale_log2;
           float alpha = 1.f;
@@ -488,45 +521,42 @@ __device__ __forceinline__ void shared_roles(const P& p, const U& un, uint8_t* b
             }
           }
           // weights as f16 pairs, high and low parts
-          if constexpr (WIDE && HD < 256) {                // (16 keys at a time: two CTAs an SM have 80 registers a thread)
+          if constexpr (TREE && WIDE) {                    // (16 keys at a time: two CTAs an SM have 80 registers a thread)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               uint32_t hi[8], lo[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float e0 = ex2_approx(fmaf(s[16 * h + 2 * i], p.scale_log2, -m_st)), e1 = ex2_approx(fmaf(s[16 * h + 2 * i + 1], p.scale_log2, -m_st));
-                l_sum += e0 + e1;
-                const __half2 x = __floats2half2_rn(e0, e1);
-                const float2 f = __half22float2(x);
-                hi[i] = *reinterpret_cast<const uint32_t*>(&x); lo[i] = pack_h2(e0 - f.x, e1 - f.y);
-              }
+              l_sum += tree_weights(s + 16 * h, p.scale_log2, m_st, hi, lo);
               tmem_st8u(t_s0 + b * 64 + 16 * wg + 8 * h + lane_addr, hi);
               tmem_st8u(t_s0 + b * 64 + 32 + 16 * wg + 8 * h + lane_addr, lo);
             }
           } else {
-          uint32_t hi[NS / 2], lo[NS / 2];
+            uint32_t hi[NS / 2], lo[NS / 2];
+            if constexpr (TREE) {
+              l_sum += tree_weights(s, p.scale_log2, m_st, hi, lo);
+            } else {
 #pragma unroll
-          for (int i = 0; i < NS / 2; ++i) {
-            const float e0 = ex2_approx(fmaf(s[2 * i], p.scale_log2, -m_st)), e1 = ex2_approx(fmaf(s[2 * i + 1], p.scale_log2, -m_st));
-            l_sum += e0 + e1;
-            const __half2 h = __floats2half2_rn(e0, e1);
-            const float2 f = __half22float2(h);
-            hi[i] = *reinterpret_cast<const uint32_t*>(&h); lo[i] = pack_h2(e0 - f.x, e1 - f.y);
-          }
-          if constexpr (WIDE) {
-            tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, hi);
-            tmem_st16u(t_s0 + b * 64 + 32 + 16 * wg + lane_addr, lo);
-          } else {
-            // the even lane's row takes the high parts of the group's 32 keys, the odd one's the low parts
-            uint32_t pw[16];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t got = __shfl_xor_sync(0xffffffffu, is_lo ? hi[i] : lo[i], 1);
-              pw[i] = is_lo ? got : hi[i];
-              pw[8 + i] = is_lo ? lo[i] : got;
+              for (int i = 0; i < NS / 2; ++i) {
+                const float e0 = ex2_approx(fmaf(s[2 * i], p.scale_log2, -m_st)), e1 = ex2_approx(fmaf(s[2 * i + 1], p.scale_log2, -m_st));
+                l_sum += e0 + e1;
+                const __half2 h = __floats2half2_rn(e0, e1);
+                const float2 f = __half22float2(h);
+                hi[i] = *reinterpret_cast<const uint32_t*>(&h); lo[i] = pack_h2(e0 - f.x, e1 - f.y);
+              }
             }
-            tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, pw);
-          }
+            if constexpr (WIDE) {
+              tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, hi);
+              tmem_st16u(t_s0 + b * 64 + 32 + 16 * wg + lane_addr, lo);
+            } else {
+              // the even lane's row takes the high parts of the group's 32 keys, the odd one's the low parts
+              uint32_t pw[16];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, is_lo ? hi[i] : lo[i], 1);
+                pw[i] = is_lo ? got : hi[i];
+                pw[8 + i] = is_lo ? lo[i] : got;
+              }
+              tmem_st16u(t_s0 + b * 64 + 16 * wg + lane_addr, pw);
+            }
           }
           tmem_wait_st();
           tc_fence_before();

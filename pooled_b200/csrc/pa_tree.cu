@@ -11,9 +11,11 @@
 //   V           a weight of zero does not make up for an infinity or NaN: the V producer looks through the tree's rows of a tile
 //               while the scores are being made, puts zeros in the place of such values and notes their rows; a token that attends
 //               one of them has its values added to its record at the end, so that it ends as the formula does
-// What bounds it: with few tokens HBM; from some 100 query rows a kv head on the tensor cores (a byte of K and V serves all row
-// tiles from L2): 64 tokens of 16 / 2 heads of 256 behind 32768 rows 75 us (0.28 of the measured rate of plain bf16 products), 16 x 60 of
-// 16 / 8 heads of 128 behind up to 4003 rows 75 us.
+// What bounds it: with few tokens HBM; from some 100 query rows a kv head on the issue of the tensor instructions, whose N is a tile's 64
+// keys (with half of the L2 traffic taken away nothing changes): 64 tokens of 16 / 2 heads of 256 behind 32768 rows 52 us (0.40 of the
+// measured rate of plain bf16 products), 16 x 60 of 16 / 8 heads of 128 behind up to 4003 rows 41 us, 6 x 26 of 32 / 8 heads of 128 with f32
+// queries behind up to 9003 rows 58 us; 8 tokens behind 300 rows 7.5 us.  (Tiles of 128 keys need one CTA an SM and the exponentials of a
+// tile are then not hidden: 49, 45 and 58 us with 16 softmax warps, and 8.2 us for the 8 tokens.)
 #include "pa_shared.cuh"
 
 namespace pa {
@@ -83,8 +85,9 @@ __device__ __forceinline__ uint32_t tree_item(const TreeFinishParams& p, uint32_
   return lo;
 }
 
-// Merge, gate, store.  Few rows: a CTA a row (or slice), as behind a shared prefix.  Many: a warp a row (head_dim 256: half of one), eight a
-// CTA, so that a row of two or three records does not take a CTA's start and two barriers.
+// Merge, gate, store.  Few rows: a CTA a row (or slice), as behind a shared prefix.  Many: a warp a piece of a row, eight a CTA, so that a
+// row of two or three records does not take a CTA's start and two barriers.  (Pieces of 64 dims, half a warp on every other record: no faster
+// with 1024 rows of 18 records, 3 to 6 us slower with thousands of rows.)
 template <int HD, bool WARPS>
 __global__ void __launch_bounds__(256, 4) pa_tree_finish_kernel(const __grid_constant__ TreeFinishParams p) {
   pdl_wait();
@@ -94,73 +97,70 @@ __global__ void __launch_bounds__(256, 4) pa_tree_finish_kernel(const __grid_con
     const uint32_t slices = HD / 4 / p.lanes, prow = blockIdx.x / slices, col = prow / p.n_heads, it = tree_item(p, col);
     shared_merge_row<HD>(p, s_acc, p.rec0[it] + (uint64_t)(prow - p.col0[it] * p.n_heads) * p.n_rec[it], blockIdx.x % slices, col, prow % p.n_heads, p.n_rec[it]);
   } else {
-    constexpr int PIECES = HD == 256 ? 2 : 1, W = HD == 64 ? 2 : 4, U = 8;       // warps of a row; values of a lane; records at once
-    const uint32_t w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, prow = w / PIECES, d = w % PIECES * 128 + lane * W;
+    constexpr int PIECE = HD == 64 ? 64 : 128, PIECES = HD / PIECE, SIDES = 128 / PIECE, U = 8;       // dims; warps of a row; records of a load; loads at once
+    const uint32_t w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, prow = w / PIECES, side = SIDES == 2 ? lane >> 4 : 0,
+                   d = w % PIECES * PIECE + (SIDES == 2 ? lane & 15 : lane) * 4;
     if (prow >= p.n_rows) return;
     const uint32_t col = prow / p.n_heads, h = prow - col * p.n_heads, it = tree_item(p, col), ns = p.n_rec[it];
     const uint64_t rec = p.rec0[it] + (uint64_t)(prow - p.col0[it] * p.n_heads) * ns;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + rec;
     const float* ob = p.part_o + rec * HD + d;
-    float x[U][W], acc[W] = {};
+    float4 x[U], acc = make_float4(0.f, 0.f, 0.f, 0.f);
     auto load = [&](uint32_t s0) {
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const float* at = ob + (uint64_t)(s0 + k) * HD;
-        if constexpr (W == 4) {
-          const float4 v = s0 + k < ns ? *reinterpret_cast<const float4*>(at) : make_float4(0.f, 0.f, 0.f, 0.f);
-          x[k][0] = v.x; x[k][1] = v.y; x[k][W - 2] = v.z; x[k][W - 1] = v.w;
-        } else {
-          const float2 v = s0 + k < ns ? *reinterpret_cast<const float2*>(at) : make_float2(0.f, 0.f);
-          x[k][0] = v.x; x[k][1] = v.y;
-        }
+        const uint32_t s = s0 + k * SIDES + side;
+        x[k] = s < ns ? *reinterpret_cast<const float4*>(ob + (uint64_t)s * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     };
     load(0);
     const uint64_t go = (uint64_t)col * p.gate_col_stride + (uint64_t)h * p.gate_head_stride + d, oo = (uint64_t)col * p.out_col_stride + (uint64_t)h * HD + d;
-    float gv[W];
+    float gv[4];
     if (p.gate) {
-      if (p.vec && W == 4) {
-        if (p.act_f16) {
-          const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.gate) + go);
-          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
-          gv[0] = a.x; gv[1] = a.y; gv[W - 2] = b.x; gv[W - 1] = b.y;
-        } else {
-          const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.gate) + go);
-          gv[0] = v.x; gv[1] = v.y; gv[W - 2] = v.z; gv[W - 1] = v.w;
-        }
+      if (p.vec && p.act_f16) {
+        const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const __half*>(p.gate) + go);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+        gv[0] = a.x; gv[1] = a.y; gv[2] = b.x; gv[3] = b.y;
+      } else if (p.vec) {
+        const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.gate) + go);
+        gv[0] = v.x; gv[1] = v.y; gv[2] = v.z; gv[3] = v.w;
       } else {
 #pragma unroll
-        for (int e = 0; e < W; ++e) gv[e] = ld_act(p.gate, go + e, p.act_f16);
+        for (int e = 0; e < 4; ++e) gv[e] = ld_act(p.gate, go + e, p.act_f16);
       }
     }
     float M, l;
     shared_row_ml(ml, ns, M, l);
-    for (uint32_t s0 = 0; s0 < ns; s0 += U) {
+    for (uint32_t s0 = 0; s0 < ns; s0 += U * SIDES) {
       if (s0) load(s0);
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const float wt = s0 + k < ns ? ex2_approx(ml[s0 + k].x - M) : 0.f;
-#pragma unroll
-        for (int e = 0; e < W; ++e) acc[e] = fmaf(x[k][e], wt, acc[e]);
+        const uint32_t s = s0 + k * SIDES + side;
+        const float wt = s < ns ? ex2_approx(ml[s].x - M) : 0.f;
+        acc.x = fmaf(x[k].x, wt, acc.x); acc.y = fmaf(x[k].y, wt, acc.y); acc.z = fmaf(x[k].z, wt, acc.z); acc.w = fmaf(x[k].w, wt, acc.w);
       }
     }
+    float t[4] = {acc.x, acc.y, acc.z, acc.w};
+    if constexpr (SIDES == 2) {
 #pragma unroll
-    for (int e = 0; e < W; ++e) {
-      acc[e] = __fdiv_rn(acc[e], l);
-      if (p.gate) acc[e] *= __fdiv_rn(1.0f, 1.0f + __expf(-gv[e]));
+      for (int e = 0; e < 4; ++e) t[e] += __shfl_down_sync(0xffffffffu, t[e], 16);
+      if (side) return;
     }
-    if (p.vec && W == 4) {
-      if (p.act_f16) {
-        const __half2 a = __floats2half2_rn(acc[0], acc[1]), b = __floats2half2_rn(acc[W - 2], acc[W - 1]);
-        *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + oo) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-      } else {
-        *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + oo) = make_float4(acc[0], acc[1], acc[W - 2], acc[W - 1]);
-      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      t[e] = __fdiv_rn(t[e], l);
+      if (p.gate) t[e] *= __fdiv_rn(1.0f, 1.0f + __expf(-gv[e]));
+    }
+    if (p.vec && p.act_f16) {
+      const __half2 a = __floats2half2_rn(t[0], t[1]), b = __floats2half2_rn(t[2], t[3]);
+      *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + oo) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else if (p.vec) {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + oo) = make_float4(t[0], t[1], t[2], t[3]);
     } else {
 #pragma unroll
-      for (int e = 0; e < W; ++e) {
-        if (p.act_f16) reinterpret_cast<__half*>(p.out)[oo + e] = __float2half_rn(acc[e]);
-        else reinterpret_cast<float*>(p.out)[oo + e] = acc[e];
+      for (int e = 0; e < 4; ++e) {
+        if (p.act_f16) reinterpret_cast<__half*>(p.out)[oo + e] = __float2half_rn(t[e]);
+        else reinterpret_cast<float*>(p.out)[oo + e] = t[e];
       }
     }
   }
@@ -189,8 +189,8 @@ cudaError_t launch_tree(const TreeParams& p, bool wide, const CUtensorMap& k, co
 }
 template <int HD>
 static cudaError_t launch_finish_t(const TreeFinishParams& p, cudaStream_t st) {
-  return p.lanes ? launch_pdl(pa_tree_finish_kernel<HD, false>, dim3(p.n_rows * (HD / 4 / p.lanes)), dim3(256), 0, st, p)
-                 : launch_pdl(pa_tree_finish_kernel<HD, true>, dim3((p.n_rows * (HD == 256 ? 2 : 1) + 7) / 8), dim3(256), 0, st, p);
+  if (p.lanes) return launch_pdl(pa_tree_finish_kernel<HD, false>, dim3(p.n_rows * (HD / 4 / p.lanes)), dim3(256), 0, st, p);
+  return launch_pdl(pa_tree_finish_kernel<HD, true>, dim3((p.n_rows * (HD == 256 ? 2 : 1) + 7) / 8), dim3(256), 0, st, p);
 }
 cudaError_t launch_tree_finish(const TreeFinishParams& p, uint32_t hd, cudaStream_t st) {
   return hd == 256 ? launch_finish_t<256>(p, st) : hd == 128 ? launch_finish_t<128>(p, st) : hd == 64 ? launch_finish_t<64>(p, st) : cudaErrorInvalidValue;

@@ -14,8 +14,9 @@ using namespace pa;
 
 static uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
-// tiles of a run: f16 outputs at most 128, f32 at most 4 (16 with several row tiles; 24 where records run short), as behind a shared
-// prefix (pa_shared_api.cu), since the tensor cores' sums round towards zero
+// tiles of a run: f16 outputs at most 128, f32 at most 4 (10 with several row tiles; 24 where records run short), since the tensor cores'
+// sums round towards zero.  (6 x 26 tokens behind up to 9003 rows: 55.5 us and off by 1.9e-6 of the largest output with runs of 16, 58 us
+// and 1.2e-6 with 10; f32 products in the plain order 1.1e-6.)
 static constexpr uint32_t kF16Tiles = 128, kF32Run = 24;
 static uint32_t record_tiles(uint32_t T, uint32_t cap) { return ceil_div(T, ceil_div(T, cap)); }
 
@@ -44,16 +45,20 @@ static TreePlan plan_tree(const pa_ctx* ctx, const TreePart* parts, const uint32
   }
   hbm *= (float)(n_kv * hd * 256) / 6.0e6f;
   TreePlan best{longest, 3.0e38f};
-  for (uint32_t s = 1; s <= std::min(longest, 512u); s += 1 + s / 24) {
-    const uint32_t T = ceil_div(longest, s), own = std::min(T, longest), records = ceil_div(own, record_tiles(T, cap));
-    const uint64_t recs = tree_records(parts, tiles, n, ctx->cfg.n_heads, T);
-    if (recs > ctx->tree_slots) break;
-    const float unit = (float)own * tile + start + (float)(records - 1) * record;
+  for (uint32_t T = longest; T >= 1; T -= 1 + T / 40) {
+    const uint32_t records = ceil_div(T, record_tiles(T, cap));
     uint32_t units = 0;
-    for (uint32_t i = 0; i < n; ++i) units += ceil_div(tiles[i], T) * row_tiles[i];
-    units *= n_kv;
-    float us = units <= sms ? unit : std::max(unit, (work_tiles * n_kv * tile + (float)units * start) / (float)sms + 0.3f * unit);
-    us = std::max(us, hbm + start) + 0.05f * us + (float)(recs * records * hd * 4) / 4.0e6f;
+    uint64_t recs = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+      const uint32_t splits = ceil_div(tiles[i], T);
+      units += splits * row_tiles[i];
+      recs += (uint64_t)parts[i].cols * splits;
+    }
+    units *= n_kv; recs *= ctx->cfg.n_heads;
+    if (recs > ctx->tree_slots) break;
+    const float unit = (float)T * tile + start + (float)(records - 1) * record;
+    float us = units <= sms ? unit : std::max(unit, (work_tiles * n_kv * tile + (float)units * start) / (float)sms + 0.5f * unit);
+    us = std::max(us, hbm + start) + (float)(recs * records * hd * 4) / 5.0e6f;
     if (us < best.us) best = TreePlan{T, us};
   }
   return best;
@@ -89,14 +94,14 @@ static int tree_launch(const TreeCall& c, const TreePart* parts, uint32_t n, uin
   }
   f.col0[n] = total;
   const bool f16_out = ctx->cfg.act_dtype == PA_F16;
-  const uint32_t cap = f16_out ? kF16Tiles : most_row_tiles > 1 ? 16u : 4u;
+  const uint32_t cap = f16_out ? kF16Tiles : most_row_tiles > 1 ? 10u : 4u;
   TreePlan plan = plan_tree(ctx, parts, tiles, row_tiles, n, false, rows_of_tile, cap);
   bool wide = false;
   if (most_row_tiles > 1 && c.q_f16 && f16_out && ctx->tune.shared_wide != 0) {
     const TreePlan w = plan_tree(ctx, parts, tiles, wide_tiles, n, true, 128, cap);
     if (w.us < plan.us || ctx->tune.shared_wide == 1) { plan = w; wide = true; }
   }
-  // tiles of a record, as behind a shared prefix: a unit's shared out evenly; more where there is no room for that many, and past the
+  // tiles of a record: a unit's shared out evenly; more where there is no room for that many, and past the
   // longest run a record adds up several
   uint32_t T = plan.T, records = ceil_div(T, cap);
   while (records > 1 && tree_records(parts, tiles, n, nH, ceil_div(T, records)) > ctx->tree_slots) --records;
@@ -136,7 +141,7 @@ static int tree_launch(const TreeCall& c, const TreePart* parts, uint32_t n, uin
   f.gate = c.gate ? reinterpret_cast<const uint8_t*>(c.gate) + (uint64_t)first_col * c.gcs * aes : nullptr; f.gate_col_stride = c.gcs; f.gate_head_stride = c.ghs;
   f.out = reinterpret_cast<uint8_t*>(c.out) + (uint64_t)first_col * c.ocs * aes; f.out_col_stride = c.ocs; f.act_f16 = f16_out;
   f.vec = !((uintptr_t)f.out % (4 * aes)) && c.ocs % 4 == 0 && (!c.gate || (!((uintptr_t)f.gate % (4 * aes)) && c.gcs % 4 == 0 && c.ghs % 4 == 0));
-  // a warp a row where that gives every SM CTAs enough; else a CTA a row, or a 64-dim slice of one with many records
+  // warps for pieces of rows where that gives every SM enough of them; else a CTA a row, or a 64-dim slice of one with many records
   f.lanes = f.n_rows >= 4 * (uint32_t)ctx->sm_count ? 0 : f.n_rows * 2 <= (uint32_t)ctx->sm_count * 4 && p.n_rec[0] > 16 ? 16 : hd / 4;
   CU_TRY(ctx, launch_tree(p, wide, L->tm_k64, L->tm_v64, hd, n_kv, ctx->device, st));
   CU_TRY(ctx, launch_tree_finish(f, hd, st));
