@@ -202,8 +202,8 @@ struct PrefillParams {
 
 constexpr int kMaxShared = 128;   // items of one pa_rotary_append / pa_decode_shared / pa_decode_weights call
 
-// rotation by a pa_rotary, and the append behind it (pa_rotary_kernel)
-struct RotaryParams {
+// rotation by a pa_rotary, and the append behind it (pa_rotary_kernel), for up to N items: a launch costs the host by its parameters' size
+struct RotaryCommon {
   const double* turns;     // [n_rot / 2] turns of a pair per position
   float mscale;
   uint32_t hd, n_rot, layout, n_cols, cpb;                                   // cpb: columns of a CTA (the launcher sets it)
@@ -216,10 +216,15 @@ struct RotaryParams {
   const void* k; const void* v; uint64_t kv_col_stride; uint32_t kv_heads;
   __half* k_cache; __half* v_cache;
   uint32_t n_items, one_each;                                               // one_each: every item has one column
-  int32_t pos[kMaxShared];
-  uint32_t col0[kMaxShared];
-  uint64_t row[kMaxShared];
 };
+template <int N>
+struct RotaryParamsOf : RotaryCommon {
+  int32_t pos[N];
+  uint32_t col0[N];
+  uint64_t row[N];
+};
+using RotaryParams = RotaryParamsOf<kMaxShared>;
+constexpr int kFewRotary = 16;        // items of an append of few
 
 // attention of one token per item against rows all items share and rows of its own (pa_shared_kernel), and the merge of its
 // records, with or without the sums of the weights (pa_shared_finish_kernel)

@@ -124,7 +124,8 @@ __device__ __forceinline__ void rot_angle(const double* turns, uint32_t i, int32
 }
 
 // the item of a column: items own consecutive columns, col0 ascending
-__device__ __forceinline__ uint32_t rot_item(const RotaryParams& p, uint32_t col) {
+template <int N>
+__device__ __forceinline__ uint32_t rot_item(const RotaryParamsOf<N>& p, uint32_t col) {
   if (p.one_each) return col;
   uint32_t lo = 0, hi = p.n_items - 1;
   while (lo < hi) { const uint32_t mid = (lo + hi + 1) / 2; if (col >= p.col0[mid]) lo = mid; else hi = mid - 1; }
@@ -132,7 +133,7 @@ __device__ __forceinline__ uint32_t rot_item(const RotaryParams& p, uint32_t col
 }
 
 // the axis whose position turns pair k: blocks of pairs, or the axes in turn for as long as they have pairs left, then the first
-__device__ __forceinline__ uint32_t rot_axis(const RotaryParams& p, uint32_t k) {
+__device__ __forceinline__ uint32_t rot_axis(const RotaryCommon& p, uint32_t k) {
   if (p.n_axes < 2) return 0;
   const uint32_t n0 = p.axis_pairs[0], n1 = p.axis_pairs[1], n2 = p.axis_pairs[2];
   if (!p.axes_cycled) return (k >= n0) + (k >= n0 + n1 && p.n_axes > 2) + (k >= n0 + n1 + n2 && p.n_axes > 3);
@@ -142,8 +143,8 @@ __device__ __forceinline__ uint32_t rot_axis(const RotaryParams& p, uint32_t k) 
 
 // V: 16-byte vectors, or 1: single values (then a unit is one pair, or two copied values), for layouts that vectors do not fit.
 // Threads (units, columns); grid (column groups, unit blocks).
-template <typename TI, typename TO, bool APPEND, int V>
-__global__ void __launch_bounds__(kRotThreads) pa_rotary_kernel(const __grid_constant__ RotaryParams p) {
+template <typename TI, typename TO, bool APPEND, int V, int N>
+__global__ void __launch_bounds__(kRotThreads) pa_rotary_kernel(const __grid_constant__ RotaryParamsOf<N> p) {
   __shared__ __align__(16) float s_c[kRotAngles], s_s[kRotAngles];
   const uint32_t tid = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
   const uint32_t half = p.n_rot / 2, pitch = (half + 3) & ~3u, c0 = blockIdx.x * p.cpb, cols = min(p.cpb, p.n_cols - c0);
@@ -219,8 +220,12 @@ __global__ void __launch_bounds__(kRotThreads) pa_rotary_kernel(const __grid_con
   }
 }
 
-template <typename TI, typename TO, bool APPEND, int V>
-static cudaError_t launch_rotary_v(RotaryParams p, uint32_t sms, cudaStream_t st) {
+template <typename TI, typename TO, bool APPEND, int V, int N>
+static cudaError_t launch_rotary_n(const RotaryParams& all, uint32_t sms, cudaStream_t st) {
+  RotaryParamsOf<N> p;
+  static_cast<RotaryCommon&>(p) = all;
+  const uint32_t n = std::max(1u, all.n_items);      // (no append: the first position)
+  std::copy(all.pos, all.pos + n, p.pos); std::copy(all.col0, all.col0 + n, p.col0); std::copy(all.row, all.row + n, p.row);
   const bool lay = p.layout == PA_ROPE_HALF;
   const uint32_t per_head = rot_units<V>(p.hd, p.n_rot, lay), units = (p.q ? p.q_heads * per_head : 0) + (APPEND ? p.kv_heads * (per_head + rot_units<V>(p.hd, 0, lay)) : 0);
   // CTAs of up to 384 units of a column, of several columns where they have few; a thread takes four columns, fewer while that
@@ -229,7 +234,12 @@ static cudaError_t launch_rotary_v(RotaryParams p, uint32_t sms, cudaStream_t st
   const uint32_t y = std::max(1u, std::min(std::min(256 / x, p.n_cols), kRotAngles / pitch));
   const uint32_t k = std::max(1u, std::min(std::min(kRotCols, kRotAngles / pitch / y), (uint32_t)((uint64_t)p.n_cols * blocks / y / (2 * sms))));
   p.cpb = y * k;
-  return launch_pdl(pa_rotary_kernel<TI, TO, APPEND, V>, dim3((p.n_cols + p.cpb - 1) / p.cpb, blocks), dim3(x, y), 0, st, p);
+  return launch_pdl(pa_rotary_kernel<TI, TO, APPEND, V, N>, dim3((p.n_cols + p.cpb - 1) / p.cpb, blocks), dim3(x, y), 0, st, p);
+}
+template <typename TI, typename TO, bool APPEND, int V>
+static cudaError_t launch_rotary_v(const RotaryParams& p, uint32_t sms, cudaStream_t st) {
+  if constexpr (!APPEND) return launch_rotary_n<TI, TO, false, V, 1>(p, sms, st);
+  else return p.n_items <= (uint32_t)kFewRotary ? launch_rotary_n<TI, TO, true, V, kFewRotary>(p, sms, st) : launch_rotary_n<TI, TO, true, V, kMaxShared>(p, sms, st);
 }
 template <typename TI, typename TO, bool APPEND>
 static cudaError_t launch_rotary_t(const RotaryParams& p, uint32_t sms, cudaStream_t st) {

@@ -134,7 +134,7 @@ extern "C" int pa_rotary_freqs(const pa_rotary* r, double* freqs, double* mscale
   return PA_OK;
 }
 
-static void set_axes(RotaryParams& p, const pa_rotary* r) {
+static void set_axes(RotaryCommon& p, const pa_rotary* r) {
   p.n_axes = r->axes.n_axes; p.axes_cycled = r->axes.order == PA_ROPE_AXES_CYCLED;
   std::copy(r->axes.pairs, r->axes.pairs + 4, p.axis_pairs);
 }
