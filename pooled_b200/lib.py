@@ -217,6 +217,8 @@ class CtypesCalls:
                                        _ptr(out), out.stride(0), stream)
 
     def cache_move(self, entry, layers, n_layers, items, lists, list_stride, stream):
+        if any(len(it) != 5 for it in items):
+            raise ValueError("the items are a sequence of (src_seq, src_row, dst_seq, dst_row, n_rows)")
         arr = (PaMoveItem * max(1, len(items)))(*[PaMoveItem(*map(u32, it), 0) for it in items])
         return self.lib.pa_cache_move(layers, u32(n_layers), arr, len(items), _ptr(lists), u32(list_stride), stream)
 
