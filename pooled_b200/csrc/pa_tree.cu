@@ -13,9 +13,10 @@
 //               one of them has its values added to its record at the end, so that it ends as the formula does
 // What bounds it: with few tokens HBM; from some 100 query rows a kv head on the issue of the tensor instructions, whose N is a tile's 64
 // keys (with half of the L2 traffic taken away nothing changes): 64 tokens of 16 / 2 heads of 256 behind 32768 rows 52 us (0.40 of the
-// measured rate of plain bf16 products), 16 x 60 of 16 / 8 heads of 128 behind up to 4003 rows 41 us, 6 x 26 of 32 / 8 heads of 128 with f32
-// queries behind up to 9003 rows 58 us; 8 tokens behind 300 rows 7.5 us.  (Tiles of 128 keys need one CTA an SM and the exponentials of a
-// tile are then not hidden: 49, 45 and 58 us with 16 softmax warps, and 8.2 us for the 8 tokens.)
+// measured rate of plain bf16 products), 16 x 60 of 16 / 8 heads of 128 behind up to 4003 rows 41 us, 6 x 26 of 24 / 4 heads of 256 with f32
+// queries behind up to 9001 rows 58 us; 8 tokens behind 301 rows 7.5 us.  (At a sustained load the clock falls to 1.5 GHz: 61, 45 and 69 us.
+// Tiles of 128 keys need one CTA an SM and the exponentials of a tile are then not hidden: 49, 45 and 55 us with 16 softmax warps, 59, 47 and
+// 67 sustained, and 8.2 us for the 8 tokens.  Merged by the last CTA of each row tile instead of a second kernel: 11.4, 133, 85 and 56 us.)
 #include "pa_shared.cuh"
 
 namespace pa {

@@ -15,7 +15,7 @@ using namespace pa;
 static uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
 // tiles of a run: f16 outputs at most 128, f32 at most 4 (10 with several row tiles; 24 where records run short), since the tensor cores'
-// sums round towards zero.  (6 x 26 tokens behind up to 9003 rows: 55.5 us and off by 1.9e-6 of the largest output with runs of 16, 58 us
+// sums round towards zero.  (6 x 26 tokens of 24 / 4 heads of 256 behind up to 9001 rows: 55.5 us and off by 1.9e-6 of the largest output with runs of 16, 58 us
 // and 1.2e-6 with 10; f32 products in the plain order 1.1e-6.)
 static constexpr uint32_t kF16Tiles = 128, kF32Run = 24;
 static uint32_t record_tiles(uint32_t T, uint32_t cap) { return ceil_div(T, ceil_div(T, cap)); }
