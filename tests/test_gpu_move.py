@@ -152,6 +152,23 @@ def test_long_rows_over_one_another_keep_their_order(gap, up):
     assert same(eng, want)
 
 
+def test_rows_past_four_gigabytes():
+    # the last of eight sequences of 300000 rows of 2 KB: a fork, a list, rows over one another
+    eng = engine(8, 128, 300000, 8)
+    caches = [eng.cache(0, w) for w in "kv"]
+    for i, x in enumerate(caches):
+        x[7, 290000:] = torch.randint(-30000, 30000, (10000, 1024), generator=torch.Generator(device="cuda").manual_seed(i), device="cuda").to(torch.int16)
+    was = [x[7, 290000:].clone() for x in caches]
+    eng.move([(7, 290000, 7, 280000, 9000), (7, 290000, 6, 291000, 9000)])
+    eng.move([(7, 290000, 7, 290007, 9000)])
+    eng.move([(7, 290007, 0, 5, 100)], lists=torch.tensor([[3, 99, 0, 50]], dtype=torch.int32, device="cuda"))
+    eng.sync()
+    for x, y in zip(caches, was):
+        assert torch.equal(x[7, 280000:289000], y[:9000]) and torch.equal(x[6, 291000:], y[:9000])
+        assert torch.equal(x[7, 290000:290007], y[:7]) and torch.equal(x[7, 290007:299007], y[:9000]) and torch.equal(x[7, 299007:], y[9007:])
+        assert torch.equal(x[0, 5:8], y[[99, 0, 50]])
+
+
 def test_some_layers_and_many():
     eng = engine(2, 64, 100, 2, layers=70)                                 # more than one launch takes
     fill(eng, 5)

@@ -167,6 +167,30 @@ def test_a_long_context(nH, nKV, hd, act):
     check(eng, k, v, [(0, 33001, 61)], trees, q, None, got)
 
 
+def test_rows_past_four_gigabytes():
+    # the last of eight sequences of 300000 rows of 2 KB
+    eng = engine(16, 8, 128, 300000, 8, F16)
+    r, n, base = random.Random(2), 30, 200
+    k, v = [torch.randn((1, base + n, 8, 128), device="cuda").half() for _ in "kv"]
+    v[0, base + 3] = math.inf                                             # looked up again for those that attend it
+    for w, x in zip("kv", (k, v)):
+        eng.cache(0, w)[7, :base + n] = x.view(base + n, -1).view(torch.int16)
+    poison_rows = eng.cache(0, "v")[7, base + n:base + n + 64]
+    poison_rows[:] = torch.tensor(POISON, dtype=F16).repeat(256).view(torch.int16).cuda()
+    parents = tree(r, n, 4)
+    parents[3], parents[5] = 2, 3
+    q = torch.randn((n, 16 * 128), device="cuda").half()
+    got = eng.decode_tree(0, [(7, base, n)], q, parents=torch.tensor(parents, dtype=torch.int32, device="cuda"))
+    eng.sync()
+    mask = mask_of(parents, base)
+    of = mask[:, base + 3]
+    assert torch.all(got[of.cuda()] == math.inf) and of.any() and not of.all()
+    v[0, base + 3] = 0.0
+    want, delta = attend(q.view(n, 16, 128), k[0], v[0], mask)
+    keep = ~of.cuda()
+    close(got[keep], want[keep], v[0], delta[keep], base + n)
+
+
 @pytest.mark.parametrize("nH,nKV,hd", [(16, 8, 128), (16, 2, 256), (8, 8, 64)])
 def test_chains_and_single_tokens_are_what_the_other_decode_gives(nH, nKV, hd):
     eng = engine(nH, nKV, hd, 1100, 3, F32, max_cols=64)
