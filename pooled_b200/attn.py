@@ -162,10 +162,12 @@ class Rotary:
         [axes, n_cols]).  Into a new [n_cols, n_heads * head_dim] of x's type, or `out`, which may be x itself (with x's head_stride)."""
         eng = self.eng
         hd = eng.cfg.head_dim
-        eng._on_device(x, out, positions)
-        if positions is not None:
-            self._places(positions, x.shape[0])
+        if not (eng._fits and eng._fits(eng.device, -1, x, 0, None, out, 0, None)):
+            eng._on_device(x, out)
         cols, have = x.shape
+        if positions is not None and not (eng._exact and eng._exact(eng.device, positions, torch.int32, self.n_axes, cols)):
+            eng._on_device(positions)
+            self._places(positions, cols)
         hs, ohs, last, dt = head_stride or hd, out_head_stride or hd, n_heads - 1, _dt(x.dtype)
         if out is None:
             out, out_have, out_dt, ohs = torch.empty_strided((cols, n_heads * hd), (n_heads * hd, 1), dtype=x.dtype, device=eng._dev), n_heads * hd, dt, hd
@@ -186,11 +188,13 @@ class Rotary:
 
 class AttnEngine:
     """The attention part of an engine: per-layer f16 K/V caches and the per-layer attention step."""
+    _fits = _exact = None               # the call module's quick looks at tensors; without them every check is made one by one
 
     def __init__(self, cfg: AttnConfig, device: int = 0):
         self.cfg, self.device = cfg, device
         self.L = _l.load()
         self._call, e = self.L.call, self.L.entry
+        self._fits, self._exact = getattr(self._call, "fits", None), getattr(self._call, "exact", None)
         self._f_layer, self._f_items, self._f_rope, self._f_gather = e["pa_attn_layer"], e["pa_attn_items"], e["pa_rope_append"], e["pa_decode_gather"]
         self._f_rot_append, self._f_shared, self._f_weights, self._f_evict = e["pa_rotary_append"], e["pa_decode_shared"], e["pa_decode_weights"], e["pa_evict"]
         self._f_rot_at, self._f_tree, self._f_move = e["pa_rotary_append_at"], e["pa_decode_tree"], e["pa_cache_move"]
@@ -474,8 +478,9 @@ class AttnEngine:
         if k.stride(0) != v.stride(0) and total > 1:
             raise _l.PaError(-1, "k and v have different column strides")
         if positions is not None:
-            self._on_device(positions)
-            rot._places(positions, total)
+            if not (self._exact and self._exact(self.device, positions, torch.int32, rot.n_axes, total)):
+                self._on_device(positions)
+                rot._places(positions, total)
             rc = self._call.rotary_append_at(self._f_rot_at, rot._h, self.layers[li].value, items, rows, positions, q, q_head_stride or self.cfg.head_dim, k, v, q_out,
                                              _l.PA_F32 if q is None else _dt(q_out.dtype), self._raw_st())
             if rc:
@@ -502,6 +507,8 @@ class AttnEngine:
     def _columns(self, n: int, q, q_head_stride, k, v, out):
         """Columns of the engine's own types: q, k, v of act_dtype, n of each, q with all its heads."""
         c = self.cfg
+        if self._fits and self._fits(self.device, n, q, self._heads(q_head_stride), c.act_dtype, k, self._kv_dim, c.act_dtype, v, self._kv_dim, c.act_dtype, out, self._q_dim, None):
+            return
         self._on_device(q, k, v, out)
         for t, width in ((q, self._heads(q_head_stride)), (k, self._kv_dim), (v, self._kv_dim)):
             if t is not None:
@@ -517,6 +524,8 @@ class AttnEngine:
         """The tensors of a decode of n single tokens; returns out, made where it is None."""
         c = self.cfg
         act = c.act_dtype
+        if self._fits and self._fits(self.device, n, q, self._heads(q_head_stride), None, gate, self._heads(gate_head_stride) if gate is not None else 0, act, out, self._q_dim, act):
+            return torch.empty_strided((n, self._q_dim), (self._q_dim, 1), dtype=act, device=self._dev) if out is None else out
         self._on_device(q, gate)
         cols, have = q.shape
         if cols != n or self._heads(q_head_stride) > have:
@@ -541,7 +550,7 @@ class AttnEngine:
         rows; None: chains.  A token attends the committed rows, its ancestors and itself."""
         total = sum([it[2] for it in items])
         out = self._batch(total, q, q_head_stride, gate, gate_head_stride, out)
-        if parents is not None:
+        if parents is not None and not (self._exact and self._exact(self.device, parents, torch.int32, None, total)):
             self._on_device(parents)
             if parents.dtype != torch.int32 or parents.shape != (total,) or not parents.is_contiguous():
                 raise _l.PaError(-1, f"{parents.dtype} parents of shape {tuple(parents.shape)}: contiguous int32, one per token of {total}, are wanted")

@@ -33,7 +33,7 @@ typedef int (*fn_decode_weights)(pa_layer*, const pa_item*, uint32_t, const void
 typedef int (*fn_evict)(pa_layer*, const pa_evict_item*, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t*, void*);
 /* Every call names the entry point (its address in the library the engine loaded) as its first argument: the module keeps
  * nothing of its own. */
-static PyObject *s_data_ptr, *s_stride, *s_size, *i_zero;
+static PyObject *s_data_ptr, *s_stride, *s_size, *s_get_device, *s_is_contiguous, *s_shape, *s_dtype, *i_zero, *i_last;
 
 static int ptr_of(PyObject* t, void** p) {
   if (t == Py_None) { *p = NULL; return 0; }
@@ -398,7 +398,72 @@ static PyObject* evict(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
+/* Does tensor `t` lie on `device`, of `dtype` (None: any), in two dimensions, or in one?  Its extents (one: [1, n]); 1, 0, or -1 with an error
+ * set. */
+static int is_of(PyObject* t, int64_t device, PyObject* dtype, int two, int one, int64_t* extent) {
+  PyObject* r = PyObject_VectorcallMethod(s_get_device, &t, 1 | PY_VECTORCALL_ARGUMENTS_OFFSET, NULL);
+  if (!r) return -1;
+  const int64_t on = PyLong_AsLongLong(r);
+  Py_DECREF(r);
+  if (on != device) return PyErr_Occurred() ? -1 : 0;
+  if (dtype != Py_None) {
+    if (!(r = PyObject_GetAttr(t, s_dtype))) return -1;
+    Py_DECREF(r);
+    if (r != dtype) return 0;                  /* (torch's types are single objects) */
+  }
+  if (!(r = PyObject_GetAttr(t, s_shape))) return -1;
+  const Py_ssize_t dims = PyTuple_Check(r) ? PyTuple_GET_SIZE(r) : 0;
+  const int ok = (two && dims == 2) || (one && dims == 1);
+  extent[0] = 1;
+  for (Py_ssize_t i = 0; ok && i < dims; ++i) extent[2 - dims + i] = PyLong_AsLongLong(PyTuple_GET_ITEM(r, i));
+  Py_DECREF(r);
+  return ok && PyErr_Occurred() ? -1 : ok;
+}
+static int is_contiguous(PyObject* t) {
+  PyObject* r = PyObject_VectorcallMethod(s_is_contiguous, &t, 1 | PY_VECTORCALL_ARGUMENTS_OFFSET, NULL);
+  if (!r) return -1;
+  Py_DECREF(r);
+  return r == Py_True;
+}
+
+/* fits(device, cols, tensor, width, dtype, ...) -> bool: every tensor that is not None is a matrix of `cols` rows (below 0: any number) of
+ * at least `width` consecutive values, of dtype (None: any), on the device.  What does not fit is looked at again by the caller, who says why. */
+static PyObject* fits(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  int64_t device, cols, width, extent[2];
+  (void)self;
+  if (n < 2 || (n - 2) % 3) { PyErr_SetString(PyExc_TypeError, "fits takes a device, a number of columns, and a width and type for every tensor"); return NULL; }
+  if (int_of(a[0], INT32_MIN, INT32_MAX, "device", &device) || int_of(a[1], INT64_MIN, INT64_MAX, "number of columns", &cols)) return NULL;
+  int ok = 1;
+  for (Py_ssize_t i = 2; ok == 1 && i < n; i += 3) {
+    if (a[i] == Py_None) continue;
+    if (int_of(a[i + 1], INT64_MIN, INT64_MAX, "width", &width)) return NULL;
+    ok = is_of(a[i], device, a[i + 2], 1, 0, extent);
+    if (ok == 1) ok = (cols < 0 || extent[0] == cols) && extent[1] >= width;
+    if (ok == 1 && (ok = is_contiguous(a[i])) == 0) {
+      PyObject* b[2] = {a[i], i_last};
+      PyObject* r = PyObject_VectorcallMethod(s_stride, b, 2 | PY_VECTORCALL_ARGUMENTS_OFFSET, NULL);
+      ok = !r ? -1 : PyLong_AsLongLong(r) == 1;
+      Py_XDECREF(r);
+    }
+  }
+  return ok < 0 ? NULL : PyBool_FromLong(ok);
+}
+/* exact(device, tensor, dtype, rows, cols) -> bool: the tensor lies on the device, contiguous, of dtype and [rows, cols]; one row: [cols] too;
+ * rows = None: [cols] */
+static PyObject* exact(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  int64_t device, want[2] = {1, 0}, extent[2];
+  (void)self;
+  if (args_are(n, 5, "exact") || int_of(a[0], INT32_MIN, INT32_MAX, "device", &device) || int_of(a[4], INT64_MIN, INT64_MAX, "number of columns", &want[1]) ||
+      (a[3] != Py_None && int_of(a[3], INT64_MIN, INT64_MAX, "number of rows", &want[0])))
+    return NULL;
+  int ok = is_of(a[1], device, a[2], a[3] != Py_None, want[0] == 1, extent);
+  if (ok == 1) ok = extent[0] == want[0] && extent[1] == want[1] ? is_contiguous(a[1]) : 0;
+  return ok < 0 ? NULL : PyBool_FromLong(ok);
+}
+
 static PyMethodDef methods[] = {
+    {"fits", (PyCFunction)(void (*)(void))fits, METH_FASTCALL, "whether tensors are what a call takes"},
+    {"exact", (PyCFunction)(void (*)(void))exact, METH_FASTCALL, "whether a tensor has a shape and type"},
     {"attn_layer", (PyCFunction)(void (*)(void))attn_layer, METH_FASTCALL, "pa_attn_layer on tensors"},
     {"attn_items", (PyCFunction)(void (*)(void))attn_items, METH_FASTCALL, "pa_attn_items on tensors"},
     {"rope_append", (PyCFunction)(void (*)(void))rope_append, METH_FASTCALL, "pa_rope_append on tensors"},
@@ -417,7 +482,12 @@ PyMODINIT_FUNC PyInit__pa_call(void) {
   s_data_ptr = PyUnicode_InternFromString("data_ptr");
   s_stride = PyUnicode_InternFromString("stride");
   s_size = PyUnicode_InternFromString("size");
+  s_get_device = PyUnicode_InternFromString("get_device");
+  s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
+  s_shape = PyUnicode_InternFromString("shape");
+  s_dtype = PyUnicode_InternFromString("dtype");
   i_zero = PyLong_FromLong(0);
-  if (!s_data_ptr || !s_stride || !s_size || !i_zero) return NULL;
+  i_last = PyLong_FromLong(-1);
+  if (!s_data_ptr || !s_stride || !s_size || !s_get_device || !s_is_contiguous || !s_shape || !s_dtype || !i_zero || !i_last) return NULL;
   return PyModule_Create(&module);
 }

@@ -33,7 +33,7 @@ def detached():
     eng.cfg = AttnConfig(n_heads=4, n_kv_heads=2, head_dim=64, n_rot=64, rope_theta=1e4, max_seq=32, act_dtype=torch.float32)
     eng.device, eng.layers, eng._call, eng.ctx, eng.slots, eng._xc_keep, eng._q_dim, eng._kv_dim = -1, [C.c_void_p(8), C.c_void_p(16)], NoCalls(), None, {}, None, 256, 128
     eng._f_rot_append = eng._f_rot_at = eng._f_tree = eng._f_move = 0
-    eng._all_layers = None
+    eng._all_layers, eng._dev = None, torch.device("cpu")
     eng._raw_st = lambda: 0
     rot = object.__new__(Rotary)
     rot.eng, rot.handle, rot._h, rot._apply, rot._f_apply, rot.n_axes = eng, C.c_void_p(8), 8, NoCalls(), 0, 2
@@ -242,3 +242,66 @@ def test_js_methods_lay_out_what_the_header_says():
     tree = call(method("decodeTree"), "pa_decode_tree")
     assert tree[3] == "parents" and tree[8:11] == ["g", "gs", "gh"] and "this._gate(gate, qFull)" in method("decodeTree")
     assert "6 * items.length" in method("move") and call(method("move"), "pa_cache_move")[4:6] == ["lists", "listStride"]
+
+
+def test_the_quick_look_at_tensors_agrees_with_the_checks_one_by_one(pa, detached):
+    eng, rot = detached
+    fits, exact = pa.call.fits, pa.call.exact
+    z = torch.zeros
+    base = z((6, 512))
+    matrices = [z((2, 256)), z((2, 256)).half(), z((3, 256)), z((2, 255)), z((2, 300))[:, :256], z((256, 2)).t(), base[::3, :256], base[:2, ::2], z((1, 256)), z((256,)), z((2, 2, 256)),
+                z((2, 256), dtype=torch.bfloat16), z((0, 256)), z((2, 1))]
+    for q in matrices:
+        for gate in (None, *matrices):
+            for out in (None, *matrices):
+                try:
+                    eng._batch(2, q, None, gate, None, out)
+                    slow = True
+                except (PaError, ValueError):
+                    slow = False
+                assert fits(-1, 2, q, 256, None, gate, 256, torch.float32, out, 256, torch.float32) == slow, (q.shape, gate is not None and gate.shape, out is not None and out.shape)
+    for k in matrices:
+        try:
+            eng._columns(2, None, None, k[..., :128], z((2, 128)), None)
+            slow = True
+        except (PaError, ValueError):
+            slow = False
+        assert fits(-1, 2, None, 256, torch.float32, k[..., :128], 128, torch.float32, z((2, 128)), 128, torch.float32, None, 256, None) == slow, k.shape
+    assert not fits(0, 2, matrices[0], 256, None) and fits(-1, -1, matrices[2], 256, None) and fits(0, 2, None, 1, None)          # of another device; any number of columns
+    for p in [z((2, 3), dtype=I32), z((2, 3)), z((3, 2), dtype=I32), z((3, 2), dtype=I32).t(), z(3, dtype=I32), z((2, 6), dtype=I32)[:, ::2], z((1, 2, 3), dtype=I32)]:
+        try:
+            rot._places(p, 3)
+            slow = True
+        except PaError:
+            slow = False
+        assert exact(-1, p, I32, 2, 3) == slow, p.shape
+        assert exact(-1, p, I32, None, 3) == (tuple(p.shape) == (3,)) and not exact(0, p, I32, 2, 3)
+        rot.n_axes = 1
+        try:
+            rot._places(p, 3)
+            slow = True
+        except PaError:
+            slow = False
+        assert exact(-1, p, I32, 1, 3) == slow, p.shape
+        rot.n_axes = 2
+    assert exact(-1, z((1, 3), dtype=I32), I32, 1, 3) and not exact(-1, z((1, 3), dtype=I32), I32, None, 3)
+    for call in (lambda: fits(-1), lambda: fits(-1, 2, base), lambda: fits(-1, 2, base, "x", None), lambda: fits(-1, 2, 3, 4, None), lambda: exact(-1, base, None, 2), lambda: exact(-1, 5, None, 2, 3)):
+        with pytest.raises((TypeError, AttributeError)):
+            call()
+
+
+def test_engines_without_the_module_check_one_by_one(detached):
+    eng, rot = detached
+    assert eng._fits is None and eng._exact is None
+    calls = []
+    eng._call = type("Calls", (), {"decode_tree": lambda self, *a: calls.append(a) or 0, "rotary_append_at": lambda self, *a: calls.append(a) or 0})()
+    rot._apply = lambda *a: calls.append(a) or 0
+    q, kv = torch.zeros((2, 256)), torch.zeros((2, 128))
+    for fast in (False, True):
+        if fast:
+            eng._fits, eng._exact = L.load().call.fits, L.load().call.exact
+        calls.clear()
+        assert eng.decode_tree(0, [(0, 0, 2)], q, torch.zeros(2, dtype=I32), out=q) is q
+        assert eng.rotary_append(0, rot, [(0, 0, 2)], q, kv, kv, q_out=q, positions=torch.zeros((2, 2), dtype=I32)) is q
+        assert rot.apply(q, 4, positions=torch.zeros((2, 2), dtype=I32), out=q) is q
+        assert len(calls) == 3
