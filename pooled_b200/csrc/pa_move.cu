@@ -15,7 +15,7 @@
 //                     took a lower number has loaded that tile or is about to, without waiting for anybody ahead of its byte, so
 //                     every wait ends.  (The next number taken when the tile's loads are out: 70 us for 57, others wait for a tile
 //                     whose CTA is still busy with the one before.)  The CTA that is done last clears the words.
-// What bounds it: HBM, a row read and written once (a prompt of 8000 rows forked to seven sequences in two layers 43 us, 0.92 of the measured rate); rows over
+// What bounds it: HBM, a row read and written once (a prompt of 8000 rows forked to seven sequences in two layers 43 us, 0.93 of the measured rate); rows over
 // one another the wait for the other tile's byte on top of it (0.79 for a gap of 2000 rows, 0.55 for one of a row); a few rows the launch and two trips to memory, list and rows.
 #include <string.h>
 
