@@ -430,7 +430,7 @@ PA_API int pa_decode_tree(pa_layer* layer, const pa_item* items, uint32_t n_item
  * sums of layers whose weights are tracked.  Rows are cache rows, whatever the layer's origin.
  *   - a prompt forked to many sequences: items with the same source read it once
  *   - source and destination of one item may overlap: the destination ends up with the rows that the source held (rows that follow an
- *     evicted stretch move up to it, or down from it); n_rows = 0 moves nothing
+ *     evicted stretch move up to it, or down from it); n_rows = 0 moves nothing and meets no other item
  *   - lists (u32 on the device, list_stride words an item, as pa_decode_gather's): [0] = n, then n offsets into the item's rows; row j of the
  *     destination gets row src_row + offset j: the accepted path of a drafted tree (dst_row = src_row = base), a selection.  At most
  *     min(n_rows, list_stride - 1) rows of an item are moved; offsets that are not below n_rows move nothing.  Where source and

@@ -261,9 +261,9 @@ extern "C" int pa_cache_move(pa_layer* const* layers, uint32_t n_layers, const p
   p.max_seq = L->max_seq; p.n_kv = ctx->cfg.n_kv_heads; p.lists = lists; p.list_stride = list_stride; p.err = ctx->dev_err;
   bool sums = false;
   for (uint32_t i = 0; i < n_layers; ++i) sums = sums || layers[i]->sums;
-  // which rows an item may read and write
+  // which rows an item may read and write (a span without rows meets none)
   struct Span { uint32_t seq, a, b; };
-  auto meet = [](const Span& x, const Span& y) { return x.seq == y.seq && x.a < y.b && y.a < x.b; };
+  auto meet = [](const Span& x, const Span& y) { return x.seq == y.seq && std::max(x.a, y.a) < std::min(x.b, y.b); };
   Span from[kMaxMoves], to[kMaxMoves];
   for (uint32_t i = 0; i < n_items; ++i) {
     const pa_move_item& it = items[i];

@@ -1,0 +1,59 @@
+"""pa_cache_move at its edges: items and lists that move no row, wherever their rows would lie."""
+import pytest
+import torch
+
+from pooled_b200 import PaError
+from tests.test_gpu_move import engine, expected, fill, same
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = [("f16", 2, 256, True), ("q8", 2, 64, False), ("f32", 1, 128, False)]
+
+
+@pytest.mark.parametrize("kv,nKV,hd,track", FORMATS)
+@pytest.mark.parametrize("items", [
+    [(0, 0, 1, 0, 100), (1, 50, 2, 0, 0)],                                # its source inside another's destination,
+    [(0, 0, 1, 0, 100), (2, 50, 1, 50, 0)],                               # its destination,
+    [(0, 0, 1, 0, 100), (2, 0, 0, 50, 0)],                                # its destination inside another's source
+    [(1, 50, 2, 0, 0), (2, 50, 1, 60, 0), (0, 0, 1, 0, 100), (2, 0, 0, 50, 0), (0, 40, 0, 70, 0)],
+    [(0, 20, 0, 10, 700), (0, 30, 0, 40, 0)],                             # among rows that move over one another
+    [(0, 10, 0, 10, 0), (0, 5, 0, 15, 40)],
+    [(0, 5, 1, 5, 0), (0, 5, 1, 5, 0)]])
+def test_items_without_rows_meet_nothing(kv, nKV, hd, track, items):
+    eng = engine(nKV, hd, 800, 3, kv, layers=2)
+    if track:
+        eng.track_weights(0)
+    fill(eng, 1)
+    want = expected(eng, items)
+    eng.move(items)
+    assert same(eng, want)
+
+
+@pytest.mark.parametrize("items", [[(0, 0, 1, 0, 100), (0, 0, 1, 50, 100)], [(0, 0, 1, 0, 100), (1, 50, 0, 20, 60)], [(0, 10, 0, 30, 60)]])
+def test_lists_without_room_for_a_row_move_nothing(items):
+    # one word a list: its count, of rows that it has no offsets for.  Sources and destinations may then lie anywhere
+    eng = engine(2, 256, 200, 2)
+    fill(eng, 2)
+    want = expected(eng, [])
+    eng.move(items, lists=torch.full((len(items), 1), 7, dtype=torch.int32, device="cuda"))
+    assert same(eng, want)
+
+
+def test_spans_that_do_meet_are_refused_beside_items_without_rows():
+    eng = engine(2, 256, 200, 3)
+    fill(eng, 3)
+    want = expected(eng, [])
+    empty = (0, 50, 1, 50, 0)
+    for items in ([(0, 0, 1, 0, 100), (1, 99, 2, 0, 1)], [(0, 0, 1, 0, 100), (2, 0, 1, 99, 1)], [(0, 0, 1, 0, 100), (2, 0, 0, 0, 1)], [(0, 0, 1, 0, 100), (2, 0, 0, 99, 1)],
+                  [(0, 0, 1, 0, 1), (2, 0, 1, 0, 1)]):
+        for at in range(3):
+            with pytest.raises(PaError):
+                eng.move(items[:at] + [empty] + items[at:])
+    for bad in ((0, 201, 1, 0, 0), (0, 0, 1, 201, 0), (3, 0, 1, 0, 0), (0, 0, 3, 0, 0)):
+        with pytest.raises(PaError):
+            eng.move([(0, 0, 1, 0, 10), bad])
+    assert same(eng, want)
+    items = [(0, 0, 1, 0, 100), (1, 100, 2, 0, 1), (2, 10, 1, 101, 20), empty]         # neighbours do not meet
+    want = expected(eng, items)
+    eng.move(items)
+    assert same(eng, want)
