@@ -578,6 +578,8 @@ class AttnEngine:
             if lists.dtype != torch.int32 or lists.dim() != 2 or lists.shape[0] != len(items) or not lists.is_contiguous():
                 raise _l.PaError(-1, f"{lists.dtype} lists of shape {tuple(lists.shape)}: contiguous int32, one row per item of {len(items)}, are wanted")
             stride = lists.shape[1]
+            if not stride:                        # (an empty tensor has no address, and a call without lists moves whole items)
+                raise _l.PaError(-1, f"lists of shape {tuple(lists.shape)}: a list holds one word at least, its count")
         rc = self._call.cache_move(self._f_move, C.addressof(arr), n, items, lists, stride, self._raw_st())
         if rc:
             self._ck(rc)

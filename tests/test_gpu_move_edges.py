@@ -57,3 +57,13 @@ def test_spans_that_do_meet_are_refused_beside_items_without_rows():
     want = expected(eng, items)
     eng.move(items)
     assert same(eng, want)
+
+
+def test_lists_without_words_are_refused():
+    # (an empty tensor has no address: without the check the call would be one without lists, which moves whole items)
+    eng = engine(2, 256, 100, 2)
+    fill(eng, 4)
+    want = expected(eng, [])
+    with pytest.raises(PaError):
+        eng.move([(0, 0, 1, 0, 50)], lists=torch.empty((1, 0), dtype=torch.int32, device="cuda"))
+    assert same(eng, want)
