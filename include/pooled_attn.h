@@ -279,7 +279,9 @@ PA_API int pa_exchange_init(pa_ctx* ctx, uint32_t rank, uint32_t world, void* co
  * The same limit (0: 2^20 looks, about a second) bounds the wait of a single-token call over an f16 cache for the records of its own
  * CTAs, which need an SM each at the same time: beside a longer kernel of another stream that leaves them none it
  * ends with status 8 and PA_ETIMEOUT.  Calls over f32 caches wait no more than 2^12 looks, or this limit if that is less, and
- * then leave their share to the CTA that finishes last: they need no SM of their own and only take longer. */
+ * then leave their share to the CTA that finishes last: they need no SM of their own and only take longer.  And it bounds (0: 2^20
+ * looks) the wait of a pa_cache_move over rows that lie over one another for the tiles ahead of each tile (status 9): a tile whose wait runs
+ * out is not stored, so every word of the destination is the one that was there or the one that was moved there. */
 PA_API int pa_set_wait_limit(pa_ctx* ctx, uint32_t sweeps);
 /* pa_decode over this rank's shard with the cross-GPU merge inside the combine kernel: each CTA stores its merged
  * (o, m, l) slice into every rank's exchange buffer over NVLink, each value as one 8-byte {value, call tag} store,

@@ -809,7 +809,8 @@ class AttnEngine:
         self._xc_keep = None
 
     def set_wait_limit(self, sweeps: int):
-        """Polling limit of the waits for other GPUs' and a call's own CTAs' records (0: the built-in limits, about a second)."""
+        """Polling limit of the waits for other GPUs' and a call's own CTAs' records, and for tiles of moved rows (0: the built-in limits, about
+        a second)."""
         self._ck(self.L.pa_set_wait_limit(self.ctx, sweeps))
 
     def decode_exchange(self, li: int, items, q: torch.Tensor, gate: torch.Tensor | None = None, out: torch.Tensor | None = None,

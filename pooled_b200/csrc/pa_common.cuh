@@ -17,10 +17,10 @@
 namespace pa {
 
 // Every device-side wait is bounded: after this many polls the waiter records PA_WAIT_* in the context's
-// error word and carries on as if the wait had succeeded, so control flow stays uniform, every thread
+// error word and carries on as if the wait had succeeded (a tile of moved rows is left unstored), so control flow stays uniform, every thread
 // reaches the end of the kernel and the host reports PA_ETIMEOUT instead of a hung GPU.
 constexpr uint32_t kWaitPolls = 1u << 24;  // with 32..64 ns back-off: well under a second
-constexpr uint32_t kMergePolls = 1u << 20; // looks for another CTA's record: about a second
+constexpr uint32_t kMergePolls = 1u << 20; // looks for another CTA's record, or its tile of moved rows: about a second
 constexpr uint32_t kMergeLeave = 1u << 12; // ... before a unit is left to the CTA that comes last (f32 tokens): some milliseconds
 
 enum : uint32_t { WAIT_KFULL = 1, WAIT_VFULL = 2, WAIT_EMPTY = 3, WAIT_MMA = 4, WAIT_TMEM = 5, WAIT_QFULL = 6, WAIT_PEER = 7, WAIT_MERGE = 8, WAIT_MOVE = 9 };
@@ -421,7 +421,7 @@ struct pa_ctx {
     bool kv_evict_first = true;  // POOLED_ATTN_KV_EVICT_FIRST=0: decode / verify K and V tiles enter L2 with the default policy instead of evict-first
     bool no_merge = false;       // POOLED_ATTN_NO_MERGE: always merge the split records in the combine kernel
     int shared_wide = -1;        // POOLED_ATTN_SHARED_WIDE: wide units of shared rows wherever they can be (1), never (0), by the plan (-1)
-    uint32_t wait_polls = 0;     // pa_set_wait_limit: limit of the waits for other CTAs' and other GPUs' records (0: the built-in limits)
+    uint32_t wait_polls = 0;     // pa_set_wait_limit: limit of the waits for other CTAs' and other GPUs' records, and for tiles of moved rows (0: the built-in limits)
   } tune;
   // device: the scores of one pa_decode_weights call, or the lists of a pa_evict call (pa_layer_track_weights makes it as large as
   // the largest tracked layer wants it); `outgrown`: earlier ones, which captured graphs may still use

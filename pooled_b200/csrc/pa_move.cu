@@ -13,8 +13,9 @@
 //                     CTAs start is not defined), a tile's byte says that it has been loaded, and a CTA waits, with its own tile in
 //                     registers and its own byte set, for the one or two earlier tiles that its stores would overwrite.  Whoever
 //                     took a lower number has loaded that tile or is about to, without waiting for anybody ahead of its byte, so
-//                     every wait ends.  (The next number taken when the tile's loads are out: 70 us for 57, others wait for a tile
-//                     whose CTA is still busy with the one before.)  The CTA that is done last clears the words.
+//                     every wait ends; one that runs out of looks all the same leaves its tile unstored.  (The next number taken
+//                     when the tile's loads are out: 70 us for 57, others wait for a tile whose CTA is still busy with the one
+//                     before.)  The CTA that is done last clears the words.
 // What bounds it: HBM, a row read and written once (a prompt of 8000 rows forked to seven sequences in two layers 43 us, 0.93 of the measured rate); rows over
 // one another the wait for the other tile's byte on top of it (0.79 for a gap of 2000 rows, 0.55 for one of a row); a few rows the launch and two trips to memory, list and rows.
 #include <string.h>
@@ -46,17 +47,20 @@ __device__ __forceinline__ uint32_t mv_below(const uint32_t* list, uint32_t n, u
   return a;
 }
 
-// The tile has been loaded; waits until the one or two earlier tiles [lo, hi] that read what it will overwrite have been, too.
-__device__ __forceinline__ void mv_in_order(const MoveParams& p, uint8_t* said, uint32_t tile, uint32_t lo, uint32_t hi) {
+// The tile has been loaded; waits until the one or two earlier tiles [lo, hi] that read what it will overwrite have been, too.  False, for all
+// threads, where that took more than p.polls looks: the tile may not be stored then, rows that nobody has read yet would be lost.
+__device__ __forceinline__ bool mv_in_order(const MoveParams& p, uint8_t* said, uint32_t tile, uint32_t lo, uint32_t hi) {
+  bool late = false;
   if (threadIdx.x < 2 && lo + threadIdx.x <= hi && lo + threadIdx.x < tile) {
     uint32_t there = 0;
-    for (uint32_t i = 0; i < kWaitPolls && !there; ++i) {
+    for (uint32_t i = 0; i < p.polls && !there; ++i) {
       asm volatile("ld.relaxed.gpu.u8 %0, [%1];" : "=r"(there) : "l"(said + lo + threadIdx.x) : "memory");
       if (!there && i > 64) __nanosleep(32);
     }
-    if (!there) atomicMax(p.err, (uint32_t)WAIT_MOVE);
+    late = !there;
+    if (late) atomicMax(p.err, (uint32_t)WAIT_MOVE);
   }
-  __syncthreads();
+  return !__syncthreads_or(late);
 }
 // All threads have their part of the tile (the barrier takes a word made of all of it: a thread without its values does not get there), so
 // the byte need not be ordered behind anything: whoever sees it overwrites what is in registers here.
@@ -93,18 +97,20 @@ __device__ __forceinline__ uint32_t move_run(const MoveParams& p, uint32_t g, ui
 #pragma unroll
   for (uint32_t k = 0; k < kMvUnits; ++k)
     if (k * kMvThreads + threadIdx.x < len) x[k] = from[k * kMvThreads];
+  bool store = true;
   if (over) {
     if (ordered) {
       mv_say(said, tile, x);
       const uint64_t gap = (uint64_t)(up ? p.dst_row[i0] - p.row[g] : p.row[g] - p.dst_row[i0]) * a.per, e1 = e0 + len;
       uint32_t lo = 1, hi = 0;
       if (e1 > gap) { lo = (uint32_t)((e0 > gap ? e0 - gap : 0) / kMoveUnits); hi = (uint32_t)((e1 - gap - 1) / kMoveUnits); }
-      mv_in_order(p, said, tile, lo, hi);
+      store = mv_in_order(p, said, tile, lo, hi);
     } else {
       __syncthreads();
     }
   }
   const uint32_t next = ORDER ? mv_next(p) : 0;
+  if (!store) return next;
   for (uint32_t i = i0; i < i1; ++i) {
     T* to = mv_at<BYTES>(a, p.dst_seq[i], p.dst_row[i]) + first + threadIdx.x;
 #pragma unroll
@@ -146,6 +152,7 @@ __device__ __forceinline__ uint32_t move_rows_of(const MoveParams& p, uint32_t g
     to_at[k] = live ? r * a.per + c : ~0u;
     if (live) x[k] = from[(uint64_t)src * a.per + c];
   }
+  bool store = true;
   if (p.flags[g] & MOVE_OVER) {
     if (ordered) {
       mv_say(said, tile, x);
@@ -155,12 +162,13 @@ __device__ __forceinline__ uint32_t move_rows_of(const MoveParams& p, uint32_t g
         const uint32_t below = mv_below(list + 1, rows, first_row > gap ? first_row - gap : 0);
         lo = below / r_tile; hi = (below + live_rows - 1) / r_tile;
       }
-      mv_in_order(p, said, tile, lo, hi);
+      store = mv_in_order(p, said, tile, lo, hi);
     } else {
       __syncthreads();
     }
   }
   const uint32_t next = ORDER ? mv_next(p) : 0;
+  if (!store) return next;
   T* to = mv_at<BYTES>(a, p.dst_seq[i0], p.dst_row[i0]) + (uint64_t)first_row * a.per;
 #pragma unroll
   for (uint32_t k = 0; k < kMvUnits; ++k)
@@ -259,6 +267,7 @@ extern "C" int pa_cache_move(pa_layer* const* layers, uint32_t n_layers, const p
   for (int k = 0; k < 2; ++k) p.inv[k] = p.per[k] > 1 ? (uint32_t)((0x100000000ull + p.per[k] - 1) / p.per[k]) : 0;
   if (lists && p.per[0] > kMoveUnits) return fail(ctx, PA_EUNSUPPORTED, "pa_cache_move: listed rows of at most %u bytes", kMoveUnits * 16);
   p.max_seq = L->max_seq; p.n_kv = ctx->cfg.n_kv_heads; p.lists = lists; p.list_stride = list_stride; p.err = ctx->dev_err;
+  p.polls = ctx->tune.wait_polls ? ctx->tune.wait_polls : kMergePolls;
   bool sums = false;
   for (uint32_t i = 0; i < n_layers; ++i) sums = sums || layers[i]->sums;
   // which rows an item may read and write (a span without rows meets none)

@@ -326,6 +326,7 @@ struct MoveParams {
   uint8_t flags[kMaxMoves];                         // MOVE_* of a group
   const uint32_t* lists; uint32_t list_stride;
   unsigned int* words;                              // != nullptr: tiles of MOVE_OVER groups that are not MOVE_COLUMNS keep their order
+  uint32_t polls;                                   // ... and look this many times for the tiles ahead of them
   uint32_t* err;
 };
 

@@ -1,9 +1,9 @@
-"""pa_cache_move at its edges: items and lists that move no row, wherever their rows would lie."""
+"""pa_cache_move at its edges: items and lists that move no row, wherever their rows would lie, and an order of tiles whose wait runs out."""
 import pytest
 import torch
 
 from pooled_b200 import PaError
-from tests.test_gpu_move import engine, expected, fill, same
+from tests.test_gpu_move import arrays, engine, expected, fill, same
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,46 @@ def test_lists_without_words_are_refused():
     with pytest.raises(PaError):
         eng.move([(0, 0, 1, 0, 50)], lists=torch.empty((1, 0), dtype=torch.int32, device="cuda"))
     assert same(eng, want)
+
+
+@pytest.mark.parametrize("up,listed", [(False, False), (True, False), (False, True)])
+def test_a_wait_that_runs_out_overwrites_no_row_that_was_not_read(up, listed):
+    # one look for the neighbour's tile: the call comes back by itself with a status, every word is the one that was there or the one that belongs
+    # there, and after a reset moves are right again
+    eng = engine(4, 256, 20000, 1)
+    n = 19999
+    if listed:
+        kept = [i for i in range(20000) if i % 3]
+        items, lists = [(0, 0, 0, 0, 20000)], [[len(kept), *kept]]
+        on_device = torch.tensor(lists, dtype=torch.int32, device="cuda")
+    else:
+        items, lists, on_device = [(0, 0, 0, 1, n) if up else (0, 1, 0, 0, n)], None, None
+    ran_out = 0
+    for trial in range(40):
+        fill(eng, trial)
+        was, want = expected(eng, []), expected(eng, items, lists)
+        eng.set_wait_limit(1)
+        eng.move(items, lists=on_device)
+        try:
+            eng.sync()
+        except PaError as e:
+            assert e.code == -5                                            # PA_ETIMEOUT
+            ran_out += 1
+            with pytest.raises(PaError) as latched:
+                eng.move(items, lists=on_device)
+            assert latched.value.code == -6                                # PA_ESTATE
+            eng.reset()
+            for layer, b, w in zip(arrays(eng), was, want):
+                for x, y, z in zip(layer, b, w):
+                    assert torch.all((x == y) | (x == z))
+        else:
+            assert same(eng, want)
+        eng.set_wait_limit(0)
+        if ran_out == 3:
+            break
+    assert ran_out
+    fill(eng, 99)
+    for _ in range(2):
+        want = expected(eng, items, lists)
+        eng.move(items, lists=on_device)
+        assert same(eng, want)
