@@ -86,11 +86,11 @@ template <int BYTES> __device__ __forceinline__ typename MvUnit<BYTES>::T* mv_at
 
 // a tile of a range: a run of units, counted from the end where rows move up over one another
 template <int BYTES, bool ORDER>
-__device__ __forceinline__ uint32_t move_run(const MoveParams& p, uint32_t g, uint32_t tile, const MvArray& a, bool ordered, uint8_t* said) {
+__device__ __forceinline__ uint32_t move_run(const MoveParams& p, uint32_t g, uint32_t tile, const MvArray& a, uint8_t* said) {
   using T = typename MvUnit<BYTES>::T;
   const uint64_t total = (uint64_t)p.n[g] * a.per, e0 = (uint64_t)tile * kMoveUnits;
   const uint32_t len = (uint32_t)min((uint64_t)kMoveUnits, total - e0), i0 = p.item0[g], i1 = p.item0[g + 1];
-  const bool over = p.flags[g] & MOVE_OVER, up = p.flags[g] & MOVE_UP;
+  const bool up = p.flags[g] & MOVE_UP;
   const uint64_t first = up ? total - e0 - len : e0;   // the tile's first unit
   const T* from = mv_at<BYTES>(a, p.seq[g], p.row[g]) + first + threadIdx.x;
   T x[kMvUnits] = {};
@@ -98,15 +98,13 @@ __device__ __forceinline__ uint32_t move_run(const MoveParams& p, uint32_t g, ui
   for (uint32_t k = 0; k < kMvUnits; ++k)
     if (k * kMvThreads + threadIdx.x < len) x[k] = from[k * kMvThreads];
   bool store = true;
-  if (over) {
-    if (ordered) {
+  if constexpr (ORDER) {                               // (ranges over one another that are no columns are always taken in order)
+    if (p.flags[g] & MOVE_OVER) {
       mv_say(said, tile, x);
       const uint64_t gap = (uint64_t)(up ? p.dst_row[i0] - p.row[g] : p.row[g] - p.dst_row[i0]) * a.per, e1 = e0 + len;
       uint32_t lo = 1, hi = 0;
       if (e1 > gap) { lo = (uint32_t)((e0 > gap ? e0 - gap : 0) / kMoveUnits); hi = (uint32_t)((e1 - gap - 1) / kMoveUnits); }
       store = mv_in_order(p, said, tile, lo, hi);
-    } else {
-      __syncthreads();
     }
   }
   const uint32_t next = ORDER ? mv_next(p) : 0;
@@ -122,7 +120,7 @@ __device__ __forceinline__ uint32_t move_run(const MoveParams& p, uint32_t g, ui
 
 // a tile of whole rows, listed ones, or of a few columns of all of an item's rows
 template <int BYTES, bool ORDER>
-__device__ __forceinline__ uint32_t move_rows_of(const MoveParams& p, uint32_t g, uint32_t tile, const MvArray& a, bool ordered, uint8_t* said) {
+__device__ __forceinline__ uint32_t move_rows_of(const MoveParams& p, uint32_t g, uint32_t tile, const MvArray& a, uint8_t* said) {
   using T = typename MvUnit<BYTES>::T;
   const uint32_t tid = threadIdx.x, n = p.n[g], i0 = p.item0[g];
   const bool columns = p.flags[g] & MOVE_COLUMNS;
@@ -153,8 +151,10 @@ __device__ __forceinline__ uint32_t move_rows_of(const MoveParams& p, uint32_t g
     if (live) x[k] = from[(uint64_t)src * a.per + c];
   }
   bool store = true;
-  if (p.flags[g] & MOVE_OVER) {
-    if (ordered) {
+  if (columns) {
+    __syncthreads();                                   // all of the item's rows are in registers
+  } else if constexpr (ORDER) {
+    if (p.flags[g] & MOVE_OVER) {
       mv_say(said, tile, x);
       uint32_t lo = 1, hi = 0;
       const uint32_t gap = p.row[g] - p.dst_row[i0], past = first_row + live_rows;        // row r of the destination is row r - gap of the source
@@ -163,8 +163,6 @@ __device__ __forceinline__ uint32_t move_rows_of(const MoveParams& p, uint32_t g
         lo = below / r_tile; hi = (below + live_rows - 1) / r_tile;
       }
       store = mv_in_order(p, said, tile, lo, hi);
-    } else {
-      __syncthreads();
     }
   }
   const uint32_t next = ORDER ? mv_next(p) : 0;
@@ -196,18 +194,17 @@ __device__ __forceinline__ uint32_t move_tile(const MoveParams& p, uint32_t unit
     tile = v - p.first[kind][g];
   }
   uint8_t* said = ORDER ? reinterpret_cast<uint8_t*>(p.words + kMoveHead) + (unit - u) + array * p.tiles[kind] + p.first[kind][g] : nullptr;      // bytes of the group's tiles of this array
-  const bool ordered = ORDER && (p.flags[g] & (MOVE_OVER | MOVE_COLUMNS)) == MOVE_OVER;
   MvArray a;
   if (kind == 0) a = MvArray{reinterpret_cast<uint8_t*>(p.rows[layer][which]), p.max_seq, p.per[0], p.inv[0]};
   else if (kind == 1) a = MvArray{reinterpret_cast<uint8_t*>(p.scales[layer][which]), p.max_seq, p.per[1], p.inv[1]};
   else a = MvArray{reinterpret_cast<uint8_t*>(p.sums[layer] ? p.sums[layer] + (uint64_t)which * p.max_seq : nullptr), (uint64_t)p.n_kv * p.max_seq, 1, 0};
   const bool run = RUNS || (!p.lists && !(p.flags[g] & MOVE_COLUMNS));
   if (kind == 0) {
-    if (run) return move_run<16, ORDER>(p, g, tile, a, ordered, said);
-    if constexpr (!RUNS) return move_rows_of<16, ORDER>(p, g, tile, a, ordered, said);
+    if (run) return move_run<16, ORDER>(p, g, tile, a, said);
+    if constexpr (!RUNS) return move_rows_of<16, ORDER>(p, g, tile, a, said);
   } else if (a.start) {
-    if (run) return move_run<4, ORDER>(p, g, tile, a, ordered, said);
-    if constexpr (!RUNS) return move_rows_of<4, ORDER>(p, g, tile, a, ordered, said);
+    if (run) return move_run<4, ORDER>(p, g, tile, a, said);
+    if constexpr (!RUNS) return move_rows_of<4, ORDER>(p, g, tile, a, said);
   }
   return ORDER ? mv_next(p) : 0;
 }
