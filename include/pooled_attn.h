@@ -420,7 +420,8 @@ PA_API int pa_rotary_append_at(pa_rotary* rotary, pa_layer* layer, const pa_item
  * device, read when the kernels run): for every column of the call the number within its tree of the token that it follows, an earlier one;
  * any other value: it follows the committed rows.  A token attends the committed rows, its ancestors and itself, whatever the other
  * tokens' rows hold (infinities and NaN too).  parents = NULL: chains, every token follows the one before it.  n_cols = 1: a single
- * token.  Items may repeat a sequence.  q, gate, out and their limits as pa_decode_shared's.  At most 32 items; f16 caches, origin 0. */
+ * token.  Items may repeat a sequence.  q, gate, out and their limits as pa_decode_shared's.  At most 32 items; f16 caches, origin 0.
+ * The context holds records for calls of max_cols tokens; a call of more adds up longer runs of rows, or takes several launches. */
 PA_API int pa_decode_tree(pa_layer* layer, const pa_item* items, uint32_t n_items, const int32_t* parents, const void* q, int q_dtype, uint64_t q_col_stride,
                           uint64_t q_head_stride, const void* gate, uint64_t gate_col_stride, uint64_t gate_head_stride, void* out, uint64_t out_col_stride,
                           void* stream);

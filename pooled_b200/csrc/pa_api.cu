@@ -189,12 +189,7 @@ extern "C" int pa_create(int device, const pa_config* cfg, pa_ctx** out) {
   }
   if (half && (e = cudaMalloc(&ctx->angles, (size_t)cfg->max_cols * half * sizeof(Angle))) != cudaSuccess) return bail(PA_ENOMEM, "cudaMalloc(angles)", e);
   if ((e = cudaMalloc(&ctx->q_rot, (size_t)cfg->max_cols * cfg->n_heads * cfg->head_dim * 4)) != cudaSuccess) return bail(PA_ENOMEM, "cudaMalloc(q_rot)", e);
-  // split partials: one (o, m, l) record per (query row, split).  A call uses rows * splits of them, about
-  // 64 rows x one CTA per SM; the split planner keeps every call inside this capacity.
-  ctx->part_slots = 16384;
-  // a prefill call of few columns splits its keys: 400 columns of 24 heads three ways are 28800 records
-  ctx->pf_slots = std::max<size_t>(ctx->part_slots, std::min<size_t>(32768, (size_t)cfg->max_cols * cfg->n_heads * kPrefillSplits));
-  ctx->tree_slots = std::max<size_t>(32768, std::min<size_t>(65536, (size_t)cfg->max_cols * cfg->n_heads * 4));
+  size_records(ctx);
   if ((e = cudaMalloc(&ctx->part_o, ctx->tree_slots * cfg->head_dim * 4)) != cudaSuccess) return bail(PA_ENOMEM, "cudaMalloc(part_o)", e);
   if ((e = cudaMalloc(&ctx->part_ml, ctx->tree_slots * 2 * 4)) != cudaSuccess) return bail(PA_ENOMEM, "cudaMalloc(part_ml)", e);
   ctx->merge_bytes = (size_t)ctx->sm_count * 16 * (cfg->head_dim + cfg->head_dim / 32) * 4;   // one CTA per SM, at most 16 query rows each

@@ -1,5 +1,7 @@
-// What the files with C entry points share: error messages, the guards of a call, the current device.
+// What the files with C entry points share: error messages, the guards of a call, the current device, the sizes of a context's buffers.
 #pragma once
+#include <algorithm>
+
 #include "pa_common.cuh"
 
 namespace pa {
@@ -22,6 +24,20 @@ class DeviceScope {
  private:
   int before_ = 0, device_ = 0;
 };
+
+// How many records, one (o, m, l) per (query row, run of tiles), the partial buffers of a context hold and a call may use.
+inline void size_records(pa_ctx* ctx) {
+  const size_t rows = (size_t)ctx->cfg.max_cols * ctx->cfg.n_heads;
+  // about 64 rows x one CTA per SM; the split planner keeps every call inside this capacity
+  ctx->part_slots = 16384;
+  // a prefill call of few columns splits its keys: 400 columns of 24 heads three ways are 28800 records
+  ctx->pf_slots = std::max<size_t>(ctx->part_slots, std::min<size_t>(32768, rows * kPrefillSplits));
+  // Trees: one for each of 64 rows of two CTAs an SM, or 136 for each row of max_cols tokens, which are runs of 4 tiles (the shortest that f32 outputs
+  // ask for) behind 34816 committed rows, up to 32768 in all; more tokens: four for each row, up to 65536.  (32768 for every context were 14 MB more at
+  // head_dim 256 for one of 8 columns and 16 heads, and no other plan for its trees.)
+  const size_t few = std::max<size_t>(rows * 136, (size_t)ctx->sm_count * 128);
+  ctx->tree_slots = std::max(ctx->pf_slots, std::min(few, std::max<size_t>(32768, std::min<size_t>(65536, rows * 4))));
+}
 
 // whether any two of the pieces of `len` values that begin at c * col_stride + h * head_stride, c < n_cols, h < n_heads, overlap
 inline bool pieces_overlap(uint64_t n_cols, uint64_t col_stride, uint64_t n_heads, uint64_t head_stride, uint64_t len) {
