@@ -51,3 +51,17 @@ def test_contexts_of_few_columns_plan_their_trees_as_if_they_held_more_records(p
             fewer += 1
             assert plan(nH, nKV, hd, f16, cols, sizes, records=32768)[1] == launches, (nH, nKV, hd, f16, sizes)
     assert fewer > 100
+
+
+def test_the_long_runs_of_the_gpu_tests_are_reached(plan):
+    # wide and narrow row tiles, units of several runs (added up in one record, or a record each) and of one, at every head_dim that tests name
+    from tests.test_gpu_tree_runs import CASES
+    reached = set()
+    for name, (nH, nKV, hd, f16, cols, sizes, wide, several, run) in CASES.items():
+        _, launches = plan(nH, nKV, hd, f16, cols, sizes)
+        kernels = [(bool(p["wide"]), p["fold"] > 1 or (bool(p["wide"]) and p["tiles"] > p["run"])) for p in launches]       # (WIDE, FOLD)
+        assert kernels[0] == (wide, several) and max(p["run"] for p in launches) == run, (name, launches)
+        reached.update((hd, *k) for k in kernels)
+        reached.update((hd, "added up" if p["fold"] > 1 else "one by one") for p in launches if p["wide"])
+    assert {(hd, True, True) for hd in (256, 128, 64)} <= reached and {(hd, False, True) for hd in (256, 128, 64)} <= reached
+    assert {(256, "added up"), (128, "added up"), (64, "added up"), (128, "one by one")} <= reached
