@@ -8,7 +8,7 @@
 //
 // Rows that move over one another (destination and source of an item overlap) may not be stored before they have been read:
 //   up to 512 rows    a tile is a few columns of all the rows, and the CTA's barrier between loading and storing is enough: no
-//                     order between tiles (the accepted paths of 8 trees in 8 layers of 8 x 128: 4.0 us)
+//                     order between tiles (the accepted paths of 8 trees in 8 layers of 8 x 128: 3.9 us)
 //   more              tiles are taken in the rows' order (from the side that they move to; from a counter, since the order in which
 //                     CTAs start is not defined), a tile's byte says that it has been loaded, and a CTA waits, with its own tile in
 //                     registers and its own byte set, for the one or two earlier tiles that its stores would overwrite.  Whoever
@@ -16,8 +16,8 @@
 //                     every wait ends; one that runs out of looks all the same leaves its tile unstored.  (The next number taken
 //                     when the tile's loads are out: 70 us for 57, others wait for a tile whose CTA is still busy with the one
 //                     before.)  The CTA that is done last clears the words.
-// What bounds it: HBM, a row read and written once (a prompt of 8000 rows forked to seven sequences in two layers 43 us, 0.93 of the measured rate); rows over
-// one another the wait for the other tile's byte on top of it (0.79 for a gap of 2000 rows, 0.55 for one of a row); a few rows the launch and two trips to memory, list and rows.
+// What bounds it: HBM, a row read and written once (a prompt of 8000 rows forked to seven sequences in two layers 43.5 us, 0.92 of the measured rate); rows over
+// one another the wait for the other tile's byte on top of it (0.78 to 0.80 for a gap of 2000 rows, 0.55 for one of a row); a few rows the launch and two trips to memory, list and rows.
 #include <string.h>
 
 #include <algorithm>
